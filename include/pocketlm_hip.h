@@ -778,6 +778,98 @@ int kv_dense_layer_decode_u16_ext(void* handle, int64_t layer, const uint16_t* h
                                   int64_t intermediate_size, int64_t num_heads, int64_t num_kv_heads, float rms_eps,
                                   float rope_theta);
 
+/* ---------------------------------------------------------------------------
+ * A batched decode step over FP8 weights and a paged cache (no counterparts in
+ * the reference, whose decode takes one sequence and fp32 activations).
+ * dtype_code: 0 fp16, 1 bf16, 2 fp32. */
+
+/* Activation rows in e4m3 with one fp32 scale for each 128 columns:
+ *   scale[r][b] = max(max |x[r][128 b ..]| / 448, 2^-126),
+ *   out[r][c] = e4m3(x[r][c] / scale[r][c / 128]), to nearest even.
+ * A block that holds an infinity or a NaN gets the scale NaN and bytes 0x7F.
+ * x [rows][cols], x_stride values from row to row (fp16, bf16 or fp32);
+ * out_fp8 [rows][cols], out_scales fp32 [rows][ceil(cols / 128)].  Codes -1
+ * null, -2 bad dimensions (cols above 65536 among them). */
+int fp8_e4m3_quantize_rows(const void* x, uint8_t* out_fp8, float* out_scales, int64_t rows, int64_t cols,
+                           int64_t x_stride, int dtype_code);
+/* The same of y = s * rsqrt(mean(s^2) + rms_eps) * weight, where s is
+ * x + residual rounded to the rows' type and written to out_sum [rows][cols]
+ * (which may be x or residual themselves, with a row stride of cols), or x
+ * itself where residual is NULL (out_sum is not written then).  y is fp32 and
+ * is not rounded before its quantization.  x, residual, weight [cols] and
+ * out_sum share dtype_code.  Codes as above. */
+int fp8_e4m3_rms_norm_rows(const void* x, const void* residual, const void* weight, void* out_sum, uint8_t* out_fp8,
+                           float* out_scales, int64_t rows, int64_t cols, int64_t x_stride, int64_t residual_stride,
+                           int dtype_code, float rms_eps);
+/* Such rows times an FP8 block-scaled weight:
+ *   out[m][n] = sum_b x_scales[m][b] * scale_inv[n / 128][b]
+ *               * sum_{k in block b} x[m][k] * W[n][k],
+ * fp32 sums, rounded once to dtype_code.  x [rows][in_cols], x_scales
+ * [rows][ceil(in_cols / 128)], fp8_weight [out_rows][in_cols], scale_inv
+ * [ceil(out_rows / 128)][scale_cols], out [rows][out_rows].  NaN bytes are
+ * NaN, in the weight too (the fp8_e4m3_block_linear family counts them as 0,
+ * as the reference's decoder does).  scratch: device memory of at least
+ * fp8_e4m3_block_matmul_scratch_bytes, 16-byte aligned, or NULL for the
+ * library's own.  Codes -1 null, -2 bad dimensions, -3 scratch. */
+int fp8_e4m3_block_matmul(const uint8_t* x, const float* x_scales, const uint8_t* fp8_weight, const float* scale_inv,
+                          void* out, void* scratch, int64_t scratch_bytes, int64_t rows, int64_t out_rows,
+                          int64_t in_cols, int64_t scale_cols, int dtype_code);
+int64_t fp8_e4m3_block_matmul_scratch_bytes(int64_t rows, int64_t out_rows, int64_t in_cols);
+
+/* A key-value cache in pages.  k_cache and v_cache [num_pages][page_size]
+ * [kv_heads][head_dim] (fp16 or bf16) share the strides page_stride,
+ * slot_stride and head_stride (values; multiples of 8; head_dim adjacent), so
+ * [page][head][slot] orders serve too.  Position p of sequence b is slot
+ * p % page_size of page page_table[b][p / page_size] (int32
+ * [sequences][table_cols]).  lengths int32 [sequences]: the positions a
+ * sequence holds before the call's rows; negative for an idle sequence.
+ * head_dim is a multiple of 8 up to 256; addresses are 16-byte aligned; a
+ * cache spans at most 64 GiB; table_cols * page_size < 2^31.
+ *
+ * Appends `rows` rows of keys and values [rows][kv_heads][head_dim] (strides
+ * in values, multiples of 8) and rotates them and the queries
+ * [rows][heads][head_dim] (heads 0 and NULLs without) to their positions:
+ * row i of sequence b has position lengths[b] + i.  Rows belong to the
+ * sequences by row_starts (int32 [sequences + 1], ascending: sequence b has
+ * rows [row_starts[b], row_starts[b + 1])), or, where that is NULL, in equal
+ * shares (rows a multiple of sequences).  rope_frequencies: double
+ * [rope_pairs], the angle of pair i at position p is p * frequency, reduced in
+ * 64 bits; pairs are (i, i + rope_pairs) of a head, or (2 i, 2 i + 1) when
+ * interleaved; values past 2 * rope_pairs and values v stay as they are
+ * (rope_pairs 0: all).  q_out [rows][heads][head_dim], contiguous: zeros for
+ * rows of no sequence or of an idle one, which are not stored either.  A row
+ * whose position has no page (past the table, or an entry outside
+ * [0, num_pages)) is not stored; their number is added to *rejected (int32,
+ * device; may be NULL).  Two rows must not share a slot.  Codes -1 null, -2
+ * bad dimensions. */
+int kv_paged_append_u16(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* q_out, uint16_t* k_cache,
+                        uint16_t* v_cache, const int* page_table, const int* lengths, const int* row_starts,
+                        const double* rope_frequencies, int* rejected, int64_t rows, int64_t sequences, int64_t heads,
+                        int64_t kv_heads, int64_t head_dim, int64_t rope_pairs, int interleaved, int64_t q_row_stride,
+                        int64_t q_head_stride, int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride,
+                        int64_t v_head_stride, int64_t table_cols, int64_t num_pages, int64_t page_size,
+                        int64_t page_stride, int64_t slot_stride, int64_t head_stride, int dtype_code);
+/* Attention of `rows` (1 to 8) new rows of each sequence over its pages, with
+ * the lengths that the append took: row r sees positions 0 .. lengths[b] + r.
+ *   out[b][r][h] = softmax(q[b][r][h] . K * softmax_scale) V
+ * with the key-value head h / (heads / kv_heads).  Positions without a page
+ * are left out, those past the table too; a row that sees nothing is zero.
+ * What a row does not see never reaches it, NaN or not.  q
+ * [sequences][rows][heads][head_dim] with strides in values (multiples of 8);
+ * out contiguous.  The work is dealt out from the lengths on the device.
+ * scratch as in fp8_e4m3_block_matmul (kv_paged_attention_scratch_bytes;
+ * capacity is table_cols * page_size).  Codes -1 null, -2 bad dimensions, -3
+ * scratch. */
+int kv_paged_attention_decode_u16(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,
+                                  const int* page_table, const int* lengths, uint16_t* out, void* scratch,
+                                  int64_t scratch_bytes, int64_t sequences, int64_t rows, int64_t heads,
+                                  int64_t kv_heads, int64_t head_dim, int64_t q_seq_stride, int64_t q_row_stride,
+                                  int64_t q_head_stride, int64_t table_cols, int64_t num_pages, int64_t page_size,
+                                  int64_t page_stride, int64_t slot_stride, int64_t head_stride, float softmax_scale,
+                                  int dtype_code);
+int64_t kv_paged_attention_scratch_bytes(int64_t sequences, int64_t rows, int64_t heads, int64_t kv_heads,
+                                         int64_t head_dim, int64_t capacity);
+
 #ifdef __cplusplus
 }
 #endif

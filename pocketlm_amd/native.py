@@ -26,6 +26,7 @@ purpose:
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from dataclasses import dataclass
 from pathlib import Path
@@ -171,6 +172,7 @@ class _launch:
         if self.previous >= 0:
             torch.cuda.set_device(self.index)
         self.lib.pocketlm_set_stream(_raw_stream(self.index))
+        return self.index
 
     def __exit__(self, *exc):
         if self.previous >= 0:
@@ -1825,3 +1827,314 @@ class NativeKvSession:
                 self._handle, int(layer), _p(x), int(rows.shape[0]), *[_p(t) for t in tensors], _p(out), *scalars)
         _check("kv_dense_layer_prefill_u16_ext_packed_rows8", code)
         return out
+
+
+# --------------------------------------------------------------------------- batched decode over FP8 rows and pages
+#
+# No counterparts in the reference, whose decode takes one sequence with fp32
+# activations.  A decode step of a batch: fp8_e4m3_rms_norm_rows, the fused
+# q/k/v projection (fp8_e4m3_block_matmul), kv_paged_append,
+# kv_paged_attention_decode, fp8_e4m3_quantize_rows and the o projection.
+# These calls take device tensors and allocate only with torch, scratch
+# included, so each captured graph has its own.
+
+_FP8_DTYPES = (torch.float8_e4m3fn, torch.uint8)
+_ROW_CODES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+class Fp8Rows(NamedTuple):
+    """Activation rows in e4m3 with a scale for each 128 columns."""
+    data: torch.Tensor    # float8_e4m3fn [rows, cols]
+    scales: torch.Tensor  # float32 [rows, ceil(cols / 128)]
+
+
+def native_fp8_rows_available() -> bool:
+    return _available("PCKETLM_DISABLE_NATIVE_FP8_LINEAR")
+
+
+def native_paged_kv_available() -> bool:
+    return _available("PCKETLM_DISABLE_NATIVE_KV")
+
+
+def _device_only(what: str, device: torch.device, *tensors: torch.Tensor | None) -> None:
+    if device.type != "cuda":
+        raise ValueError(f"{what} takes tensors on a HIP device")
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"{what} takes tensors on one HIP device")
+
+
+def _norm_input(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """Rows [rows, cols] with adjacent columns, and their stride."""
+    rows = t if t.ndim == 2 else t.reshape(-1, t.shape[-1])
+    if rows.stride(1) != 1 and rows.shape[1] != 1:
+        rows = rows.contiguous()
+    return rows, rows.stride(0)
+
+
+def _new_fp8_rows(rows: int, cols: int, device: torch.device) -> Fp8Rows:
+    return Fp8Rows(torch.empty((rows, cols), dtype=torch.float8_e4m3fn, device=device),
+                   torch.empty((rows, (cols + 127) // 128), dtype=torch.float32, device=device))
+
+
+def fp8_e4m3_quantize_rows(x: torch.Tensor) -> Fp8Rows:
+    """Rows [..., cols] of fp16, bf16 or fp32 in e4m3 with a scale of
+    max|x| / 448 for each 128 columns (pocketlm_hip.h)."""
+    lib = _require("PCKETLM_DISABLE_NATIVE_FP8_LINEAR", "Native FP8 rows")
+    code = _ROW_CODES.get(x.dtype)
+    if code is None:
+        raise TypeError("fp8_e4m3_quantize_rows requires torch.float16, torch.bfloat16 or torch.float32 rows")
+    if x.ndim < 1 or x.shape[-1] == 0:
+        raise ValueError("x must have shape [..., cols]")
+    device = x.device
+    _device_only("fp8_e4m3_quantize_rows", device)
+    x, stride = _norm_input(x)
+    rows, cols = x.shape
+    out = _new_fp8_rows(rows, cols, device)
+    if rows:
+        with _launch(lib, device):
+            code = lib.fp8_e4m3_quantize_rows(x.data_ptr(), out.data.data_ptr(), out.scales.data_ptr(), rows, cols,
+                                              stride, code)
+        _check("fp8_e4m3_quantize_rows", code)
+    return out
+
+
+def fp8_e4m3_rms_norm_rows(x: torch.Tensor, weight: torch.Tensor, *, rms_eps: float,
+                           residual: torch.Tensor | None = None) -> tuple[Fp8Rows, torch.Tensor]:
+    """(rows, sum): sum = x + residual in x's type (x itself without a
+    residual), rows the RMS norm of sum times weight in e4m3 with a scale for
+    each 128 columns.  x [..., cols]; sum has x's shape."""
+    lib = _require("PCKETLM_DISABLE_NATIVE_FP8_LINEAR", "Native FP8 rows")
+    dtype = x.dtype
+    code = _ROW_CODES.get(dtype)
+    if code is None:
+        raise TypeError("fp8_e4m3_rms_norm_rows requires torch.float16, torch.bfloat16 or torch.float32 rows")
+    if weight.dtype != dtype or (residual is not None and residual.dtype != dtype):
+        raise TypeError("fp8_e4m3_rms_norm_rows requires rows, weight and residual to share dtype")
+    shape, device = x.shape, x.device
+    if x.ndim < 1 or shape[-1] == 0:
+        raise ValueError("x must have shape [..., cols]")
+    if weight.shape != shape[-1:]:
+        raise ValueError("weight must hold one value per column")
+    if residual is not None and residual.shape != shape:
+        raise ValueError("residual must have the shape of x")
+    _device_only("fp8_e4m3_rms_norm_rows", device, weight, residual)
+    xr, stride = _norm_input(x)
+    rows, cols = xr.shape
+    w = weight if weight.is_contiguous() else weight.contiguous()
+    out = _new_fp8_rows(rows, cols, device)
+    if residual is None:
+        summed, rr, r_stride = x, None, 0
+    else:
+        summed = torch.empty(shape, dtype=dtype, device=device)
+        rr, r_stride = _norm_input(residual)
+    if rows:
+        with _launch(lib, device):
+            code = lib.fp8_e4m3_rms_norm_rows(xr.data_ptr(), None if rr is None else rr.data_ptr(), w.data_ptr(),
+                                              None if rr is None else summed.data_ptr(), out.data.data_ptr(),
+                                              out.scales.data_ptr(), rows, cols, stride, r_stride, code, rms_eps)
+        _check("fp8_e4m3_rms_norm_rows", code)
+    return out, summed
+
+
+@functools.lru_cache(maxsize=4096)
+def _matmul_scratch(rows: int, out_rows: int, in_cols: int, device_index: int) -> int:
+    return int(_lib.load().fp8_e4m3_block_matmul_scratch_bytes(rows, out_rows, in_cols))
+
+
+def fp8_e4m3_block_matmul(rows: Fp8Rows, fp8_weight: torch.Tensor, scale_inv: torch.Tensor, *,
+                          out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """FP8 rows [rows, in_cols] times an FP8 block-scaled weight
+    [out_rows, in_cols]: [rows, out_rows] in out_dtype (fp16, bf16 or fp32),
+    summed in fp32.  NaN bytes are NaN on both sides."""
+    lib = _require("PCKETLM_DISABLE_NATIVE_FP8_LINEAR", "Native FP8 matmul")
+    x, xs = rows
+    code = _ROW_CODES.get(out_dtype)
+    if code is None:
+        raise TypeError("out_dtype must be torch.float16, torch.bfloat16 or torch.float32")
+    if x.dtype not in _FP8_DTYPES or fp8_weight.dtype not in _FP8_DTYPES:
+        raise TypeError("FP8 rows and weights must be torch.uint8 raw e4m3 bytes or torch.float8_e4m3fn")
+    if xs.dtype != torch.float32 or scale_inv.dtype != torch.float32:
+        raise TypeError("FP8 scales must be torch.float32")
+    if x.ndim != 2:
+        raise ValueError("rows must have shape [rows, in_cols]")
+    if fp8_weight.ndim != 2:
+        raise ValueError("fp8_weight must have shape [out_rows, in_cols]")
+    m, k = x.shape
+    n, wk = fp8_weight.shape
+    blocks = (k + 127) // 128
+    if wk != k or k == 0:
+        raise ValueError("rows' columns do not match FP8 weight columns")
+    if xs.shape != (m, blocks):
+        raise ValueError("scales' shape does not match one scale for each 128 columns of a row")
+    if scale_inv.shape != ((n + 127) // 128, blocks):
+        raise ValueError("scale_inv shape does not match FP8 128x128 block layout")
+    device = x.device
+    _device_only("fp8_e4m3_block_matmul", device, xs, fp8_weight, scale_inv)
+    if not (x.is_contiguous() and xs.is_contiguous() and fp8_weight.is_contiguous() and scale_inv.is_contiguous()):
+        x, xs, fp8_weight, scale_inv = (t.contiguous() for t in (x, xs, fp8_weight, scale_inv))
+    out = torch.empty((m, n), dtype=out_dtype, device=device)
+    if m and n:
+        with _launch(lib, device) as index:
+            nbytes = _matmul_scratch(m, n, k, index)
+            scratch = torch.empty((nbytes,), dtype=torch.uint8, device=device) if nbytes else None
+            code = lib.fp8_e4m3_block_matmul(x.data_ptr(), xs.data_ptr(), fp8_weight.data_ptr(), scale_inv.data_ptr(),
+                                             out.data_ptr(), None if scratch is None else scratch.data_ptr(), nbytes,
+                                             m, n, k, blocks, code)
+        _check("fp8_e4m3_block_matmul", code)
+    return out
+
+
+def kv_rope_frequencies(head_dim: int, rope_theta: float, *, device: torch.device | str | None = None) -> torch.Tensor:
+    """The rotation's frequencies theta^(-2 i / head_dim) in float64, as
+    kv_paged_append takes them (a caller may scale them, or pass fewer than
+    head_dim / 2 to rotate the first values of a head alone)."""
+    at = torch.arange(int(head_dim) // 2, dtype=torch.float64)
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+    return torch.pow(torch.tensor(float(rope_theta), dtype=torch.float64), -2.0 * at / int(head_dim)).to(device)
+
+
+def _rows_of_heads(t: torch.Tensor) -> torch.Tensor:
+    """[..., heads, head_dim] in place where the kernels can read it (adjacent
+    head values, strides and address of 16 bytes), else a copy."""
+    s = t.stride()
+    if s[-1] != 1 or any(x % 8 for x in s[:-1]) or t.data_ptr() & 15:
+        # clone: a contiguous tensor at an odd address is copied too
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _check_pages(what: str, k_cache, v_cache, page_table, lengths):
+    """Shared checks; (device, dtype code, table's columns, cache sizes and strides)."""
+    dtype, device = k_cache.dtype, k_cache.device
+    if dtype == torch.bfloat16:
+        code = 1
+    elif dtype == torch.float16:
+        code = 0
+    else:
+        raise TypeError(f"{what} requires torch.float16 or torch.bfloat16 caches")
+    if v_cache.dtype != dtype:
+        raise TypeError(f"{what} requires caches to share dtype")
+    if page_table.dtype != torch.int32 or lengths.dtype != torch.int32:
+        raise TypeError("page_table and lengths must be torch.int32")
+    shape, stride = k_cache.shape, k_cache.stride()
+    if len(shape) != 4 or v_cache.shape != shape or v_cache.stride() != stride or stride[3] != 1:
+        raise ValueError("caches must have shape [pages, page_size, kv_heads, head_dim], the same strides and adjacent "
+                         "head values")
+    if page_table.ndim != 2 or lengths.ndim != 1 or lengths.shape[0] != page_table.shape[0]:
+        raise ValueError("page_table must have shape [sequences, pages], lengths one entry per sequence")
+    if not page_table.is_contiguous() or not lengths.is_contiguous():
+        raise ValueError("page_table and lengths must be contiguous")
+    return device, dtype, code, shape, stride
+
+
+def kv_paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
+                    v_cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, *,
+                    row_starts: torch.Tensor | None = None, rope_frequencies: torch.Tensor | None = None,
+                    interleaved: bool = False, rejected: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Writes rows of keys and values into their sequences' pages, rotated to
+    their positions, and returns the queries rotated alike (None without q).
+
+    q [rows, heads, head_dim], k and v [rows, kv_heads, head_dim] (views of a
+    fused projection are read in place), caches [pages, page_size, kv_heads,
+    head_dim] (any strides that keep head values adjacent), page_table int32
+    [sequences, pages of a sequence], lengths int32 [sequences]: what each
+    sequence holds before the call (negative: idle, its rows are not stored and
+    its queries zero).  Rows belong to the sequences in equal shares, or by
+    row_starts int32 [sequences + 1].  rope_frequencies float64 [pairs]
+    (kv_rope_frequencies) or None for no rotation; pairs are (i, i + pairs), or
+    neighbours when interleaved.  Rows without a page are not stored; their
+    number is added to rejected (int32, one value).  The lengths are not
+    advanced."""
+    lib = _require("PCKETLM_DISABLE_NATIVE_KV", "Native paged KV cache")
+    device, dtype, code, shape, stride = _check_pages("kv_paged_append", k_cache, v_cache, page_table, lengths)
+    if k.dtype != dtype or v.dtype != dtype or (q is not None and q.dtype != dtype):
+        raise TypeError(f"kv_paged_append requires {dtype} rows")
+    pages, page_size, kv_heads, head_dim = shape
+    if k.ndim != 3 or k.shape[1:] != shape[2:] or v.shape != k.shape:
+        raise ValueError("k and v must have shape [rows, kv_heads, head_dim]")
+    rows, (sequences, table_cols) = k.shape[0], page_table.shape
+    if q is not None and (q.ndim != 3 or q.shape[0] != rows or q.shape[2] != head_dim):
+        raise ValueError("q must have shape [rows, heads, head_dim]")
+    if row_starts is None:
+        if sequences == 0 or rows % sequences:
+            raise ValueError("rows must be a multiple of the sequences (or give row_starts)")
+    elif row_starts.dtype != torch.int32:
+        raise TypeError("row_starts must be torch.int32")
+    elif row_starts.shape != (sequences + 1,) or not row_starts.is_contiguous():
+        raise ValueError("row_starts must hold sequences + 1 entries")
+    pairs = 0
+    if rope_frequencies is not None:
+        if rope_frequencies.dtype != torch.float64:
+            raise TypeError("rope_frequencies must be torch.float64")
+        if rope_frequencies.ndim != 1 or not rope_frequencies.is_contiguous() or 2 * len(rope_frequencies) > head_dim:
+            raise ValueError("rope_frequencies must hold at most head_dim / 2 values")
+        pairs = rope_frequencies.shape[0]
+    if rejected is not None and (rejected.dtype != torch.int32 or rejected.numel() != 1):
+        raise TypeError("rejected must be one torch.int32 value")
+    _device_only("kv_paged_append", device, q, k, v, v_cache, page_table, lengths, row_starts, rope_frequencies, rejected)
+    k, v = _rows_of_heads(k), _rows_of_heads(v)
+    ks, vs = k.stride(), v.stride()
+    q_out, heads, qs = None, 0, (0, 0)
+    if q is not None:
+        q = _rows_of_heads(q)
+        heads, qs = q.shape[1], q.stride()
+        q_out = torch.empty(q.shape, dtype=dtype, device=device)
+    if rows:
+        with _launch(lib, device):
+            code = lib.kv_paged_append_u16(
+                q.data_ptr() if heads else None, k.data_ptr(), v.data_ptr(), q_out.data_ptr() if heads else None,
+                k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), _p(row_starts),
+                _p(rope_frequencies) if pairs else None, _p(rejected), rows, sequences, heads, kv_heads, head_dim, pairs,
+                1 if interleaved else 0, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], table_cols, pages, page_size,
+                stride[0], stride[1], stride[2], code)
+        _check("kv_paged_append_u16", code)
+    return q_out
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_scratch(sequences: int, rows: int, heads: int, kv_heads: int, head_dim: int, capacity: int,
+                       device_index: int) -> int:
+    return int(_lib.load().kv_paged_attention_scratch_bytes(sequences, rows, heads, kv_heads, head_dim, capacity))
+
+
+def kv_paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                              lengths: torch.Tensor, *, softmax_scale: float | None = None) -> torch.Tensor:
+    """Attention of the new rows of each sequence over its pages, after
+    kv_paged_append with the same page_table and lengths: row r of sequence b
+    sees the positions up to lengths[b] + r.
+
+    q [sequences, heads, head_dim], or [sequences, rows, heads, head_dim] with
+    1 to 8 rows (a verifier's candidates); the result has q's shape.
+    softmax_scale: head_dim ** -0.5 by default.  Idle sequences (negative
+    lengths) get zeros."""
+    lib = _require("PCKETLM_DISABLE_NATIVE_KV", "Native paged KV cache")
+    device, dtype, code, shape, stride = _check_pages("kv_paged_attention_decode", k_cache, v_cache, page_table, lengths)
+    if q.dtype != dtype:
+        raise TypeError(f"kv_paged_attention_decode requires {dtype} queries")
+    pages, page_size, kv_heads, head_dim = shape
+    sequences, table_cols = page_table.shape
+    q_shape = q.shape
+    if len(q_shape) not in (3, 4) or q_shape[0] != sequences or q_shape[-1] != head_dim:
+        raise ValueError("q must have shape [sequences, heads, head_dim] or [sequences, rows, heads, head_dim]")
+    rows = 1 if len(q_shape) == 3 else q_shape[1]
+    heads = q_shape[-2]
+    if not 1 <= rows <= 8:
+        raise ValueError("kv_paged_attention_decode takes 1 to 8 rows of a sequence")
+    if kv_heads == 0 or heads % kv_heads or not heads:
+        raise ValueError("heads must be a multiple of kv_heads")
+    _device_only("kv_paged_attention_decode", device, q, v_cache, page_table, lengths)
+    q = _rows_of_heads(q)
+    qs = q.stride()
+    out = torch.empty(q_shape, dtype=dtype, device=device)
+    if sequences:
+        with _launch(lib, device) as index:
+            nbytes = _attention_scratch(sequences, rows, heads, kv_heads, head_dim, table_cols * page_size, index)
+            scratch = torch.empty((nbytes,), dtype=torch.uint8, device=device) if nbytes > 0 else None
+            code = lib.kv_paged_attention_decode_u16(
+                q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
+                out.data_ptr(), None if scratch is None else scratch.data_ptr(), nbytes, sequences, rows, heads, kv_heads,
+                head_dim, qs[0], qs[1] if len(q_shape) == 4 else 0, qs[-2], table_cols, pages, page_size, stride[0],
+                stride[1], stride[2], head_dim ** -0.5 if softmax_scale is None else softmax_scale, code)
+        _check("kv_paged_attention_decode_u16", code)
+    return out

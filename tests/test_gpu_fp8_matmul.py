@@ -1,0 +1,120 @@
+"""FP8 rows times an FP8 block-scaled weight, against the sum in 64 bits."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import batched_refs as ref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def nat():
+    from pocketlm_amd import native
+
+    assert native.native_fp8_rows_available(), "libpocketlm_hip.so must load on the GPU box"
+    return native
+
+
+def make(m, n, k, seed):
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn((m, k), generator=g) * 100).clamp(-448, 448).to(torch.float8_e4m3fn)
+    w = torch.randn((n, k), generator=g).to(torch.float8_e4m3fn)
+    xs = torch.rand((m, (k + 127) // 128), generator=g) * 9e-3 + 1e-3
+    ws = torch.rand(((n + 127) // 128, (k + 127) // 128), generator=g) * 0.9 + 0.1
+    return x, xs, w, ws
+
+
+def run(nat, x, xs, w, ws, dtype):
+    return nat.fp8_e4m3_block_matmul(nat.Fp8Rows(x.cuda(), xs.cuda()), w.cuda(), ws.cuda(), out_dtype=dtype)
+
+
+SHAPES = [(1, 576, 7168), (1, 1, 16), (2, 130, 128), (8, 100, 144), (16, 128, 256), (17, 33, 400), (31, 257, 1536),
+          (33, 200, 384), (63, 640, 896), (64, 1024, 1040), (65, 96, 272), (100, 513, 2048), (128, 256, 512),
+          (129, 384, 4096), (200, 1000, 640), (255, 48, 16384), (257, 300, 1552), (500, 700, 1280), (1, 5000, 128),
+          (300, 129, 130), (7, 40, 1), (5, 3, 137)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_against_64_bits(nat, dtype, m, n, k):
+    x, xs, w, ws = make(m, n, k, m + n + k)
+    got = run(nat, x, xs, w, ws, dtype)
+    assert got.dtype == dtype and got.shape == (m, n)
+    want, size = ref.matmul(x, xs, w, ws)
+    ref.within(got, want, ref.matmul_bound(want, size, k, dtype))
+
+
+@pytest.mark.parametrize("m,n,k", [(600, 2304, 1024), (1025, 1100, 528), (2048, 512, 896)])
+def test_prompts(nat, m, n, k):
+    x, xs, w, ws = make(m, n, k, m)
+    want, size = ref.matmul(x, xs, w, ws)
+    ref.within(run(nat, x, xs, w, ws, torch.bfloat16), want, ref.matmul_bound(want, size, k, torch.bfloat16))
+
+
+def test_whole_numbers_are_exact(nat):
+    """Small whole numbers and scales that are powers of two: every sum is exact."""
+    g = torch.Generator().manual_seed(9)
+    for m, n, k in ((3, 50, 640), (40, 300, 2176), (300, 520, 1280)):
+        x = torch.randint(-4, 5, (m, k), generator=g).float().to(torch.float8_e4m3fn)
+        w = torch.randint(-4, 5, (n, k), generator=g).float().to(torch.float8_e4m3fn)
+        xs = torch.exp2(torch.randint(-2, 3, (m, k // 128), generator=g).float())
+        ws = torch.exp2(torch.randint(-2, 3, ((n + 127) // 128, k // 128), generator=g).float())
+        want, _ = ref.matmul(x, xs, w, ws)
+        assert torch.equal(run(nat, x, xs, w, ws, torch.float32).cpu().double(), want)
+
+
+@pytest.mark.parametrize("m", [1, 20, 50, 90, 300])
+def test_nan_rows_weights_and_scales_stay_where_they_are(nat, m):
+    n, k = 200, 656
+    x, xs, w, ws = make(m, n, k, 21)
+    want, size = ref.matmul(x, xs, w, ws)
+    bound = ref.matmul_bound(want, size, k, torch.bfloat16)
+    xb, wb, xs2 = x.view(torch.uint8).clone(), w.view(torch.uint8).clone(), xs.clone()
+    wb[17, k - 1] = 0x7F
+    wb[199, 0] = 0xFF
+    if m > 1:
+        xb[m - 1, 3] = 0x7F
+        xs2[m // 2, 5] = float("nan")
+    got = run(nat, xb, xs2, wb, ws, torch.bfloat16).cpu()
+    hit = torch.zeros((m, n), dtype=torch.bool)
+    hit[:, 17] = hit[:, 199] = True
+    if m > 1:
+        hit[m - 1] = hit[m // 2] = True
+    assert torch.equal(got.isnan(), hit)
+    ref.within(got[~hit], want[~hit], bound[~hit])
+
+
+def test_offset_and_strided_operands(nat):
+    m, n, k = 70, 150, 512
+    x, xs, w, ws = make(m, n, k, 30)
+    want = run(nat, x, xs, w, ws, torch.float32)
+    wide = torch.zeros((m, 2 * k), dtype=torch.uint8, device="cuda")
+    wide[:, k:] = x.cuda().view(torch.uint8)
+    odd = torch.zeros(n * k + 1, dtype=torch.uint8, device="cuda")[1:].view(n, k)
+    odd.copy_(w.cuda().view(torch.uint8))
+    got = nat.fp8_e4m3_block_matmul(nat.Fp8Rows(wide[:, k:], xs.cuda()), w.cuda(), ws.cuda().t().contiguous().t(),
+                                    out_dtype=torch.float32)
+    assert torch.equal(got, want)
+    exact, size = ref.matmul(x, xs, w, ws)
+    # an odd address: one result a thread
+    ref.within(nat.fp8_e4m3_block_matmul(nat.Fp8Rows(x.cuda(), xs.cuda()), odd, ws.cuda(), out_dtype=torch.float32),
+               exact, ref.matmul_bound(exact, size, k, torch.float32))
+    assert nat.fp8_e4m3_block_matmul(nat.Fp8Rows(x.cuda()[:0], xs.cuda()[:0]), w.cuda(), ws.cuda()).shape == (0, n)
+
+
+def test_the_library_s_own_scratch(nat):
+    """The C entry without scratch gives the bits of the call with it."""
+    from pocketlm_amd import _lib
+
+    lib = _lib.load()
+    for m, n, k in ((1, 300, 7168), (40, 256, 4096), (300, 384, 8192)):
+        x, xs, w, ws = (t.cuda() for t in make(m, n, k, 40 + m))
+        want = nat.fp8_e4m3_block_matmul(nat.Fp8Rows(x, xs), w, ws)
+        out = torch.zeros_like(want)
+        lib.pocketlm_set_stream(torch.cuda.current_stream().cuda_stream)
+        assert lib.fp8_e4m3_block_matmul(x.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), out.data_ptr(), None,
+                                         0, m, n, k, k // 128, 1) == 0
+        assert torch.equal(out, want)
