@@ -7,6 +7,7 @@
 // the block's inner sum, and the scaled sum over the blocks is kept in fp32 by
 // vector fma.  NaN bytes, in the rows or in the weight, are NaN.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "fp8_mfma.h"
@@ -184,6 +185,223 @@ int launch_rows(const MatmulArgs& a, int waves, hipStream_t st) {
     return plm::check_launch("fp8_e4m3_block_matmul");
 }
 
+// Many rows: a workgroup owns 16 TN GN weight rows and 16 TM GM activation
+// rows, wave (i, j) of GN x GM of them 16 TN by 16 TM.  Both operands' block
+// of 128 columns goes to LDS by loads that write it there (no registers), the
+// next block's while this one is multiplied; one barrier a block.
+//
+// A row's eight 16-byte pieces lie in LDS at piece ^ f(row), so that the
+// eight lanes which read together (the same piece of eight rows) touch eight
+// different groups of banks; the loads write LDS in lane order, so it is
+// their addresses that are permuted.  Weight tile i of a wave holds the rows
+// 16 (r / 4) + 4 i + r % 4: a lane then has 4 TN adjacent results of an
+// output row.
+template <int TN, int TM, int GN, int GM>
+struct Tile {
+    static constexpr int kWaves = GN * GM;
+    static constexpr int kN = 16 * TN * GN, kM = 16 * TM * GM;
+    static constexpr int kStage = (kN + kM) * 128;      // bytes of a block's operands
+    static constexpr int kLds = 2 * kStage + 2 * kM * 4;  // and of its row scales
+};
+
+// Eight results in the output's 16-bit type.
+template <bool BF16>
+__device__ __forceinline__ plm_u32x4 pack8(const plm_f32x4 a, const plm_f32x4 b) {
+    typedef float f32x8 __attribute__((ext_vector_type(8)));
+    typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+    const f32x8 v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    if constexpr (BF16)
+        return __builtin_bit_cast(plm_u32x4, __builtin_convertvector(v, plm_bf16x8));
+    else
+        return __builtin_bit_cast(plm_u32x4, __builtin_convertvector(v, f16x8));
+}
+
+template <int TN>
+__device__ __forceinline__ int swizzle_w(int row) {
+    return (row & 3) | ((row / (4 * TN)) & 1) << 2;
+}
+__device__ __forceinline__ int swizzle_x(int row) { return row & 7; }
+
+// 16 bytes a lane from base + offset to LDS, the wave's KB in lane order at
+// `to`.  Not the compiler's builtin: it waits for every load to LDS before any
+// read of LDS, also of the other stage.  The wait is load_to_lds_wait's.
+__device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :
+                 : "v"(offset), "s"(base), "s"(to)
+                 : "memory");
+}
+__device__ __forceinline__ void load_to_lds_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+template <int TN, int TM, int GN, int GM>
+__global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const MatmulArgs a) {
+    using T = Tile<TN, TM, GN, GM>;
+    extern __shared__ char lds[];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int li = lane & 15, qd = lane >> 4;
+    const int wn = wave % GN, wm = wave / GN;
+    const int64_t n0 = static_cast<int64_t>(blockIdx.x) * T::kN, m0 = static_cast<int64_t>(blockIdx.y) * T::kM;
+
+    constexpr int kLag = 2;
+    // a wave's loads: 8 rows each, rows past the end repeat the last one
+    constexpr int kLoads = (T::kN + T::kM) / 8 / T::kWaves;
+    static_assert((T::kN + T::kM) % (8 * T::kWaves) == 0 && T::kN % (8 * T::kWaves) == 0, "whole loads");
+    const uint8_t* wbase = a.w + n0 * a.k;
+    const uint8_t* xbase = a.x + m0 * a.k;
+    uint32_t src[kLoads];  // from the operand's first row of the workgroup
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        const int r = (i * T::kWaves + wave) * 8 + (lane >> 3);  // of both operands' rows
+        const bool is_w = i < T::kN / 8 / T::kWaves;
+        const int rr = is_w ? r : r - T::kN;
+        const int f = is_w ? swizzle_w<TN>(rr) : swizzle_x(rr);
+        const int last = static_cast<int>(min(is_w ? a.n - 1 - n0 : a.m - 1 - m0, static_cast<int64_t>(T::kN + T::kM)));
+        src[i] = static_cast<uint32_t>(min(rr, last)) * static_cast<uint32_t>(a.k) + 16 * ((lane & 7) ^ f);
+    }
+    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
+    auto load_stage = [&](int b) {
+        const uint32_t to = lds_at + (b & 1) * T::kStage + wave * 1024;
+        const int64_t at = static_cast<int64_t>(b) * 128;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+            load_to_lds((i < T::kN / 8 / T::kWaves ? wbase : xbase) + at, src[i], to + i * T::kWaves * 1024);
+    };
+    float* scales = reinterpret_cast<float*>(lds + 2 * T::kStage);
+    // every thread keeps a row's scale moving, several the same one: no branch splits a block's work
+    const int srow = threadIdx.x % T::kM;
+    const float* xs = a.xs + min(m0 + srow, a.m - 1) * a.blocks;
+    const float* ws = a.ws + (min(n0 + 16 * TN * wn, a.n - 1) >> 7) * a.scale_cols;
+
+    plm_f32x4 acc[TN][TM];
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int j = 0; j < TM; ++j) acc[i][j] = plm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    const int wrow = 16 * TN * wn + 4 * TN * (li >> 2) + (li & 3);  // + 4 i
+    const int xrow = 16 * TM * wm + li;                              // + 16 j
+    const int fw = swizzle_w<TN>(wrow), fx = swizzle_x(xrow);
+    const int w0 = wrow * 128 + 16 * (qd ^ fw), w1 = wrow * 128 + 16 * ((qd + 4) ^ fw);
+    const int x0 = (T::kN + xrow) * 128 + 16 * (qd ^ fx), x1 = (T::kN + xrow) * 128 + 16 * ((qd + 4) ^ fx);
+
+    load_stage(0);
+    scales[srow] = xs[0];
+    float sw = ws[0];
+    auto block = [&](int b, auto masked) {
+        constexpr bool MASKED = decltype(masked)::value;
+        load_to_lds_wait();
+        __syncthreads();
+        const int ahead = min(b + 1, a.blocks - 1);
+        if (b + 1 < a.blocks) load_stage(b + 1);
+        const float next = xs[ahead], next_w = ws[ahead];
+        const char* stage = lds + (b & 1) * T::kStage;
+        const float* sx = scales + (b & 1) * T::kM + xrow;
+        auto piece = [&](int at, int h) {
+            plm_u32x4 v = *reinterpret_cast<const plm_u32x4*>(stage + at);
+            if constexpr (MASKED) {  // columns past the end
+                if (static_cast<int64_t>(b) * 128 + 64 * h + 16 * qd >= a.k) v = plm_u32x4{0, 0, 0, 0};
+            }
+            return v;
+        };
+        plm_u32x4 w[TN][2];
+#pragma unroll
+        for (int i = 0; i < TN; ++i) {
+            w[i][0] = piece(w0 + i * 512, 0);
+            w[i][1] = piece(w1 + i * 512, 1);
+        }
+        plm_u32x4 v[2][2];
+        plm_f32x4 d[kLag + 1];
+        float scale[2];
+        v[0][0] = piece(x0, 0);
+        v[0][1] = piece(x1, 1);
+        scale[0] = sx[0] * sw;
+        // the adds of a result follow the matrix instruction kLag later
+#pragma unroll
+        for (int at = 0; at < TN * TM + kLag; ++at) {
+            const int i = at % TN, j = at / TN;
+            if (i == 0 && j + 1 < TM) {
+                v[(j + 1) & 1][0] = piece(x0 + (j + 1) * 2048, 0);
+                v[(j + 1) & 1][1] = piece(x1 + (j + 1) * 2048, 1);
+            }
+            if (j < TM)
+                d[at % (kLag + 1)] =
+                    mfma_fp8(w[i][0], w[i][1], v[j & 1][0], v[j & 1][1], plm_f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+            if (at >= kLag) {
+                const int was = at - kLag, wi = was % TN, wj = was / TN;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    acc[wi][wj][e] = fmaf(d[was % (kLag + 1)][e], scale[wj & 1], acc[wi][wj][e]);
+                if (wi == TN - 1 && wj + 1 < TM) scale[(wj + 1) & 1] = sx[16 * (wj + 1)] * sw;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        scales[((b + 1) & 1) * T::kM + srow] = next;
+        sw = next_w;
+    };
+    const bool ragged = (a.k & 127) != 0;
+    const int whole = a.blocks - (ragged ? 1 : 0);
+    for (int b = 0; b < whole; ++b) block(b, std::false_type{});
+    if (ragged) block(whole, std::true_type{});
+
+    // A lane has 4 TN adjacent results of TM rows.  Whole ones of aligned rows
+    // are stored by 16 bytes, others by single values through LDS.
+    const int64_t n = n0 + 16 * TN * wn + 4 * TN * qd;
+    const int per = a.out_type == kOutF32 ? 4 : 8;
+    const bool wide = a.n % per == 0 && n0 + T::kN <= a.n && (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0;
+    if (wide) {
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+            const int64_t m = m0 + 16 * TM * wm + 16 * j + li;
+            if (m >= a.m) continue;
+            const int64_t at = m * a.n + n;
+            if (a.out_type == kOutF32) {
+#pragma unroll
+                for (int i = 0; i < TN; ++i) *reinterpret_cast<plm_f32x4*>(static_cast<float*>(a.out) + at + 4 * i) = acc[i][j];
+            } else if (a.out_type == kOutBF16) {
+#pragma unroll
+                for (int i = 0; i < TN; i += 2)
+                    *reinterpret_cast<plm_u32x4*>(static_cast<uint16_t*>(a.out) + at + 4 * i) =
+                        pack8<true>(acc[i][j], acc[i + 1][j]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < TN; i += 2)
+                    *reinterpret_cast<plm_u32x4*>(static_cast<uint16_t*>(a.out) + at + 4 * i) =
+                        pack8<false>(acc[i][j], acc[i + 1][j]);
+            }
+        }
+        return;
+    }
+    __syncthreads();
+    constexpr int kRow = 16 * TN;
+    plm_f32x4* mine = reinterpret_cast<plm_f32x4*>(lds) + wave * 16 * (kRow / 4);
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+#pragma unroll
+        for (int i = 0; i < TN; ++i) mine[li * (kRow / 4) + TN * qd + i] = acc[i][j];
+        // the wave's own: its LDS operations are done in order
+        __builtin_amdgcn_wave_barrier();
+        for (int e = lane; e < 16 * kRow; e += 64) {
+            const int64_t m = m0 + 16 * TM * wm + 16 * j + e / kRow, c = n0 + 16 * TN * wn + e % kRow;
+            if (m < a.m && c < a.n) store_out(a, m * a.n + c, reinterpret_cast<const float*>(mine)[e]);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+template <int TN, int TM, int GN, int GM>
+int launch_tile(const MatmulArgs& a, hipStream_t st) {
+    using T = Tile<TN, TM, GN, GM>;
+    const int64_t gx = plm::ceil_div(a.n, T::kN), gy = plm::ceil_div(a.m, T::kM);
+    if (gx > 0x7FFFFFFF || gy > 65535) return plm::fail(-2, "too many rows");
+    const void* fn = reinterpret_cast<const void*>(&fp8_matmul_tile_kernel<TN, TM, GN, GM>);
+    const int code = plm::allow_large_lds(fn, T::kLds);
+    if (code != 0) return code;
+    hipLaunchKernelGGL((fp8_matmul_tile_kernel<TN, TM, GN, GM>), dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy)),
+                       dim3(64 * T::kWaves), T::kLds, st, a);
+    return plm::check_launch("fp8_e4m3_block_matmul");
+}
+
 }  // namespace
 
 PLM_EXPORT int64_t fp8_e4m3_block_matmul_scratch_bytes(int64_t rows, int64_t out_rows, int64_t in_cols) {
@@ -215,5 +433,6 @@ PLM_EXPORT int fp8_e4m3_block_matmul(const uint8_t* x, const float* x_scales, co
     const int waves = std::min(8, a.blocks);
     if (rows <= 16) return launch_rows<1, 1, 4, 8>(a, waves, st);
     if (rows <= 32) return launch_rows<2, 2, 2, 8>(a, waves, st);
-    return launch_rows<2, 4, 2, 8>(a, waves, st);
+    if (rows <= 64) return launch_rows<2, 4, 2, 8>(a, waves, st);
+    return launch_tile<4, 8, 4, 2>(a, st);
 }
