@@ -201,7 +201,7 @@ struct Tile {
     static constexpr int kWaves = GN * GM;
     static constexpr int kN = 16 * TN * GN, kM = 16 * TM * GM;
     static constexpr int kStage = (kN + kM) * 128;      // bytes of a block's operands
-    static constexpr int kLds = 2 * kStage + 2 * kM * 4;  // and of its row scales
+    static constexpr int kLds = 2 * kStage + 4 * kM * 4;  // and four blocks' row scales
 };
 
 // Eight results in the output's 16-bit type.
@@ -231,7 +231,19 @@ __device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, u
                  : "v"(offset), "s"(base), "s"(to)
                  : "memory");
 }
-__device__ __forceinline__ void load_to_lds_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void load4_to_lds(const void* base, uint32_t offset, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
+                 :
+                 : "v"(offset), "s"(base), "s"(to)
+                 : "memory");
+}
+// Until all but the last LEFT of the wave's loads to LDS are there, then until
+// the workgroup's waves are here.  One statement: no read of LDS moves in
+// between.
+template <int LEFT>
+__device__ __forceinline__ void load_to_lds_barrier() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+}
 
 template <int TN, int TM, int GN, int GM>
 __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const MatmulArgs a) {
@@ -244,6 +256,8 @@ __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const Mat
     const int64_t n0 = static_cast<int64_t>(blockIdx.x) * T::kN, m0 = static_cast<int64_t>(blockIdx.y) * T::kM;
 
     constexpr int kLag = 2;
+    constexpr int kAtOnce = 2;
+    constexpr int kScalesAt = TM - 1;
     // a wave's loads: 8 rows each, rows past the end repeat the last one
     constexpr int kLoads = (T::kN + T::kM) / 8 / T::kWaves;
     static_assert((T::kN + T::kM) % (8 * T::kWaves) == 0 && T::kN % (8 * T::kWaves) == 0, "whole loads");
@@ -260,18 +274,16 @@ __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const Mat
         src[i] = static_cast<uint32_t>(min(rr, last)) * static_cast<uint32_t>(a.k) + 16 * ((lane & 7) ^ f);
     }
     const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
-    auto load_stage = [&](int b) {
-        const uint32_t to = lds_at + (b & 1) * T::kStage + wave * 1024;
-        const int64_t at = static_cast<int64_t>(b) * 128;
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i)
-            load_to_lds((i < T::kN / 8 / T::kWaves ? wbase : xbase) + at, src[i], to + i * T::kWaves * 1024);
+    auto load_part = [&](int b, int i) {
+        load_to_lds((i < T::kN / 8 / T::kWaves ? wbase : xbase) + static_cast<int64_t>(b) * 128, src[i],
+                    lds_at + (b & 1) * T::kStage + (i * T::kWaves + wave) * 1024);
     };
-    float* scales = reinterpret_cast<float*>(lds + 2 * T::kStage);
-    // every thread keeps a row's scale moving, several the same one: no branch splits a block's work
-    const int srow = threadIdx.x % T::kM;
-    const float* xs = a.xs + min(m0 + srow, a.m - 1) * a.blocks;
-    const float* ws = a.ws + (min(n0 + 16 * TN * wn, a.n - 1) >> 7) * a.scale_cols;
+    const float* scales = reinterpret_cast<const float*>(lds + 2 * T::kStage);
+    const int sfirst = wave * 64 % T::kM;
+    const float* xs = a.xs + m0 * a.blocks;
+    const uint32_t ssrc = static_cast<uint32_t>(min(static_cast<int64_t>((sfirst + lane) % T::kM), a.m - 1 - m0)) * a.blocks * 4;
+    const auto ws = (const __attribute__((address_space(4))) float*)(
+        a.ws + (min(n0 + 16 * TN * wn, a.n - 1) >> 7) * a.scale_cols);
 
     plm_f32x4 acc[TN][TM];
 #pragma unroll
@@ -285,18 +297,20 @@ __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const Mat
     const int w0 = wrow * 128 + 16 * (qd ^ fw), w1 = wrow * 128 + 16 * ((qd + 4) ^ fw);
     const int x0 = (T::kN + xrow) * 128 + 16 * (qd ^ fx), x1 = (T::kN + xrow) * 128 + 16 * ((qd + 4) ^ fx);
 
-    load_stage(0);
-    scales[srow] = xs[0];
+    auto load_scales = [&](int b) {
+        load4_to_lds(xs + min(b, a.blocks - 1), ssrc, lds_at + 2 * T::kStage + ((b & 3) * T::kM + sfirst) * 4);
+    };
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) load_part(0, i);
+    load_scales(0);
+    load_scales(1);
     float sw = ws[0];
-    auto block = [&](int b, auto masked) {
-        constexpr bool MASKED = decltype(masked)::value;
-        load_to_lds_wait();
-        __syncthreads();
-        const int ahead = min(b + 1, a.blocks - 1);
-        if (b + 1 < a.blocks) load_stage(b + 1);
-        const float next = xs[ahead], next_w = ws[ahead];
+    auto block = [&](int b, auto more, auto masked) {
+        constexpr bool MORE = decltype(more)::value, MASKED = decltype(masked)::value;
+        load_to_lds_barrier<MORE ? 1 : 0>();
+        const float next_w = ws[min(b + 1, a.blocks - 1)];
         const char* stage = lds + (b & 1) * T::kStage;
-        const float* sx = scales + (b & 1) * T::kM + xrow;
+        const float* sx = scales + (b & 3) * T::kM + xrow;
         auto piece = [&](int at, int h) {
             plm_u32x4 v = *reinterpret_cast<const plm_u32x4*>(stage + at);
             if constexpr (MASKED) {  // columns past the end
@@ -320,6 +334,13 @@ __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const Mat
 #pragma unroll
         for (int at = 0; at < TN * TM + kLag; ++at) {
             const int i = at % TN, j = at / TN;
+            // the next block's loads go out one at a time: all at once they wait for each other before the
+            // first product
+            if (MORE && i == 0) {
+#pragma unroll
+                for (int x = kAtOnce * j; x < min(kLoads, kAtOnce * (j + 1)); ++x) load_part(b + 1, x);
+                if (j == kScalesAt) load_scales(b + 2);
+            }
             if (i == 0 && j + 1 < TM) {
                 v[(j + 1) & 1][0] = piece(x0 + (j + 1) * 2048, 0);
                 v[(j + 1) & 1][1] = piece(x1 + (j + 1) * 2048, 1);
@@ -336,13 +357,15 @@ __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const Mat
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-        scales[((b + 1) & 1) * T::kM + srow] = next;
+        // the adds stay in their block: moved past a branch, all results would wait for them in registers
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+            for (int j = 0; j < TM; ++j) asm volatile("" : "+v"(acc[i][j]));
         sw = next_w;
     };
-    const bool ragged = (a.k & 127) != 0;
-    const int whole = a.blocks - (ragged ? 1 : 0);
-    for (int b = 0; b < whole; ++b) block(b, std::false_type{});
-    if (ragged) block(whole, std::true_type{});
+    for (int b = 0; b + 1 < a.blocks; ++b) block(b, std::true_type{}, std::false_type{});
+    block(a.blocks - 1, std::false_type{}, std::true_type{});
 
     // A lane has 4 TN adjacent results of TM rows.  Whole ones of aligned rows
     // are stored by 16 bytes, others by single values through LDS.
