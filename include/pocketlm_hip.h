@@ -806,7 +806,9 @@ int fp8_e4m3_rms_norm_rows(const void* x, const void* residual, const void* weig
  *               * sum_{k in block b} x[m][k] * W[n][k],
  * fp32 sums, rounded once to dtype_code.  x [rows][in_cols], x_scales
  * [rows][ceil(in_cols / 128)], fp8_weight [out_rows][in_cols], scale_inv
- * [ceil(out_rows / 128)][scale_cols], out [rows][out_rows].  NaN bytes are
+ * [ceil(out_rows / 128)][scale_cols], out [rows][out_rows]; x and fp8_weight
+ * 16-byte aligned (in_cols may be any; multiples of 16 are read in place,
+ * others are copied to padded rows first).  NaN bytes are
  * NaN, in the weight too (the fp8_e4m3_block_linear family counts them as 0,
  * as the reference's decoder does).  scratch: device memory of at least
  * fp8_e4m3_block_matmul_scratch_bytes, 16-byte aligned, or NULL for the

@@ -19,6 +19,10 @@ using namespace plm_fp8;
 enum OutType { kOutF16 = 0, kOutBF16 = 1, kOutF32 = 2 };
 
 typedef int plm_i32x8 __attribute__((ext_vector_type(8)));
+// stored at the alignment of one value
+typedef plm_f32x4 any_f32x4 __attribute__((aligned(4)));
+typedef plm_u32x4 any_u32x4 __attribute__((aligned(2)));
+typedef uint32_t any_u32x2 __attribute__((ext_vector_type(2), aligned(2)));
 
 struct MatmulArgs {
     const uint8_t* x;
@@ -32,6 +36,7 @@ struct MatmulArgs {
     int64_t scale_cols;  // of ws
     int blocks;          // of 128 columns; the row length of xs
     int out_type;
+    float* part;
 };
 
 __device__ __forceinline__ void store_out(const MatmulArgs& a, int64_t at, float v) {
@@ -43,23 +48,27 @@ __device__ __forceinline__ void store_out(const MatmulArgs& a, int64_t at, float
         static_cast<float*>(a.out)[at] = v;
 }
 
-// One result a thread, for rows that are not whole 16-byte pieces.
-__global__ __launch_bounds__(256) void fp8_matmul_scalar_kernel(const MatmulArgs a) {
+// Rows of k bytes to rows of k16, k up to a multiple of 16, zeros behind: the
+// other kernels read whole 16-byte pieces.  A thread: one piece.
+__global__ __launch_bounds__(256) void fp8_pad_rows_kernel(const uint8_t* __restrict__ from, uint8_t* __restrict__ to,
+                                                           int64_t rows, int64_t k, int64_t k16) {
+    const int64_t per = k16 / 16;
     const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (at >= a.m * a.n) return;
-    const int64_t m = at / a.n, n = at - m * a.n;
-    const uint8_t* x = a.x + m * a.k;
-    const uint8_t* w = a.w + n * a.k;
-    float sum = 0.0f;
-    for (int b = 0; b < a.blocks; ++b) {
-        const int64_t end = min(a.k, static_cast<int64_t>(b + 1) * 128);
-        float s = 0.0f;
-        for (int64_t k = static_cast<int64_t>(b) * 128; k < end; ++k)
-            s = fmaf(__builtin_amdgcn_cvt_f32_fp8(static_cast<int>(x[k]), 0),
-                     __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(w[k]), 0), s);
-        sum = fmaf(s, a.xs[m * a.blocks + b] * a.ws[(n >> 7) * a.scale_cols + b], sum);
-    }
-    store_out(a, at, sum);
+    if (at >= rows * per) return;
+    const int64_t row = at / per, c = (at - row * per) * 16;
+    const uint8_t* src = from + row * k + c;
+    uint32_t v[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        if (c + i < k) v[i >> 2] |= static_cast<uint32_t>(src[i]) << (8 * (i & 3));
+    *reinterpret_cast<uint4*>(to + row * k16 + c) = make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+int pad_rows(const uint8_t* from, uint8_t* to, int64_t rows, int64_t k, int64_t k16, hipStream_t st) {
+    const int64_t groups = plm::ceil_div(rows * (k16 / 16), 256);
+    if (groups > 0x7FFFFFFF) return plm::fail(-2, "too many rows");
+    hipLaunchKernelGGL(fp8_pad_rows_kernel, dim3(static_cast<unsigned>(groups)), dim3(256), 0, st, from, to, rows, k, k16);
+    return plm::check_launch("fp8_e4m3_block_matmul, pad");
 }
 
 __device__ __forceinline__ plm_f32x4 mfma_fp8(const plm_u32x4 a0, const plm_u32x4 a1, const plm_u32x4 b0,
@@ -186,22 +195,26 @@ int launch_rows(const MatmulArgs& a, int waves, hipStream_t st) {
 }
 
 // Many rows: a workgroup owns 16 TN GN weight rows and 16 TM GM activation
-// rows, wave (i, j) of GN x GM of them 16 TN by 16 TM.  Both operands' block
-// of 128 columns goes to LDS by loads that write it there (no registers), the
-// next block's while this one is multiplied; one barrier a block.
+// rows, wave (i, j) of GN x GM of them 16 TN by 16 TM.  Both operands' blocks
+// of 128 columns go to LDS by loads that write it there (no registers), S - 1
+// blocks ahead; one barrier a block.  blockIdx.z takes a share of the blocks;
+// where there are several, their sums go to `part` in fp32 and
+// fp8_matmul_join_kernel adds them.
 //
 // A row's eight 16-byte pieces lie in LDS at piece ^ f(row), so that the
 // eight lanes which read together (the same piece of eight rows) touch eight
 // different groups of banks; the loads write LDS in lane order, so it is
 // their addresses that are permuted.  Weight tile i of a wave holds the rows
-// 16 (r / 4) + 4 i + r % 4: a lane then has 4 TN adjacent results of an
+// 4 TN (r / 4) + 4 i + r % 4: a lane then has 4 TN adjacent results of an
 // output row.
-template <int TN, int TM, int GN, int GM>
+template <int TN, int TM, int GN, int GM, int S>
 struct Tile {
     static constexpr int kWaves = GN * GM;
     static constexpr int kN = 16 * TN * GN, kM = 16 * TM * GM;
-    static constexpr int kStage = (kN + kM) * 128;      // bytes of a block's operands
-    static constexpr int kLds = 2 * kStage + 4 * kM * 4;  // and four blocks' row scales
+    static constexpr int kStage = (kN + kM) * 128;  // bytes of a block's operands
+    static constexpr int kScales = kM < 64 ? 64 : kM;
+    static constexpr int kScaleSlots = S < 4 ? 4 : 8;  // of kScales row scales: more than S blocks ahead
+    static constexpr int kLds = S * kStage + kScaleSlots * kScales * 4;
 };
 
 // Eight results in the output's 16-bit type.
@@ -245,9 +258,9 @@ __device__ __forceinline__ void load_to_lds_barrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
 }
 
-template <int TN, int TM, int GN, int GM>
+template <int TN, int TM, int GN, int GM, int S>
 __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const MatmulArgs a) {
-    using T = Tile<TN, TM, GN, GM>;
+    using T = Tile<TN, TM, GN, GM, S>;
     extern __shared__ char lds[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -255,35 +268,53 @@ __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const Mat
     const int wn = wave % GN, wm = wave / GN;
     const int64_t n0 = static_cast<int64_t>(blockIdx.x) * T::kN, m0 = static_cast<int64_t>(blockIdx.y) * T::kM;
 
-    constexpr int kLag = 2;
-    constexpr int kAtOnce = 2;
-    constexpr int kScalesAt = TM - 1;
-    // a wave's loads: 8 rows each, rows past the end repeat the last one
-    constexpr int kLoads = (T::kN + T::kM) / 8 / T::kWaves;
-    static_assert((T::kN + T::kM) % (8 * T::kWaves) == 0 && T::kN % (8 * T::kWaves) == 0, "whole loads");
-    const uint8_t* wbase = a.w + n0 * a.k;
-    const uint8_t* xbase = a.x + m0 * a.k;
-    uint32_t src[kLoads];  // from the operand's first row of the workgroup
+    // this workgroup's blocks
+    const int first = static_cast<int>(static_cast<int64_t>(a.blocks) * blockIdx.z / gridDim.z);
+    const int blocks = static_cast<int>(static_cast<int64_t>(a.blocks) * (blockIdx.z + 1) / gridDim.z) - first;
+
+    constexpr int kLag = 2;  // matrix instructions between a result and its adds
+    // A wave's loads of a block: 8 rows each, LW of the weight's and LX of the activations' (of few
+    // rows several waves load the same ones).  Rows past the end repeat the last one.
+    constexpr int LW = T::kN / 8 / T::kWaves, LX = T::kM / 8 >= T::kWaves ? T::kM / 8 / T::kWaves : 1, L = LW + LX;
+    static_assert(T::kN % (8 * T::kWaves) == 0 && (T::kM % (8 * T::kWaves) == 0 || T::kWaves * 8 % T::kM == 0),
+                  "whole loads");
+    static_assert(T::kWaves % TN == 0, "rows of an operand's loads share their piece");
+    const uint8_t* wbase = a.w + n0 * a.k + static_cast<int64_t>(first) * 128;
+    const uint8_t* xbase = a.x + m0 * a.k + static_cast<int64_t>(first) * 128;
+    uint32_t src[L];  // from the operand's first row of the workgroup
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-        const int r = (i * T::kWaves + wave) * 8 + (lane >> 3);  // of both operands' rows
-        const bool is_w = i < T::kN / 8 / T::kWaves;
-        const int rr = is_w ? r : r - T::kN;
-        const int f = is_w ? swizzle_w<TN>(rr) : swizzle_x(rr);
-        const int last = static_cast<int>(min(is_w ? a.n - 1 - n0 : a.m - 1 - m0, static_cast<int64_t>(T::kN + T::kM)));
-        src[i] = static_cast<uint32_t>(min(rr, last)) * static_cast<uint32_t>(a.k) + 16 * ((lane & 7) ^ f);
+    for (int i = 0; i < L; ++i) {
+        const bool is_w = i < LW;
+        const int r = ((is_w ? i : i - LW) * T::kWaves + wave) * 8 % (is_w ? T::kN : T::kM) + (lane >> 3);
+        const int f = is_w ? swizzle_w<TN>(r) : swizzle_x(r);
+        const int last = static_cast<int>(min((is_w ? a.n : a.m) - 1 - (is_w ? n0 : m0), static_cast<int64_t>(T::kN + T::kM)));
+        src[i] = static_cast<uint32_t>(min(r, last)) * static_cast<uint32_t>(a.k) + 16 * ((lane & 7) ^ f);
     }
     const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
-    auto load_part = [&](int b, int i) {
-        load_to_lds((i < T::kN / 8 / T::kWaves ? wbase : xbase) + static_cast<int64_t>(b) * 128, src[i],
-                    lds_at + (b & 1) * T::kStage + (i * T::kWaves + wave) * 1024);
+    // in a last block of fewer columns the pieces past a row's end read its last one instead (the
+    // columns are cleared when they are used); a lane's piece is the same in all loads of an operand
+    const int64_t inside = a.k - 16 - static_cast<int64_t>(a.blocks - 1) * 128;
+    auto past = [&](int f) {
+        return static_cast<uint32_t>(max(static_cast<int64_t>(16 * ((lane & 7) ^ f)) - inside, static_cast<int64_t>(0)));
     };
-    const float* scales = reinterpret_cast<const float*>(lds + 2 * T::kStage);
-    const int sfirst = wave * 64 % T::kM;
-    const float* xs = a.xs + m0 * a.blocks;
+    const uint32_t wpast = past(swizzle_w<TN>(wave * 8 + (lane >> 3))), xpast = past(swizzle_x(lane >> 3));
+    auto load_part = [&](int b, int i) {
+        const bool is_w = i < LW;
+        const uint32_t back = first + b + 1 < a.blocks ? 0u : is_w ? wpast : xpast;
+        const int row = is_w ? (i * T::kWaves + wave) * 8 : T::kN + ((i - LW) * T::kWaves + wave) * 8 % T::kM;
+        load_to_lds((is_w ? wbase : xbase) + static_cast<int64_t>(b) * 128, src[i] - back,
+                    lds_at + b % S * T::kStage + row * 128);
+    };
+    const float* scales = reinterpret_cast<const float*>(lds + S * T::kStage);
+    const int sfirst = wave * 64 % T::kScales;
+    const float* xs = a.xs + m0 * a.blocks + first;
     const uint32_t ssrc = static_cast<uint32_t>(min(static_cast<int64_t>((sfirst + lane) % T::kM), a.m - 1 - m0)) * a.blocks * 4;
+    auto load_scales = [&](int b) {
+        load4_to_lds(xs + min(b, blocks - 1), ssrc,
+                     lds_at + S * T::kStage + (b % T::kScaleSlots * T::kScales + sfirst) * 4);
+    };
     const auto ws = (const __attribute__((address_space(4))) float*)(
-        a.ws + (min(n0 + 16 * TN * wn, a.n - 1) >> 7) * a.scale_cols);
+        a.ws + (min(n0 + 16 * TN * wn, a.n - 1) >> 7) * a.scale_cols + first);
 
     plm_f32x4 acc[TN][TM];
 #pragma unroll
@@ -297,24 +328,28 @@ __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const Mat
     const int w0 = wrow * 128 + 16 * (qd ^ fw), w1 = wrow * 128 + 16 * ((qd + 4) ^ fw);
     const int x0 = (T::kN + xrow) * 128 + 16 * (qd ^ fx), x1 = (T::kN + xrow) * 128 + 16 * ((qd + 4) ^ fx);
 
-    auto load_scales = [&](int b) {
-        load4_to_lds(xs + min(b, a.blocks - 1), ssrc, lds_at + 2 * T::kStage + ((b & 3) * T::kM + sfirst) * 4);
-    };
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) load_part(0, i);
+    // In the order of their use: scales 0, block 0, scales 1, block 1, ..., scales S - 1.  Block b sends
+    // block b + S - 1 and scales b + S, so behind its own operands S - 1 scales and S - 2 blocks are on
+    // their way.
     load_scales(0);
-    load_scales(1);
+    for (int b = 0; b < S - 1; ++b) {
+        if (b < blocks) {
+#pragma unroll
+            for (int i = 0; i < L; ++i) load_part(b, i);
+        }
+        load_scales(b + 1);
+    }
     float sw = ws[0];
     auto block = [&](int b, auto more, auto masked) {
         constexpr bool MORE = decltype(more)::value, MASKED = decltype(masked)::value;
-        load_to_lds_barrier<MORE ? 1 : 0>();
-        const float next_w = ws[min(b + 1, a.blocks - 1)];
-        const char* stage = lds + (b & 1) * T::kStage;
-        const float* sx = scales + (b & 3) * T::kM + xrow;
+        load_to_lds_barrier<MORE ? S - 1 + (S - 2) * L : 0>();
+        const float next_w = ws[min(b + 1, blocks - 1)];
+        const char* stage = lds + b % S * T::kStage;
+        const float* sx = scales + b % T::kScaleSlots * T::kScales + xrow;
         auto piece = [&](int at, int h) {
             plm_u32x4 v = *reinterpret_cast<const plm_u32x4*>(stage + at);
             if constexpr (MASKED) {  // columns past the end
-                if (static_cast<int64_t>(b) * 128 + 64 * h + 16 * qd >= a.k) v = plm_u32x4{0, 0, 0, 0};
+                if (static_cast<int64_t>(first + b) * 128 + 64 * h + 16 * qd >= a.k) v = plm_u32x4{0, 0, 0, 0};
             }
             return v;
         };
@@ -334,12 +369,13 @@ __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const Mat
 #pragma unroll
         for (int at = 0; at < TN * TM + kLag; ++at) {
             const int i = at % TN, j = at / TN;
-            // the next block's loads go out one at a time: all at once they wait for each other before the
-            // first product
+            // A later block's loads go out two at a time: all at once they hold up the first products (one
+            // row of 256 x 256 tiles 526 us, two at a time 414, one 477).
             if (MORE && i == 0) {
+                constexpr int kAtOnce = 2 * TM >= L ? 2 : L;
 #pragma unroll
-                for (int x = kAtOnce * j; x < min(kLoads, kAtOnce * (j + 1)); ++x) load_part(b + 1, x);
-                if (j == kScalesAt) load_scales(b + 2);
+                for (int x = kAtOnce * j; x < min(L, kAtOnce * (j + 1)); ++x) load_part(b + S - 1, x);
+                if (j == TM - 1) load_scales(b + S);
             }
             if (i == 0 && j + 1 < TM) {
                 v[(j + 1) & 1][0] = piece(x0 + (j + 1) * 2048, 0);
@@ -364,72 +400,183 @@ __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const Mat
             for (int j = 0; j < TM; ++j) asm volatile("" : "+v"(acc[i][j]));
         sw = next_w;
     };
-    for (int b = 0; b + 1 < a.blocks; ++b) block(b, std::true_type{}, std::false_type{});
-    block(a.blocks - 1, std::false_type{}, std::true_type{});
+    int b = 0;
+    for (; b + S - 1 < blocks; ++b) block(b, std::true_type{}, std::false_type{});
+    for (; b < blocks; ++b) block(b, std::false_type{}, std::true_type{});
 
-    // A lane has 4 TN adjacent results of TM rows.  Whole ones of aligned rows
-    // are stored by 16 bytes, others by single values through LDS.
+    // A lane has 4 TN adjacent results of TM rows, stored by 16 bytes (rows need no alignment: such
+    // stores may start at any value) up to the last columns.
     const int64_t n = n0 + 16 * TN * wn + 4 * TN * qd;
-    const int per = a.out_type == kOutF32 ? 4 : 8;
-    const bool wide = a.n % per == 0 && n0 + T::kN <= a.n && (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0;
-    if (wide) {
+    if (gridDim.z > 1) {  // a.part [share][m][n4], n4 the columns up to a multiple of 4
+        const int64_t n4 = (a.n + 3) & ~static_cast<int64_t>(3);
 #pragma unroll
         for (int j = 0; j < TM; ++j) {
             const int64_t m = m0 + 16 * TM * wm + 16 * j + li;
+#pragma unroll
+            for (int i = 0; i < TN; ++i)
+                if (m < a.m && n + 4 * i < a.n)
+                    *reinterpret_cast<plm_f32x4*>(a.part + (blockIdx.z * a.m + m) * n4 + n + 4 * i) = acc[i][j];
+        }
+        return;
+    }
+    if (a.out_type == kOutF32) {
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+            const int64_t m = m0 + 16 * TM * wm + 16 * j + li;
+            float* to = static_cast<float*>(a.out) + m * a.n + n;
             if (m >= a.m) continue;
-            const int64_t at = m * a.n + n;
-            if (a.out_type == kOutF32) {
 #pragma unroll
-                for (int i = 0; i < TN; ++i) *reinterpret_cast<plm_f32x4*>(static_cast<float*>(a.out) + at + 4 * i) = acc[i][j];
-            } else if (a.out_type == kOutBF16) {
+            for (int i = 0; i < TN; ++i) {
+                if (n + 4 * i + 4 <= a.n) {
+                    *reinterpret_cast<any_f32x4*>(to + 4 * i) = acc[i][j];
+                } else {
 #pragma unroll
-                for (int i = 0; i < TN; i += 2)
-                    *reinterpret_cast<plm_u32x4*>(static_cast<uint16_t*>(a.out) + at + 4 * i) =
-                        pack8<true>(acc[i][j], acc[i + 1][j]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < TN; i += 2)
-                    *reinterpret_cast<plm_u32x4*>(static_cast<uint16_t*>(a.out) + at + 4 * i) =
-                        pack8<false>(acc[i][j], acc[i + 1][j]);
+                    for (int e = 0; e < 4; ++e)
+                        if (n + 4 * i + e < a.n) to[4 * i + e] = acc[i][j][e];
+                }
             }
         }
         return;
     }
-    __syncthreads();
-    constexpr int kRow = 16 * TN;
-    plm_f32x4* mine = reinterpret_cast<plm_f32x4*>(lds) + wave * 16 * (kRow / 4);
+    constexpr int kSide = TN == 1 ? 1 : 2;  // tiles stored together
 #pragma unroll
     for (int j = 0; j < TM; ++j) {
+        const int64_t m = m0 + 16 * TM * wm + 16 * j + li;
+        uint16_t* to = static_cast<uint16_t*>(a.out) + m * a.n + n;
+        if (m >= a.m) continue;
 #pragma unroll
-        for (int i = 0; i < TN; ++i) mine[li * (kRow / 4) + TN * qd + i] = acc[i][j];
-        // the wave's own: its LDS operations are done in order
-        __builtin_amdgcn_wave_barrier();
-        for (int e = lane; e < 16 * kRow; e += 64) {
-            const int64_t m = m0 + 16 * TM * wm + 16 * j + e / kRow, c = n0 + 16 * TN * wn + e % kRow;
-            if (m < a.m && c < a.n) store_out(a, m * a.n + c, reinterpret_cast<const float*>(mine)[e]);
+        for (int i = 0; i < TN; i += kSide) {
+            const plm_u32x4 v = a.out_type == kOutBF16 ? pack8<true>(acc[i][j], acc[i + kSide - 1][j])
+                                                       : pack8<false>(acc[i][j], acc[i + kSide - 1][j]);
+            if (n + 4 * i + 4 * kSide <= a.n) {
+                if constexpr (kSide == 2)
+                    *reinterpret_cast<any_u32x4*>(to + 4 * i) = v;
+                else
+                    *reinterpret_cast<any_u32x2*>(to + 4 * i) = any_u32x2{v.x, v.y};
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4 * kSide; ++e)
+                    if (n + 4 * i + e < a.n) to[4 * i + e] = static_cast<uint16_t>(v[e >> 1] >> (16 * (e & 1)));
+            }
         }
-        __builtin_amdgcn_wave_barrier();
     }
 }
 
-template <int TN, int TM, int GN, int GM>
-int launch_tile(const MatmulArgs& a, hipStream_t st) {
-    using T = Tile<TN, TM, GN, GM>;
+// The shares' sums in their order, rounded once.  A thread: four columns.
+__global__ __launch_bounds__(256) void fp8_matmul_join_kernel(const MatmulArgs a, int shares) {
+    const int64_t n4 = (a.n + 3) / 4;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (at >= a.m * n4) return;
+    const plm_f32x4* part = reinterpret_cast<const plm_f32x4*>(a.part) + at;
+    plm_f32x4 v = part[0];
+    for (int s = 1; s < shares; ++s) v = v + part[s * a.m * n4];
+    const int64_t m = at / n4, n = (at - m * n4) * 4;
+    for (int e = 0; e < 4; ++e)
+        if (n + e < a.n) store_out(a, m * a.n + n + e, v[e]);
+}
+
+template <int TN, int TM, int GN, int GM, int S>
+int launch_tile(const MatmulArgs& a, int shares, hipStream_t st) {
+    using T = Tile<TN, TM, GN, GM, S>;
     const int64_t gx = plm::ceil_div(a.n, T::kN), gy = plm::ceil_div(a.m, T::kM);
     if (gx > 0x7FFFFFFF || gy > 65535) return plm::fail(-2, "too many rows");
-    const void* fn = reinterpret_cast<const void*>(&fp8_matmul_tile_kernel<TN, TM, GN, GM>);
-    const int code = plm::allow_large_lds(fn, T::kLds);
+    const void* fn = reinterpret_cast<const void*>(&fp8_matmul_tile_kernel<TN, TM, GN, GM, S>);
+    int code = T::kLds > 64 * 1024 ? plm::allow_large_lds(fn, T::kLds) : 0;
     if (code != 0) return code;
-    hipLaunchKernelGGL((fp8_matmul_tile_kernel<TN, TM, GN, GM>), dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy)),
+    hipLaunchKernelGGL((fp8_matmul_tile_kernel<TN, TM, GN, GM, S>),
+                       dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy), static_cast<unsigned>(shares)),
                        dim3(64 * T::kWaves), T::kLds, st, a);
-    return plm::check_launch("fp8_e4m3_block_matmul");
+    code = plm::check_launch("fp8_e4m3_block_matmul");
+    if (code != 0 || shares == 1) return code;
+    hipLaunchKernelGGL(fp8_matmul_join_kernel, dim3(static_cast<unsigned>(plm::ceil_div(a.m * plm::ceil_div(a.n, 4), 256))),
+                       dim3(256), 0, st, a, shares);
+    return plm::check_launch("fp8_e4m3_block_matmul, join");
+}
+
+// How a product runs, from its sizes alone: the least of the times (us, an
+// MI355X) that these straight lines give, fitted to 860 timings of 139 shapes
+// of 1 to 4096 rows, 134 to 24576 weight rows and 544 to 16384 columns (the
+// choice is 2 % slower than the fastest of all that were timed, 13 % at worst).
+//   tile   a workgroup's time per K block, alone on its compute unit or two on
+//          one, for the rounds that the grid takes; 8 us for launch, first loads
+//          and stores; at least the weight at 5.85 TB/s
+//   shares of the blocks (for grids that leave compute units idle): 3.85 us for
+//          the join, its sums written and read at 3.6 TB/s
+//   rows   its waves' blocks, or the weight at 3.6 TB/s (2.4 above 8 rows)
+struct Choice {
+    int tile;    // activation rows of a workgroup; 0: the rows kernel
+    int shares;  // of the blocks
+};
+
+struct TileCost {
+    int tile, weight_rows;
+    double alone, paired;  // paired 0: only grids of one workgroup per compute unit
+};
+constexpr TileCost kTileCosts[] = {
+    {256, 256, 1.42, 0.0}, {128, 128, 0.64, 1.33}, {64, 128, 0.49, 0.0}, {32, 128, 0.48, 0.0}, {16, 128, 0.33, 0.72}};
+constexpr int kMostShares = 9;
+constexpr int kMostRows = 32;  // of the rows kernel
+
+Choice choice_of(int64_t m, int64_t n, int64_t k) {
+    const int64_t blocks = plm::ceil_div(k, 128);
+    const double bytes = static_cast<double>(n) * static_cast<double>(k);
+    const int64_t cus = plm::cu_count();
+    if (k >= (1 << 23)) return {0, 1};  // a workgroup's rows pass 32-bit offsets
+    Choice best = {0, 1};
+    double least = 1e30;
+    if (m <= kMostRows)
+        least = std::max(3.2 + (m <= 8 ? 0.75 : m <= 16 ? 1.0 : 1.6) * static_cast<double>(plm::ceil_div(blocks, 8)),
+                         3.5 + bytes / (m <= 8 ? 3.6e6 : 2.4e6));
+    for (const TileCost& c : kTileCosts) {
+        if (c.tile >= 2 * m && c.tile > 16) continue;
+        const int64_t tiles = plm::ceil_div(n, c.weight_rows) * plm::ceil_div(m, c.tile);
+        for (int64_t s = 1; s <= kMostShares && s <= blocks; ++s) {
+            const int64_t groups = tiles * s, per = plm::ceil_div(blocks, s);
+            double t = static_cast<double>(per) * c.alone;
+            if (c.tile == 256)
+                t *= static_cast<double>(plm::ceil_div(groups, cus));
+            else if (groups > cus && c.paired > 0.0)
+                t = static_cast<double>(per) * c.paired *
+                    std::max(1.0, static_cast<double>(groups) / static_cast<double>(2 * cus));
+            else if (groups > cus)
+                break;
+            t = std::max(t + 8.0, bytes / 5.85e6);
+            if (s > 1) t += 3.85 + static_cast<double>(s * m) * static_cast<double>(n) * 8.0 / 3.6e6;
+            if (t < least) {
+                least = t;
+                best = {c.tile, static_cast<int>(s)};
+            }
+        }
+    }
+    return best;
+}
+
+// The call's scratch: the shares' sums, then both operands in rows of whole
+// pieces where theirs are not.
+struct Scratch {
+    int64_t sums;  // bytes
+    int64_t k16;   // columns of a row
+    int64_t all;   // bytes
+};
+
+Scratch scratch_of(const Choice& c, int64_t m, int64_t n, int64_t k) {
+    Scratch s;
+    s.sums = c.shares > 1 ? c.shares * m * plm::ceil_div(n, 4) * 16 : 0;
+    s.k16 = plm::ceil_div(k, 16) * 16;
+    s.all = s.sums + (s.k16 != k ? (m + n) * s.k16 : 0);
+    return s;
+}
+
+bool bad_sizes(int64_t m, int64_t n, int64_t k) {
+    const int64_t most = static_cast<int64_t>(1) << 31;
+    return m <= 0 || n <= 0 || k <= 0 || m >= most || n >= most || k >= most;
 }
 
 }  // namespace
 
 PLM_EXPORT int64_t fp8_e4m3_block_matmul_scratch_bytes(int64_t rows, int64_t out_rows, int64_t in_cols) {
-    if (rows <= 0 || out_rows <= 0 || in_cols <= 0) return plm::fail(-2, "bad dimensions");
-    return 0;
+    if (bad_sizes(rows, out_rows, in_cols)) return plm::fail(-2, "bad dimensions");
+    return scratch_of(choice_of(rows, out_rows, in_cols), rows, out_rows, in_cols).all;
 }
 
 PLM_EXPORT int fp8_e4m3_block_matmul(const uint8_t* x, const float* x_scales, const uint8_t* fp8_weight,
@@ -438,24 +585,42 @@ PLM_EXPORT int fp8_e4m3_block_matmul(const uint8_t* x, const float* x_scales, co
                                      int dtype_code) {
     if (x == nullptr || x_scales == nullptr || fp8_weight == nullptr || scale_inv == nullptr || out == nullptr)
         return plm::fail(-1, "null pointer");
-    const int64_t most = static_cast<int64_t>(1) << 31;
-    if (rows <= 0 || out_rows <= 0 || in_cols <= 0 || rows >= most || out_rows >= most || in_cols >= most ||
-        scale_cols < plm::ceil_div(in_cols, 128) || dtype_code < 0 || dtype_code > 2)
+    if (bad_sizes(rows, out_rows, in_cols) || scale_cols < plm::ceil_div(in_cols, 128) || dtype_code < 0 || dtype_code > 2)
         return plm::fail(-2, "bad dimensions");
-    const MatmulArgs a = {x,    x_scales, fp8_weight, scale_inv,  out,
-                          rows, out_rows, in_cols,    scale_cols, static_cast<int>(plm::ceil_div(in_cols, 128)),
-                          dtype_code};
-    (void)scratch, (void)scratch_bytes;
+    if (!plm::aligned16(x) || !plm::aligned16(fp8_weight)) return plm::fail(-2, "rows and weight must be 16-byte aligned");
+    MatmulArgs a = {x,    x_scales, fp8_weight, scale_inv,  out,
+                    rows, out_rows, in_cols,    scale_cols, static_cast<int>(plm::ceil_div(in_cols, 128)),
+                    dtype_code, nullptr};
+    const Choice c = choice_of(rows, out_rows, in_cols);
+    const Scratch need = scratch_of(c, rows, out_rows, in_cols);
     const hipStream_t st = plm::current_stream();
-    if (in_cols % 16 != 0 || !plm::aligned16(x) || !plm::aligned16(fp8_weight)) {
-        const int64_t groups = plm::ceil_div(rows * out_rows, 256);
-        if (groups > 0x7FFFFFFF) return plm::fail(-2, "too many results");
-        hipLaunchKernelGGL(fp8_matmul_scalar_kernel, dim3(static_cast<unsigned>(groups)), dim3(256), 0, st, a);
-        return plm::check_launch("fp8_e4m3_block_matmul");
+    if (need.all > 0) {
+        char* at = static_cast<char*>(scratch);
+        if (at == nullptr) {
+            at = static_cast<char*>(plm::workspace(static_cast<size_t>(need.all)));
+            if (at == nullptr) return -3;
+        } else if (scratch_bytes < need.all || !plm::aligned16(at)) {
+            return plm::fail(-3, "scratch must hold fp8_e4m3_block_matmul_scratch_bytes, 16-byte aligned");
+        }
+        a.part = reinterpret_cast<float*>(at);
+        if (need.k16 != in_cols) {
+            uint8_t* to = reinterpret_cast<uint8_t*>(at) + need.sums;
+            int code = pad_rows(x, to, rows, in_cols, need.k16, st);
+            if (code == 0) code = pad_rows(fp8_weight, to + rows * need.k16, out_rows, in_cols, need.k16, st);
+            if (code != 0) return code;
+            a.x = to;
+            a.w = to + rows * need.k16;
+            a.k = need.k16;
+        }
+    }
+    switch (c.tile) {
+        case 16: return launch_tile<1, 1, 8, 1, 4>(a, c.shares, st);
+        case 32: return launch_tile<1, 2, 8, 1, 3>(a, c.shares, st);
+        case 64: return launch_tile<2, 2, 4, 2, 3>(a, c.shares, st);
+        case 128: return launch_tile<2, 4, 4, 2, 2>(a, c.shares, st);
+        case 256: return launch_tile<4, 8, 4, 2, 2>(a, c.shares, st);
+        default: break;
     }
     const int waves = std::min(8, a.blocks);
-    if (rows <= 16) return launch_rows<1, 1, 4, 8>(a, waves, st);
-    if (rows <= 32) return launch_rows<2, 2, 2, 8>(a, waves, st);
-    if (rows <= 64) return launch_rows<2, 4, 2, 8>(a, waves, st);
-    return launch_tile<4, 8, 4, 2>(a, st);
+    return rows <= 16 ? launch_rows<1, 1, 4, 8>(a, waves, st) : launch_rows<2, 2, 2, 8>(a, waves, st);
 }

@@ -1973,6 +1973,10 @@ def fp8_e4m3_block_matmul(rows: Fp8Rows, fp8_weight: torch.Tensor, scale_inv: to
     _device_only("fp8_e4m3_block_matmul", device, xs, fp8_weight, scale_inv)
     if not (x.is_contiguous() and xs.is_contiguous() and fp8_weight.is_contiguous() and scale_inv.is_contiguous()):
         x, xs, fp8_weight, scale_inv = (t.contiguous() for t in (x, xs, fp8_weight, scale_inv))
+    if x.data_ptr() & 15:
+        x = x.clone()
+    if fp8_weight.data_ptr() & 15:
+        fp8_weight = fp8_weight.clone()
     out = torch.empty((m, n), dtype=out_dtype, device=device)
     if m and n:
         with _launch(lib, device) as index:

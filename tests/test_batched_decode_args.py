@@ -42,7 +42,7 @@ def test_matmul_codes(lib):
 
     for name in ("x", "xs", "w", "ws", "out"):
         assert call(**{name: N}) == -1
-    for bad in (dict(m=0), dict(n=-1), dict(k=0), dict(k=129), dict(code=3), dict(m=1 << 31), dict(n=1 << 31)):
+    for bad in (dict(m=0), dict(n=-1), dict(k=0), dict(k=129), dict(code=3), dict(m=1 << 31), dict(n=1 << 31), dict(x=ODD), dict(w=ODD)):
         assert call(**bad) == -2
     assert lib.fp8_e4m3_block_matmul_scratch_bytes(0, 1, 1) == -2
     assert lib.fp8_e4m3_block_matmul_scratch_bytes(1, 16, 128) >= 0

@@ -99,7 +99,7 @@ def test_offset_and_strided_operands(nat):
                                     out_dtype=torch.float32)
     assert torch.equal(got, want)
     exact, size = ref.matmul(x, xs, w, ws)
-    # an odd address: one result a thread
+    # an odd address: copied first
     ref.within(nat.fp8_e4m3_block_matmul(nat.Fp8Rows(x.cuda(), xs.cuda()), odd, ws.cuda(), out_dtype=torch.float32),
                exact, ref.matmul_bound(exact, size, k, torch.float32))
     assert nat.fp8_e4m3_block_matmul(nat.Fp8Rows(x.cuda()[:0], xs.cuda()[:0]), w.cuda(), ws.cuda()).shape == (0, n)
