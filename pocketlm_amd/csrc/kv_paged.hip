@@ -682,17 +682,39 @@ __global__ __launch_bounds__(64 * kAttnWaves, CT * DP > 128 ? 1 : 2) void paged_
     }
 }
 
-// Joins the splits of a sequence: a wave per query row and head, its lanes
-// over the head's values.  Sequences of one split were written already.
+// Joins the splits of a sequence, a workgroup per query row and head.  Its
+// threads first take the splits' maxima and sums (the weights of the splits go
+// to LDS), then each a quad of head values of every kSets-th split, and the
+// sets meet in LDS.  Sequences of one split were written already.
+constexpr int kJoinThreads = 256;
+constexpr int kJoinSplits = 1024;  // at a time
+
+__device__ __forceinline__ float join_reduce(float v, bool is_max, float* red) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        const float o = __shfl_xor(v, off);
+        v = is_max ? fmaxf(v, o) : v + o;
+    }
+    if (lane == 0) red[wave] = v;
+    __syncthreads();
+    v = is_max ? fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])) : (red[0] + red[1]) + (red[2] + red[3]);
+    __syncthreads();
+    return v;
+}
+
 template <bool BF16>
-__global__ __launch_bounds__(256) void paged_join_kernel(const AttnArgs a, int ct) {
+__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const AttnArgs a, int ct) {
+    __shared__ float weights[kJoinSplits];
+    __shared__ f32x4 sums[kJoinThreads];
+    __shared__ float red[4];
     const int lane = threadIdx.x & 63;
     const int all = a.rows * a.heads;
-    const int per = (all + 3) / 4;
-    int seq = blockIdx.x / per;
-    const int at = (blockIdx.x - seq * per) * 4 + (threadIdx.x >> 6);
+    int seq = blockIdx.x / all;
+    const int at = blockIdx.x - seq * all;
     Plan plan;
-    if (!find_plan(a, lane, false, 0, seq, plan) || plan.splits <= 1 || at >= all) return;
+    if (!find_plan(a, lane, false, 0, seq, plan) || plan.splits <= 1) return;
+    const int splits = __builtin_amdgcn_readfirstlane(plan.splits);
     const int r = at / a.heads, head = at - r * a.heads;
     const int kvh = head / a.group, col = r * a.group + head - kvh * a.group;
     const int hc_count = a.kv_heads * a.column_blocks;
@@ -700,35 +722,41 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const AttnArgs a, int c
     const int hc = kvh * a.column_blocks + col / wide;
     // partial of split s: first + s * stride
     const int64_t stride = static_cast<int64_t>(hc_count) * wide;
-    const int64_t first = (static_cast<int64_t>(plan.first) * hc_count + hc) * wide + col % wide;
+    const int64_t first = (static_cast<int64_t>(__builtin_amdgcn_readfirstlane(plan.first)) * hc_count + hc) * wide + col % wide;
+    const f32x2* ml = reinterpret_cast<const f32x2*>(a.part_ml) + first;
     float m = -INFINITY;
-    for (int s = lane; s < plan.splits; s += 64) m = fmaxf(m, a.part_ml[2 * (first + s * stride)]);
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+    for (int s = threadIdx.x; s < splits; s += kJoinThreads) m = fmaxf(m, ml[s * stride][0]);
+    m = join_reduce(m, true, red);
+    const int quads = a.head_dim / 4;  // threads of a set
+    const int sets = kJoinThreads / quads;
+    const int set = threadIdx.x / quads, d = 4 * (threadIdx.x - set * quads);
+    const float* part = a.part + first * a.head_dim + d;
     float sum = 0.0f;
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    const int d = 4 * lane;
-    for (int base = 0; base < plan.splits; base += 64) {
-        float weight = 0.0f, part = 0.0f;
-        if (base + lane < plan.splits) {
-            const f32x2 ml = *reinterpret_cast<const f32x2*>(a.part_ml + 2 * (first + (base + lane) * stride));
-            weight = exp2_from(ml[0], m);
-            part = ml[1] * weight;
+    for (int base = 0; base < splits; base += kJoinSplits) {
+        const int n = min(kJoinSplits, splits - base);
+        if (base > 0) __syncthreads();
+        for (int s = threadIdx.x; s < n; s += kJoinThreads) {
+            const f32x2 v = ml[(base + s) * stride];
+            const float w = exp2_from(v[0], m);
+            weights[s] = w;
+            sum = fmaf(v[1], w, sum);
         }
+        __syncthreads();
+        if (set < sets) {
+#pragma unroll 4
+            for (int s = set; s < n; s += sets) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(part + (base + s) * stride * a.head_dim);
+                const float w = weights[s];
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) part += __shfl_xor(part, off);
-        sum += part;
-        const int n = min(64, plan.splits - base);
-        for (int s = 0; s < n; ++s) {
-            const float f = __shfl(weight, s);
-            if (d < a.head_dim) {
-                const f32x4 x = *reinterpret_cast<const f32x4*>(a.part + (first + (base + s) * stride) * a.head_dim + d);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[i] = fmaf(x[i], f, acc[i]);
+                for (int i = 0; i < 4; ++i) acc[i] = fmaf(x[i], w, acc[i]);
             }
         }
     }
-    if (d >= a.head_dim) return;
+    sums[threadIdx.x] = acc;
+    sum = join_reduce(sum, false, red);
+    if (threadIdx.x >= quads) return;
+    for (int s = 1; s < sets; ++s) acc = acc + sums[s * quads + threadIdx.x];
     const bool empty = m == -INFINITY;
     const float inv = 1.0f / sum;
     u32x2 o;
@@ -840,7 +868,7 @@ void launch_attention(const AttnArgs& a, const AttnShape& s, hipStream_t st) {
 #undef PLM_ATTN
     if (s.joined)
         hipLaunchKernelGGL((paged_join_kernel<BF16>),
-                           dim3(static_cast<unsigned>(a.p.sequences * plm::ceil_div(a.rows * a.heads, 4))), dim3(256), 0,
+                           dim3(static_cast<unsigned>(a.p.sequences * a.rows * a.heads)), dim3(kJoinThreads), 0,
                            st, a, s.ct);
 }
 
@@ -938,7 +966,7 @@ PLM_EXPORT int kv_paged_attention_decode_u16(const uint16_t* q, const uint16_t* 
         return plm::fail(-2, "query strides and addresses must be multiples of 16 bytes");
     a.capacity = table_cols * page_size;
     const AttnShape s = shape_of(sequences, rows, heads, kv_heads, head_dim, a.capacity);
-    if (s.items * kv_heads * s.column_blocks > kMostInt || sequences * plm::ceil_div(rows * heads, 4) > kMostInt)
+    if (s.items * kv_heads * s.column_blocks > kMostInt || sequences * rows * heads > kMostInt)
         return plm::fail(-2, "too many sequences and heads");
     void* part = scratch;
     if (s.bytes > 0) {
