@@ -8,6 +8,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
+#include <type_traits>
 
 #include "common.h"
 
@@ -239,21 +240,26 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(const Appe
 
 // ---------------------------------------------------------------- attention
 //
-// A unit is 128 positions of a sequence.  The work is dealt out on the device
-// from the lengths: with c units to an item, sequence b has ceil(units / c)
-// items, c the least that keeps their number at about `budget`.  Each
-// workgroup finds its item from the lengths itself; no launch, copy or host
-// value depends on them.
+// A unit is 128 positions of a sequence (an idle or empty one has one unit,
+// whose result is the zeros).  The units of all sequences, one after another,
+// are dealt to the workgroups of a key-value head in equal runs, on the device
+// from the lengths: no launch, copy or host value depends on them, and ragged
+// batches stay balanced (48 sequences of 8000 to 16000 positions, 4 heads of 128:
+// 253 -> 228 us against runs that end with their sequence).  A run
+// that holds a sequence's every unit writes its result; the others write a
+// partial, in slot run + sequence, which grows by at least one from partial to
+// partial.
 
 constexpr int kUnit = 128;
 constexpr int kAttnWaves = 4;
 constexpr int kMaxQueryRows = 8;
+constexpr uint32_t kShortRuns = 4;  // units for each run, below which sequences are short
 
 struct AttnArgs {
     Pages p;
     const uint16_t* q;
     uint16_t* out;     // [sequences][rows][heads][head_dim]
-    float* part;       // [item][head and column block][column][head_dim], then the maxima and sums
+    float* part;       // [slot][head and column block][column][head_dim], then the maxima and sums
     float* part_ml;
     int64_t q_seq, q_row, q_head;  // strides, values
     int64_t capacity;  // positions of a table row
@@ -264,7 +270,9 @@ struct AttnArgs {
     int head_dim;
     int columns;       // rows * group: column r * group + h is row r, head h of the group
     int column_blocks;
-    int budget;
+    uint32_t budget;      // runs of long sequences
+    uint32_t short_runs;  // runs of short ones, about
+    uint32_t streamed;    // units from which on the values are read past the caches
     float scale;       // softmax scale * log2(e)
 };
 
@@ -273,52 +281,88 @@ __device__ __forceinline__ int64_t seen_of(int length, int rows, int64_t capacit
     return length < 0 ? 0 : min(static_cast<int64_t>(length) + rows, capacity);
 }
 
-// Items start at least one per sequence: an idle one's writes the zeros.
 __device__ __forceinline__ uint32_t units_of(int length, int rows, int64_t capacity) {
     return max(1u, static_cast<uint32_t>((seen_of(length, rows, capacity) + kUnit - 1) / kUnit));
 }
 
-struct Plan {
-    int first;   // item of the sequence's first split
-    int splits;
-};
-
-__device__ __forceinline__ uint32_t item_units(const AttnArgs& a, int lane) {
-    unsigned long long total = 0;
-    for (int base = 0; base < a.p.sequences; base += 64) {
-        const int i = base + lane;
-        if (i < a.p.sequences) total += units_of(a.p.lengths[i], a.rows, a.capacity);
-    }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off);
-    return static_cast<uint32_t>((total + a.budget - 1) / a.budget);
+// Inclusive prefix sum over the lanes of a wave (DPP, no LDS).
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t v) {
+#define PLM_PREFIX(ctrl, rows) \
+    v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), ctrl, rows, 0xF, false))
+    PLM_PREFIX(0x111, 0xF);  // row_shr:1, 2, 4, 8
+    PLM_PREFIX(0x112, 0xF);
+    PLM_PREFIX(0x114, 0xF);
+    PLM_PREFIX(0x118, 0xF);
+    PLM_PREFIX(0x142, 0xA);  // row_bcast:15 into rows 1 and 3
+    PLM_PREFIX(0x143, 0xC);  // row_bcast:31 into rows 2 and 3
+#undef PLM_PREFIX
+    return v;
 }
 
-// The sequence that holds item `item` (`by_item`), or the plan of sequence
-// `seq`.  Every lane of a wave calls it.  False past the last item.
-__device__ __forceinline__ bool find_plan(const AttnArgs& a, int lane, bool by_item, int item, int& seq, Plan& plan) {
-    const uint32_t c = item_units(a, lane);
-    int before = 0;
-    for (int base = 0; base < a.p.sequences; base += 64) {
+struct Plan {
+    uint32_t total;   // units of all sequences, each rounded up to whole multiples of `align`
+    uint32_t runs;
+    uint32_t align;
+    int seq;
+    uint32_t before;  // units of the sequences before seq, rounded
+    uint32_t units;   // of seq
+
+    __device__ __forceinline__ uint32_t rounded(uint32_t n) const { return (n + align - 1) / align * align; }
+    // run * total / runs
+    __device__ __forceinline__ uint32_t start(uint32_t run) const {
+        const uint32_t each = total / runs;
+        return run * each + run * (total - each * runs) / runs;
+    }
+    // The run that holds a unit: the last that starts at or before it.
+    __device__ __forceinline__ uint32_t run_of(uint32_t unit) const {
+        if (total == runs * align) return unit / align;
+        return static_cast<uint32_t>(((static_cast<uint64_t>(unit) + 1) * runs + total - 1) / total - 1);
+    }
+};
+
+// The plan, at the sequence that holds the first unit of run `run` (by_run),
+// or at sequence `seq`.  Every lane of a wave calls it; false for a run past
+// the last.
+__device__ __forceinline__ bool find_plan(const AttnArgs& a, int lane, bool by_run, uint32_t run, int seq, Plan& plan) {
+    // a lane's sequence of each 64: the first 64 are read once
+    const uint32_t n0 = lane < a.p.sequences ? units_of(a.p.lengths[lane], a.rows, a.capacity) : 0;
+    auto units_at = [&](int base) {
+        if (base == 0) return n0;
         const int i = base + lane;
-        const int n =
-            i < a.p.sequences ? static_cast<int>((units_of(a.p.lengths[i], a.rows, a.capacity) + c - 1) / c) : 0;
-        int upto = n;  // inclusive prefix
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int o = __shfl_up(upto, off);
-            if (lane >= off) upto += o;
-        }
-        const unsigned long long past =
-            by_item ? __ballot(before + upto > item) : __ballot(i == seq);
+        return i < a.p.sequences ? units_of(a.p.lengths[i], a.rows, a.capacity) : 0;
+    };
+    auto sum = [&] {
+        uint32_t total = 0;
+        for (int base = 0; base < a.p.sequences; base += 64)
+            total += __builtin_amdgcn_readlane(wave_prefix(plan.rounded(units_at(base))), 63);
+        return total;
+    };
+    // Long sequences: `budget` equal runs, as many as there is room for.  Short ones: runs of `align`
+    // units that end with their sequence (starting on another costs more than a unit or two), as many as
+    // there are compute units (their partials cost as well).
+    plan.align = 1;
+    plan.total = sum();
+    plan.runs = a.budget;
+    if (plan.total < kShortRuns * a.budget) {
+        plan.align = max(1u, (plan.total + a.short_runs - 1) / a.short_runs);
+        if (plan.align > 1) plan.total = sum();
+        plan.runs = plan.total / plan.align;
+    }
+    if (by_run && run >= plan.runs) return false;
+    const uint32_t unit = by_run ? plan.start(run) : 0;
+    uint32_t before = 0;
+    for (int base = 0; base < a.p.sequences; base += 64) {
+        const uint32_t n = units_at(base);
+        const uint32_t upto = wave_prefix(plan.rounded(n));
+        const unsigned long long past = by_run ? __ballot(before + upto > unit) : __ballot(base + lane == seq);
         if (past != 0) {
-            const int at = __ffsll(past) - 1;
-            seq = base + at;
-            plan.splits = __shfl(n, at);
-            plan.first = before + __shfl(upto, at) - plan.splits;
+            const int at = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
+            plan.seq = base + at;
+            plan.units = __builtin_amdgcn_readlane(n, at);
+            plan.before = before + __builtin_amdgcn_readlane(upto, at) - plan.rounded(plan.units);
             return true;
         }
-        before += __shfl(upto, 63);
+        before += __builtin_amdgcn_readlane(upto, 63);
     }
     return false;
 }
@@ -352,9 +396,9 @@ __device__ __forceinline__ float exp2_from(float x, float m) { return exp2f(x - 
 
 constexpr uint32_t kNoRow = 0xFFFFFFFFu;
 
-// Workgroup (item, kv head, column block): 4 waves take every fourth tile of
-// 32 positions of the item's range, each with a running maximum and sum of its
-// own; they meet in LDS at the end.
+// Workgroup (run, kv head, column block): for each sequence of the run, 4
+// waves take every fourth tile of 32 positions, each with a running maximum and
+// sum of its own; they meet in LDS at the end.
 //
 //   scores  S^T = K Q^T: A holds 16 positions x 32 head values as they lie in
 //           the cache, B the 16 columns' queries; a lane gets, of column
@@ -373,184 +417,204 @@ constexpr uint32_t kNoRow = 0xFFFFFFFFu;
 // DP: head_dim rounded up to 64, 128 or 256; EXACT: no rounding.  CT: blocks
 // of 16 columns.
 template <bool BF16, int DP, bool EXACT, int CT>
-__global__ __launch_bounds__(64 * kAttnWaves, CT * DP > 128 ? 1 : 2) void paged_attention_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(64 * kAttnWaves, DP > 128 || CT * DP > 256 ? 1 : 2) void paged_attention_kernel(const AttnArgs a) {
     constexpr int KS = DP / 32;               // score steps of 32 head values
     constexpr int NV = DP / 16;               // value instructions
     constexpr int PV = DP == 64 ? 4 : 8;      // adjacent head values of a lane
     constexpr int SETS = NV / PV;             // pieces of a lane per position
     constexpr float kBias = BF16 ? 0.0f : 15.0f;
-    __shared__ float meet[2][CT * (NV * 4 + 2)][64];
+    __shared__ float meet[2][CT * (NV * 4 + 2)][64];  // at most 70 KB
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int li = lane & 15, g = lane >> 4;
     const int hc_count = a.kv_heads * a.column_blocks;
-    const int item = blockIdx.x / hc_count, hc = blockIdx.x - item * hc_count;
+    const int run = blockIdx.x / hc_count, hc = blockIdx.x - run * hc_count;
     const int kvh = hc / a.column_blocks, col0 = (hc - kvh * a.column_blocks) * 16 * CT;
-    int seq = 0;
     Plan plan;
-    if (!find_plan(a, lane, true, item, seq, plan)) return;
-    seq = __builtin_amdgcn_readfirstlane(seq);
-    const int splits = __builtin_amdgcn_readfirstlane(plan.splits);
-    const int split = item - __builtin_amdgcn_readfirstlane(plan.first);
-    const int length = a.p.lengths[seq];
-    const int seen = static_cast<int>(seen_of(length, a.rows, a.capacity));
-    const int64_t units = (seen + kUnit - 1) / kUnit;
-    const int begin = static_cast<int>(units * split / splits * kUnit);
-    const int end = min(seen, static_cast<int>(units * (split + 1) / splits * kUnit));
+    if (!find_plan(a, lane, true, static_cast<uint32_t>(run), 0, plan)) return;
+    const uint32_t run_end = plan.start(run + 1);
+    const bool streamed = EXACT && DP >= 128 && plan.total >= a.streamed;
+    uint32_t unit = plan.start(run);
+    int seq = plan.seq;
+    uint32_t before = plan.before;
+    uint32_t units = plan.units;
+    while (unit < run_end) {  // a sequence of the run's
+        const int length = a.p.lengths[seq];
+        const int seen = static_cast<int>(seen_of(length, a.rows, a.capacity));
+        const bool whole = unit == before && run_end >= before + units;
+        const int begin = static_cast<int>(unit - before) * kUnit;
+        const int end = min(seen, static_cast<int>(min(run_end - before, units)) * kUnit);
 
-    // this lane's columns: queries, and the positions that each sees
-    u32x4 q[CT][KS];
-    int limit[CT];
+        // The lane's place anew for each sequence: what follows from it is not kept in registers over the
+        // others.
+        int again = lane;
+        asm volatile("" : "+v"(again));
+        const int li = again & 15, g = again >> 4;
+        // this lane's columns: queries, and the positions that each sees
+        u32x4 q[CT][KS];
+        int limit[CT];
 #pragma unroll
-    for (int t = 0; t < CT; ++t) {
-        const int col = col0 + 16 * t + li;
-        const int r = min(col, a.columns - 1) / a.group, h = min(col, a.columns - 1) - r * a.group;
-        const uint16_t* src = a.q + seq * a.q_seq + r * a.q_row + (kvh * a.group + h) * a.q_head;
-        limit[t] = col < a.columns ? static_cast<int>(seen_of(length, r + 1, a.capacity)) : 0;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const int d = 32 * s + 8 * g;
-            q[t][s] = *reinterpret_cast<const u32x4*>(src + (EXACT || d < a.head_dim ? d : 0));
-            if (col >= a.columns || (!EXACT && d >= a.head_dim)) q[t][s] = u32x4{0, 0, 0, 0};
-        }
-    }
-    const int least = static_cast<int>(seen_of(length, 1, a.capacity));  // what every row sees
-    const uint16_t* kbase = a.p.k + kvh * a.p.head_stride;
-    const uint16_t* vbase = a.p.v + kvh * a.p.head_stride;
-    const int* table = a.p.table + static_cast<int64_t>(seq) * a.p.table_cols;
-
-    float m[CT], l[CT];
-    f32x4 acc[CT][NV];
-#pragma unroll
-    for (int t = 0; t < CT; ++t) {
-        m[t] = -INFINITY;
-        l[t] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) acc[t][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-
-    // lane l looks up position t0 + (l & 31) of a tile
-    auto page_of = [&](int t0) {
-        const int pos = min(t0 + (lane & 31), seen - 1);
-        return table[static_cast<uint32_t>(pos) / a.p.page_size];
-    };
-    auto row_of = [&](int page, int t0) {
-        const int pos = t0 + (lane & 31);
-        const uint32_t slot = static_cast<uint32_t>(pos) % a.p.page_size;
-        const bool there = pos < seen && page >= 0 && static_cast<uint32_t>(page) < a.p.num_pages;
-        return there ? static_cast<uint32_t>(page) * a.p.page_stride + slot * a.p.slot_stride : kNoRow;
-    };
-    u32x4 k[2][KS];
-    u32x4 v[8][SETS];
-    auto load_k = [&](uint32_t row) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint32_t o = __shfl(row, 16 * i + li);
-            // a position that is not there reads the cache's first row; its score is replaced
-            const uint16_t* src = kbase + static_cast<int64_t>(o == kNoRow ? 0u : o) * 8;
+        for (int t = 0; t < CT; ++t) {
+            const int col = col0 + 16 * t + li;
+            const int r = min(col, a.columns - 1) / a.group, h = min(col, a.columns - 1) - r * a.group;
+            const uint16_t* src = a.q + seq * a.q_seq + r * a.q_row + (kvh * a.group + h) * a.q_head;
+            limit[t] = col < a.columns ? static_cast<int>(seen_of(length, r + 1, a.capacity)) : 0;
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 const int d = 32 * s + 8 * g;
-                k[i][s] = *reinterpret_cast<const u32x4*>(src + (EXACT || d < a.head_dim ? d : 0));
-                if (!EXACT && d >= a.head_dim) k[i][s] = u32x4{0, 0, 0, 0};
+                q[t][s] = *reinterpret_cast<const u32x4*>(src + (EXACT || d < a.head_dim ? d : 0));
+                if (col >= a.columns || (!EXACT && d >= a.head_dim)) q[t][s] = u32x4{0, 0, 0, 0};
             }
         }
-    };
-    uint32_t vrow[8];
-    auto load_v = [&](uint32_t row) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            vrow[j] = __shfl(row, (j < 4 ? 0 : 12) + 4 * g + j);
-            const uint16_t* src = vbase + static_cast<int64_t>(vrow[j] == kNoRow ? 0u : vrow[j]) * 8;
-#pragma unroll
-            for (int s = 0; s < SETS; ++s) {
-                const int d = PV * li + 128 * s;
-                const uint16_t* at = src + (EXACT || d < a.head_dim ? d : 0);
-                if constexpr (PV == 8) {
-                    v[j][s] = *reinterpret_cast<const u32x4*>(at);
-                } else {
-                    const u32x2 two = *reinterpret_cast<const u32x2*>(at);
-                    v[j][s] = u32x4{two.x, two.y, 0, 0};
-                }
-                if (!EXACT && d >= a.head_dim) v[j][s] = u32x4{0, 0, 0, 0};
-            }
-        }
-    };
-    // eight positions of head value PV s + i of the lane's pieces
-    auto across = [&](int s, int i, uint32_t low = 0x05040100u, uint32_t high = 0x07060302u) {
-        const uint32_t pick = (i & 1) ? high : low;
-        u32x4 t;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) t[j] = __builtin_amdgcn_perm(v[2 * j + 1][s][i >> 1], v[2 * j][s][i >> 1], pick);
-        return t;
-    };
+        const int least = static_cast<int>(seen_of(length, 1, a.capacity));  // what every row sees
+        const uint16_t* kbase = a.p.k + kvh * a.p.head_stride;
+        const uint16_t* vbase = a.p.v + kvh * a.p.head_stride;
+        const int* table = a.p.table + static_cast<int64_t>(seq) * a.p.table_cols;
 
-    int t0 = begin + 32 * wave;
-    if (t0 < end) {
-        uint32_t row = row_of(page_of(t0), t0);
-        load_k(row);
-        load_v(row);
-        int page = page_of(t0 + kUnit);
-        for (; t0 < end; t0 += kUnit) {
-            const bool more = t0 + kUnit < end;
-            const uint32_t next = row_of(page, t0 + kUnit);
-            page = page_of(t0 + 2 * kUnit);
-            f32x4 s[CT][2];
+        float m[CT], l[CT];
+        f32x4 acc[CT][NV];
 #pragma unroll
-            for (int t = 0; t < CT; ++t)
+        for (int t = 0; t < CT; ++t) {
+            m[t] = -INFINITY;
+            l[t] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    s[t][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int i = 0; i < NV; ++i) acc[t][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+
+        // lane l looks up position t0 + (l & 31) of a tile
+        auto page_of = [&](int t0) {
+            const int pos = min(t0 + (lane & 31), seen - 1);
+            return table[static_cast<uint32_t>(pos) / a.p.page_size];
+        };
+        auto row_of = [&](int page, int t0) {
+            const int pos = t0 + (lane & 31);
+            const uint32_t slot = static_cast<uint32_t>(pos) % a.p.page_size;
+            const bool there = pos < end && page >= 0 && static_cast<uint32_t>(page) < a.p.num_pages;
+            return there ? static_cast<uint32_t>(page) * a.p.page_stride + slot * a.p.slot_stride : kNoRow;
+        };
+        u32x4 k[2][KS];
+        u32x4 v[8][SETS];
+        auto load_k = [&](uint32_t row) {
 #pragma unroll
-                    for (int x = 0; x < KS; ++x) s[t][i] = mfma16<BF16>(k[i][x], q[t][x], s[t][i]);
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t o = __shfl(row, 16 * i + li);
+                // a position that is not there reads the cache's first row; its score is replaced
+                const uint16_t* src = kbase + static_cast<int64_t>(o == kNoRow ? 0u : o) * 8;
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    const int d = 32 * s + 8 * g;
+                    k[i][s] = *reinterpret_cast<const u32x4*>(src + (EXACT || d < a.head_dim ? d : 0));
+                    if (!EXACT && d >= a.head_dim) k[i][s] = u32x4{0, 0, 0, 0};
                 }
+            }
+        };
+        uint32_t vrow[8];
+        auto load_v = [&](uint32_t row, auto nontemporal) {
+            constexpr bool past = decltype(nontemporal)::value;
 #pragma unroll
-            for (int t = 0; t < CT; ++t)
+            for (int j = 0; j < 8; ++j) {
+                vrow[j] = __shfl(row, (j < 4 ? 0 : 12) + 4 * g + j);
+                const uint16_t* src = vbase + static_cast<int64_t>(vrow[j] == kNoRow ? 0u : vrow[j]) * 8;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) s[t][i] = s[t][i] * a.scale;
-            if (more) load_k(next);
-            const bool full = t0 + 32 <= least && __all(row != kNoRow);
-            // A row that sees a position has a maximum of at least the lowest number, one that sees
-            // none keeps -inf: its result is 0, while scores that are all -inf give 0 / 0.
-            float floor[CT];
+                for (int s = 0; s < SETS; ++s) {
+                    const int d = PV * li + 128 * s;
+                    const uint16_t* at = src + (EXACT || d < a.head_dim ? d : 0);
+                    if constexpr (PV == 8) {
+                        v[j][s] = past ? __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at))
+                                       : *reinterpret_cast<const u32x4*>(at);
+                    } else {
+                        const u32x2 two = *reinterpret_cast<const u32x2*>(at);
+                        v[j][s] = u32x4{two.x, two.y, 0, 0};
+                    }
+                    if (!EXACT && d >= a.head_dim) v[j][s] = u32x4{0, 0, 0, 0};
+                }
+            }
+        };
+        // eight positions of head value PV s + i of the lane's pieces
+        auto across = [&](int s, int i) {
+            const uint32_t pick = (i & 1) ? 0x07060302u : 0x05040100u;
+            u32x4 t;
 #pragma unroll
-            for (int t = 0; t < CT; ++t) floor[t] = full ? -FLT_MAX : -INFINITY;
-            if (!full) {
+            for (int j = 0; j < 4; ++j) t[j] = __builtin_amdgcn_perm(v[2 * j + 1][s][i >> 1], v[2 * j][s][i >> 1], pick);
+            return t;
+        };
+
+        int t0 = begin + 32 * wave;
+        if (t0 < end) {
+            uint32_t row = row_of(page_of(t0), t0);
+            load_k(row);
+            load_v(row, std::false_type{});
+            int page = page_of(t0 + kUnit);
+            for (; t0 < end; t0 += kUnit) {
+                // past the range: no position is there, every lane reads the cache's first row
+                const uint32_t next = row_of(page, t0 + kUnit);
+                page = page_of(t0 + 2 * kUnit);
+                f32x4 s[CT][2];
 #pragma unroll
                 for (int t = 0; t < CT; ++t)
 #pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        s[t][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int x = 0; x < KS; ++x) s[t][i] = mfma16<BF16>(k[i][x], q[t][x], s[t][i]);
+                    }
+#pragma unroll
+                for (int t = 0; t < CT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) s[t][i] = s[t][i] * a.scale;
+                __builtin_amdgcn_sched_barrier(0);
+                load_k(next);
+                const bool full = t0 + 32 <= least && __all(row != kNoRow);
+                // A row that sees a position has a maximum of at least the lowest number, one that sees
+                // none keeps -inf: its result is 0, while scores that are all -inf give 0 / 0.
+                float floor[CT];
+#pragma unroll
+                for (int t = 0; t < CT; ++t) floor[t] = full ? -FLT_MAX : -INFINITY;
+                if (!full) {
+#pragma unroll
+                    for (int t = 0; t < CT; ++t)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const int pos = t0 + (j < 4 ? 0 : 12) + 4 * g + j;
+                            if (pos >= limit[t] || vrow[j] == kNoRow)
+                                s[t][j >> 2][j & 3] = -INFINITY;
+                            else
+                                floor[t] = -FLT_MAX;
+                        }
+                }
+                u32x4 w[CT];
+#pragma unroll
+                for (int t = 0; t < CT; ++t) {
+                    float top = fmaxf(fmaxf(fmaxf(s[t][0][0], s[t][0][1]), fmaxf(s[t][0][2], s[t][0][3])),
+                                      fmaxf(fmaxf(s[t][1][0], s[t][1][1]), fmaxf(s[t][1][2], s[t][1][3])));
+                    top = fmaxf(m[t], swap_max(fmaxf(top, floor[t])));
+                    const float fade = exp2_from(m[t], top);
+                    m[t] = top;
+                    const float from = (top == -INFINITY ? 0.0f : top) - kBias;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            s[t][i][j] = exp2f(s[t][i][j] - from);
+                            sum += s[t][i][j];
+                        }
+                    l[t] = fmaf(l[t], fade, sum);
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) acc[t][i] = acc[t][i] * fade;
+                    w[t] = u32x4{pack2<BF16>(s[t][0][0], s[t][0][1]), pack2<BF16>(s[t][0][2], s[t][0][3]),
+                                 pack2<BF16>(s[t][1][0], s[t][1][1]), pack2<BF16>(s[t][1][2], s[t][1][3])};
+                }
+                if (!full) {
+                    // What a row does not see has weight 0, but 0 times a NaN or an infinity left there is
+                    // NaN: only what every row sees goes to the matrix cores.
+#pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const int pos = t0 + (j < 4 ? 0 : 12) + 4 * g + j;
-                        if (pos >= limit[t] || vrow[j] == kNoRow)
-                            s[t][j >> 2][j & 3] = -INFINITY;
-                        else
-                            floor[t] = -FLT_MAX;
+                        const uint32_t keep = pos < least && vrow[j] != kNoRow ? 0xFFFFFFFFu : 0u;
+#pragma unroll
+                        for (int x = 0; x < SETS; ++x) v[j][x] = v[j][x] & keep;
                     }
-            }
-            u32x4 w[CT];
-#pragma unroll
-            for (int t = 0; t < CT; ++t) {
-                float top = fmaxf(fmaxf(fmaxf(s[t][0][0], s[t][0][1]), fmaxf(s[t][0][2], s[t][0][3])),
-                                  fmaxf(fmaxf(s[t][1][0], s[t][1][1]), fmaxf(s[t][1][2], s[t][1][3])));
-                top = fmaxf(m[t], swap_max(fmaxf(top, floor[t])));
-                const float fade = exp2_from(m[t], top);
-                m[t] = top;
-                const float from = (top == -INFINITY ? 0.0f : top) - kBias;
-                float sum = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        s[t][i][j] = exp2f(s[t][i][j] - from);
-                        sum += s[t][i][j];
-                    }
-                l[t] = fmaf(l[t], fade, sum);
-#pragma unroll
-                for (int i = 0; i < NV; ++i) acc[t][i] = acc[t][i] * fade;
-                w[t] = u32x4{pack2<BF16>(s[t][0][0], s[t][0][1]), pack2<BF16>(s[t][0][2], s[t][0][3]),
-                             pack2<BF16>(s[t][1][0], s[t][1][1]), pack2<BF16>(s[t][1][2], s[t][1][3])};
-            }
-            if (full) {
+                }
 #pragma unroll
                 for (int x = 0; x < SETS; ++x)
 #pragma unroll
@@ -559,89 +623,124 @@ __global__ __launch_bounds__(64 * kAttnWaves, CT * DP > 128 ? 1 : 2) void paged_
 #pragma unroll
                         for (int t = 0; t < CT; ++t) acc[t][PV * x + i] = mfma16<BF16>(values, w[t], acc[t][PV * x + i]);
                     }
-            } else {
-                // What a row does not see has weight 0, but 0 times a NaN or an infinity left there is
-                // NaN: the values are cleared, row by row as the rows see different positions.
-                for (int r = 0; r < a.rows; ++r) {
-                    const int sees = static_cast<int>(seen_of(length, r + 1, a.capacity));
-                    // the permutes stay in the loop: kept across it they would take as many registers as v
-                    uint32_t low = 0x05040100u, high = 0x07060302u;
-                    asm volatile("" : "+s"(low), "+s"(high));
-                    u32x4 keep;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int pos = t0 + (j < 2 ? 0 : 12) + 4 * g + 2 * j;
-                        keep[j] = (pos < sees && vrow[2 * j] != kNoRow ? 0x0000FFFFu : 0u) |
-                                  (pos + 1 < sees && vrow[2 * j + 1] != kNoRow ? 0xFFFF0000u : 0u);
-                    }
+                // the positions that some of the rows see, at most rows - 1 of them, one at a time
+                for (int pos = max(least, t0); pos < min(t0 + 32, seen); ++pos) {
+                    const uint32_t there = __builtin_amdgcn_readlane(row, pos - t0);
+                    if (there == kNoRow) continue;
+                    const int at = pos - t0, from = (at & 12) * 4 + li;  // the lane that has this column's weight of it
+                    u32x4 value[SETS][4];
+                    const uint16_t* src = vbase + static_cast<int64_t>(there) * 8;
 #pragma unroll
                     for (int x = 0; x < SETS; ++x)
 #pragma unroll
-                        for (int i = 0; i < PV; ++i) {
-                            const u32x4 values = across(x, i, low, high) & keep;
-#pragma unroll
-                            for (int t = 0; t < CT; ++t) {
-                                const int col = col0 + 16 * t + li;
-                                const bool mine = col >= r * a.group && col < (r + 1) * a.group;
-                                const f32x4 sum = mfma16<BF16>(values, w[t], acc[t][PV * x + i]);
-#pragma unroll
-                                for (int j = 0; j < 4; ++j)
-                                    acc[t][PV * x + i][j] = mine ? sum[j] : acc[t][PV * x + i][j];
+                        for (int j = 0; j < 4; ++j) {
+                            const int d = PV * (4 * g + j) + 128 * x;
+                            const uint16_t* piece = src + (EXACT || d < a.head_dim ? d : 0);
+                            if constexpr (PV == 8) {
+                                value[x][j] = *reinterpret_cast<const u32x4*>(piece);
+                            } else {
+                                const u32x2 two = *reinterpret_cast<const u32x2*>(piece);
+                                value[x][j] = u32x4{two.x, two.y, 0, 0};
                             }
-                            __builtin_amdgcn_sched_barrier(0);  // one sum's registers, not all of them
                         }
+#pragma unroll
+                    for (int t = 0; t < CT; ++t) {
+                        float p = s[t][0][0];
+#pragma unroll
+                        for (int j = 1; j < 8; ++j) p = (at >> 4) * 4 + (at & 3) == j ? s[t][j >> 2][j & 3] : p;
+                        p = __shfl(p, from);
+                        const bool sees = pos < limit[t];
+#pragma unroll
+                        for (int x = 0; x < SETS; ++x)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const f32x8 f = widen8<BF16>(value[x][j]);
+#pragma unroll
+                                for (int i = 0; i < PV; ++i) {
+                                    const float was = acc[t][PV * x + i][j];
+                                    acc[t][PV * x + i][j] = sees ? fmaf(p, f[i], was) : was;
+                                }
+                            }
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                if (streamed) {
+                    asm volatile("");  // two sets of loads: merged into one they would all be ordinary ones
+                    load_v(next, std::true_type{});
+                    asm volatile("");
+                } else {
+                    load_v(next, std::false_type{});
+                }
+                row = next;
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < CT; ++t) l[t] = swap_sum(l[t]);
+
+        asm volatile("" : "+v"(again));
+        {
+        const int lane = again, li = again & 15, g = again >> 4;
+        // the waves' parts: 2 and 3 into 0 and 1, then 1 into 0
+#pragma unroll
+        for (int step = 2; step > 0; step >>= 1) {
+            if (wave >= step && wave < 2 * step) {
+                float(*to)[64] = meet[wave - step];
+#pragma unroll
+                for (int t = 0; t < CT; ++t) {
+                    to[t * (NV * 4 + 2)][lane] = m[t];
+                    to[t * (NV * 4 + 2) + 1][lane] = l[t];
+#pragma unroll
+                    for (int i = 0; i < NV; ++i)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) to[t * (NV * 4 + 2) + 2 + 4 * i + j][lane] = acc[t][i][j];
                 }
             }
-            if (more) load_v(next);
-            row = next;
-        }
-    }
+            __syncthreads();
+            if (wave < step) {
+                const float(*from)[64] = meet[wave];
 #pragma unroll
-    for (int t = 0; t < CT; ++t) l[t] = swap_sum(l[t]);
-
-    // the waves' parts: 2 and 3 into 0 and 1, then 1 into 0
+                for (int t = 0; t < CT; ++t) {
+                    const float om = from[t * (NV * 4 + 2)][lane], ol = from[t * (NV * 4 + 2) + 1][lane];
+                    const float top = fmaxf(m[t], om);
+                    const float f0 = exp2_from(m[t], top), f1 = exp2_from(om, top);
+                    m[t] = top;
+                    l[t] = l[t] * f0 + ol * f1;
 #pragma unroll
-    for (int step = 2; step > 0; step >>= 1) {
-        if (wave >= step && wave < 2 * step) {
-            float(*to)[64] = meet[wave - step];
+                    for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int t = 0; t < CT; ++t) {
-                to[t * (NV * 4 + 2)][lane] = m[t];
-                to[t * (NV * 4 + 2) + 1][lane] = l[t];
-#pragma unroll
-                for (int i = 0; i < NV; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) to[t * (NV * 4 + 2) + 2 + 4 * i + j][lane] = acc[t][i][j];
+                        for (int j = 0; j < 4; ++j)
+                            acc[t][i][j] = acc[t][i][j] * f0 + from[t * (NV * 4 + 2) + 2 + 4 * i + j][lane] * f1;
+                }
             }
+            __syncthreads();
         }
-        __syncthreads();
-        if (wave < step) {
-            const float(*from)[64] = meet[wave];
 #pragma unroll
-            for (int t = 0; t < CT; ++t) {
-                const float om = from[t * (NV * 4 + 2)][lane], ol = from[t * (NV * 4 + 2) + 1][lane];
-                const float top = fmaxf(m[t], om);
-                const float f0 = exp2_from(m[t], top), f1 = exp2_from(om, top);
-                m[t] = top;
-                l[t] = l[t] * f0 + ol * f1;
+        for (int t = 0; t < CT; ++t) {
+            const int col = col0 + 16 * t + li;
+            if (wave != 0 || col >= a.columns) continue;
+            if (!whole) {
+                const int64_t at = ((static_cast<int64_t>(run) + seq) * hc_count * CT + hc * CT + t) * 16 + li;
+                if (g == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * at) = f32x2{m[t], l[t]};
+                float* to = a.part + at * a.head_dim;
 #pragma unroll
-                for (int i = 0; i < NV; ++i)
+                for (int s = 0; s < SETS; ++s)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        acc[t][i][j] = acc[t][i][j] * f0 + from[t * (NV * 4 + 2) + 2 + 4 * i + j][lane] * f1;
+                    for (int j = 0; j < 4; ++j) {
+                        const int d = PV * (4 * g + j) + 128 * s;
+                        if (!EXACT && d >= a.head_dim) continue;
+#pragma unroll
+                        for (int i = 0; i < PV; i += 4)
+                            *reinterpret_cast<f32x4*>(to + d + i) =
+                                f32x4{acc[t][PV * s + i][j], acc[t][PV * s + i + 1][j], acc[t][PV * s + i + 2][j],
+                                      acc[t][PV * s + i + 3][j]};
+                    }
+                continue;
             }
-        }
-        __syncthreads();
-    }
-    if (wave != 0) return;
-#pragma unroll
-    for (int t = 0; t < CT; ++t) {
-        const int col = col0 + 16 * t + li;
-        if (col >= a.columns) continue;
-        if (splits > 1) {
-            const int64_t at = (static_cast<int64_t>(blockIdx.x) * CT + t) * 16 + li;
-            if (g == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * at) = f32x2{m[t], l[t]};
-            float* to = a.part + at * a.head_dim;
+            // a row that sees nothing is zero
+            const int r = col / a.group, h = col - r * a.group;
+            const bool empty = m[t] == -INFINITY;
+            const float inv = 1.0f / l[t];
+            uint16_t* to = a.out + ((static_cast<int64_t>(seq) * a.rows + r) * a.heads + kvh * a.group + h) * a.head_dim;
 #pragma unroll
             for (int s = 0; s < SETS; ++s)
 #pragma unroll
@@ -649,36 +748,21 @@ __global__ __launch_bounds__(64 * kAttnWaves, CT * DP > 128 ? 1 : 2) void paged_
                     const int d = PV * (4 * g + j) + 128 * s;
                     if (!EXACT && d >= a.head_dim) continue;
 #pragma unroll
-                    for (int i = 0; i < PV; i += 4)
-                        *reinterpret_cast<f32x4*>(to + d + i) =
-                            f32x4{acc[t][PV * s + i][j], acc[t][PV * s + i + 1][j], acc[t][PV * s + i + 2][j],
-                                  acc[t][PV * s + i + 3][j]};
-                }
-            continue;
-        }
-        // a row that sees nothing is zero
-        const int r = col / a.group, h = col - r * a.group;
-        const bool empty = m[t] == -INFINITY;
-        const float inv = 1.0f / l[t];
-        uint16_t* to = a.out + ((static_cast<int64_t>(seq) * a.rows + r) * a.heads + kvh * a.group + h) * a.head_dim;
+                    for (int i = 0; i < PV; i += 4) {
+                        u32x2 o;
 #pragma unroll
-        for (int s = 0; s < SETS; ++s)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int d = PV * (4 * g + j) + 128 * s;
-                if (!EXACT && d >= a.head_dim) continue;
-#pragma unroll
-                for (int i = 0; i < PV; i += 4) {
-                    u32x2 o;
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const float y0 = empty ? 0.0f : acc[t][PV * s + i + 2 * x][j] * inv;
-                        const float y1 = empty ? 0.0f : acc[t][PV * s + i + 2 * x + 1][j] * inv;
-                        o[x] = pack2<BF16>(y0, y1);
+                        for (int x = 0; x < 2; ++x) {
+                            const float y0 = empty ? 0.0f : acc[t][PV * s + i + 2 * x][j] * inv;
+                            const float y1 = empty ? 0.0f : acc[t][PV * s + i + 2 * x + 1][j] * inv;
+                            o[x] = pack2<BF16>(y0, y1);
+                        }
+                        *reinterpret_cast<u32x2*>(to + d + i) = o;
                     }
-                    *reinterpret_cast<u32x2*>(to + d + i) = o;
                 }
-            }
+        }
+        }
+        unit = before += plan.rounded(units);
+        if (unit < run_end) units = units_of(a.p.lengths[++seq], a.rows, a.capacity);
     }
 }
 
@@ -710,11 +794,13 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const AttnArgs
     __shared__ float red[4];
     const int lane = threadIdx.x & 63;
     const int all = a.rows * a.heads;
-    int seq = blockIdx.x / all;
+    const int seq = blockIdx.x / all;
     const int at = blockIdx.x - seq * all;
     Plan plan;
-    if (!find_plan(a, lane, false, 0, seq, plan) || plan.splits <= 1) return;
-    const int splits = __builtin_amdgcn_readfirstlane(plan.splits);
+    if (!find_plan(a, lane, false, 0, seq, plan)) return;
+    const uint32_t run = plan.run_of(plan.before);
+    const int splits = static_cast<int>(plan.run_of(plan.before + plan.units - 1) - run) + 1;
+    if (splits == 1) return;
     const int r = at / a.heads, head = at - r * a.heads;
     const int kvh = head / a.group, col = r * a.group + head - kvh * a.group;
     const int hc_count = a.kv_heads * a.column_blocks;
@@ -722,7 +808,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const AttnArgs
     const int hc = kvh * a.column_blocks + col / wide;
     // partial of split s: first + s * stride
     const int64_t stride = static_cast<int64_t>(hc_count) * wide;
-    const int64_t first = (static_cast<int64_t>(__builtin_amdgcn_readfirstlane(plan.first)) * hc_count + hc) * wide + col % wide;
+    const int64_t first = (static_cast<int64_t>(run + seq) * hc_count + hc) * wide + col % wide;
     const f32x2* ml = reinterpret_cast<const f32x2*>(a.part_ml) + first;
     float m = -INFINITY;
     for (int s = threadIdx.x; s < splits; s += kJoinThreads) m = fmaxf(m, ml[s * stride][0]);
@@ -813,36 +899,57 @@ void launch_append(const AppendArgs& a, int mode, dim3 grid, dim3 block, hipStre
     }
 }
 
+// A call that reads more than this reads its values past the caches, where they
+// would displace what is read again (the same batch 226 -> 210 us, 5.8 TB/s;
+// calls of 30 to 70 MB, which the last-level cache holds, are 3 % faster without).
+constexpr int64_t kStreamedBytes = static_cast<int64_t>(128) << 20;
+
 struct AttnShape {
     int ct;             // blocks of 16 columns in a workgroup
     int column_blocks;
-    int budget;
-    int64_t items;      // at most
-    bool joined;        // a sequence can have more than one item
-    size_t bytes;       // of partials
+    int64_t budget;     // runs of long sequences
+    int64_t short_runs; // of short ones, about
+    int64_t runs;       // at most
+    bool joined;        // a sequence can be in more than one run
+    int64_t slots;      // of partials
+    size_t bytes;
 };
 
 AttnShape shape_of(int64_t sequences, int64_t rows, int64_t heads, int64_t kv_heads, int64_t head_dim,
                    int64_t capacity) {
     AttnShape s;
     const int64_t columns = rows * (heads / kv_heads);
-    s.ct = columns > 16 && head_dim <= 128 ? 2 : 1;
+    // several blocks of columns share what they read of the cache
+    s.ct = head_dim > 128 || columns <= 16 ? 1 : columns <= 32 ? 2 : 4;
     s.column_blocks = static_cast<int>(plm::ceil_div(columns, 16 * s.ct));
     const int64_t hc = kv_heads * s.column_blocks;
-    s.budget = static_cast<int>(std::max<int64_t>(1, 2 * plm::cu_count() / hc));
     const int64_t units = std::max<int64_t>(1, plm::ceil_div(capacity, kUnit));
-    s.items = std::min(sequences * units, s.budget + sequences);
+    // as many workgroups as the compute units hold at once, and as there are compute units
+    const int resident = head_dim > 128 || s.ct * head_dim > 256 ? 1 : 2;
+    s.budget = std::max<int64_t>(1, resident * plm::cu_count() / hc);
+    s.short_runs = std::max<int64_t>(1, plm::cu_count() / hc);
+    s.runs = std::min(sequences * units, s.budget + std::min(sequences, kShortRuns * s.budget));
     s.joined = units > 1;
-    s.bytes = s.joined ? static_cast<size_t>(s.items) * hc * s.ct * 16 * (head_dim + 2) * sizeof(float) : 0;
+    s.slots = s.joined ? s.runs + sequences : 0;
+    s.bytes = static_cast<size_t>(s.slots) * hc * s.ct * 16 * (head_dim + 2) * sizeof(float);
     return s;
 }
 
 template <bool BF16>
 void launch_attention(const AttnArgs& a, const AttnShape& s, hipStream_t st) {
-    const dim3 grid(static_cast<unsigned>(s.items * a.kv_heads * a.column_blocks)), block(64 * kAttnWaves);
+    const dim3 grid(static_cast<unsigned>(s.runs * a.kv_heads * a.column_blocks)), block(64 * kAttnWaves);
     const int d = a.head_dim;
 #define PLM_ATTN(DP, EXACT, CT) hipLaunchKernelGGL((paged_attention_kernel<BF16, DP, EXACT, CT>), grid, block, 0, st, a)
-    if (s.ct == 2) {
+    if (s.ct == 4) {
+        if (d == 64)
+            PLM_ATTN(64, true, 4);
+        else if (d < 64)
+            PLM_ATTN(64, false, 4);
+        else if (d == 128)
+            PLM_ATTN(128, true, 4);
+        else
+            PLM_ATTN(128, false, 4);
+    } else if (s.ct == 2) {
         if (d == 64)
             PLM_ATTN(64, true, 2);
         else if (d < 64)
@@ -966,8 +1073,8 @@ PLM_EXPORT int kv_paged_attention_decode_u16(const uint16_t* q, const uint16_t* 
         return plm::fail(-2, "query strides and addresses must be multiples of 16 bytes");
     a.capacity = table_cols * page_size;
     const AttnShape s = shape_of(sequences, rows, heads, kv_heads, head_dim, a.capacity);
-    if (s.items * kv_heads * s.column_blocks > kMostInt || sequences * rows * heads > kMostInt)
-        return plm::fail(-2, "too many sequences and heads");
+    if (sequences * plm::ceil_div(a.capacity, kUnit) > kMostInt / 4 || s.runs * kv_heads * s.column_blocks > kMostInt || sequences * rows * heads > kMostInt)
+        return plm::fail(-2, "too many sequences, heads or pages");
     void* part = scratch;
     if (s.bytes > 0) {
         if (scratch == nullptr) {
@@ -989,10 +1096,12 @@ PLM_EXPORT int kv_paged_attention_decode_u16(const uint16_t* q, const uint16_t* 
     a.head_dim = static_cast<int>(head_dim);
     a.columns = a.rows * a.group;
     a.column_blocks = s.column_blocks;
-    a.budget = s.budget;
+    a.budget = static_cast<uint32_t>(s.budget);
+    a.short_runs = static_cast<uint32_t>(s.short_runs);
+    a.streamed = static_cast<uint32_t>(kStreamedBytes / (kUnit * 4 * kv_heads * head_dim));
     a.scale = softmax_scale * 1.44269504088896340736f;
     a.part = static_cast<float*>(part);
-    a.part_ml = a.part + s.items * kv_heads * s.column_blocks * s.ct * 16 * head_dim;
+    a.part_ml = a.part + s.slots * kv_heads * s.column_blocks * s.ct * 16 * head_dim;
     const hipStream_t st = plm::current_stream();
     if (dtype_code == 1)
         launch_attention<true>(a, s, st);
