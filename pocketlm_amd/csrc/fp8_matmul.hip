@@ -271,6 +271,11 @@ __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const Mat
     // this workgroup's blocks
     const int first = static_cast<int>(static_cast<int64_t>(a.blocks) * blockIdx.z / gridDim.z);
     const int blocks = static_cast<int>(static_cast<int64_t>(a.blocks) * (blockIdx.z + 1) / gridDim.z) - first;
+    // Rows a multiple of 4096 bytes apart meet in the same memory channels: there each workgroup starts
+    // at another of its blocks (16 x 7168 x 16384 33.5 -> 27.1 us, 64 rows 39.8 -> 36.4; with more rows the
+    // activations are shared at one block, and 256 rows were 5 % slower).
+    const int turn = T::kM <= 64 && gridDim.y == 1 && (a.k & 4095) == 0 ? static_cast<int>(blockIdx.x % blocks) : 0;
+    auto turned = [&](int b) { return b + turn >= blocks ? b + turn - blocks : b + turn; };
 
     constexpr int kLag = 2;  // matrix instructions between a result and its adds
     // A wave's loads of a block: 8 rows each, LW of the weight's and LX of the activations' (of few
@@ -300,9 +305,10 @@ __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const Mat
     const uint32_t wpast = past(swizzle_w<TN>(wave * 8 + (lane >> 3))), xpast = past(swizzle_x(lane >> 3));
     auto load_part = [&](int b, int i) {
         const bool is_w = i < LW;
-        const uint32_t back = first + b + 1 < a.blocks ? 0u : is_w ? wpast : xpast;
+        const int from = turned(b);
+        const uint32_t back = first + from + 1 < a.blocks ? 0u : is_w ? wpast : xpast;
         const int row = is_w ? (i * T::kWaves + wave) * 8 : T::kN + ((i - LW) * T::kWaves + wave) * 8 % T::kM;
-        load_to_lds((is_w ? wbase : xbase) + static_cast<int64_t>(b) * 128, src[i] - back,
+        load_to_lds((is_w ? wbase : xbase) + static_cast<int64_t>(from) * 128, src[i] - back,
                     lds_at + b % S * T::kStage + row * 128);
     };
     const float* scales = reinterpret_cast<const float*>(lds + S * T::kStage);
@@ -310,7 +316,7 @@ __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const Mat
     const float* xs = a.xs + m0 * a.blocks + first;
     const uint32_t ssrc = static_cast<uint32_t>(min(static_cast<int64_t>((sfirst + lane) % T::kM), a.m - 1 - m0)) * a.blocks * 4;
     auto load_scales = [&](int b) {
-        load4_to_lds(xs + min(b, blocks - 1), ssrc,
+        load4_to_lds(xs + turned(min(b, blocks - 1)), ssrc,
                      lds_at + S * T::kStage + (b % T::kScaleSlots * T::kScales + sfirst) * 4);
     };
     const auto ws = (const __attribute__((address_space(4))) float*)(
@@ -339,11 +345,11 @@ __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const Mat
         }
         load_scales(b + 1);
     }
-    float sw = ws[0];
+    float sw = ws[turned(0)];
     auto block = [&](int b, auto more, auto masked) {
         constexpr bool MORE = decltype(more)::value, MASKED = decltype(masked)::value;
         load_to_lds_barrier<MORE ? S - 1 + (S - 2) * L : 0>();
-        const float next_w = ws[min(b + 1, blocks - 1)];
+        const float next_w = ws[turned(min(b + 1, blocks - 1))];
         const char* stage = lds + b % S * T::kStage;
         const float* sx = scales + b % T::kScaleSlots * T::kScales + xrow;
         auto piece = [&](int at, int h) {
@@ -502,7 +508,7 @@ int launch_tile(const MatmulArgs& a, int shares, hipStream_t st) {
 //          and stores; at least the weight at 5.85 TB/s
 //   shares of the blocks (for grids that leave compute units idle): 3.85 us for
 //          the join, its sums written and read at 3.6 TB/s
-//   rows   its waves' blocks, or the weight at 3.6 TB/s (2.4 above 8 rows)
+//   rows   its waves' blocks, or the weight at 3.6 TB/s (3.0 above 8 rows)
 struct Choice {
     int tile;    // activation rows of a workgroup; 0: the rows kernel
     int shares;  // of the blocks
@@ -525,8 +531,8 @@ Choice choice_of(int64_t m, int64_t n, int64_t k) {
     Choice best = {0, 1};
     double least = 1e30;
     if (m <= kMostRows)
-        least = std::max(3.2 + (m <= 8 ? 0.75 : m <= 16 ? 1.0 : 1.6) * static_cast<double>(plm::ceil_div(blocks, 8)),
-                         3.5 + bytes / (m <= 8 ? 3.6e6 : 2.4e6));
+        least = std::max(3.2 + (m <= 8 ? 0.75 : m <= 16 ? 1.0 : 2.2) * static_cast<double>(plm::ceil_div(blocks, 8)),
+                         3.5 + bytes / (m <= 8 ? 3.6e6 : 3.0e6));
     for (const TileCost& c : kTileCosts) {
         if (c.tile >= 2 * m && c.tile > 16) continue;
         const int64_t tiles = plm::ceil_div(n, c.weight_rows) * plm::ceil_div(m, c.tile);

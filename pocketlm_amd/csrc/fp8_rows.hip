@@ -253,7 +253,7 @@ int run_rows(RowsArgs& a, int dtype_code, bool norm) {
     a.vec = a.cols % kPiece == 0 && whole(a.x, a.x_stride) && whole(a.residual, a.residual_stride) &&
             whole(a.weight, 0) && whole(a.sum, a.cols) && (reinterpret_cast<uintptr_t>(a.out) & 7u) == 0;
     const bool few = a.rows <= 2 * plm::cu_count();
-    int steps = few ? 1 : 4;
+    int steps = few ? 1 : 2;  // 8192 x 7168 bf16: 1 93 us, 2 79 (5.2 TB/s), 4 102
     while (plm::ceil_div(pieces, steps) > kMaxThreads) steps *= 2;
     while (steps > 1 && pieces <= static_cast<int64_t>(64) * (steps / 2)) steps /= 2;
     a.waves = static_cast<int>(plm::ceil_div(plm::ceil_div(pieces, steps), 64));

@@ -34,7 +34,8 @@ def run(nat, x, xs, w, ws, dtype):
 SHAPES = [(1, 576, 7168), (1, 1, 16), (2, 130, 128), (8, 100, 144), (16, 128, 256), (17, 33, 400), (31, 257, 1536),
           (33, 200, 384), (63, 640, 896), (64, 1024, 1040), (65, 96, 272), (100, 513, 2048), (128, 256, 512),
           (129, 384, 4096), (200, 1000, 640), (255, 48, 16384), (257, 300, 1552), (500, 700, 1280), (1, 5000, 128),
-          (300, 129, 130), (7, 40, 1), (5, 3, 137)]
+          (300, 129, 130), (7, 40, 1), (5, 3, 137),
+          (20, 300, 4096), (64, 200, 8192), (12, 400, 16384)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
