@@ -146,7 +146,7 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "fp8_e4m3_quantize_rows": (_i32, [_vp] * 3 + [_i64] * 3 + [_i32]),
     "fp8_e4m3_rms_norm_rows": (_i32, [_vp] * 6 + [_i64] * 4 + [_i32, _f32]),
     "fp8_e4m3_block_matmul": (_i32, [_vp] * 6 + [_i64] * 5 + [_i32]),
-    "fp8_e4m3_block_matmul_scratch_bytes": (_i64, [_i64] * 3),
+    "fp8_e4m3_block_matmul_scratch_bytes": (_i64, [_i64] * 3 + [_i32]),
     "kv_paged_append_u16": (_i32, [_vp] * 11 + [_i64] * 6 + [_i32] + [_i64] * 12 + [_i32]),
     "kv_paged_attention_decode_u16": (_i32, [_vp] * 7 + [_i64] * 15 + [_f32, _i32]),
     "kv_paged_attention_scratch_bytes": (_i64, [_i64] * 6),

@@ -1974,16 +1974,18 @@ def fp8_e4m3_rms_norm_rows(x: torch.Tensor, weight: torch.Tensor, *, rms_eps: fl
 
 
 @functools.lru_cache(maxsize=4096)
-def _matmul_scratch(rows: int, out_rows: int, in_cols: int, device_index: int) -> int:
+def _matmul_scratch(rows: int, out_rows: int, in_cols: int, dtype_code: int, device_index: int) -> int:
     with torch.cuda.device(device_index):
-        return int(_lib.load().fp8_e4m3_block_matmul_scratch_bytes(rows, out_rows, in_cols))
+        return int(_lib.load().fp8_e4m3_block_matmul_scratch_bytes(rows, out_rows, in_cols, dtype_code))
 
 
 def fp8_e4m3_block_matmul(rows: Fp8Rows, fp8_weight: torch.Tensor, scale_inv: torch.Tensor, *,
                           out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """FP8 rows [rows, in_cols] times an FP8 block-scaled weight
     [out_rows, in_cols]: [rows, out_rows] in out_dtype (fp16, bf16 or fp32),
-    summed in fp32.  NaN bytes are NaN on both sides."""
+    summed in fp32 (16-bit results: of products that the matrix cores cut off
+    below 2^-13 of the largest of eight; fp32 results: of exact ones).  NaN
+    bytes are NaN on both sides."""
     lib = _fp8_rows_lib("Native FP8 matmul")
     x, xs = rows
     code = _ROW_CODES.get(out_dtype)
@@ -2016,7 +2018,7 @@ def fp8_e4m3_block_matmul(rows: Fp8Rows, fp8_weight: torch.Tensor, scale_inv: to
     device = x.device
     out = torch.empty((m, n), dtype=out_dtype, device=device)
     if m and n:
-        nbytes = _matmul_scratch(m, n, k, index)
+        nbytes = _matmul_scratch(m, n, k, code, index)
         scratch = torch.empty((nbytes,), dtype=torch.uint8, device=device) if nbytes else None
         _call(lib, index, "fp8_e4m3_block_matmul", x_ptr, xs.data_ptr(), w_ptr, scale_inv.data_ptr(), out.data_ptr(),
               None if scratch is None else scratch.data_ptr(), nbytes, m, n, k, blocks, code)

@@ -46,13 +46,22 @@ def matmul(x, xs, w, ws):
     return xf @ wf.t(), xf.abs() @ wf.abs().t()
 
 
-def matmul_bound(want, size, cols, dtype):
+def matmul_bound(want, size, x, xs, w, ws, dtype):
     """A sum in fp32 of blocks of 128 products, each step off by at most a
     whole step (2^-23: matrix instructions cut off rather than round) of the
     magnitudes' sum: 128 in a block, the scale's two products, one for each
-    block and each join; then the output's rounding."""
-    steps = 128 + 4 + (cols + 127) // 128 + 32
-    off = steps * 2.0 ** -23 * size
+    block and each join.  For a 16-bit result seven of each eight products of
+    adjacent columns are also off by up to 2^-13 of the largest one's power of
+    two (at most the product of the eights' largest values).  Then the output's
+    rounding."""
+    k, n = x.shape[1], w.shape[0]
+    off = (128 + 4 + (k + 127) // 128 + 32) * 2.0 ** -23 * size
+    if dtype != torch.float32:
+        def largest(t, scales):
+            t = torch.nn.functional.pad(t.view(torch.float8_e4m3fn).double().abs(), (0, -k % 8))
+            return t.unflatten(1, (-1, 8)).amax(2) * scales.double().repeat_interleave(16, dim=1)[:, :(k + 7) // 8]
+
+        off = off + 7 * 2.0 ** -13 * (largest(x, xs) @ largest(w, ws.repeat_interleave(128, dim=0)[:n]).t())
     return off + HALF[dtype] * (want.abs() + off) + TINY[dtype]
 
 

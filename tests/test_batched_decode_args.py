@@ -44,8 +44,12 @@ def test_matmul_codes(lib):
         assert call(**{name: N}) == -1
     for bad in (dict(m=0), dict(n=-1), dict(k=0), dict(k=129), dict(code=3), dict(m=1 << 31), dict(n=1 << 31), dict(x=ODD), dict(w=ODD)):
         assert call(**bad) == -2
-    assert lib.fp8_e4m3_block_matmul_scratch_bytes(0, 1, 1) == -2
-    assert lib.fp8_e4m3_block_matmul_scratch_bytes(1, 16, 128) >= 0
+    assert lib.fp8_e4m3_block_matmul_scratch_bytes(0, 1, 1, 1) == -2
+    assert lib.fp8_e4m3_block_matmul_scratch_bytes(1, 1, 1, 3) == -2
+    need = lib.fp8_e4m3_block_matmul_scratch_bytes(64, 7168, 16384, 1)
+    assert need > 0
+    assert call(m=64, n=7168, k=16384, sc=128, scratch=A, nbytes=need - 1) == -3
+    assert call(m=64, n=7168, k=16384, sc=128, scratch=ODD, nbytes=need) == -3
 
 
 def append(lib, q=A, k=A, v=A, q_out=A, kc=A, vc=A, table=A, lengths=A, starts=N, freq=A, rejected=N, rows=2, seqs=2,

@@ -45,14 +45,14 @@ def test_against_64_bits(nat, dtype, m, n, k):
     got = run(nat, x, xs, w, ws, dtype)
     assert got.dtype == dtype and got.shape == (m, n)
     want, size = ref.matmul(x, xs, w, ws)
-    ref.within(got, want, ref.matmul_bound(want, size, k, dtype))
+    ref.within(got, want, ref.matmul_bound(want, size, x, xs, w, ws, dtype))
 
 
 @pytest.mark.parametrize("m,n,k", [(600, 2304, 1024), (1025, 1100, 528), (2048, 512, 896)])
 def test_prompts(nat, m, n, k):
     x, xs, w, ws = make(m, n, k, m)
     want, size = ref.matmul(x, xs, w, ws)
-    ref.within(run(nat, x, xs, w, ws, torch.bfloat16), want, ref.matmul_bound(want, size, k, torch.bfloat16))
+    ref.within(run(nat, x, xs, w, ws, torch.bfloat16), want, ref.matmul_bound(want, size, x, xs, w, ws, torch.bfloat16))
 
 
 def test_whole_numbers_are_exact(nat):
@@ -67,12 +67,27 @@ def test_whole_numbers_are_exact(nat):
         assert torch.equal(run(nat, x, xs, w, ws, torch.float32).cpu().double(), want)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("m", [3, 20, 60, 120, 400])
+def test_outliers_that_cancel(nat, m, dtype):
+    """Columns of large values that cancel each other: fp32 results keep the
+    small ones, 16-bit results what the matrix cores leave of them."""
+    n, k = 260, 2048
+    x, xs, w, ws = make(m, n, k, m)
+    xf, wf = x.float() / 60, w.float()
+    xf[:, 5::128], xf[:, 70::128] = 448.0, -448.0
+    wf[:, 70::128] = wf[:, 5::128]
+    x, w = xf.to(torch.float8_e4m3fn), wf.to(torch.float8_e4m3fn)
+    want, size = ref.matmul(x, xs, w, ws)
+    ref.within(run(nat, x, xs, w, ws, dtype), want, ref.matmul_bound(want, size, x, xs, w, ws, dtype))
+
+
 @pytest.mark.parametrize("m", [1, 20, 50, 90, 300])
 def test_nan_rows_weights_and_scales_stay_where_they_are(nat, m):
     n, k = 200, 656
     x, xs, w, ws = make(m, n, k, 21)
     want, size = ref.matmul(x, xs, w, ws)
-    bound = ref.matmul_bound(want, size, k, torch.bfloat16)
+    bound = ref.matmul_bound(want, size, x, xs, w, ws, torch.bfloat16)
     xb, wb, xs2 = x.view(torch.uint8).clone(), w.view(torch.uint8).clone(), xs.clone()
     wb[17, k - 1] = 0x7F
     wb[199, 0] = 0xFF
@@ -102,7 +117,7 @@ def test_offset_and_strided_operands(nat):
     exact, size = ref.matmul(x, xs, w, ws)
     # an odd address: copied first
     ref.within(nat.fp8_e4m3_block_matmul(nat.Fp8Rows(x.cuda(), xs.cuda()), odd, ws.cuda(), out_dtype=torch.float32),
-               exact, ref.matmul_bound(exact, size, k, torch.float32))
+               exact, ref.matmul_bound(exact, size, x, xs, w, ws, torch.float32))
     assert nat.fp8_e4m3_block_matmul(nat.Fp8Rows(x.cuda()[:0], xs.cuda()[:0]), w.cuda(), ws.cuda()).shape == (0, n)
 
 

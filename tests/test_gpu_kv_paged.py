@@ -326,8 +326,9 @@ def test_decode_steps_one_after_another(nat, dtype, rows):
         at = [b + i * rows if b >= 0 else -1 for b in before]
         lengths[3] = -1
         s = step(x, r, lengths)
-        want, size = ref.matmul(s["normed"].data.cpu(), s["normed"].scales.cpu(), step.qkv[0].cpu(), step.qkv[1].cpu())
-        ref.within(s["qkv"], want, ref.matmul_bound(want, size, step.hidden, dtype), "qkv")
+        given = [t.cpu() for t in (*s["normed"], *step.qkv)]
+        want, size = ref.matmul(*given)
+        ref.within(s["qkv"], want, ref.matmul_bound(want, size, *given, dtype), "qkv")
         qkv = s["qkv"].cpu()
         parts = qkv.split([step.heads * step.dim, step.kvh * step.dim, step.kvh * step.dim], 1)
         q, k, v = (t.unflatten(1, (-1, step.dim)) for t in parts)
@@ -347,8 +348,9 @@ def test_decode_steps_one_after_another(nat, dtype, rows):
         want, bound = ref.attention(s["q"].cpu().view(5, rows, step.heads, step.dim), step.k.cpu(), step.v.cpu(),
                                     step.table.cpu(), at, step.dim ** -0.5)
         ref.within(s["heads"], want, bound, "attention")
-        want, size = ref.matmul(s["back"].data.cpu(), s["back"].scales.cpu(), step.o[0].cpu(), step.o[1].cpu())
-        ref.within(s["out"], want, ref.matmul_bound(want, size, step.heads * step.dim, dtype), "out")
+        given = [t.cpu() for t in (*s["back"], *step.o)]
+        want, size = ref.matmul(*given)
+        ref.within(s["out"], want, ref.matmul_bound(want, size, *given, dtype), "out")
 
 
 def test_a_captured_step_follows_its_lengths(nat):
