@@ -130,6 +130,14 @@ __device__ __forceinline__ int pack4(float a, float b, float c, float d) {
     return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, v, true);
 }
 
+// y / scale: the reciprocal's product and one correction by its remainder, so
+// that the value that is rounded to e4m3 has been rounded once (values on a
+// border between two e4m3 values are common where both operands are 16-bit).
+__device__ __forceinline__ float quotient(float y, float scale, float inv) {
+    const float q = y * inv;
+    return fmaf(fmaf(-q, scale, y), inv, q);
+}
+
 // Quantizes the piece of block c / 16 that the 16 lanes of a DPP row hold.
 __device__ __forceinline__ void quantize_piece(const RowsArgs& a, int64_t row, int64_t c, const f32x8 y) {
     uint32_t m = 0;
@@ -143,8 +151,11 @@ __device__ __forceinline__ void quantize_piece(const RowsArgs& a, int64_t row, i
     if ((c & 15) == 0) a.scales[row * a.blocks + (c >> 4)] = scale;
     int lo = 0x7F7F7F7F, hi = 0x7F7F7F7F;
     if (finite) {
-        lo = pack4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
-        hi = pack4(y[4] * inv, y[5] * inv, y[6] * inv, y[7] * inv);
+        float q[kPiece];
+#pragma unroll
+        for (int i = 0; i < kPiece; ++i) q[i] = quotient(y[i], scale, inv);
+        lo = pack4(q[0], q[1], q[2], q[3]);
+        hi = pack4(q[4], q[5], q[6], q[7]);
     }
     uint8_t* p = a.out + row * a.cols + c * kPiece;
     if (a.vec) {

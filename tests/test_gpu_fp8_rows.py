@@ -57,6 +57,18 @@ def test_norm_and_quantize_against_the_definition(nat, dtype, rows, cols):
     check_rows(nat.fp8_e4m3_quantize_rows(x.cuda()), x.double(), 0.0)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_quotients_are_rounded_once(nat, dtype):
+    """Bytes are those of the fp32 quotient by the scale (half a step of fp32, then of
+    e4m3): with 16-bit values many quotients lie on a border between two bytes."""
+    x = randn((400, 2048), dtype, 9)
+    got = nat.fp8_e4m3_quantize_rows(x.cuda())
+    scales = got.scales.cpu()
+    assert torch.equal(scales, ref.pad_blocks(x.float()).abs().amax(-1) / 448)
+    want = (x.double() / ref.widen_scales(scales.double(), 2048)).float().clamp(-448, 448)
+    assert torch.equal(got.data.cpu().float(), want.to(torch.float8_e4m3fn).float())
+
+
 def test_rows_do_not_depend_on_the_batch(nat):
     """A row's bytes are the same alone (one workgroup of many waves) and in a
     long prompt (few waves) up to the order of its sum of squares; without the
