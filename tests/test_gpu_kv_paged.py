@@ -199,6 +199,26 @@ def test_attention_splits(nat, sequences, longest):
     check_attention(nat, lengths, 1, 64, 2, 1, 64, torch.bfloat16, seed=sequences, hide=sequences < 100)
 
 
+@pytest.mark.parametrize("share", [1, 2])
+@pytest.mark.parametrize("dtype,kvh,group,dim,rows", [
+    (torch.bfloat16, 64, 1, 64, 1), (torch.float16, 64, 3, 64, 5), (torch.bfloat16, 64, 10, 64, 2),
+    (torch.bfloat16, 64, 17, 64, 3), (torch.float16, 32, 4, 128, 1), (torch.bfloat16, 32, 9, 128, 2),
+    (torch.float16, 32, 33, 128, 1), (torch.bfloat16, 64, 2, 80, 1), (torch.bfloat16, 16, 3, 256, 1),
+    (torch.float16, 16, 2, 256, 4)])
+def test_attention_runs_across_sequences(nat, share, dtype, kvh, group, dim, rows):
+    """Many heads and enough positions that a workgroup's run goes on from one
+    sequence into the next; in whole (share 1) also more than the cache holds,
+    so that the values pass it by."""
+    lengths = [n // share for n in (2500, 0, 127, 2099, -20, 128, 900, 1, 3000)]
+    check_attention(nat, lengths, rows, 64, kvh * group, kvh, dim, dtype, seed=dim + rows)
+
+
+def test_attention_runs_across_many_sequences(nat):
+    lengths = [(37 * b) % 190 - 3 for b in range(90)]
+    check_attention(nat, lengths, 1, 16, 128, 64, 64, torch.bfloat16, seed=4)
+    check_attention(nat, lengths, 2, 16, 64, 32, 128, torch.float16, seed=5)
+
+
 def test_attention_leaves_out_bad_pages(nat):
     def spoil(table):
         table[0, 1] = -1
