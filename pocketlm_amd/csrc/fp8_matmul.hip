@@ -246,9 +246,9 @@ struct Tile {
     static constexpr int kWaves = GN * GM;
     static constexpr int kN = 16 * TN * GN, kM = 16 * TM * GM;
     static constexpr int kStage = (kN + kM) * 128;  // bytes of a block's operands
-    static constexpr int kScales = kM < 64 ? 64 : kM;
-    static constexpr int kScaleSlots = S < 4 ? 4 : 8;  // of kScales row scales: more than S blocks ahead
-    static constexpr int kLds = S * kStage + kScaleSlots * kScales * 4;
+    static constexpr int kScales = kM / kWaves;        // of a block's row scales, a wave's
+    static constexpr int kScaleSlots = S < 4 ? 4 : 8;  // of kM row scales: more than S blocks ahead
+    static constexpr int kLds = S * kStage + kScaleSlots * kM * 4;
 };
 
 // Eight results in the output's 16-bit type.
@@ -270,18 +270,30 @@ __device__ __forceinline__ int swizzle_w(int row) {
 __device__ __forceinline__ int swizzle_x(int row) { return row & 7; }
 
 // 16 bytes a lane from base + offset to LDS, the wave's KB in lane order at
-// `to`.  Not the compiler's builtin: it waits for every load to LDS before any
-// read of LDS, also of the other stage.  The wait is load_to_lds_wait's.
+// `to`; ONCE: past the caches.  Not the compiler's builtin: it waits for every
+// load to LDS before any read of LDS, also of the other stage.  The wait is
+// load_to_lds_barrier's.
+template <bool ONCE>
 __device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-                 :
-                 : "v"(offset), "s"(base), "s"(to)
-                 : "memory");
+    if constexpr (ONCE)
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt"
+                     :
+                     : "v"(offset), "s"(base), "s"(to)
+                     : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                     :
+                     : "v"(offset), "s"(base), "s"(to)
+                     : "memory");
 }
+// Four bytes each of the first LANES lanes.  All lanes are active before and after.
+template <int LANES>
 __device__ __forceinline__ void load4_to_lds(const void* base, uint32_t offset, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
+    static_assert(LANES < 64, "a mask of 64 bits");
+    asm volatile("s_mov_b32 m0, %2\n\ts_mov_b64 exec, %3\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1\n\t"
+                 "s_mov_b64 exec, -1"
                  :
-                 : "v"(offset), "s"(base), "s"(to)
+                 : "v"(offset), "s"(base), "s"(to), "s"((1ull << LANES) - 1)
                  : "memory");
 }
 // Until all but the last LEFT of the wave's loads to LDS are there, then until
@@ -292,7 +304,7 @@ __device__ __forceinline__ void load_to_lds_barrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
 }
 
-template <int TN, int TM, int GN, int GM, int S, bool EXACT>
+template <int TN, int TM, int GN, int GM, int S, bool EXACT, bool ONCE>
 __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const MatmulArgs a) {
     using T = Tile<TN, TM, GN, GM, S>;
     extern __shared__ char lds[];
@@ -306,8 +318,8 @@ __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const Mat
     const int first = static_cast<int>(static_cast<int64_t>(a.blocks) * blockIdx.z / gridDim.z);
     const int blocks = static_cast<int>(static_cast<int64_t>(a.blocks) * (blockIdx.z + 1) / gridDim.z) - first;
     // Rows a multiple of 4096 bytes apart meet in the same memory channels: there each workgroup starts
-    // at another of its blocks (16 x 7168 x 16384 33.5 -> 27.1 us, 64 rows 39.8 -> 36.4; with more rows the
-    // activations are shared at one block, and 256 rows were 5 % slower).
+    // at another of its blocks (16 x 7168 x 16384 33.5 -> 27.1 us, 64 rows 39.8 -> 36.4 when this was
+    // tried; with more rows the activations are shared at one block, and 256 rows were 5 % slower).
     const int turn = T::kM <= 64 && gridDim.y == 1 && (a.k & 4095) == 0 ? static_cast<int>(blockIdx.x % blocks) : 0;
     auto turned = [&](int b) { return b + turn >= blocks ? b + turn - blocks : b + turn; };
 
@@ -342,16 +354,22 @@ __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const Mat
         const int from = turned(b);
         const uint32_t back = first + from + 1 < a.blocks ? 0u : is_w ? wpast : xpast;
         const int row = is_w ? (i * T::kWaves + wave) * 8 : T::kN + ((i - LW) * T::kWaves + wave) * 8 % T::kM;
-        load_to_lds((is_w ? wbase : xbase) + static_cast<int64_t>(from) * 128, src[i] - back,
-                    lds_at + b % S * T::kStage + row * 128);
+        const uint32_t to = lds_at + b % S * T::kStage + row * 128;
+        if (is_w)
+            load_to_lds<ONCE>(wbase + static_cast<int64_t>(from) * 128, src[i] - back, to);
+        else
+            load_to_lds<false>(xbase + static_cast<int64_t>(from) * 128, src[i] - back, to);
     };
     const float* scales = reinterpret_cast<const float*>(lds + S * T::kStage);
-    const int sfirst = wave * 64 % T::kScales;
+    // Each wave its part of the rows' scales: they lie a row's blocks apart, so each is a cache line of its
+    // own, and the lines are what the loads take (all of them by every wave: 64 x 7168 x 16384 36.9 us, now
+    // 33.0; 1024 x 7168 x 7168 76, now 67).
+    const int sfirst = wave * T::kScales;
     const float* xs = a.xs + m0 * a.blocks + first;
-    const uint32_t ssrc = static_cast<uint32_t>(min(static_cast<int64_t>((sfirst + lane) % T::kM), a.m - 1 - m0)) * a.blocks * 4;
+    const uint32_t ssrc = static_cast<uint32_t>(min(static_cast<int64_t>(sfirst + lane % T::kScales), a.m - 1 - m0)) * a.blocks * 4;
     auto load_scales = [&](int b) {
-        load4_to_lds(xs + turned(min(b, blocks - 1)), ssrc,
-                     lds_at + S * T::kStage + (b % T::kScaleSlots * T::kScales + sfirst) * 4);
+        load4_to_lds<T::kScales>(xs + turned(min(b, blocks - 1)), ssrc,
+                                 lds_at + S * T::kStage + (b % T::kScaleSlots * T::kM + sfirst) * 4);
     };
     const auto ws = (const __attribute__((address_space(4))) float*)(
         a.ws + (min(n0 + 16 * TN * wn, a.n - 1) >> 7) * a.scale_cols + first);
@@ -385,7 +403,7 @@ __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const Mat
         load_to_lds_barrier<MORE ? S - 1 + (S - 2) * L : 0>();
         const float next_w = ws[turned(min(b + 1, blocks - 1))];
         const char* stage = lds + b % S * T::kStage;
-        const float* sx = scales + b % T::kScaleSlots * T::kScales + xrow;
+        const float* sx = scales + b % T::kScaleSlots * T::kM + xrow;
         auto piece = [&](int at, int h) {
             plm_u32x4 v = *reinterpret_cast<const plm_u32x4*>(stage + at);
             if constexpr (MASKED) {  // columns past the end
@@ -506,15 +524,22 @@ __global__ __launch_bounds__(256) void fp8_matmul_join_kernel(const MatmulArgs a
         if (n + e < a.n) store_out(a, m * a.n + n + e, v[e]);
 }
 
-template <int TN, int TM, int GN, int GM, int S, bool EXACT = false>
+// A weight of this size is not in the caches when the next call reads it (other weights come between), and
+// few rows read it once: its loads leave the caches to the activations.  64, 24 and 16 rows with 7168 x 16384:
+// 33.0, 27.9, 27.3 us without, 31.7, 25.7, 24.4 with; 64 x 7168 x 7168 18.9 without, 19.7 with.
+constexpr int64_t kStreamedBytes = static_cast<int64_t>(64) << 20;
+
+template <int TN, int TM, int GN, int GM, int S, bool EXACT = false, bool ONCE = false>
 int launch_tile(const MatmulArgs& a, int shares, hipStream_t st) {
+    if constexpr (!ONCE && 16 * TM * GM <= 64)
+        if (a.n * a.k >= kStreamedBytes) return launch_tile<TN, TM, GN, GM, S, EXACT, true>(a, shares, st);
     using T = Tile<TN, TM, GN, GM, S>;
     const int64_t gx = plm::ceil_div(a.n, T::kN), gy = plm::ceil_div(a.m, T::kM);
     if (gx > 0x7FFFFFFF || gy > 65535) return plm::fail(-2, "too many rows");
-    const void* fn = reinterpret_cast<const void*>(&fp8_matmul_tile_kernel<TN, TM, GN, GM, S, EXACT>);
+    const void* fn = reinterpret_cast<const void*>(&fp8_matmul_tile_kernel<TN, TM, GN, GM, S, EXACT, ONCE>);
     int code = T::kLds > 64 * 1024 ? plm::allow_large_lds(fn, T::kLds) : 0;
     if (code != 0) return code;
-    hipLaunchKernelGGL((fp8_matmul_tile_kernel<TN, TM, GN, GM, S, EXACT>),
+    hipLaunchKernelGGL((fp8_matmul_tile_kernel<TN, TM, GN, GM, S, EXACT, ONCE>),
                        dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy), static_cast<unsigned>(shares)),
                        dim3(64 * T::kWaves), T::kLds, st, a);
     code = plm::check_launch("fp8_e4m3_block_matmul");

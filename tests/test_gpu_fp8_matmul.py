@@ -55,6 +55,18 @@ def test_prompts(nat, m, n, k):
     ref.within(run(nat, x, xs, w, ws, torch.bfloat16), want, ref.matmul_bound(want, size, x, xs, w, ws, torch.bfloat16))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m", [12, 16, 30, 64])
+@pytest.mark.parametrize("k", [16384, 16400])
+def test_weights_larger_than_the_caches(nat, m, k, dtype):
+    n = 4200
+    x, xs, w, ws = make(m, n, k, m)
+    got = run(nat, x, xs, w, ws, dtype)
+    for rows, grid in ((slice(0, 128), ws[:1]), (slice(4096, n), ws[32:])):
+        want, size = ref.matmul(x, xs, w[rows], grid)
+        ref.within(got[:, rows], want, ref.matmul_bound(want, size, x, xs, w[rows], grid, dtype))
+
+
 def test_whole_numbers_are_exact(nat):
     """Small whole numbers and scales that are powers of two: every sum is exact."""
     g = torch.Generator().manual_seed(9)
