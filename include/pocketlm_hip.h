@@ -811,9 +811,9 @@ int fp8_e4m3_rms_norm_rows(const void* x, const void* residual, const void* weig
  * others are copied to padded rows first).  fp32 results are sums of exact
  * products; for 16-bit results the matrix cores add the products of eight
  * adjacent columns at a time, each cut off below 2^-13 of the largest one's
- * power of two.  NaN bytes are
- * NaN, in the weight too (the fp8_e4m3_block_linear family counts them as 0,
- * as the reference's decoder does).  scratch: device memory of at least
+ * power of two.  NaN bytes are NaN, in the weight too (the
+ * fp8_e4m3_block_linear family counts them as 0, as the reference's decoder
+ * does).  scratch: device memory of at least
  * fp8_e4m3_block_matmul_scratch_bytes, 16-byte aligned, or NULL for the
  * library's own.  Codes -1 null, -2 bad dimensions, -3 scratch. */
 int fp8_e4m3_block_matmul(const uint8_t* x, const float* x_scales, const uint8_t* fp8_weight, const float* scale_inv,
@@ -829,7 +829,7 @@ int64_t fp8_e4m3_block_matmul_scratch_bytes(int64_t rows, int64_t out_rows, int6
  * [sequences][table_cols]).  lengths int32 [sequences]: the positions a
  * sequence holds before the call's rows; negative for an idle sequence.
  * head_dim is a multiple of 8 up to 256; addresses are 16-byte aligned; a
- * cache spans at most 64 GiB; table_cols * page_size < 2^31.
+ * cache spans at most 64 GiB; table_cols * page_size <= 2^31 - 1024.
  *
  * Appends `rows` rows of keys and values [rows][kv_heads][head_dim] (strides
  * in values, multiples of 8) and rotates them and the queries

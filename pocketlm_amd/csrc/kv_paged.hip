@@ -855,6 +855,8 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const AttnArgs
 // ---------------------------------------------------------------- host side
 
 constexpr int64_t kMostInt = 0x7FFFFFFF;
+// Positions are ints, and the attention looks two units ahead of its last one.
+constexpr int64_t kMostPositions = kMostInt - 1023;
 
 // The checks and layout that both calls share; 0, or the code of the failure.
 int pages_of(Pages& p, void* k_cache, void* v_cache, const int* page_table, const int* lengths, int64_t sequences,
@@ -864,7 +866,7 @@ int pages_of(Pages& p, void* k_cache, void* v_cache, const int* page_table, cons
         return plm::fail(-1, "null pointer");
     if (sequences <= 0 || table_cols <= 0 || num_pages <= 0 || page_size <= 0 || kv_heads <= 0 || head_dim <= 0 ||
         sequences > 65535 || kv_heads > 65535 || num_pages > kMostInt || page_size > kMostInt ||
-        table_cols > kMostInt / page_size || (dtype_code != 0 && dtype_code != 1))
+        table_cols > kMostPositions / page_size || (dtype_code != 0 && dtype_code != 1))
         return plm::fail(-2, "bad dimensions");
     if (head_dim % 8 != 0 || head_dim > 256) return plm::fail(-2, "head_dim must be a multiple of 8 up to 256");
     if (page_stride < 0 || slot_stride < 0 || head_stride < 0 || page_stride % 8 != 0 || slot_stride % 8 != 0 ||
@@ -1048,7 +1050,7 @@ PLM_EXPORT int kv_paged_append_u16(const uint16_t* q, const uint16_t* k, const u
 PLM_EXPORT int64_t kv_paged_attention_scratch_bytes(int64_t sequences, int64_t rows, int64_t heads, int64_t kv_heads,
                                                     int64_t head_dim, int64_t capacity) {
     if (sequences <= 0 || sequences > 65535 || bad_heads(rows, heads, kv_heads) || head_dim <= 0 || head_dim > 256 ||
-        capacity <= 0 || capacity > kMostInt)
+        capacity <= 0 || capacity > kMostPositions)
         return plm::fail(-2, "bad dimensions");
     return static_cast<int64_t>(shape_of(sequences, rows, heads, kv_heads, head_dim, capacity).bytes);
 }
@@ -1073,7 +1075,8 @@ PLM_EXPORT int kv_paged_attention_decode_u16(const uint16_t* q, const uint16_t* 
         return plm::fail(-2, "query strides and addresses must be multiples of 16 bytes");
     a.capacity = table_cols * page_size;
     const AttnShape s = shape_of(sequences, rows, heads, kv_heads, head_dim, a.capacity);
-    if (sequences * plm::ceil_div(a.capacity, kUnit) > kMostInt / 4 || s.runs * kv_heads * s.column_blocks > kMostInt || sequences * rows * heads > kMostInt)
+    if (sequences * plm::ceil_div(a.capacity, kUnit) > kMostInt / 4 ||
+        s.runs * kv_heads * s.column_blocks > kMostInt || sequences * rows * heads > kMostInt)
         return plm::fail(-2, "too many sequences, heads or pages");
     void* part = scratch;
     if (s.bytes > 0) {

@@ -2102,7 +2102,7 @@ def kv_paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_
             raise ValueError("q must have shape [rows, heads, head_dim]")
         heads = q_shape[1]
     if row_starts is None:
-        if sequences == 0 or rows % sequences:
+        if rows % sequences if sequences else rows:
             raise ValueError("rows must be a multiple of the sequences (or give row_starts)")
     elif row_starts.dtype != torch.int32:
         raise TypeError("row_starts must be torch.int32")

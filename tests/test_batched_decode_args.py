@@ -64,7 +64,8 @@ def test_append_codes(lib):
         assert append(lib, **{name: N}) == -1, name
     for bad in (dict(rows=0), dict(rows=3), dict(seqs=0), dict(seqs=65536, rows=65536), dict(kvh=0), dict(dim=0),
                 dict(dim=12, pairs=0), dict(dim=264), dict(pairs=33), dict(pairs=-1), dict(cols=0), dict(pages=0),
-                dict(page=0), dict(code=2), dict(cols=1 << 20, page=1 << 12), dict(heads=-1), dict(kc=ODD), dict(q=ODD),
+                dict(page=0), dict(code=2), dict(cols=1 << 20, page=1 << 12), dict(cols=1 << 21, page=1 << 10),
+                dict(cols=(1 << 31) - 1023, page=1), dict(heads=-1), dict(kc=ODD), dict(q=ODD),
                 dict(cache=(2048, 128, 4)), dict(cache=(-8, 128, 64)), dict(pages=1 << 30, cache=(1 << 10, 128, 64)),
                 dict(strides=(256, 64, 128, 64, 130, 64)), dict(strides=(256, -64, 128, 64, 128, 64))):
         assert append(lib, **bad) == -2, bad
@@ -91,6 +92,10 @@ def test_attention_codes(lib):
     assert lib.kv_paged_attention_scratch_bytes(2, 1, 4, 2, 64, 128) == 0  # one split at most
     assert lib.kv_paged_attention_scratch_bytes(2, 9, 4, 2, 64, 128) == -2
     assert lib.kv_paged_attention_scratch_bytes(2, 1, 4, 2, 64, 0) == -2
+    # positions are ints with room for two units behind the last
+    assert lib.kv_paged_attention_scratch_bytes(1, 1, 4, 2, 64, 2 ** 31 - 1024) > 0
+    assert lib.kv_paged_attention_scratch_bytes(1, 1, 4, 2, 64, 2 ** 31 - 1023) == -2
+    assert attention(lib, cols=1 << 21, page=1 << 10) == -2
 
 
 @pytest.fixture

@@ -283,6 +283,51 @@ def test_attention_other_orders(nat):
     ref.within(shared[:, :1], want[:, :1, 0], bound[:, :1, 0])
 
 
+def test_offsets_past_32_bits(nat):
+    """Pages behind the 2^32nd value of a cache that holds keys and values."""
+    page, kvh, dim, heads, lengths = 16, 4, 128, 8, [40, 3, -1, 77]
+    pages = 2 ** 32 // (page * kvh * dim) + 1000
+    both = torch.empty((pages, 2, page, kvh, dim), dtype=torch.bfloat16, device="cuda")
+    k, v = both[:, 0], both[:, 1]
+    small_k, small_v, small = ref.make_pages([x + 1 for x in lengths], page, kvh, dim, torch.bfloat16, 12)
+    at = pages - 1 - 7 * torch.arange(small_k.shape[0])
+    k[at], v[at] = small_k.cuda(), small_v.cuda()
+    table = torch.where(small >= 0, at[small.clamp(min=0).long()].int(), small)
+    g = torch.Generator().manual_seed(13)
+    new = torch.randn((4, kvh, dim), generator=g).bfloat16()
+    q = torch.randn((4, heads, dim), generator=g).bfloat16()
+    got_q = nat.kv_paged_append(q.cuda(), new.cuda(), -new.cuda(), k, v, table.cuda(), i32(lengths))
+    for b, n in enumerate(lengths):
+        if n >= 0:
+            small_k[int(small[b, n // page]), n % page], small_v[int(small[b, n // page]), n % page] = new[b], -new[b]
+    assert torch.equal(k[at].cpu(), small_k) and torch.equal(v[at].cpu(), small_v)
+    want, bound = ref.attention(q[:, None], small_k, small_v, small, lengths, dim ** -0.5)
+    got = nat.kv_paged_attention_decode(got_q, k, v, table.cuda(), i32(lengths))
+    ref.within(got, want[:, 0], bound[:, 0])
+
+
+def test_attention_at_far_positions(nat):
+    """A sequence of 2^30 positions of which the last page alone is there."""
+    page, dim, far = 2 ** 16, 64, 2 ** 30 + 100
+    g = torch.Generator().manual_seed(14)
+    k, v = (torch.randn((1, page, 1, dim), generator=g).half() for _ in range(2))
+    q = torch.randn((1, 2, dim), generator=g).half()
+    table = torch.full((1, far // page + 1), -1, dtype=torch.int32)
+    table[0, -1] = 0
+    want, bound = ref.attention(q[:, None], k, v, torch.zeros((1, 1), dtype=torch.int32), [100], dim ** -0.5)
+    got = nat.kv_paged_attention_decode(q.cuda(), k.cuda(), v.cuda(), table.cuda(), i32([far]))
+    ref.within(got, want[:, 0], bound[:, 0])
+
+
+def test_no_sequences(nat):
+    cache = torch.zeros((2, 4, 1, 16), dtype=torch.float16, device="cuda")
+    none = torch.empty((0, 1, 16), dtype=torch.float16, device="cuda")
+    table, lengths = torch.empty((0, 3), dtype=torch.int32, device="cuda"), i32([])
+    got = nat.kv_paged_append(none, none, none, cache, cache.clone(), table, lengths)
+    assert got.shape == (0, 1, 16)
+    assert nat.kv_paged_attention_decode(got, cache, cache.clone(), table, lengths).shape == (0, 1, 16)
+
+
 def test_attention_the_library_s_own_scratch(nat):
     from pocketlm_amd import _lib
 
