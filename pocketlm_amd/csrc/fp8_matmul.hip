@@ -114,7 +114,9 @@ __device__ __forceinline__ plm_f32x4 block_sums(const Operand<true>& a, const Op
 // waves take the K blocks w, w + nw, ... and their sums meet in LDS, added in
 // wave order.  Lane l holds, of weight row (activation row) l & 15, the bytes
 // 16 (l >> 4) .. + 15 of each half of a block: the same columns on both
-// sides, which is all that the inner sum needs.
+// sides, which is all that the inner sum needs.  Operands go straight to
+// registers, P blocks ahead; bound by the latency of the few loads a wave has
+// (1 x 576 x 7168 6.6 us, 1 x 4096 x 4096 5.9).
 template <int TA, int TB, int P, int MAXW, bool EXACT>
 __global__ __launch_bounds__(64 * MAXW) void fp8_matmul_rows_kernel(const MatmulArgs a) {
     extern __shared__ plm_f32x4 red[];  // [wave][tile][lane]
@@ -223,8 +225,8 @@ int launch_rows(const MatmulArgs& a, int waves, hipStream_t st) {
         const int code = plm::allow_large_lds(fn, MAXW * TA * TB * 1024);
         if (code != 0) return code;
     }
-    hipLaunchKernelGGL((fp8_matmul_rows_kernel<TA, TB, P, MAXW, EXACT>), dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy)),
-                       dim3(static_cast<unsigned>(64 * waves)), static_cast<unsigned>(bytes), st, a);
+    const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(gy)), block(static_cast<unsigned>(64 * waves));
+    hipLaunchKernelGGL((fp8_matmul_rows_kernel<TA, TB, P, MAXW, EXACT>), grid, block, static_cast<unsigned>(bytes), st, a);
     return plm::check_launch("fp8_e4m3_block_matmul");
 }
 
@@ -241,6 +243,12 @@ int launch_rows(const MatmulArgs& a, int waves, hipStream_t st) {
 // their addresses that are permuted.  Weight tile i of a wave holds the rows
 // 4 TN (r / 4) + 4 i + r % 4: a lane then has 4 TN adjacent results of an
 // output row.
+//
+// Bound by the weight's bytes up to 64 rows (64 x 7168 x 16384 31.8 us with
+// the join, 3.8 TB/s: every workgroup also reads its 64 rows, half as many
+// bytes again, through the same cache) and by the matrix cores from 256 x 256
+// tiles on: 4096 x 7168 x 16384 420 us, 2290 TFLOP/s, of which 448 tiles on 256
+// compute units leave an eighth unused.
 template <int TN, int TM, int GN, int GM, int S>
 struct Tile {
     static constexpr int kWaves = GN * GM;
@@ -338,7 +346,8 @@ __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const Mat
         const bool is_w = i < LW;
         const int r = ((is_w ? i : i - LW) * T::kWaves + wave) * 8 % (is_w ? T::kN : T::kM) + (lane >> 3);
         const int f = is_w ? swizzle_w<TN>(r) : swizzle_x(r);
-        const int last = static_cast<int>(min((is_w ? a.n : a.m) - 1 - (is_w ? n0 : m0), static_cast<int64_t>(T::kN + T::kM)));
+        const int64_t left = is_w ? a.n - 1 - n0 : a.m - 1 - m0;
+        const int last = static_cast<int>(min(left, static_cast<int64_t>(T::kN + T::kM)));
         src[i] = static_cast<uint32_t>(min(r, last)) * static_cast<uint32_t>(a.k) + 16 * ((lane & 7) ^ f);
     }
     const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
@@ -366,7 +375,8 @@ __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const Mat
     // 33.0; 1024 x 7168 x 7168 76, now 67).
     const int sfirst = wave * T::kScales;
     const float* xs = a.xs + m0 * a.blocks + first;
-    const uint32_t ssrc = static_cast<uint32_t>(min(static_cast<int64_t>(sfirst + lane % T::kScales), a.m - 1 - m0)) * a.blocks * 4;
+    const int64_t srow = min(static_cast<int64_t>(sfirst + lane % T::kScales), a.m - 1 - m0);
+    const uint32_t ssrc = static_cast<uint32_t>(srow) * a.blocks * 4;
     auto load_scales = [&](int b) {
         load4_to_lds<T::kScales>(xs + turned(min(b, blocks - 1)), ssrc,
                                  lds_at + S * T::kStage + (b % T::kScaleSlots * T::kM + sfirst) * 4);
@@ -422,8 +432,8 @@ __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const Mat
 #pragma unroll
         for (int at = 0; at < TN * TM + kLag; ++at) {
             const int i = at % TN, j = at / TN;
-            // A later block's loads go out two at a time: all at once they hold up the first products (one
-            // row of 256 x 256 tiles 526 us, two at a time 414, one 477).
+            // A later block's loads go out two at a time: all at once they hold up the first products
+            // (4096 x 7168 x 16384 all at once 526 us, two 414, one 477 when this was tried).
             if (MORE && i == 0) {
                 constexpr int kAtOnce = 2 * TM >= L ? 2 : L;
 #pragma unroll
@@ -512,6 +522,7 @@ __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const Mat
 }
 
 // The shares' sums in their order, rounded once.  A thread: four columns.
+// Bound by its launch: 4 shares of 64 x 7168 5 us.
 __global__ __launch_bounds__(256) void fp8_matmul_join_kernel(const MatmulArgs a, int shares) {
     const int64_t n4 = (a.n + 3) / 4;
     const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;

@@ -169,7 +169,10 @@ __device__ __forceinline__ void quantize_piece(const RowsArgs& a, int64_t row, i
 
 // `waves` waves per row, several rows a workgroup where a row is short; a
 // thread keeps its NS pieces of the sum in registers between the two passes,
-// so every value is read once.
+// so every value is read once (8 pieces, rows above 32768 columns, spill).
+// Bound by memory: 8192 x 7168 bf16 with a residual 80 us, 5.2 TB/s.  One row
+// of 7168, 3.6 us, and 509 rows of 3584, 5.3 us, are the launch, a trip to
+// memory and the workgroup's sum.
 template <int DT, int NS, bool NORM>
 __global__ __launch_bounds__(kMaxThreads) void fp8_rows_kernel(const RowsArgs a) {
     using T = typename Row<DT>::T;

@@ -109,7 +109,10 @@ constexpr int kAppendThreads = 256;
 // Workgroup (row, part of the row's heads): the angles of the row's position
 // once per workgroup (their reduction to one turn in 64 bits: a position of
 // 10^6 has its angle to 10^-10), then one unit a thread: 8 pairs of a head
-// (16 values), or 8 values of it in the modes for any size.
+// (16 values), or 8 values of it in the modes for any size.  The row's values
+// are on their way while its sequence, page and angles are found.  Bound by
+// that chain for a step (64 rows of 28 and 2 x 4 heads of 128 3.6 us), by
+// memory for prompts (6800 such rows, 125 MB moved, 25 us, 4.9 TB/s).
 template <bool BF16, int MODE>
 __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(const AppendArgs a) {
     __shared__ float cs[128], sn[128];
@@ -411,13 +414,20 @@ constexpr uint32_t kNoRow = 0xFFFFFFFFu;
 //
 // Weights are rounded to the cache's type for the second product (their sum is
 // not): at most 2^-8 (2^-11) of each, of either sign, so less in their sum than
-// the output's own rounding.  In fp16 they are kept times 2^15, so that a weight is only lost
-// below 2^-40 of the row's largest.
+// the output's own rounding.  In fp16 they are kept times 2^15, so that a
+// weight is only lost below 2^-40 of the row's largest.
+//
+// Bound by the cache's bytes in large batches: 48 sequences of 8000 to 16000
+// positions, 4 key-value heads of 128, 1.2 GB 211 us with the join, 5.8 TB/s.
+// Small calls are a chain of trips to memory, lengths, table, keys and values,
+// then the join: 700 positions 7 + 5 us, 6 sequences of up to 5000 positions
+// with 4 rows each, 49 MB, 17 + 5 us.
 //
 // DP: head_dim rounded up to 64, 128 or 256; EXACT: no rounding.  CT: blocks
 // of 16 columns.
 template <bool BF16, int DP, bool EXACT, int CT>
-__global__ __launch_bounds__(64 * kAttnWaves, DP > 128 || CT * DP > 256 ? 1 : 2) void paged_attention_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(64 * kAttnWaves, DP > 128 || CT * DP > 256 ? 1 : 2) void paged_attention_kernel(
+    const AttnArgs a) {
     constexpr int KS = DP / 32;               // score steps of 32 head values
     constexpr int NV = DP / 16;               // value instructions
     constexpr int PV = DP == 64 ? 4 : 8;      // adjacent head values of a lane
@@ -768,8 +778,10 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 || CT * DP > 256 ? 1 : 2)
 
 // Joins the splits of a sequence, a workgroup per query row and head.  Its
 // threads first take the splits' maxima and sums (the weights of the splits go
-// to LDS), then each a quad of head values of every kSets-th split, and the
-// sets meet in LDS.  Sequences of one split were written already.
+// to LDS), then each a quad of head values of every sets-th split, and the
+// sets meet in LDS.  Sequences of one split were written already.  Bound by its
+// launch and three trips to memory: 28 to 672 workgroups 5 to 6 us, 48 x 28
+// with 4 partials on average 7.5.
 constexpr int kJoinThreads = 256;
 constexpr int kJoinSplits = 1024;  // at a time
 
