@@ -244,19 +244,27 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(const Appe
 // ---------------------------------------------------------------- attention
 //
 // A unit is 128 positions of a sequence (an idle or empty one has one unit,
-// whose result is the zeros).  The units of all sequences, one after another,
-// are dealt to the workgroups of a key-value head in equal runs, on the device
-// from the lengths: no launch, copy or host value depends on them, and ragged
-// batches stay balanced (48 sequences of 8000 to 16000 positions, 4 heads of 128:
-// 253 -> 228 us against runs that end with their sequence).  A run
-// that holds a sequence's every unit writes its result; the others write a
-// partial, in slot run + sequence, which grows by at least one from partial to
-// partial.
+// whose result is the zeros).  The units are dealt to the workgroups of a
+// key-value head on the device, from the lengths: no launch, copy or host value
+// depends on them.  Where no sequence is much longer than the others' share,
+// or all are short, each has a workgroup of its own (Plan::single; 300 of up to
+// 250 positions, 4 heads of 128: 29 us, 59 in runs).  Otherwise the units of
+// all sequences, one after another, make equal runs, so that ragged batches stay
+// balanced (48 sequences of 8000 to 16000 positions: 253 -> 228 us against runs
+// that end with their sequence).  A run that holds a sequence's every unit
+// writes its result; the others write a partial, in slot run + sequence, which
+// grows by at least one from partial to partial.
 
 constexpr int kUnit = 128;
 constexpr int kAttnWaves = 4;
 constexpr int kMaxQueryRows = 8;
 constexpr uint32_t kShortRuns = 4;  // units for each run, below which sequences are short
+constexpr uint32_t kFewUnits = 4;   // of a sequence that a workgroup takes alone whatever the others are
+// Where such workgroups fill the device, a sequence may have 1.5 times the equal share of a run and 12 units:
+// runs that cross sequences and their joins cost more than that much unevenness (4 heads of 128; alone / in
+// runs, us: 64 of up to 1000 positions 24 / 35, 4000 79 / 82, 16000 291 / 271; 300 of 250 29 / 50, of 3000
+// 236 / 254; 63 of 100 and one of 4096 47 / 15).
+constexpr uint32_t kUnevenHalves = 3, kUnevenUnits = 12;
 
 struct AttnArgs {
     Pages p;
@@ -264,6 +272,7 @@ struct AttnArgs {
     uint16_t* out;     // [sequences][rows][heads][head_dim]
     float* part;       // [slot][head and column block][column][head_dim], then the maxima and sums
     float* part_ml;
+    uint4* plan;       // {total, runs, align, single}, then {before, units} of each sequence (uint2); null: no join
     int64_t q_seq, q_row, q_head;  // strides, values
     int64_t capacity;  // positions of a table row
     int rows;
@@ -275,6 +284,8 @@ struct AttnArgs {
     int column_blocks;
     uint32_t budget;      // runs of long sequences
     uint32_t short_runs;  // runs of short ones, about
+    int single;           // no table row holds more than a few units: each sequence has a workgroup
+    int wide;             // a workgroup for each sequence fills the device
     uint32_t streamed;    // units from which on the values are read past the caches
     float scale;       // softmax scale * log2(e)
 };
@@ -306,11 +317,14 @@ struct Plan {
     uint32_t total;   // units of all sequences, each rounded up to whole multiples of `align`
     uint32_t runs;
     uint32_t align;
+    bool single;      // run r is sequence r
     int seq;
     uint32_t before;  // units of the sequences before seq, rounded
     uint32_t units;   // of seq
 
-    __device__ __forceinline__ uint32_t rounded(uint32_t n) const { return (n + align - 1) / align * align; }
+    __device__ __forceinline__ uint32_t rounded(uint32_t n) const {
+        return align == 1 ? n : (n + align - 1) / align * align;
+    }
     // run * total / runs
     __device__ __forceinline__ uint32_t start(uint32_t run) const {
         const uint32_t each = total / runs;
@@ -323,41 +337,80 @@ struct Plan {
     }
 };
 
-// The plan, at the sequence that holds the first unit of run `run` (by_run),
-// or at sequence `seq`.  Every lane of a wave calls it; false for a run past
-// the last.
-__device__ __forceinline__ bool find_plan(const AttnArgs& a, int lane, bool by_run, uint32_t run, int seq, Plan& plan) {
-    // a lane's sequence of each 64: the first 64 are read once
-    const uint32_t n0 = lane < a.p.sequences ? units_of(a.p.lengths[lane], a.rows, a.capacity) : 0;
+// Of the lanes of a wave (lane 63 has it).
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+#define PLM_MAX(ctrl, rows) \
+    v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), ctrl, rows, 0xF, false)))
+    PLM_MAX(0x111, 0xF);
+    PLM_MAX(0x112, 0xF);
+    PLM_MAX(0x114, 0xF);
+    PLM_MAX(0x118, 0xF);
+    PLM_MAX(0x142, 0xA);
+    PLM_MAX(0x143, 0xC);
+#undef PLM_MAX
+    return __builtin_amdgcn_readlane(v, 63);
+}
+
+// The plan, at the sequence that holds the first unit of run `run`.  Every lane
+// of a wave calls it; false for a run past the last.
+__device__ __forceinline__ bool find_plan(const AttnArgs& a, int lane, uint32_t run, Plan& plan) {
+    // a lane's sequence of each 64: the first 512 are read at once
+    constexpr int kHeld = 8;
+    uint32_t held[kHeld];
+#pragma unroll
+    for (int c = 0; c < kHeld; ++c) {
+        held[c] = 0;
+        if (64 * c < a.p.sequences) {
+            const int i = 64 * c + lane;
+            held[c] = i < a.p.sequences ? units_of(a.p.lengths[i], a.rows, a.capacity) : 0;
+        }
+    }
     auto units_at = [&](int base) {
-        if (base == 0) return n0;
         const int i = base + lane;
         return i < a.p.sequences ? units_of(a.p.lengths[i], a.rows, a.capacity) : 0;
     };
+    uint32_t longest = 0;
     auto sum = [&] {
-        uint32_t total = 0;
-        for (int base = 0; base < a.p.sequences; base += 64)
-            total += __builtin_amdgcn_readlane(wave_prefix(plan.rounded(units_at(base))), 63);
-        return total;
+        uint32_t mine = 0;
+#pragma unroll
+        for (int c = 0; c < kHeld; ++c) {
+            if (64 * c >= a.p.sequences) break;
+            mine += plan.rounded(held[c]);
+            longest = max(longest, held[c]);
+        }
+        for (int base = 64 * kHeld; base < a.p.sequences; base += 64) {
+            const uint32_t n = units_at(base);
+            mine += plan.rounded(n);
+            longest = max(longest, n);
+        }
+        return static_cast<uint32_t>(__builtin_amdgcn_readlane(wave_prefix(mine), 63));
     };
-    // Long sequences: `budget` equal runs, as many as there is room for.  Short ones: runs of `align`
-    // units that end with their sequence (starting on another costs more than a unit or two), as many as
-    // there are compute units (their partials cost as well).
+    // A workgroup for each sequence; or, of long sequences, `budget` equal runs, as many as there is room
+    // for; or, of short ones, runs of `align` units that end with their sequence (starting on another costs
+    // more than a unit or two), as many as there are compute units (their partials cost as well).
     plan.align = 1;
     plan.total = sum();
-    plan.runs = a.budget;
-    if (plan.total < kShortRuns * a.budget) {
+    longest = wave_max(longest);
+    const uint64_t most = 2 * kUnevenUnits * a.budget + kUnevenHalves * static_cast<uint64_t>(plan.total);
+    plan.single = longest <= kFewUnits || (a.wide != 0 && 2 * static_cast<uint64_t>(longest) * a.budget <= most);
+    plan.runs = plan.single ? a.p.sequences : a.budget;
+    if (!plan.single && plan.total < kShortRuns * a.budget) {
         plan.align = max(1u, (plan.total + a.short_runs - 1) / a.short_runs);
         if (plan.align > 1) plan.total = sum();
         plan.runs = plan.total / plan.align;
     }
-    if (by_run && run >= plan.runs) return false;
-    const uint32_t unit = by_run ? plan.start(run) : 0;
+    if (run >= plan.runs) return false;
+    if (plan.single) {
+        plan.seq = static_cast<int>(run);
+        plan.before = 0;
+        plan.units = units_of(a.p.lengths[run], a.rows, a.capacity);
+        return true;
+    }
+    const uint32_t unit = plan.start(run);
     uint32_t before = 0;
-    for (int base = 0; base < a.p.sequences; base += 64) {
-        const uint32_t n = units_at(base);
+    auto found = [&](int base, uint32_t n) {
         const uint32_t upto = wave_prefix(plan.rounded(n));
-        const unsigned long long past = by_run ? __ballot(before + upto > unit) : __ballot(base + lane == seq);
+        const unsigned long long past = __ballot(before + upto > unit);
         if (past != 0) {
             const int at = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
             plan.seq = base + at;
@@ -366,7 +419,13 @@ __device__ __forceinline__ bool find_plan(const AttnArgs& a, int lane, bool by_r
             return true;
         }
         before += __builtin_amdgcn_readlane(upto, 63);
-    }
+        return false;
+    };
+#pragma unroll
+    for (int c = 0; c < kHeld; ++c)
+        if (64 * c < a.p.sequences && found(64 * c, held[c])) return true;
+    for (int base = 64 * kHeld; base < a.p.sequences; base += 64)
+        if (found(base, units_at(base))) return true;
     return false;
 }
 
@@ -440,16 +499,29 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 || CT * DP > 256 ? 1 : 2)
     const int run = blockIdx.x / hc_count, hc = blockIdx.x - run * hc_count;
     const int kvh = hc / a.column_blocks, col0 = (hc - kvh * a.column_blocks) * 16 * CT;
     Plan plan;
-    if (!find_plan(a, lane, true, static_cast<uint32_t>(run), 0, plan)) return;
-    const uint32_t run_end = plan.start(run + 1);
+    uint32_t unit = 0, run_end;
+    if (a.single != 0) {
+        plan.align = 1;
+        plan.seq = run;
+        plan.before = 0;
+        plan.units = units_of(a.p.lengths[run], a.rows, a.capacity);
+        plan.total = plan.units * static_cast<uint32_t>(a.p.sequences);  // about
+        run_end = plan.units;
+    } else {
+        if (!find_plan(a, lane, static_cast<uint32_t>(run), plan)) return;
+        unit = plan.single ? 0 : plan.start(run);
+        run_end = plan.single ? plan.units : plan.start(run + 1);
+        if (blockIdx.x == 0 && threadIdx.x == 0) *a.plan = make_uint4(plan.total, plan.runs, plan.align, plan.single);
+    }
     const bool streamed = EXACT && DP >= 128 && plan.total >= a.streamed;
-    uint32_t unit = plan.start(run);
+    const bool noted = a.single == 0 && !plan.single && hc == 0 && threadIdx.x == 0;
     int seq = plan.seq;
     uint32_t before = plan.before;
     uint32_t units = plan.units;
     while (unit < run_end) {  // a sequence of the run's
         const int length = a.p.lengths[seq];
         const int seen = static_cast<int>(seen_of(length, a.rows, a.capacity));
+        if (noted && unit == before) reinterpret_cast<uint2*>(a.plan + 1)[seq] = make_uint2(before, units);
         const bool whole = unit == before && run_end >= before + units;
         const int begin = static_cast<int>(unit - before) * kUnit;
         const int end = min(seen, static_cast<int>(min(run_end - before, units)) * kUnit);
@@ -804,14 +876,19 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const AttnArgs
     __shared__ float weights[kJoinSplits];
     __shared__ f32x4 sums[kJoinThreads];
     __shared__ float red[4];
-    const int lane = threadIdx.x & 63;
     const int all = a.rows * a.heads;
     const int seq = blockIdx.x / all;
     const int at = blockIdx.x - seq * all;
+    // as the first kernel left it; of no sequence where each had a workgroup
+    const uint4 noted = *a.plan;
+    const uint2 own = reinterpret_cast<const uint2*>(a.plan + 1)[seq];
+    if (noted.w != 0) return;
     Plan plan;
-    if (!find_plan(a, lane, false, 0, seq, plan)) return;
-    const uint32_t run = plan.run_of(plan.before);
-    const int splits = static_cast<int>(plan.run_of(plan.before + plan.units - 1) - run) + 1;
+    plan.total = noted.x;
+    plan.runs = noted.y;
+    plan.align = noted.z;
+    const uint32_t run = plan.run_of(own.x);
+    const int splits = static_cast<int>(plan.run_of(own.x + own.y - 1) - run) + 1;
     if (splits == 1) return;
     const int r = at / a.heads, head = at - r * a.heads;
     const int kvh = head / a.group, col = r * a.group + head - kvh * a.group;
@@ -924,6 +1001,8 @@ struct AttnShape {
     int64_t budget;     // runs of long sequences
     int64_t short_runs; // of short ones, about
     int64_t runs;       // at most
+    bool single;        // a run for each sequence
+    bool wide;          // such runs fill the device
     bool joined;        // a sequence can be in more than one run
     int64_t slots;      // of partials
     size_t bytes;
@@ -942,10 +1021,14 @@ AttnShape shape_of(int64_t sequences, int64_t rows, int64_t heads, int64_t kv_he
     const int resident = head_dim > 128 || s.ct * head_dim > 256 ? 1 : 2;
     s.budget = std::max<int64_t>(1, resident * plm::cu_count() / hc);
     s.short_runs = std::max<int64_t>(1, plm::cu_count() / hc);
-    s.runs = std::min(sequences * units, s.budget + std::min(sequences, kShortRuns * s.budget));
-    s.joined = units > 1;
-    s.slots = s.joined ? s.runs + sequences : 0;
+    s.single = units <= kFewUnits;
+    s.wide = sequences * hc >= plm::cu_count();
+    const int64_t shared = std::min(sequences * units, s.budget + std::min(sequences, kShortRuns * s.budget));
+    s.runs = s.single ? sequences : std::max(sequences, shared);
+    s.joined = !s.single;
+    s.slots = s.joined ? shared + sequences : 0;
     s.bytes = static_cast<size_t>(s.slots) * hc * s.ct * 16 * (head_dim + 2) * sizeof(float);
+    if (s.joined) s.bytes += sizeof(uint4) + sizeof(uint2) * sequences;
     return s;
 }
 
@@ -1113,10 +1196,14 @@ PLM_EXPORT int kv_paged_attention_decode_u16(const uint16_t* q, const uint16_t* 
     a.column_blocks = s.column_blocks;
     a.budget = static_cast<uint32_t>(s.budget);
     a.short_runs = static_cast<uint32_t>(s.short_runs);
+    a.single = s.single ? 1 : 0;
+    a.wide = s.wide ? 1 : 0;
     a.streamed = static_cast<uint32_t>(kStreamedBytes / (kUnit * 4 * kv_heads * head_dim));
     a.scale = softmax_scale * 1.44269504088896340736f;
     a.part = static_cast<float*>(part);
     a.part_ml = a.part + s.slots * kv_heads * s.column_blocks * s.ct * 16 * head_dim;
+    // whole vectors of 16 bytes before it: 16 columns or more of head_dim + 2 values
+    a.plan = s.joined ? reinterpret_cast<uint4*>(a.part_ml + s.slots * kv_heads * s.column_blocks * s.ct * 32) : nullptr;
     const hipStream_t st = plm::current_stream();
     if (dtype_code == 1)
         launch_attention<true>(a, s, st);

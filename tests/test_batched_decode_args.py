@@ -89,7 +89,8 @@ def test_attention_codes(lib):
     assert need > 0
     assert attention(lib, scratch=A, nbytes=need - 1) == -3
     assert attention(lib, scratch=ODD, nbytes=need) == -3
-    assert lib.kv_paged_attention_scratch_bytes(2, 1, 4, 2, 64, 128) == 0  # one split at most
+    assert lib.kv_paged_attention_scratch_bytes(2, 1, 4, 2, 64, 512) == 0  # a workgroup for each sequence
+    assert lib.kv_paged_attention_scratch_bytes(2, 1, 4, 2, 64, 513) > 0
     assert lib.kv_paged_attention_scratch_bytes(2, 9, 4, 2, 64, 128) == -2
     assert lib.kv_paged_attention_scratch_bytes(2, 1, 4, 2, 64, 0) == -2
     # positions are ints with room for two units behind the last

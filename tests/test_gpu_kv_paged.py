@@ -147,9 +147,9 @@ def test_append_into_other_orders(nat):
 # ---------------------------------------------------------------- attention
 
 def check_attention(nat, lengths, rows, page, heads, kvh, dim, dtype, *, seed=0, scale=None, spoil=None, hide=True,
-                    values=1.0):
+                    values=1.0, room=1):
     seen = [max(0, x + rows) for x in lengths]
-    k_cache, v_cache, table = ref.make_pages(seen, page, kvh, dim, dtype, seed)
+    k_cache, v_cache, table = ref.make_pages(seen, page, kvh, dim, dtype, seed, extra_cols=-(-room // page))
     v_cache *= values
     if spoil is not None:
         spoil(table)
@@ -182,8 +182,9 @@ def test_attention_lengths_and_heads(nat, dtype, heads, kvh, dim):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("rows", [2, 3, 5, 8])
 @pytest.mark.parametrize("heads,kvh,dim", [(7, 1, 128), (4, 4, 64), (8, 2, 256), (12, 2, 96)])
-def test_attention_of_several_rows(nat, dtype, rows, heads, kvh, dim):
-    check_attention(nat, [0, 1, 29, 60, 125, -8, 333], rows, 8, heads, kvh, dim, dtype, seed=rows)
+@pytest.mark.parametrize("longest", [333, 813])
+def test_attention_of_several_rows(nat, dtype, rows, heads, kvh, dim, longest):
+    check_attention(nat, [0, 1, 29, 60, 125, -8, longest], rows, 8, heads, kvh, dim, dtype, seed=rows)
 
 
 @pytest.mark.parametrize("page", [1, 3, 8, 31, 100, 256, 1024])
@@ -209,14 +210,35 @@ def test_attention_runs_across_sequences(nat, share, dtype, kvh, group, dim, row
     """Many heads and enough positions that a workgroup's run goes on from one
     sequence into the next; in whole (share 1) also more than the cache holds,
     so that the values pass it by."""
-    lengths = [n // share for n in (2500, 0, 127, 2099, -20, 128, 900, 1, 3000)]
+    lengths = [n // share for n in (5200, 0, 127, 99, -20, 128, 900, 1, 3000)]
     check_attention(nat, lengths, rows, 64, kvh * group, kvh, dim, dtype, seed=dim + rows)
 
 
 def test_attention_runs_across_many_sequences(nat):
     lengths = [(37 * b) % 190 - 3 for b in range(90)]
+    lengths[40] = 9000
     check_attention(nat, lengths, 1, 16, 128, 64, 64, torch.bfloat16, seed=4)
     check_attention(nat, lengths, 2, 16, 64, 32, 128, torch.float16, seed=5)
+
+
+@pytest.mark.parametrize("rows", [1, 3])
+def test_attention_many_sequences_alone(nat, rows):
+    """Each sequence is one workgroup's: all short, in tables of any length, and
+    so many that the device is full."""
+    lengths = [(53 * b) % 400 - 20 for b in range(70)]
+    check_attention(nat, lengths, rows, 16, 4, 1, 128, torch.bfloat16, seed=6)
+    check_attention(nat, lengths, rows, 16, 4, 1, 128, torch.float16, seed=6, room=2000)
+    lengths = [(211 * b) % 1400 - 20 for b in range(40)]
+    check_attention(nat, lengths, rows, 16, 16, 8, 64, torch.bfloat16, seed=7)
+
+
+@pytest.mark.parametrize("kvh,longest", [(1, 3000), (8, 6000), (2, 40)])
+def test_attention_of_more_than_512_sequences(nat, kvh, longest):
+    lengths = [(7 * b) % 45 - 2 for b in range(620)]
+    lengths[570] = longest
+    check_attention(nat, lengths, 1, 16, 2 * kvh, kvh, 64, torch.bfloat16, seed=8)
+    lengths[570], lengths[2] = 5, longest
+    check_attention(nat, lengths, 1, 16, 2 * kvh, kvh, 64, torch.float16, seed=9, room=600)
 
 
 def test_attention_leaves_out_bad_pages(nat):
@@ -333,6 +355,7 @@ def test_attention_the_library_s_own_scratch(nat):
 
     lib = _lib.load()
     k, v, table = (t.cuda() for t in ref.make_pages([900, 300], 16, 2, 64, torch.bfloat16, 5))
+    assert lib.kv_paged_attention_scratch_bytes(2, 1, 4, 2, 64, 16 * table.shape[1]) > 0
     q = torch.randn((2, 4, 64), device="cuda").bfloat16()
     lengths = i32([899, 299])
     want = nat.kv_paged_attention_decode(q, k, v, table, lengths)
@@ -445,6 +468,28 @@ def test_a_captured_step_follows_its_lengths(nat):
         assert torch.equal(held["out"], want["out"]) and torch.equal(held["heads"], want["heads"])
         assert torch.equal(captured.k, eager.k) and torch.equal(glen, elen)
         torch.randn((64, 64), device="cuda").matmul(torch.randn((64, 64), device="cuda"))
+
+
+def test_a_captured_attention_follows_its_lengths(nat):
+    """One graph over short, ragged, long and idle sequences in turn: each deal
+    of the units, from the lengths that the replay finds."""
+    sequences, dim = 40, 64
+    k, v, table = ref.make_pages([1500] * sequences, 16, 8, dim, torch.bfloat16, 31)
+    q = torch.randn((sequences, 16, dim), generator=torch.Generator().manual_seed(32)).bfloat16()
+    dk, dv, dtable, dq, lengths = k.cuda(), v.cuda(), table.cuda(), q.cuda(), i32([7] * sequences)
+    nat.kv_paged_attention_decode(dq, dk, dv, dtable, lengths)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = nat.kv_paged_attention_decode(dq, dk, dv, dtable, lengths)
+    for now in ([9] * sequences, [1499] + [3] * 39, [300 + 30 * b for b in range(40)], [-1] * 39 + [1200],
+                [-1] * sequences, [1499] * 3 + [100] * 37, [1400] * sequences):
+        lengths.copy_(i32(now))
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        want, bound = ref.attention(q[:, None], k, v, table, now, dim ** -0.5)
+        ref.within(out, want[:, 0], bound[:, 0])
+        assert torch.equal(out, nat.kv_paged_attention_decode(dq, dk, dv, dtable, lengths))
 
 
 def test_two_captured_graphs_at_once(nat):
