@@ -563,7 +563,8 @@ int launch_tile(const MatmulArgs& a, int shares, hipStream_t st) {
 // How a product runs, from its sizes alone: the least of the times (us, an
 // MI355X) that these straight lines give, fitted to 860 timings of 139 shapes
 // of 1 to 4096 rows, 134 to 24576 weight rows and 544 to 16384 columns (the
-// choice is 2 % slower than the fastest of all that were timed, 13 % at worst).
+// choice is 2 % slower than the fastest of all that were timed, 13 % at worst;
+// on 800 other shapes 2.3 %).
 //   tile   a workgroup's time per K block, alone on its compute unit or two on
 //          one, for the rounds that the grid takes; 8 us for launch, first loads
 //          and stores; at least the weight at 5.85 TB/s
@@ -684,12 +685,17 @@ PLM_EXPORT int fp8_e4m3_block_matmul(const uint8_t* x, const float* x_scales, co
         }
     }
     const int waves = std::min(8, a.blocks);
+    // Tiles of 128 rows: two workgroups fit a compute unit with two stages each; where there is one for each,
+    // it takes three (300 x 3000 x 16000 44 -> 36 us, 256 x 7168 x 16384 68 -> 63).
+    const bool alone = plm::ceil_div(out_rows, 128) * plm::ceil_div(rows, 128) * c.shares <= plm::cu_count();
     if (exact) {
         switch (c.tile) {
             case 16: return launch_tile<1, 1, 8, 1, 4, true>(a, c.shares, st);
             case 32: return launch_tile<1, 2, 8, 1, 3, true>(a, c.shares, st);
             case 64: return launch_tile<2, 2, 4, 2, 3, true>(a, c.shares, st);
-            case 128: return launch_tile<2, 4, 4, 2, 2, true>(a, c.shares, st);
+            case 128:
+                return alone ? launch_tile<2, 4, 4, 2, 3, true>(a, c.shares, st)
+                             : launch_tile<2, 4, 4, 2, 2, true>(a, c.shares, st);
             default: break;
         }
         return rows <= 16 ? launch_rows<1, 1, 4, 8, true>(a, waves, st) : launch_rows<2, 2, 2, 8, true>(a, waves, st);
@@ -698,7 +704,8 @@ PLM_EXPORT int fp8_e4m3_block_matmul(const uint8_t* x, const float* x_scales, co
         case 16: return launch_tile<1, 1, 8, 1, 4>(a, c.shares, st);
         case 32: return launch_tile<1, 2, 8, 1, 3>(a, c.shares, st);
         case 64: return launch_tile<2, 2, 4, 2, 3>(a, c.shares, st);
-        case 128: return launch_tile<2, 4, 4, 2, 2>(a, c.shares, st);
+        case 128:
+            return alone ? launch_tile<2, 4, 4, 2, 3>(a, c.shares, st) : launch_tile<2, 4, 4, 2, 2>(a, c.shares, st);
         case 256: return launch_tile<4, 8, 4, 2, 2>(a, c.shares, st);
         default: break;
     }

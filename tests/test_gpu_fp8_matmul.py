@@ -48,6 +48,18 @@ def test_against_64_bits(nat, dtype, m, n, k):
     ref.within(got, want, ref.matmul_bound(want, size, x, xs, w, ws, dtype))
 
 
+# on 256 compute units: tiles of 32, 64, 128 (one and two workgroups on a unit) and 256 rows (one and two rounds),
+# each with a share of the blocks and all of them, over rows and columns that end within a tile and a block
+@pytest.mark.parametrize("m,n,k", [(2122, 132, 928), (401, 130, 2272), (2870, 257, 928), (453, 131, 3120),
+                                   (2793, 655, 912), (2808, 129, 2896), (515, 6541, 912), (159, 5430, 10640),
+                                   (1305, 6313, 912), (130, 5474, 9136), (1947, 8779, 944), (77, 3000, 3001)])
+def test_every_tile(nat, m, n, k):
+    x, xs, w, ws = make(m, n, k, m)
+    want, size = ref.matmul(x, xs, w, ws)
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        ref.within(run(nat, x, xs, w, ws, dtype), want, ref.matmul_bound(want, size, x, xs, w, ws, dtype), str(dtype))
+
+
 @pytest.mark.parametrize("m,n,k", [(600, 2304, 1024), (1025, 1100, 528), (2048, 512, 896)])
 def test_prompts(nat, m, n, k):
     x, xs, w, ws = make(m, n, k, m)
