@@ -887,9 +887,10 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const AttnArgs
     plan.total = noted.x;
     plan.runs = noted.y;
     plan.align = noted.z;
-    const uint32_t run = plan.run_of(own.x);
-    const int splits = static_cast<int>(plan.run_of(own.x + own.y - 1) - run) + 1;
-    if (splits == 1) return;
+    // (within the runs also where the lengths were changed under the first kernel)
+    const uint32_t run = min(plan.run_of(own.x), plan.runs - 1);
+    const int splits = static_cast<int>(min(plan.run_of(own.x + own.y - 1), plan.runs - 1)) - static_cast<int>(run) + 1;
+    if (splits <= 1) return;
     const int r = at / a.heads, head = at - r * a.heads;
     const int kvh = head / a.group, col = r * a.group + head - kvh * a.group;
     const int hc_count = a.kv_heads * a.column_blocks;
