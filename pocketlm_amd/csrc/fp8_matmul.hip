@@ -411,7 +411,7 @@ __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const Mat
     auto block = [&](int b, auto more, auto masked) {
         constexpr bool MORE = decltype(more)::value, MASKED = decltype(masked)::value;
         load_to_lds_barrier<MORE ? S - 1 + (S - 2) * L : 0>();
-        const float next_w = ws[turned(min(b + 1, blocks - 1))];
+        float next_w = 0.0f;
         const char* stage = lds + b % S * T::kStage;
         const float* sx = scales + b % T::kScaleSlots * T::kM + xrow;
         auto piece = [&](int at, int h) {
@@ -422,12 +422,17 @@ __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const Mat
             return v;
         };
         Operand<EXACT> w[TN], v[2];
-#pragma unroll
-        for (int i = 0; i < TN; ++i) w[i] = Operand<EXACT>(piece(w0 + i * 512, 0), piece(w1 + i * 512, 1));
         plm_f32x4 d[kLag + 1];
-        float scale[2];
+        float raw[TM], scale = 0.0f;
+        // What the first product takes is read first.  In the large tile a row tile's operands and scale are
+        // read behind the first product of the one before it, and the weight's next scale, which no read of LDS
+        // may wait beside, at the block's end (4096 x 7168 x 16384 440 us without this order, 419 with).
+        w[0] = Operand<EXACT>(piece(w0, 0), piece(w1, 1));
         v[0] = Operand<EXACT>(piece(x0, 0), piece(x1, 1));
-        scale[0] = sx[0] * sw;
+        raw[0] = sx[0];
+        if constexpr (TN > 2) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 1; i < TN; ++i) w[i] = Operand<EXACT>(piece(w0 + i * 512, 0), piece(w1 + i * 512, 1));
         // the adds of a result follow the matrix instruction kLag later
 #pragma unroll
         for (int at = 0; at < TN * TM + kLag; ++at) {
@@ -440,15 +445,18 @@ __global__ __launch_bounds__(64 * GN * GM) void fp8_matmul_tile_kernel(const Mat
                 for (int x = kAtOnce * j; x < min(L, kAtOnce * (j + 1)); ++x) load_part(b + S - 1, x);
                 if (j == TM - 1) load_scales(b + S);
             }
-            if (i == 0 && j + 1 < TM)
+            if (i == (TN > 2 ? 1 : 0) && j + 1 < TM) {
                 v[(j + 1) & 1] = Operand<EXACT>(piece(x0 + (j + 1) * 2048, 0), piece(x1 + (j + 1) * 2048, 1));
+                raw[j + 1] = sx[16 * (j + 1)];
+            }
+            if (at == TN * TM - 1) next_w = ws[turned(min(b + 1, blocks - 1))];
             if (j < TM) d[at % (kLag + 1)] = block_sums(w[i], v[j & 1]);
             if (at >= kLag) {
                 const int was = at - kLag, wi = was % TN, wj = was / TN;
+                if (wi == 0) scale = raw[wj] * sw;
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    acc[wi][wj][e] = fmaf(d[was % (kLag + 1)][e], scale[wj & 1], acc[wi][wj][e]);
-                if (wi == TN - 1 && wj + 1 < TM) scale[(wj + 1) & 1] = sx[16 * (wj + 1)] * sw;
+                    acc[wi][wj][e] = fmaf(d[was % (kLag + 1)][e], scale, acc[wi][wj][e]);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
