@@ -260,11 +260,11 @@ constexpr int kAttnWaves = 4;
 constexpr int kMaxQueryRows = 8;
 constexpr uint32_t kShortRuns = 4;  // units for each run, below which sequences are short
 constexpr uint32_t kFewUnits = 4;   // of a sequence that a workgroup takes alone whatever the others are
-// Where such workgroups fill the device, a sequence may have 1.5 times the equal share of a run and 12 units:
-// runs that cross sequences and their joins cost more than that much unevenness (4 heads of 128; alone / in
-// runs, us: 64 of up to 1000 positions 24 / 35, 4000 79 / 82, 16000 291 / 271; 300 of 250 29 / 50, of 3000
-// 236 / 254; 63 of 100 and one of 4096 47 / 15).
-constexpr uint32_t kUnevenHalves = 3, kUnevenUnits = 12;
+// Where such workgroups fill the device, a sequence may have 1.5 times the equal share of a run and 12 units, 8
+// where they fill half of it: runs that cross sequences and their joins cost more than that much unevenness
+// (4 heads of 128; alone / in runs, us: 32 of up to 1000 positions 18 / 21, 64 24 / 35, 64 of 4000 79 / 82, of
+// 16000 291 / 271; 300 of 250 29 / 50, of 3000 236 / 254; 63 of 100 and one of 4096 47 / 15).
+constexpr uint32_t kUnevenHalves = 3, kUnevenUnits = 12, kUnevenUnitsHalf = 8;
 
 struct AttnArgs {
     Pages p;
@@ -285,7 +285,7 @@ struct AttnArgs {
     uint32_t budget;      // runs of long sequences
     uint32_t short_runs;  // runs of short ones, about
     int single;           // no table row holds more than a few units: each sequence has a workgroup
-    int wide;             // a workgroup for each sequence fills the device
+    uint32_t uneven;      // units of a sequence more than its share that a workgroup may take; 0: never
     uint32_t streamed;    // units from which on the values are read past the caches
     float scale;       // softmax scale * log2(e)
 };
@@ -391,8 +391,8 @@ __device__ __forceinline__ bool find_plan(const AttnArgs& a, int lane, uint32_t 
     plan.align = 1;
     plan.total = sum();
     longest = wave_max(longest);
-    const uint64_t most = 2 * kUnevenUnits * a.budget + kUnevenHalves * static_cast<uint64_t>(plan.total);
-    plan.single = longest <= kFewUnits || (a.wide != 0 && 2 * static_cast<uint64_t>(longest) * a.budget <= most);
+    const uint64_t most = 2 * a.uneven * a.budget + kUnevenHalves * static_cast<uint64_t>(plan.total);
+    plan.single = longest <= kFewUnits || (a.uneven > 0 && 2 * static_cast<uint64_t>(longest) * a.budget <= most);
     plan.runs = plan.single ? a.p.sequences : a.budget;
     if (!plan.single && plan.total < kShortRuns * a.budget) {
         plan.align = max(1u, (plan.total + a.short_runs - 1) / a.short_runs);
@@ -483,21 +483,29 @@ constexpr uint32_t kNoRow = 0xFFFFFFFFu;
 // with 4 rows each, 49 MB, 17 + 5 us.
 //
 // DP: head_dim rounded up to 64, 128 or 256; EXACT: no rounding.  CT: blocks
-// of 16 columns.
+// of 16 columns, 1 or 2.  More have workgroups of their own which read the same
+// through an L2 that they share: with 4 in a workgroup, one wave a SIMD, 8 rows
+// of 7 heads took 29 us for 700 positions and 137 for 50 sequences of 4000, now
+// 17 and 108.
 template <bool BF16, int DP, bool EXACT, int CT>
-__global__ __launch_bounds__(64 * kAttnWaves, DP > 128 || CT * DP > 256 ? 1 : 2) void paged_attention_kernel(
+__global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void paged_attention_kernel(
     const AttnArgs a) {
     constexpr int KS = DP / 32;               // score steps of 32 head values
     constexpr int NV = DP / 16;               // value instructions
     constexpr int PV = DP == 64 ? 4 : 8;      // adjacent head values of a lane
     constexpr int SETS = NV / PV;             // pieces of a lane per position
     constexpr float kBias = BF16 ? 0.0f : 15.0f;
-    __shared__ float meet[2][CT * (NV * 4 + 2)][64];  // at most 70 KB
+    __shared__ float meet[2][CT * (NV * 4 + 2)][64];  // at most 35 KB
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int hc_count = a.kv_heads * a.column_blocks;
-    const int run = blockIdx.x / hc_count, hc = blockIdx.x - run * hc_count;
-    const int kvh = hc / a.column_blocks, col0 = (hc - kvh * a.column_blocks) * 16 * CT;
+    // The column blocks of a run and head are eight workgroups apart: those are dispatched to one XCD.
+    const uint32_t pairs = gridDim.x / a.column_blocks;  // of run and head
+    const uint32_t group = blockIdx.x / (8 * a.column_blocks), rest = blockIdx.x - group * 8 * a.column_blocks;
+    const uint32_t together = min(8u, pairs - 8 * group);
+    const int block = rest / together, pair = 8 * group + (rest - block * together);
+    const int run = pair / a.kv_heads, kvh = pair - run * a.kv_heads;
+    const int hc = kvh * a.column_blocks + block, col0 = block * 16 * CT;
     Plan plan;
     uint32_t unit = 0, run_end;
     if (a.single != 0) {
@@ -995,6 +1003,7 @@ void launch_append(const AppendArgs& a, int mode, dim3 grid, dim3 block, hipStre
 // would displace what is read again (the same batch 226 -> 210 us, 5.8 TB/s;
 // calls of 30 to 70 MB, which the last-level cache holds, are 3 % faster without).
 constexpr int64_t kStreamedBytes = static_cast<int64_t>(128) << 20;
+constexpr double kLittleBytes = 64.0 * (1 << 20);
 
 struct AttnShape {
     int ct;             // blocks of 16 columns in a workgroup
@@ -1003,7 +1012,7 @@ struct AttnShape {
     int64_t short_runs; // of short ones, about
     int64_t runs;       // at most
     bool single;        // a run for each sequence
-    bool wide;          // such runs fill the device
+    uint32_t uneven;    // see AttnArgs
     bool joined;        // a sequence can be in more than one run
     int64_t slots;      // of partials
     size_t bytes;
@@ -1013,17 +1022,22 @@ AttnShape shape_of(int64_t sequences, int64_t rows, int64_t heads, int64_t kv_he
                    int64_t capacity) {
     AttnShape s;
     const int64_t columns = rows * (heads / kv_heads);
-    // several blocks of columns share what they read of the cache
-    s.ct = head_dim > 128 || columns <= 16 ? 1 : columns <= 32 ? 2 : 4;
+    // Two blocks of columns share what a workgroup reads of the cache, unless all that the tables reach is
+    // little for their columns (4 rows of 7 heads of 128, 4 kv heads, us with 1 / 2: 16000 positions 17.7 / 19.7,
+    // 16 times 8192 78 / 63).
+    const int64_t blocks = plm::ceil_div(columns, 16);
+    const double reach = static_cast<double>(sequences * blocks) * static_cast<double>(capacity * kv_heads * head_dim * 4);
+    s.ct = head_dim > 128 || blocks == 1 || reach <= kLittleBytes ? 1 : 2;
     s.column_blocks = static_cast<int>(plm::ceil_div(columns, 16 * s.ct));
     const int64_t hc = kv_heads * s.column_blocks;
     const int64_t units = std::max<int64_t>(1, plm::ceil_div(capacity, kUnit));
     // as many workgroups as the compute units hold at once, and as there are compute units
-    const int resident = head_dim > 128 || s.ct * head_dim > 256 ? 1 : 2;
+    const int resident = head_dim > 128 ? 1 : 2;
     s.budget = std::max<int64_t>(1, resident * plm::cu_count() / hc);
     s.short_runs = std::max<int64_t>(1, plm::cu_count() / hc);
     s.single = units <= kFewUnits;
-    s.wide = sequences * hc >= plm::cu_count();
+    const int64_t groups = sequences * hc;
+    s.uneven = groups >= plm::cu_count() ? kUnevenUnits : 2 * groups >= plm::cu_count() ? kUnevenUnitsHalf : 0;
     const int64_t shared = std::min(sequences * units, s.budget + std::min(sequences, kShortRuns * s.budget));
     s.runs = s.single ? sequences : std::max(sequences, shared);
     s.joined = !s.single;
@@ -1038,16 +1052,7 @@ void launch_attention(const AttnArgs& a, const AttnShape& s, hipStream_t st) {
     const dim3 grid(static_cast<unsigned>(s.runs * a.kv_heads * a.column_blocks)), block(64 * kAttnWaves);
     const int d = a.head_dim;
 #define PLM_ATTN(DP, EXACT, CT) hipLaunchKernelGGL((paged_attention_kernel<BF16, DP, EXACT, CT>), grid, block, 0, st, a)
-    if (s.ct == 4) {
-        if (d == 64)
-            PLM_ATTN(64, true, 4);
-        else if (d < 64)
-            PLM_ATTN(64, false, 4);
-        else if (d == 128)
-            PLM_ATTN(128, true, 4);
-        else
-            PLM_ATTN(128, false, 4);
-    } else if (s.ct == 2) {
+    if (s.ct == 2) {
         if (d == 64)
             PLM_ATTN(64, true, 2);
         else if (d < 64)
@@ -1198,7 +1203,7 @@ PLM_EXPORT int kv_paged_attention_decode_u16(const uint16_t* q, const uint16_t* 
     a.budget = static_cast<uint32_t>(s.budget);
     a.short_runs = static_cast<uint32_t>(s.short_runs);
     a.single = s.single ? 1 : 0;
-    a.wide = s.wide ? 1 : 0;
+    a.uneven = s.uneven;
     a.streamed = static_cast<uint32_t>(kStreamedBytes / (kUnit * 4 * kv_heads * head_dim));
     a.scale = softmax_scale * 1.44269504088896340736f;
     a.part = static_cast<float*>(part);

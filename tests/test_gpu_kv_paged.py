@@ -175,16 +175,18 @@ def check_attention(nat, lengths, rows, page, heads, kvh, dim, dtype, *, seed=0,
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("heads,kvh,dim", [(28, 4, 128), (2, 2, 64), (12, 1, 256), (40, 2, 64), (17, 1, 128),
                                            (6, 3, 96), (4, 2, 8), (5, 1, 40), (6, 2, 192), (33, 1, 112), (3, 1, 200)])
-def test_attention_lengths_and_heads(nat, dtype, heads, kvh, dim):
-    check_attention(nat, [0, 30, 31, 32, 126, 127, 128, 299, -1, 700], 1, 16, heads, kvh, dim, dtype, seed=dim)
+@pytest.mark.parametrize("room", [1, 200000])
+def test_attention_lengths_and_heads(nat, dtype, heads, kvh, dim, room):
+    check_attention(nat, [0, 30, 31, 32, 126, 127, 128, 299, -1, 700], 1, 16, heads, kvh, dim, dtype, seed=dim, room=room)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("rows", [2, 3, 5, 8])
 @pytest.mark.parametrize("heads,kvh,dim", [(7, 1, 128), (4, 4, 64), (8, 2, 256), (12, 2, 96)])
-@pytest.mark.parametrize("longest", [333, 813])
-def test_attention_of_several_rows(nat, dtype, rows, heads, kvh, dim, longest):
-    check_attention(nat, [0, 1, 29, 60, 125, -8, longest], rows, 8, heads, kvh, dim, dtype, seed=rows)
+@pytest.mark.parametrize("longest,room", [(333, 1), (813, 1), (813, 200000)])
+def test_attention_of_several_rows(nat, dtype, rows, heads, kvh, dim, longest, room):
+    """Of small and of large tables, whose workgroups take 16 and 32 rows and heads."""
+    check_attention(nat, [0, 1, 29, 60, 125, -8, longest], rows, 8, heads, kvh, dim, dtype, seed=rows, room=room)
 
 
 @pytest.mark.parametrize("page", [1, 3, 8, 31, 100, 256, 1024])
