@@ -351,34 +351,27 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
     return __builtin_amdgcn_readlane(v, 63);
 }
 
-// The plan, at the sequence that holds the first unit of run `run`.  Every lane
-// of a wave calls it; false for a run past the last.
-__device__ __forceinline__ bool find_plan(const AttnArgs& a, int lane, uint32_t run, Plan& plan) {
-    // a lane's sequence of each 64: the first 512 are read at once
-    constexpr int kHeld = 8;
-    uint32_t held[kHeld];
-#pragma unroll
-    for (int c = 0; c < kHeld; ++c) {
-        held[c] = 0;
-        if (64 * c < a.p.sequences) {
-            const int i = 64 * c + lane;
-            held[c] = i < a.p.sequences ? units_of(a.p.lengths[i], a.rows, a.capacity) : 0;
-        }
+// The plan, at the sequence that holds the first unit of run `run`.  Every
+// thread of a workgroup calls it; false for a run past the last.  (Kept short:
+// a small call waits for its instructions as for its data.)
+constexpr int kHeld = 2048;  // sequences whose units are read once
+__device__ __forceinline__ bool find_plan(const AttnArgs& a, int lane, uint32_t run, uint32_t* held, Plan& plan) {
+    const uint32_t n0 = lane < a.p.sequences ? units_of(a.p.lengths[lane], a.rows, a.capacity) : 0;
+    if (a.p.sequences > 64) {
+        for (int i = threadIdx.x; i < min(a.p.sequences, kHeld); i += 64 * kAttnWaves)
+            held[i] = units_of(a.p.lengths[i], a.rows, a.capacity);
+        __syncthreads();
     }
     auto units_at = [&](int base) {
+        if (base == 0) return n0;
         const int i = base + lane;
-        return i < a.p.sequences ? units_of(a.p.lengths[i], a.rows, a.capacity) : 0;
+        return i >= a.p.sequences ? 0 : base < kHeld ? held[i] : units_of(a.p.lengths[i], a.rows, a.capacity);
     };
     uint32_t longest = 0;
     auto sum = [&] {
         uint32_t mine = 0;
-#pragma unroll
-        for (int c = 0; c < kHeld; ++c) {
-            if (64 * c >= a.p.sequences) break;
-            mine += plan.rounded(held[c]);
-            longest = max(longest, held[c]);
-        }
-        for (int base = 64 * kHeld; base < a.p.sequences; base += 64) {
+#pragma unroll 1
+        for (int base = 0; base < a.p.sequences; base += 64) {
             const uint32_t n = units_at(base);
             mine += plan.rounded(n);
             longest = max(longest, n);
@@ -408,7 +401,9 @@ __device__ __forceinline__ bool find_plan(const AttnArgs& a, int lane, uint32_t 
     }
     const uint32_t unit = plan.start(run);
     uint32_t before = 0;
-    auto found = [&](int base, uint32_t n) {
+#pragma unroll 1
+    for (int base = 0; base < a.p.sequences; base += 64) {
+        const uint32_t n = units_at(base);
         const uint32_t upto = wave_prefix(plan.rounded(n));
         const unsigned long long past = __ballot(before + upto > unit);
         if (past != 0) {
@@ -419,13 +414,7 @@ __device__ __forceinline__ bool find_plan(const AttnArgs& a, int lane, uint32_t 
             return true;
         }
         before += __builtin_amdgcn_readlane(upto, 63);
-        return false;
-    };
-#pragma unroll
-    for (int c = 0; c < kHeld; ++c)
-        if (64 * c < a.p.sequences && found(64 * c, held[c])) return true;
-    for (int base = 64 * kHeld; base < a.p.sequences; base += 64)
-        if (found(base, units_at(base))) return true;
+    }
     return false;
 }
 
@@ -496,6 +485,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void paged_atten
     constexpr int SETS = NV / PV;             // pieces of a lane per position
     constexpr float kBias = BF16 ? 0.0f : 15.0f;
     __shared__ float meet[2][CT * (NV * 4 + 2)][64];  // at most 35 KB
+    __shared__ uint32_t held[kHeld];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int hc_count = a.kv_heads * a.column_blocks;
@@ -516,7 +506,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void paged_atten
         plan.total = plan.units * static_cast<uint32_t>(a.p.sequences);  // about
         run_end = plan.units;
     } else {
-        if (!find_plan(a, lane, static_cast<uint32_t>(run), plan)) return;
+        if (!find_plan(a, lane, static_cast<uint32_t>(run), &held[0], plan)) return;
         unit = plan.single ? 0 : plan.start(run);
         run_end = plan.single ? plan.units : plan.start(run + 1);
         if (blockIdx.x == 0 && threadIdx.x == 0) *a.plan = make_uint4(plan.total, plan.runs, plan.align, plan.single);
