@@ -327,6 +327,7 @@ struct Plan {
     }
     // run * total / runs
     __device__ __forceinline__ uint32_t start(uint32_t run) const {
+        if (total == runs * align) return run * align;
         const uint32_t each = total / runs;
         return run * each + run * (total - each * runs) / runs;
     }
@@ -490,10 +491,14 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void paged_atten
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int hc_count = a.kv_heads * a.column_blocks;
     // The column blocks of a run and head are eight workgroups apart: those are dispatched to one XCD.
-    const uint32_t pairs = gridDim.x / a.column_blocks;  // of run and head
-    const uint32_t group = blockIdx.x / (8 * a.column_blocks), rest = blockIdx.x - group * 8 * a.column_blocks;
-    const uint32_t together = min(8u, pairs - 8 * group);
-    const int block = rest / together, pair = 8 * group + (rest - block * together);
+    int block = 0, pair = blockIdx.x;  // of run and head
+    if (a.column_blocks > 1) {
+        const uint32_t pairs = gridDim.x / a.column_blocks;
+        const uint32_t group = blockIdx.x / (8 * a.column_blocks), rest = blockIdx.x - group * 8 * a.column_blocks;
+        const uint32_t together = min(8u, pairs - 8 * group);
+        block = rest / together;
+        pair = 8 * group + (rest - block * together);
+    }
     const int run = pair / a.kv_heads, kvh = pair - run * a.kv_heads;
     const int hc = kvh * a.column_blocks + block, col0 = block * 16 * CT;
     Plan plan;
