@@ -467,10 +467,10 @@ constexpr uint32_t kNoRow = 0xFFFFFFFFu;
 // weight is only lost below 2^-40 of the row's largest.
 //
 // Bound by the cache's bytes in large batches: 48 sequences of 8000 to 16000
-// positions, 4 key-value heads of 128, 1.2 GB 211 us with the join, 5.8 TB/s.
+// positions, 4 key-value heads of 128, 1.2 GB 212 us with the join, 5.7 TB/s.
 // Small calls are a chain of trips to memory, lengths, table, keys and values,
-// then the join: 700 positions 7 + 5 us, 6 sequences of up to 5000 positions
-// with 4 rows each, 49 MB, 17 + 5 us.
+// then the join: 700 positions 7.6 + 4.7 us, 6 sequences of up to 5000 positions
+// with 4 rows each, 49 MB, 17.8 + 5.1 us.
 //
 // DP: head_dim rounded up to 64, 128 or 256; EXACT: no rounding.  CT: blocks
 // of 16 columns, 1 or 2.  More have workgroups of their own which read the same
@@ -855,8 +855,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void paged_atten
 // threads first take the splits' maxima and sums (the weights of the splits go
 // to LDS), then each a quad of head values of every sets-th split, and the
 // sets meet in LDS.  Sequences of one split were written already.  Bound by its
-// launch and three trips to memory: 28 to 672 workgroups 5 to 6 us, 48 x 28
-// with 4 partials on average 7.5.
+// launch and three trips to memory: 28 to 672 workgroups about 5 us, 48 x 28
+// with 4 partials on average 7.4.
 constexpr int kJoinThreads = 256;
 constexpr int kJoinSplits = 1024;  // at a time
 
