@@ -796,8 +796,9 @@ int fp8_e4m3_quantize_rows(const void* x, uint8_t* out_fp8, float* out_scales, i
  * x + residual rounded to the rows' type and written to out_sum [rows][cols]
  * (which may be x or residual themselves, with a row stride of cols), or x
  * itself where residual is NULL (out_sum is not written then).  y is fp32 and
- * is not rounded before its quantization.  x, residual, weight [cols] and
- * out_sum share dtype_code.  Codes as above. */
+ * is not rounded before its quantization; finite rows of any size have finite
+ * means (a sum of squares that leaves fp32's range is taken in 64 bits).  x,
+ * residual, weight [cols] and out_sum share dtype_code.  Codes as above. */
 int fp8_e4m3_rms_norm_rows(const void* x, const void* residual, const void* weight, void* out_sum, uint8_t* out_fp8,
                            float* out_scales, int64_t rows, int64_t cols, int64_t x_stride, int64_t residual_stride,
                            int dtype_code, float rms_eps);

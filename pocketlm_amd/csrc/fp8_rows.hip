@@ -4,7 +4,8 @@
 // first (fp8_e4m3_rms_norm_rows).
 //
 //   sum = T(x + residual)                       T: the rows' type, to nearest even
-//   y   = sum * rsqrt(mean(sum^2) + eps) * w    fp32, as the dense layer's norms
+//   y   = sum * rsqrt(mean(sum^2) + eps) * w    fp32, as the dense layer's norms; sums of squares
+//                                               that leave fp32's range in 64 bits
 //   s_b = max(max |y| over block b / 448, 2^-126)
 //   q   = e4m3(y / s_b)                         to nearest even
 //
@@ -125,6 +126,23 @@ __device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
     return v;
 }
 
+// plm_wave_sum in 64 bits; every lane has it.
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) v += __shfl_xor(v, off);
+    return v;
+}
+
+// Whether a row's sum of squares has left fp32: the squares of finite values
+// pass its largest number from 2^64 on, and below 2^-63 they lose bits, which
+// counts where rms_eps is tiny too.  Such rows are summed again in 64 bits
+// (one with an infinity or a NaN comes out as it went in); the others keep the
+// fp32 sum's bits and time (one row of 7168 bf16 3.98 us, 509 rows of 3584 4.75;
+// with all sums in 64 bits 4.16 and 4.87).
+__device__ __forceinline__ bool beyond(float total, const RowsArgs& a) {
+    return !(total < 0x1p127f) || total + a.eps * static_cast<float>(a.cols) < 0x1p-80f;
+}
+
 __device__ __forceinline__ int pack4(float a, float b, float c, float d) {
     int v = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
     return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, v, true);
@@ -177,6 +195,7 @@ template <int DT, int NS, bool NORM>
 __global__ __launch_bounds__(kMaxThreads) void fp8_rows_kernel(const RowsArgs a) {
     using T = typename Row<DT>::T;
     __shared__ float red[kMaxThreads / 64];
+    __shared__ double red64[kMaxThreads / 64];
     const int wave = threadIdx.x >> 6;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x / (64 * a.waves)) + wave / a.waves;
     const int t = threadIdx.x - wave / a.waves * a.waves * 64;
@@ -215,14 +234,46 @@ __global__ __launch_bounds__(kMaxThreads) void fp8_rows_kernel(const RowsArgs a)
             for (int j = 0; j < kPiece; ++j) s = fmaf(h[i][j], h[i][j], s);
         s = plm_wave_sum(s);
         float total = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, s), kSumLane));
+        const int own = wave / a.waves;  // of the workgroup's rows
+        bool far = false;                // one of them, where they share barriers
         if (a.waves > 1) {
             if ((threadIdx.x & 63) == 0) red[wave] = total;
             __syncthreads();
-            total = 0.0f;
-            const int first = wave / a.waves * a.waves;
-            for (int w = 0; w < a.waves; ++w) total += red[first + w];
+            const int rows = blockDim.x / (64 * a.waves);
+            for (int r = 0; r < rows; ++r) {
+                float all = 0.0f;
+                for (int w = 0; w < a.waves; ++w) all += red[r * a.waves + w];
+                far |= beyond(all, a);
+                if (r == own) total = all;
+            }
+        } else {
+            far = beyond(total, a);
         }
-        const float scale = 1.0f / sqrtf(total / static_cast<float>(a.cols) + a.eps);
+        float scale = 1.0f / sqrtf(total / static_cast<float>(a.cols) + a.eps);
+        if (__builtin_expect(far, 0)) {
+            double wide = 0.0;
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+#pragma unroll
+                for (int j = 0; j < kPiece; ++j) wide = fma(static_cast<double>(h[i][j]), static_cast<double>(h[i][j]), wide);
+            wide = wave_sum64(wide);
+            if (a.waves > 1) {
+                if ((threadIdx.x & 63) == 0) red64[wave] = wide;
+                __syncthreads();
+                wide = 0.0;
+                for (int w = 0; w < a.waves; ++w) wide += red64[own * a.waves + w];
+            }
+            if (beyond(total, a)) {
+                // the root's power of two goes to the values, which it leaves exact, so that both stay in range
+                const double mean = wide / static_cast<double>(a.cols) + static_cast<double>(a.eps);
+                const int half = -(__builtin_amdgcn_frexp_exp(mean) >> 1);
+                scale = 1.0f / sqrtf(static_cast<float>(__builtin_ldexp(mean, 2 * half)));
+#pragma unroll
+                for (int i = 0; i < NS; ++i)
+#pragma unroll
+                    for (int j = 0; j < kPiece; ++j) h[i][j] = ldexpf(h[i][j], half);
+            }
+        }
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             const int64_t c = t + static_cast<int64_t>(i) * step;

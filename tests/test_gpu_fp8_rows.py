@@ -139,3 +139,19 @@ def test_the_c_entry_adds_in_place(nat):
                                           scales.data_ptr(), 40, 512, 512, 512, 1, 1e-6) == 0
         assert torch.equal(to, summed) and torch.equal(data, want.data.view(torch.uint8))
         assert torch.equal(scales, want.scales)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,cols", [(5, 7168), (7, 129), (1030, 520), (1100, 100), (2, 20008), (1, 65536)])
+def test_norm_of_rows_whose_squares_leave_fp32(nat, dtype, rows, cols):
+    """Finite rows from near the type's largest value down to 2^-120, in one
+    batch: the sum of squares passes fp32 both ways, y does not."""
+    x = randn((rows, cols), torch.float32, cols + 3)
+    powers = torch.tensor([124.0, 0.0, 63.0, -120.0, 90.0, -66.0, 64.0])[torch.arange(rows) % 7]
+    x = (x * torch.exp2(powers)[:, None]).to(dtype)
+    if rows > 1:
+        x[1, 3] = 2.0 ** 100  # one value beside ordinary ones
+    w = randn((cols,), dtype, cols + 4)
+    for eps in (0.0, 1e-6):
+        got, _ = nat.fp8_e4m3_rms_norm_rows(x.cuda(), w.cuda(), rms_eps=eps)
+        check_rows(got, ref.rms_norm(x, w, eps), NORM_OFF)
