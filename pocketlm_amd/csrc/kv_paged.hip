@@ -674,13 +674,14 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void paged_atten
                     top = fmaxf(m[t], swap_max(fmaxf(top, floor[t])));
                     const float fade = exp2_from(m[t], top);
                     m[t] = top;
-                    const float from = (top == -INFINITY ? 0.0f : top) - kBias;
+                    const float from = top == -INFINITY ? 0.0f : top;
                     float sum = 0.0f;
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            s[t][i][j] = exp2f(s[t][i][j] - from);
+                            // the bias last: a score of 2^24 or more has no room for it
+                            s[t][i][j] = exp2f((s[t][i][j] - from) + kBias);
                             sum += s[t][i][j];
                         }
                     l[t] = fmaf(l[t], fade, sum);

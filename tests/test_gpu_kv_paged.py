@@ -531,3 +531,26 @@ def test_calls_on_another_stream(nat):
         got = other(x, x, lengths)
     stream.synchronize()
     assert torch.equal(got["out"], want["out"]) and torch.equal(other.k, step.k)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("room", [1, 200000])
+def test_attention_of_scores_past_2_to_the_24(nat, dtype, room):
+    """Scores that fp32 holds in steps of whole numbers, exact ones: 2^15 apart
+    at least, so the largest position's value is the result."""
+    n, dim, page = 40, 64, 16
+    lengths = [20 + 13 * b for b in range(n)]
+    k, v, table = ref.make_pages([x + 1 for x in lengths], page, 1, dim, dtype, 41, extra_cols=-(-room // page))
+    k.zero_()
+    want = torch.zeros((n, 2, dim), dtype=dtype)
+    for b, length in enumerate(lengths):
+        for p in range(length + 1):
+            k[int(table[b, p // page]), p % page, 0, :8] = p % 97
+        at = (7 * b) % (length + 1)
+        slot = (int(table[b, at // page]), at % page, 0)
+        k[slot][:8] = 128 + 3 * b
+        want[b, :] = v[slot]
+    q = torch.zeros((n, 2, dim), dtype=dtype)
+    q[..., :8] = 2.0 ** 15
+    got = nat.kv_paged_attention_decode(q.cuda(), k.cuda(), v.cuda(), table.cuda(), i32(lengths), softmax_scale=1.0)
+    assert torch.equal(got.cpu(), want)
