@@ -446,6 +446,28 @@ __device__ __forceinline__ f32x4 mfma16(const u32x4 a, const u32x4 b, const f32x
 // exp2(x - m) for a running maximum that may be -inf (nothing seen yet).
 __device__ __forceinline__ float exp2_from(float x, float m) { return exp2f(x - (m == -INFINITY ? 0.0f : m)); }
 
+// Two weights as sums of two values of the cache's type each: cut off, so that
+// the rest is not negative, and the rest, rounded; together they keep 15 bits
+// (fp16 21) of each weight.  The rest of a weight above 0 is not 0: times an
+// infinity 0 is NaN, as is the sum of infinities of both signs.
+struct Halves {
+    uint32_t high, low;
+};
+template <bool BF16>
+__device__ __forceinline__ Halves halves(float a, float b) {
+    if constexpr (BF16) {
+        const uint32_t ia = __float_as_uint(a), ib = __float_as_uint(b);
+        const float ra = a - __uint_as_float(ia & 0xFFFF0000u), rb = b - __uint_as_float(ib & 0xFFFF0000u);
+        return {__builtin_amdgcn_perm(ib, ia, 0x07060302u),
+                pack2<true>(__builtin_amdgcn_fmed3f(ra, a, 0x1p-126f), __builtin_amdgcn_fmed3f(rb, b, 0x1p-126f))};
+    } else {
+        const f16x2 high = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(a, b));
+        const float ra = a - static_cast<float>(high[0]), rb = b - static_cast<float>(high[1]);
+        return {__builtin_bit_cast(uint32_t, high),
+                pack2<false>(__builtin_amdgcn_fmed3f(ra, a, 0x1p-24f), __builtin_amdgcn_fmed3f(rb, b, 0x1p-24f))};
+    }
+}
+
 constexpr uint32_t kNoRow = 0xFFFFFFFFu;
 
 // Workgroup (run, kv head, column block): for each sequence of the run, 4
@@ -461,10 +483,14 @@ constexpr uint32_t kNoRow = 0xFFFFFFFFu;
 //           and transposes 8 x 8 values by register permutes.  Matrix
 //           instruction i has head values 8 r + i in its row r.
 //
-// Weights are rounded to the cache's type for the second product (their sum is
-// not): at most 2^-8 (2^-11) of each, of either sign, so less in their sum than
-// the output's own rounding.  In fp16 they are kept times 2^15, so that a
-// weight is only lost below 2^-40 of the row's largest.
+// Weights go to the second product as two values of the cache's type each
+// (halves below), so that the result is as close to 64 bits as with fp32
+// weights: rounded once, the error is 2.1e-3 of the results' size in bf16 and
+// 2.6e-4 in fp16, so 1.66e-3 and 2.07e-4, which are the output's rounding.  The
+// second instruction waits for memory with the first (48 sequences of 8000 to
+// 16000 positions 211.5 us with one, 211.7 with two; 6 of 5000 with 4 rows each
+// 23.0, 23.7).  In fp16 weights are kept times 2^15, so that a weight is only
+// lost below 2^-40 of the row's largest.
 //
 // Bound by the cache's bytes in large batches: 48 sequences of 8000 to 16000
 // positions, 4 key-value heads of 128, 1.2 GB 212 us with the join, 5.7 TB/s.
@@ -666,7 +692,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void paged_atten
                                 floor[t] = -FLT_MAX;
                         }
                 }
-                u32x4 w[CT];
+                u32x4 w[CT], w_low[CT];
 #pragma unroll
                 for (int t = 0; t < CT; ++t) {
                     float top = fmaxf(fmaxf(fmaxf(s[t][0][0], s[t][0][1]), fmaxf(s[t][0][2], s[t][0][3])),
@@ -687,8 +713,12 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void paged_atten
                     l[t] = fmaf(l[t], fade, sum);
 #pragma unroll
                     for (int i = 0; i < NV; ++i) acc[t][i] = acc[t][i] * fade;
-                    w[t] = u32x4{pack2<BF16>(s[t][0][0], s[t][0][1]), pack2<BF16>(s[t][0][2], s[t][0][3]),
-                                 pack2<BF16>(s[t][1][0], s[t][1][1]), pack2<BF16>(s[t][1][2], s[t][1][3])};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const Halves x = halves<BF16>(s[t][i >> 1][2 * (i & 1)], s[t][i >> 1][2 * (i & 1) + 1]);
+                        w[t][i] = x.high;
+                        w_low[t][i] = x.low;
+                    }
                 }
                 if (!full) {
                     // What a row does not see has weight 0, but 0 times a NaN or an infinity left there is
@@ -707,7 +737,9 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void paged_atten
                     for (int i = 0; i < PV; ++i) {
                         const u32x4 values = across(x, i);
 #pragma unroll
-                        for (int t = 0; t < CT; ++t) acc[t][PV * x + i] = mfma16<BF16>(values, w[t], acc[t][PV * x + i]);
+                        for (int t = 0; t < CT; ++t)
+                            acc[t][PV * x + i] =
+                                mfma16<BF16>(values, w_low[t], mfma16<BF16>(values, w[t], acc[t][PV * x + i]));
                     }
                 // the positions that some of the rows see, at most rows - 1 of them, one at a time
                 for (int pos = max(least, t0); pos < min(t0 + 32, seen); ++pos) {

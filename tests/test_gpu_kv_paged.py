@@ -554,3 +554,48 @@ def test_attention_of_scores_past_2_to_the_24(nat, dtype, room):
     q[..., :8] = 2.0 ** 15
     got = nat.kv_paged_attention_decode(q.cuda(), k.cuda(), v.cuda(), table.cuda(), i32(lengths), softmax_scale=1.0)
     assert torch.equal(got.cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [1, 4])
+@pytest.mark.parametrize("heads,kvh,dim", [(28, 4, 128), (8, 8, 64), (4, 2, 256), (6, 3, 96)])
+def test_attention_weights_keep_more_bits_than_the_cache(nat, dtype, rows, heads, kvh, dim):
+    """The bound of ref.attention with 2^-15 (fp16 2^-21, and 2^-38 of the row's largest) for a
+    weight's rounding: a weight is a value of the cache's type, cut off (2^-7 of it, fp16 2^-10),
+    and the rest in that type, rounded (2^-8 of the rest, fp16 2^-11)."""
+    lengths = [600, 17, 1200]
+    k, v, table = ref.make_pages([x + rows for x in lengths], 16, kvh, dim, dtype, 51)
+    q = torch.randn((3, rows, heads, dim), generator=torch.Generator().manual_seed(52)).to(dtype)
+    want, _ = ref.attention(q, k, v, table, lengths, dim ** -0.5)
+    bound = torch.zeros_like(want)
+    for b, length in enumerate(lengths):
+        for r in range(rows):
+            at = torch.arange(length + r + 1)
+            page, slot = table[b][at // 16].long(), at % 16
+            for h in range(kvh):
+                group = slice(h * (heads // kvh), (h + 1) * (heads // kvh))
+                ks, vs, qs = k[page, slot, h].double(), v[page, slot, h].double().abs(), q[b, r, group].double()
+                off = (qs.abs() @ ks.abs().t()) * dim ** -0.5 * (dim + 4) * 2.0 ** -23
+                p = torch.softmax(qs @ ks.t() * dim ** -0.5, dim=1)
+                share = 2 * off + 2.0 ** -20 + (len(at) / 32 + 64) * 2.0 ** -23
+                weight = 2.0 ** -15 * p if dtype == torch.bfloat16 else 2.0 ** -21 * p + 2.0 ** -38 * p.amax(1, keepdim=True)
+                wide = (p * share + weight) @ vs + share.amax(1, keepdim=True) * (p @ vs)
+                o = want[b, r, group].abs()
+                bound[b, r, group] = wide + ref.HALF[dtype] * (o + wide) + ref.TINY[dtype]
+    got = nat.kv_paged_attention_decode(q.cuda() if rows > 1 else q[:, 0].cuda(), k.cuda(), v.cuda(), table.cuda(),
+                                        i32(lengths))
+    ref.within(got.reshape(q.shape), want, bound)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attention_of_infinite_values_that_are_seen(nat, dtype):
+    """An infinite value with a weight above 0 is the result's, with its sign; equal weights are 1."""
+    k, v, table = ref.make_pages([300, 300, 40], 16, 2, 64, dtype, 53)
+    for b, (pos, sign) in enumerate(((200, 1), (3, -1), (39, 1))):
+        v[int(table[b, pos // 16]), pos % 16] = sign * float("inf")
+    q = torch.randn((3, 4, 64), generator=torch.Generator().manual_seed(54)).to(dtype)
+    q[2] = 0.0
+    got = nat.kv_paged_attention_decode(q.cuda(), k.cuda(), v.cuda(), table.cuda(), i32([299, 299, 39])).cpu()
+    assert torch.equal(got[0], torch.full_like(got[0], float("inf")))
+    assert torch.equal(got[1], torch.full_like(got[1], -float("inf")))
+    assert torch.equal(got[2], torch.full_like(got[2], float("inf")))
