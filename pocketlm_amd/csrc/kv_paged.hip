@@ -252,8 +252,9 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(const Appe
 // all sequences, one after another, make equal runs, so that ragged batches stay
 // balanced (48 sequences of 8000 to 16000 positions: 253 -> 228 us against runs
 // that end with their sequence).  A run that holds a sequence's every unit
-// writes its result; the others write a partial, in slot run + sequence, which
-// grows by at least one from partial to partial.
+// writes its result; of the others a run leaves two partials at most: that of
+// the sequence it goes on with (slot 2 run) and that of the one it begins and
+// does not end (slot 2 run + 1), whatever the number of sequences.
 
 constexpr int kUnit = 128;
 constexpr int kAttnWaves = 4;
@@ -837,7 +838,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void paged_atten
             const int col = col0 + 16 * t + li;
             if (wave != 0 || col >= a.columns) continue;
             if (!whole) {
-                const int64_t at = ((static_cast<int64_t>(run) + seq) * hc_count * CT + hc * CT + t) * 16 + li;
+                const int64_t slot = 2 * static_cast<int64_t>(run) + (unit == before ? 1 : 0);
+                const int64_t at = (slot * hc_count * CT + hc * CT + t) * 16 + li;
                 if (g == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * at) = f32x2{m[t], l[t]};
                 float* to = a.part + at * a.head_dim;
 #pragma unroll
@@ -932,12 +934,13 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const AttnArgs
     const int hc_count = a.kv_heads * a.column_blocks;
     const int wide = 16 * ct;
     const int hc = kvh * a.column_blocks + col / wide;
-    // partial of split s: first + s * stride
+    // partial of split s: first + slot(s) * stride; the first split's is its run's second
     const int64_t stride = static_cast<int64_t>(hc_count) * wide;
-    const int64_t first = (static_cast<int64_t>(run + seq) * hc_count + hc) * wide + col % wide;
+    const int64_t first = (2 * static_cast<int64_t>(run) * hc_count + hc) * wide + col % wide;
+    auto slot = [](int s) { return max(2 * s, 1); };
     const f32x2* ml = reinterpret_cast<const f32x2*>(a.part_ml) + first;
     float m = -INFINITY;
-    for (int s = threadIdx.x; s < splits; s += kJoinThreads) m = fmaxf(m, ml[s * stride][0]);
+    for (int s = threadIdx.x; s < splits; s += kJoinThreads) m = fmaxf(m, ml[slot(s) * stride][0]);
     m = join_reduce(m, true, red);
     const int quads = a.head_dim / 4;  // threads of a set
     const int sets = kJoinThreads / quads;
@@ -949,7 +952,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const AttnArgs
         const int n = min(kJoinSplits, splits - base);
         if (base > 0) __syncthreads();
         for (int s = threadIdx.x; s < n; s += kJoinThreads) {
-            const f32x2 v = ml[(base + s) * stride];
+            const f32x2 v = ml[slot(base + s) * stride];
             const float w = exp2_from(v[0], m);
             weights[s] = w;
             sum = fmaf(v[1], w, sum);
@@ -958,7 +961,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const AttnArgs
         if (set < sets) {
 #pragma unroll 4
             for (int s = set; s < n; s += sets) {
-                const f32x4 x = *reinterpret_cast<const f32x4*>(part + (base + s) * stride * a.head_dim);
+                const f32x4 x = *reinterpret_cast<const f32x4*>(part + slot(base + s) * stride * a.head_dim);
                 const float w = weights[s];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[i] = fmaf(x[i], w, acc[i]);
@@ -1069,7 +1072,7 @@ AttnShape shape_of(int64_t sequences, int64_t rows, int64_t heads, int64_t kv_he
     const int64_t shared = std::min(sequences * units, s.budget + std::min(sequences, kShortRuns * s.budget));
     s.runs = s.single ? sequences : std::max(sequences, shared);
     s.joined = !s.single;
-    s.slots = s.joined ? shared + sequences : 0;
+    s.slots = s.joined ? 2 * shared : 0;
     s.bytes = static_cast<size_t>(s.slots) * hc * s.ct * 16 * (head_dim + 2) * sizeof(float);
     if (s.joined) s.bytes += sizeof(uint4) + sizeof(uint2) * sequences;
     return s;

@@ -195,3 +195,14 @@ def test_kill_switches(monkeypatch):
         native.fp8_e4m3_quantize_rows(x)
     with pytest.raises(RuntimeError, match="unavailable: disabled"):
         native.kv_paged_append(None, x, x, x, x, x, x)
+
+
+def test_attention_scratch_does_not_grow_with_the_sequences(lib):
+    """A run leaves two partials at most, and there are as many runs for 512 sequences as for 65535: what
+    grows is the deal's note of each sequence, 8 bytes."""
+    need = lib.kv_paged_attention_scratch_bytes
+    for rows, heads, kvh, dim, capacity in ((1, 64, 64, 128, 8192), (1, 128, 128, 128, 8192), (1, 32, 8, 128, 131072),
+                                            (8, 28, 4, 128, 32768), (1, 16, 4, 256, 4096)):
+        few = need(1000, rows, heads, kvh, dim, capacity)
+        assert need(65535, rows, heads, kvh, dim, capacity) - few == 8 * (65535 - 1000)
+        assert 0 < few < 1 << 28

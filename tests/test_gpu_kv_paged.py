@@ -599,3 +599,27 @@ def test_attention_of_infinite_values_that_are_seen(nat, dtype):
     assert torch.equal(got[0], torch.full_like(got[0], float("inf")))
     assert torch.equal(got[1], torch.full_like(got[1], -float("inf")))
     assert torch.equal(got[2], torch.full_like(got[2], float("inf")))
+
+
+@pytest.mark.parametrize("sequences,longest,kvh", [(1, 9000, 2), (40, 3000, 2), (300, 1500, 8), (90, 9000, 64), (1200, 700, 1)])
+def test_attention_writes_within_its_scratch(nat, sequences, longest, kvh):
+    """The C entry with as much scratch as it asks for, at the end of a buffer whose front and back stay as they are."""
+    from pocketlm_amd import _lib
+
+    lib, dim, page, guard = _lib.load(), 64, 16, 1 << 20
+    lengths = [(97 * b) % 190 - 3 for b in range(sequences)]
+    lengths[sequences // 2] = longest
+    k, v, table = (t.cuda() for t in ref.make_pages([max(0, x + 1) for x in lengths], page, kvh, dim, torch.float16, 61))
+    q = torch.randn((sequences, 2 * kvh, dim), generator=torch.Generator().manual_seed(62)).half().cuda()
+    dl = i32(lengths)
+    need = lib.kv_paged_attention_scratch_bytes(sequences, 1, 2 * kvh, kvh, dim, page * table.shape[1])
+    assert need > 0 and need % 8 == 0
+    room = torch.full((2 * guard + need,), 0xA5, dtype=torch.uint8, device="cuda")
+    out = torch.zeros_like(q)
+    lib.pocketlm_set_stream(torch.cuda.current_stream().cuda_stream)
+    assert lib.kv_paged_attention_decode_u16(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), dl.data_ptr(), out.data_ptr(), room.data_ptr() + guard,
+        need, sequences, 1, 2 * kvh, kvh, dim, 2 * kvh * dim, 0, dim, table.shape[1], k.shape[0], page, k.stride(0),
+        k.stride(1), k.stride(2), 0.125, 0) == 0
+    assert torch.equal(out, nat.kv_paged_attention_decode(q, k, v, table, dl))
+    assert bool((room[:guard] == 0xA5).all()) and bool((room[guard + need:] == 0xA5).all())
