@@ -553,8 +553,21 @@ int launch_tile(const MatmulArgs& a, int shares, hipStream_t st) {
     if constexpr (!ONCE && 16 * TM * GM <= 64)
         if (a.n * a.k >= kStreamedBytes) return launch_tile<TN, TM, GN, GM, S, EXACT, true>(a, shares, st);
     using T = Tile<TN, TM, GN, GM, S>;
+    constexpr int64_t kMostTiles = 65535;  // of a grid's second dimension
+    if (plm::ceil_div(a.m, T::kM) > kMostTiles) {  // passes, one after another on the stream
+        for (int64_t m = 0; m < a.m; m += kMostTiles * T::kM) {
+            MatmulArgs part = a;
+            part.m = std::min(a.m - m, kMostTiles * T::kM);
+            part.x = a.x + m * a.k;
+            part.xs = a.xs + m * a.blocks;
+            part.out = static_cast<char*>(a.out) + m * a.n * (a.out_type == kOutF32 ? 4 : 2);
+            const int code = launch_tile<TN, TM, GN, GM, S, EXACT, ONCE>(part, shares, st);
+            if (code != 0) return code;
+        }
+        return 0;
+    }
     const int64_t gx = plm::ceil_div(a.n, T::kN), gy = plm::ceil_div(a.m, T::kM);
-    if (gx > 0x7FFFFFFF || gy > 65535) return plm::fail(-2, "too many rows");
+    if (gx > 0x7FFFFFFF) return plm::fail(-2, "too many weight rows");
     const void* fn = reinterpret_cast<const void*>(&fp8_matmul_tile_kernel<TN, TM, GN, GM, S, EXACT, ONCE>);
     int code = T::kLds > 64 * 1024 ? plm::allow_large_lds(fn, T::kLds) : 0;
     if (code != 0) return code;

@@ -158,3 +158,15 @@ def test_the_library_s_own_scratch(nat):
         assert lib.fp8_e4m3_block_matmul(x.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), out.data_ptr(), None,
                                          0, m, n, k, k // 128, 1) == 0
         assert torch.equal(out, want)
+
+
+def test_more_rows_than_a_grid_s_second_dimension_holds(nat):
+    """More than 65535 tiles of 128 rows (a long batch through a narrow weight)."""
+    m, n, k = 65535 * 128 + 300, 8, 16
+    x, xs, w, ws = make(251, n, k, 50)
+    of = torch.arange(m, device="cuda") % 251
+    got = nat.fp8_e4m3_block_matmul(nat.Fp8Rows(x.view(torch.uint8).cuda()[of], xs.cuda()[of]), w.cuda(), ws.cuda(),
+                                    out_dtype=torch.float32)
+    want, size = ref.matmul(x, xs, w, ws)
+    bound = ref.matmul_bound(want, size, x, xs, w, ws, torch.float32)
+    assert bool(((got.double() - want.cuda()[of]).abs() <= bound.cuda()[of]).all())
