@@ -544,14 +544,16 @@ __global__ __launch_bounds__(256) void fp8_matmul_join_kernel(const MatmulArgs a
 }
 
 // A weight of this size is not in the caches when the next call reads it (other weights come between), and
-// few rows read it once: its loads leave the caches to the activations.  64, 24 and 16 rows with 7168 x 16384:
-// 33.0, 27.9, 27.3 us without, 31.7, 25.7, 24.4 with; 64 x 7168 x 7168 18.9 without, 19.7 with.
+// where one group of rows reads it, it is read once: its loads leave the caches to the activations.  64, 24 and
+// 16 rows with 7168 x 16384: 33.0, 27.9, 27.3 us without, 31.7, 25.7, 24.4 with; 64 x 7168 x 7168 18.9 without,
+// 19.7 with.  Several groups find in the caches what the first of them read: 18 rows (two of 16) with
+// 12967 x 5936 42.8 us with, 32.2 without, 91 (two of 64) with 14964 x 6800 62.8 and 44.3.
 constexpr int64_t kStreamedBytes = static_cast<int64_t>(64) << 20;
 
 template <int TN, int TM, int GN, int GM, int S, bool EXACT = false, bool ONCE = false>
 int launch_tile(const MatmulArgs& a, int shares, hipStream_t st) {
     if constexpr (!ONCE && 16 * TM * GM <= 64)
-        if (a.n * a.k >= kStreamedBytes) return launch_tile<TN, TM, GN, GM, S, EXACT, true>(a, shares, st);
+        if (a.m <= 16 * TM * GM && a.n * a.k >= kStreamedBytes) return launch_tile<TN, TM, GN, GM, S, EXACT, true>(a, shares, st);
     using T = Tile<TN, TM, GN, GM, S>;
     constexpr int64_t kMostTiles = 65535;  // of a grid's second dimension
     if (plm::ceil_div(a.m, T::kM) > kMostTiles) {  // passes, one after another on the stream

@@ -170,3 +170,18 @@ def test_more_rows_than_a_grid_s_second_dimension_holds(nat):
     want, size = ref.matmul(x, xs, w, ws)
     bound = ref.matmul_bound(want, size, x, xs, w, ws, torch.float32)
     assert bool(((got.double() - want.cuda()[of]).abs() <= bound.cuda()[of]).all())
+
+
+@pytest.mark.parametrize("m,n,k,dtype", [
+    (18, 12967, 5936, torch.bfloat16), (91, 14964, 6800, torch.bfloat16), (128, 12332, 7728, torch.float16),
+    (420, 4202, 16352, torch.float32), (64, 37888, 3584, torch.bfloat16), (40, 33000, 2048, torch.float32),
+    (16, 33000, 2048, torch.bfloat16), (60, 24576, 4096, torch.bfloat16)])
+def test_large_weights_and_groups_of_rows(nat, m, n, k, dtype):
+    """Weights larger than the caches under one group of rows and several, in one share of the columns and several."""
+    x, xs, w, ws = make(m, n, k, m)
+    got = run(nat, x, xs, w, ws, dtype)
+    last = (n - 1) // 128
+    for rows, grid in ((slice(0, 256), ws[:2]), (slice(128 * (last // 2), 128 * (last // 2) + 128), ws[last // 2:last // 2 + 1]),
+                       (slice(128 * last, n), ws[last:])):
+        want, size = ref.matmul(x, xs, w[rows], grid)
+        ref.within(got[:, rows], want, ref.matmul_bound(want, size, x, xs, w[rows], grid, dtype))
