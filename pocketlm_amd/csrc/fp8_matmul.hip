@@ -277,6 +277,10 @@ __device__ __forceinline__ int swizzle_w(int row) {
 }
 __device__ __forceinline__ int swizzle_x(int row) { return row & 7; }
 
+// These loads take the LDS address from M0, which the compiler has to know as
+// written (it warns of any reserved register that is named so).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 // 16 bytes a lane from base + offset to LDS, the wave's KB in lane order at
 // `to`; ONCE: past the caches.  Not the compiler's builtin: it waits for every
 // load to LDS before any read of LDS, also of the other stage.  The wait is
@@ -287,12 +291,12 @@ __device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, u
         asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt"
                      :
                      : "v"(offset), "s"(base), "s"(to)
-                     : "memory");
+                     : "m0", "memory");
     else
         asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                      :
                      : "v"(offset), "s"(base), "s"(to)
-                     : "memory");
+                     : "m0", "memory");
 }
 // Four bytes each of the first LANES lanes.  All lanes are active before and after.
 template <int LANES>
@@ -302,8 +306,9 @@ __device__ __forceinline__ void load4_to_lds(const void* base, uint32_t offset, 
                  "s_mov_b64 exec, -1"
                  :
                  : "v"(offset), "s"(base), "s"(to), "s"((1ull << LANES) - 1)
-                 : "memory");
+                 : "m0", "memory");
 }
+#pragma clang diagnostic pop
 // Until all but the last LEFT of the wave's loads to LDS are there, then until
 // the workgroup's waves are here.  One statement: no read of LDS moves in
 // between.
