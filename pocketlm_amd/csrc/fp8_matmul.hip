@@ -115,8 +115,9 @@ __device__ __forceinline__ plm_f32x4 block_sums(const Operand<true>& a, const Op
 // wave order.  Lane l holds, of weight row (activation row) l & 15, the bytes
 // 16 (l >> 4) .. + 15 of each half of a block: the same columns on both
 // sides, which is all that the inner sum needs.  Operands go straight to
-// registers, P blocks ahead; bound by the latency of the few loads a wave has
-// (1 x 576 x 7168 6.6 us, 1 x 4096 x 4096 5.9).
+// registers, P blocks ahead once a wave's blocks beyond a multiple of P have
+// gone one at a time; bound by the latency of the few loads a wave has (1 x 576
+// x 7168 6.6 us, of whose 7 blocks a wave 3 go alone; 1 x 4096 x 4096 5.9).
 template <int TA, int TB, int P, int MAXW, bool EXACT>
 __global__ __launch_bounds__(64 * MAXW) void fp8_matmul_rows_kernel(const MatmulArgs a) {
     extern __shared__ plm_f32x4 red[];  // [wave][tile][lane]
@@ -219,12 +220,8 @@ template <int TA, int TB, int P, int MAXW, bool EXACT>
 int launch_rows(const MatmulArgs& a, int waves, hipStream_t st) {
     const int64_t gx = plm::ceil_div(a.n, 16 * TA), gy = plm::ceil_div(a.m, 16 * TB);
     if (gx > 0x7FFFFFFF || gy > 65535) return plm::fail(-2, "too many rows");
+    static_assert(MAXW * TA * TB * 1024 <= 64 * 1024, "LDS that needs no leave");
     const int bytes = waves * TA * TB * 1024;
-    const void* fn = reinterpret_cast<const void*>(&fp8_matmul_rows_kernel<TA, TB, P, MAXW, EXACT>);
-    if (bytes > 64 * 1024) {
-        const int code = plm::allow_large_lds(fn, MAXW * TA * TB * 1024);
-        if (code != 0) return code;
-    }
     const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(gy)), block(static_cast<unsigned>(64 * waves));
     hipLaunchKernelGGL((fp8_matmul_rows_kernel<TA, TB, P, MAXW, EXACT>), grid, block, static_cast<unsigned>(bytes), st, a);
     return plm::check_launch("fp8_e4m3_block_matmul");
