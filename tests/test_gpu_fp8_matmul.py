@@ -185,3 +185,21 @@ def test_large_weights_and_groups_of_rows(nat, m, n, k, dtype):
                        (slice(128 * last, n), ws[last:])):
         want, size = ref.matmul(x, xs, w[rows], grid)
         ref.within(got[:, rows], want, ref.matmul_bound(want, size, x, xs, w[rows], grid, dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,n,k", [(3, 50, 640), (12, 400, 16384), (40, 300, 2176), (64, 640, 16384), (300, 520, 1280),
+                                   (515, 6541, 896), (1947, 8779, 944)])
+def test_whole_numbers_are_exact_in_16_bits(nat, m, n, k, dtype):
+    """Small whole numbers and scales that are powers of two: no product of at
+    most 16 is cut off beside another, every sum is exact, and the result is
+    rounded once."""
+    g = torch.Generator().manual_seed(m)
+    x = torch.randint(-4, 5, (m, k), generator=g).float().to(torch.float8_e4m3fn)
+    w = torch.randint(-4, 5, (n, k), generator=g).float().to(torch.float8_e4m3fn)
+    xs = torch.exp2(torch.randint(-2, 3, (m, (k + 127) // 128), generator=g).float())
+    ws = torch.exp2(torch.randint(-2, 3, ((n + 127) // 128, (k + 127) // 128), generator=g).float())
+    want, size = ref.matmul(x, xs, w, ws)
+    # every partial sum is a multiple of 1/16 below 2^20: 24 bits hold it
+    assert float(size.max()) < 2 ** 20
+    assert torch.equal(run(nat, x, xs, w, ws, dtype).cpu(), want.to(dtype))

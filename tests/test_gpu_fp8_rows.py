@@ -155,3 +155,15 @@ def test_norm_of_rows_whose_squares_leave_fp32(nat, dtype, rows, cols):
     for eps in (0.0, 1e-6):
         got, _ = nat.fp8_e4m3_rms_norm_rows(x.cuda(), w.cuda(), rms_eps=eps)
         check_rows(got, ref.rms_norm(x, w, eps), NORM_OFF)
+
+
+def test_norm_rows_do_not_depend_on_the_batch(nat):
+    """A row's norm alone (one workgroup of many waves) and in a long prompt
+    (few waves): the order of the sum of squares differs, the bounds hold for
+    both and the scales agree within them."""
+    x, w = randn((1500, 896), torch.bfloat16, 14), randn((896,), torch.bfloat16, 15)
+    every, _ = nat.fp8_e4m3_rms_norm_rows(x.cuda(), w.cuda(), rms_eps=1e-6)
+    one, _ = nat.fp8_e4m3_rms_norm_rows(x[777:778].cuda(), w.cuda(), rms_eps=1e-6)
+    want = ref.rms_norm(x, w, 1e-6)
+    check_rows(every, want, NORM_OFF)
+    check_rows(one, want[777:778], NORM_OFF)

@@ -623,3 +623,20 @@ def test_attention_writes_within_its_scratch(nat, sequences, longest, kvh):
         k.stride(1), k.stride(2), 0.125, 0) == 0
     assert torch.equal(out, nat.kv_paged_attention_decode(q, k, v, table, dl))
     assert bool((room[:guard] == 0xA5).all()) and bool((room[guard + need:] == 0xA5).all())
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append_far_positions_store_their_keys(nat, interleaved):
+    """Keys and values of a position beyond 2^30, in caches of their own whose pages share one row."""
+    dim, far, page = 64, 2 ** 30 + 12345, 2 ** 20
+    rows = [torch.zeros((1, 1, 1, dim), dtype=torch.float16, device="cuda") for _ in range(2)]
+    k_cache, v_cache = (t.expand(1, page, 1, dim) for t in rows)
+    freq = nat.kv_rope_frequencies(dim, 1e6)
+    g = torch.Generator().manual_seed(3)
+    k, v = (torch.randn((1, 1, dim), generator=g).half() for _ in range(2))
+    table = torch.zeros((1, 2 ** 10 + 1), dtype=torch.int32, device="cuda")
+    nat.kv_paged_append(None, k.cuda(), v.cuda(), k_cache, v_cache, table, i32([far]), rope_frequencies=freq,
+                        interleaved=interleaved)
+    want, bound = ref.rotate(k[0], far, freq.cpu(), interleaved)
+    ref.within(rows[0][0, 0], want, bound + ref.HALF[torch.float16] * (want.abs() + bound) + ref.TINY[torch.float16])
+    assert torch.equal(rows[1][0].cpu(), v)
