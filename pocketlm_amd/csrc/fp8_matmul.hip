@@ -593,9 +593,20 @@ int launch_tile(const MatmulArgs& a, int shares, hipStream_t st) {
 //   tile   a workgroup's time per K block, alone on its compute unit or two on
 //          one, for the rounds that the grid takes; 8 us for launch, first loads
 //          and stores; at least the weight at 5.85 TB/s
+//          (read again by each group of rows where the weight's tiles alone fill
+//          the compute units: the groups come one after another then)
 //   shares of the blocks (for grids that leave compute units idle): 3.85 us for
 //          the join, its sums written and read at 3.6 TB/s
 //   rows   its waves' blocks, or the weight at 3.6 TB/s (3.0 above 8 rows)
+// Above 24576 weight rows the lines are carried on, checked at 51 sizes up to
+// 200000 weight rows and 391 rows: tiles of 32 and 64 rows run in rounds there
+// (64 x 36864 x 7168 74 us, with tiles of 16 rows 145; 64 x 129280 x 7168 181 and
+// 618; 32 x 37888 x 3584 34 and 45), and groups that read such a weight one after
+// another are fewer (391 x 33801 x 11568 with tiles of 256 rows 363, of 128 455).
+// EXACT products are chosen by the same lines, without the tile of 256 rows: an
+// EXACT block takes four instructions and its operands' conversion, which the
+// lines do not know (64 x 7168 x 16384 38.8 us, 2048 x 7168 x 7168 244, 4096 x 7168
+// x 16384 1047: 0.92 PFLOP/s of bf16 products).
 struct Choice {
     int tile;    // activation rows of a workgroup; 0: the rows kernel
     int shares;  // of the blocks
@@ -603,15 +614,14 @@ struct Choice {
 
 struct TileCost {
     int tile, weight_rows;
-    double alone, paired;  // paired 0: only grids of one workgroup per compute unit
+    double alone, paired;  // paired 0: one workgroup per compute unit at a time
 };
 constexpr TileCost kTileCosts[] = {
     {256, 256, 1.42, 0.0}, {128, 128, 0.64, 1.33}, {64, 128, 0.49, 0.0}, {32, 128, 0.48, 0.0}, {16, 128, 0.33, 0.72}};
 constexpr int kMostShares = 9;
 constexpr int kMostRows = 32;  // of the rows kernel
 
-// EXACT products take four instructions and their operands' conversion for one:
-// the tiles up to 128 rows have the registers for them.
+// EXACT: the tiles up to 128 rows have the registers for its operands.
 Choice choice_of(int64_t m, int64_t n, int64_t k, bool exact) {
     const int64_t blocks = plm::ceil_div(k, 128);
     const double bytes = static_cast<double>(n) * static_cast<double>(k);
@@ -624,18 +634,20 @@ Choice choice_of(int64_t m, int64_t n, int64_t k, bool exact) {
                          3.5 + bytes / (m <= 8 ? 3.6e6 : 3.0e6));
     for (const TileCost& c : kTileCosts) {
         if ((c.tile >= 2 * m && c.tile > 16) || (exact && c.tile == 256)) continue;
-        const int64_t tiles = plm::ceil_div(n, c.weight_rows) * plm::ceil_div(m, c.tile);
+        const int64_t along = plm::ceil_div(n, c.weight_rows), groups_of_rows = plm::ceil_div(m, c.tile);
+        const int64_t tiles = along * groups_of_rows;
+        const double reads = along > cus ? static_cast<double>(groups_of_rows) : 1.0;
         for (int64_t s = 1; s <= kMostShares && s <= blocks; ++s) {
             const int64_t groups = tiles * s, per = plm::ceil_div(blocks, s);
             double t = static_cast<double>(per) * c.alone;
-            if (c.tile == 256)
+            if (c.tile == 256 || (c.paired == 0.0 && s == 1 && groups_of_rows == 1))
                 t *= static_cast<double>(plm::ceil_div(groups, cus));
             else if (groups > cus && c.paired > 0.0)
                 t = static_cast<double>(per) * c.paired *
                     std::max(1.0, static_cast<double>(groups) / static_cast<double>(2 * cus));
             else if (groups > cus)
                 break;
-            t = std::max(t + 8.0, bytes / 5.85e6);
+            t = std::max(t + 8.0, reads * bytes / 5.85e6);
             if (s > 1) t += 3.85 + static_cast<double>(s * m) * static_cast<double>(n) * 8.0 / 3.6e6;
             if (t < least) {
                 least = t;

@@ -203,3 +203,17 @@ def test_whole_numbers_are_exact_in_16_bits(nat, m, n, k, dtype):
     # every partial sum is a multiple of 1/16 below 2^20: 24 bits hold it
     assert float(size.max()) < 2 ** 20
     assert torch.equal(run(nat, x, xs, w, ws, dtype).cpu(), want.to(dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m", [5, 17, 32, 33, 64, 200])
+@pytest.mark.parametrize("n,k", [(32769, 1040), (70000, 256)])
+def test_weights_of_more_tiles_than_compute_units(nat, m, n, k, dtype):
+    """Fused projections and vocabularies: several rounds of weight tiles."""
+    x, xs, w, ws = make(m, n, k, m)
+    got = run(nat, x, xs, w, ws, dtype)
+    assert got.shape == (m, n)
+    for first in (0, 128 * (n // 384), n // 128 * 128):
+        rows, grid = slice(first, min(first + 128, n)), ws[first // 128:first // 128 + 1]
+        want, size = ref.matmul(x, xs, w[rows], grid)
+        ref.within(got[:, rows], want, ref.matmul_bound(want, size, x, xs, w[rows], grid, dtype))
