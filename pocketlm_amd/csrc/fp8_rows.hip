@@ -61,6 +61,7 @@ struct RowsArgs {
     int64_t residual_stride;
     int blocks;          // scales per row
     int waves;           // per row
+    int rows_per;        // rows of a workgroup
     int vec;             // whole pieces, 16-byte aligned rows
     float eps;
 };
@@ -197,7 +198,7 @@ __global__ __launch_bounds__(kMaxThreads) void fp8_rows_kernel(const RowsArgs a)
     __shared__ float red[kMaxThreads / 64];
     __shared__ double red64[kMaxThreads / 64];
     const int wave = threadIdx.x >> 6;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x / (64 * a.waves)) + wave / a.waves;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * a.rows_per + wave / a.waves;
     const int t = threadIdx.x - wave / a.waves * a.waves * 64;
     const int step = a.waves * 64;
     const bool live = row < a.rows;
@@ -239,8 +240,7 @@ __global__ __launch_bounds__(kMaxThreads) void fp8_rows_kernel(const RowsArgs a)
         if (a.waves > 1) {
             if ((threadIdx.x & 63) == 0) red[wave] = total;
             __syncthreads();
-            const int rows = blockDim.x / (64 * a.waves);
-            for (int r = 0; r < rows; ++r) {
+            for (int r = 0; r < a.rows_per; ++r) {
                 float all = 0.0f;
                 for (int w = 0; w < a.waves; ++w) all += red[r * a.waves + w];
                 far |= beyond(all, a);
@@ -322,10 +322,10 @@ int run_rows(RowsArgs& a, int dtype_code, bool norm) {
     while (plm::ceil_div(pieces, steps) > kMaxThreads) steps *= 2;
     while (steps > 1 && pieces <= static_cast<int64_t>(64) * (steps / 2)) steps /= 2;
     a.waves = static_cast<int>(plm::ceil_div(plm::ceil_div(pieces, steps), 64));
-    const int rows_per = few ? 1 : (a.waves >= 4 ? 1 : 4 / a.waves);
-    const int64_t groups = plm::ceil_div(a.rows, rows_per);
+    a.rows_per = few ? 1 : (a.waves >= 4 ? 1 : 4 / a.waves);
+    const int64_t groups = plm::ceil_div(a.rows, a.rows_per);
     if (groups > 0x7FFFFFFF) return plm::fail(-2, "too many rows");
-    const dim3 grid(static_cast<unsigned>(groups)), block(static_cast<unsigned>(64 * a.waves * rows_per));
+    const dim3 grid(static_cast<unsigned>(groups)), block(static_cast<unsigned>(64 * a.waves * a.rows_per));
     const hipStream_t st = plm::current_stream();
     if (dtype_code == kF16)
         launch_steps<kF16>(a, steps, norm, grid, block, st);
