@@ -2013,7 +2013,10 @@ def fp8_e4m3_block_matmul(rows: Fp8Rows, fp8_weight: torch.Tensor, scale_inv: to
         x, xs, fp8_weight, scale_inv = (t.contiguous() for t in (x, xs, fp8_weight, scale_inv))
     x_ptr, w_ptr = x.data_ptr(), fp8_weight.data_ptr()
     if (x_ptr | w_ptr) & 15:  # the kernels read 16 bytes at a time
-        x, fp8_weight = x.clone(), fp8_weight.clone()
+        if x_ptr & 15:
+            x = x.clone()
+        if w_ptr & 15:
+            fp8_weight = fp8_weight.clone()
         x_ptr, w_ptr = x.data_ptr(), fp8_weight.data_ptr()
     device = x.device
     out = torch.empty((m, n), dtype=out_dtype, device=device)
@@ -2028,7 +2031,8 @@ def fp8_e4m3_block_matmul(rows: Fp8Rows, fp8_weight: torch.Tensor, scale_inv: to
 def kv_rope_frequencies(head_dim: int, rope_theta: float, *, device: torch.device | str | None = None) -> torch.Tensor:
     """The rotation's frequencies theta^(-2 i / head_dim) in float64, as
     kv_paged_append takes them (a caller may scale them, or pass fewer than
-    head_dim / 2 to rotate the first values of a head alone)."""
+    head_dim / 2 to rotate the first values of a head alone).  Made on the host
+    and copied: call it once, before a capture."""
     at = torch.arange(int(head_dim) // 2, dtype=torch.float64)
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
     return torch.pow(torch.tensor(float(rope_theta), dtype=torch.float64), -2.0 * at / int(head_dim)).to(device)

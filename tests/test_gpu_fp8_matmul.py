@@ -217,3 +217,16 @@ def test_weights_of_more_tiles_than_compute_units(nat, m, n, k, dtype):
         rows, grid = slice(first, min(first + 128, n)), ws[first // 128:first // 128 + 1]
         want, size = ref.matmul(x, xs, w[rows], grid)
         ref.within(got[:, rows], want, ref.matmul_bound(want, size, x, xs, w[rows], grid, dtype))
+
+
+def test_only_the_operand_at_an_odd_address_is_copied(nat):
+    m, n, k = 3, 4096, 2048
+    x, xs, w, ws = (t.cuda() for t in make(m, n, k, 31))
+    want = nat.fp8_e4m3_block_matmul(nat.Fp8Rows(x, xs), w, ws)
+    odd = torch.zeros(m * k + 1, dtype=torch.uint8, device="cuda")[1:].view(m, k)
+    odd.copy_(x.view(torch.uint8))
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    got = nat.fp8_e4m3_block_matmul(nat.Fp8Rows(odd, xs), w, ws)
+    assert torch.equal(got, want)
+    assert torch.cuda.max_memory_allocated() - before < n * k  # the rows, the result and the scratch
