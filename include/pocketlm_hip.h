@@ -805,7 +805,8 @@ int fp8_e4m3_rms_norm_rows(const void* x, const void* residual, const void* weig
 /* Such rows times an FP8 block-scaled weight:
  *   out[m][n] = sum_b x_scales[m][b] * scale_inv[n / 128][b]
  *               * sum_{k in block b} x[m][k] * W[n][k],
- * fp32 sums, rounded once to dtype_code.  x [rows][in_cols], x_scales
+ * fp32 sums, rounded once to dtype_code; the scales are multiplied with each
+ * other first, in fp32.  x [rows][in_cols], x_scales
  * [rows][ceil(in_cols / 128)], fp8_weight [out_rows][in_cols], scale_inv
  * [ceil(out_rows / 128)][scale_cols], out [rows][out_rows]; x and fp8_weight
  * 16-byte aligned (in_cols may be any; multiples of 16 are read in place,

@@ -497,7 +497,7 @@ constexpr uint32_t kNoRow = 0xFFFFFFFFu;
 // positions, 4 key-value heads of 128, 1.2 GB 212 us with the join, 5.7 TB/s.
 // Small calls are a chain of trips to memory, lengths, table, keys and values,
 // then the join: 700 positions 7.6 + 4.7 us, 6 sequences of up to 5000 positions
-// with 4 rows each, 49 MB, 17.8 + 5.1 us.
+// with 4 rows each, 49 MB, 18.6 + 5.0 us.
 //
 // DP: head_dim rounded up to 64, 128 or 256; EXACT: no rounding.  CT: blocks
 // of 16 columns, 1 or 2.  More have workgroups of their own which read the same

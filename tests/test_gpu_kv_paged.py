@@ -640,3 +640,30 @@ def test_append_far_positions_store_their_keys(nat, interleaved):
     want, bound = ref.rotate(k[0], far, freq.cpu(), interleaved)
     ref.within(rows[0][0, 0], want, bound + ref.HALF[torch.float16] * (want.abs() + bound) + ref.TINY[torch.float16])
     assert torch.equal(rows[1][0].cpu(), v)
+
+
+def test_captured_steps_with_an_idle_sequence(nat):
+    """The step with the lengths of live sequences advanced behind it, captured
+    once and replayed for five tokens: an idle sequence stays idle."""
+    eager, captured = Step(nat), Step(nat)
+    captured.k.copy_(eager.k)
+    captured.v.copy_(eager.v)
+
+    def step(of, x, lengths):
+        out = of(x, x, lengths.clone())
+        lengths += lengths >= 0
+        return out["out"]
+
+    x = torch.randn((5, 1, eager.hidden), generator=torch.Generator().manual_seed(71)).bfloat16().cuda()
+    lengths, glen, gx = i32([0, 100, -1, 31, 127]), i32([0, 100, -1, 31, 127]), x.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(captured, gx, glen)
+    for i in range(5):
+        want = step(eager, x, lengths)
+        gx.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, want) and torch.equal(captured.k, eager.k) and torch.equal(captured.v, eager.v)
+        assert lengths.tolist() == glen.tolist() == [i + 1, 101 + i, -1, 32 + i, 128 + i]
+        x = torch.randn((5, 1, eager.hidden), generator=torch.Generator().manual_seed(72 + i)).bfloat16().cuda()
