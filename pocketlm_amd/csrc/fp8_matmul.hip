@@ -555,7 +555,8 @@ constexpr int64_t kStreamedBytes = static_cast<int64_t>(64) << 20;
 template <int TN, int TM, int GN, int GM, int S, bool EXACT = false, bool ONCE = false>
 int launch_tile(const MatmulArgs& a, int shares, hipStream_t st) {
     if constexpr (!ONCE && 16 * TM * GM <= 64)
-        if (a.m <= 16 * TM * GM && a.n * a.k >= kStreamedBytes) return launch_tile<TN, TM, GN, GM, S, EXACT, true>(a, shares, st);
+        if (a.m <= 16 * TM * GM && a.n * a.k >= kStreamedBytes)
+            return launch_tile<TN, TM, GN, GM, S, EXACT, true>(a, shares, st);
     using T = Tile<TN, TM, GN, GM, S>;
     constexpr int64_t kMostTiles = 65535;  // of a grid's second dimension
     if (plm::ceil_div(a.m, T::kM) > kMostTiles) {  // passes, one after another on the stream

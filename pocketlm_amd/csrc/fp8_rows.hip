@@ -255,7 +255,10 @@ __global__ __launch_bounds__(kMaxThreads) void fp8_rows_kernel(const RowsArgs a)
 #pragma unroll
             for (int i = 0; i < NS; ++i)
 #pragma unroll
-                for (int j = 0; j < kPiece; ++j) wide = fma(static_cast<double>(h[i][j]), static_cast<double>(h[i][j]), wide);
+                for (int j = 0; j < kPiece; ++j) {
+                    const double v = h[i][j];
+                    wide = fma(v, v, wide);
+                }
             wide = wave_sum64(wide);
             if (a.waves > 1) {
                 if ((threadIdx.x & 63) == 0) red64[wave] = wide;

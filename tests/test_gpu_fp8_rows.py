@@ -142,7 +142,7 @@ def test_the_c_entry_adds_in_place(nat):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("rows,cols", [(5, 7168), (7, 129), (1030, 520), (1100, 100), (2, 20008), (1, 65536)])
+@pytest.mark.parametrize("rows,cols", [(5, 7168), (7, 129), (1030, 520), (1100, 100), (601, 1500), (2, 20008), (1, 65536)])
 def test_norm_of_rows_whose_squares_leave_fp32(nat, dtype, rows, cols):
     """Finite rows from near the type's largest value down to 2^-120, in one
     batch: the sum of squares passes fp32 both ways, y does not."""
