@@ -877,6 +877,90 @@ int kv_paged_attention_decode_u16(const uint16_t* q, const uint16_t* k_cache, co
 int64_t kv_paged_attention_scratch_bytes(int64_t sequences, int64_t rows, int64_t heads, int64_t kv_heads,
                                          int64_t head_dim, int64_t capacity);
 
+/* kv_paged_append_u16 with queries and keys normed head by head before their
+ * rotation:
+ *   y = x * rsqrt(mean(x^2) + rms_eps) * weight      over a head's head_dim values
+ * in fp32 (a sum of squares that leaves fp32's range in 64 bits), rounded once,
+ * after the rotation.  q_norm_weight and k_norm_weight [head_dim] share
+ * dtype_code and are 16-byte aligned (q_norm_weight may be NULL without
+ * queries); values v are not normed.  rms_eps >= 0.  Codes as there. */
+int kv_paged_norm_append_u16(const uint16_t* q, const uint16_t* k, const uint16_t* v, const uint16_t* q_norm_weight,
+                             const uint16_t* k_norm_weight, uint16_t* q_out, uint16_t* k_cache, uint16_t* v_cache,
+                             const int* page_table, const int* lengths, const int* row_starts,
+                             const double* rope_frequencies, int* rejected, int64_t rows, int64_t sequences,
+                             int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t rope_pairs, int interleaved,
+                             int64_t q_row_stride, int64_t q_head_stride, int64_t k_row_stride, int64_t k_head_stride,
+                             int64_t v_row_stride, int64_t v_head_stride, int64_t table_cols, int64_t num_pages,
+                             int64_t page_size, int64_t page_stride, int64_t slot_stride, int64_t head_stride,
+                             float rms_eps, int dtype_code);
+
+/* The same into a cache of e4m3 values with one fp32 scale for each position
+ * and key-value head:
+ *   scale = max(max |z| / 448, 2^-126),   byte = e4m3(z / scale), to nearest even,
+ * where z are the head's values in fp32, normed and rotated (a NULL weight: not
+ * normed), not rounded before.  A head that holds an infinity or a NaN gets the
+ * scale NaN and bytes 0x7F.  k_cache and v_cache are laid out as the 16-bit
+ * caches, with head_dim and the strides (in values) multiples of 16; the scale
+ * of slot s of page p and head h is k_scales[p * scale_page_stride + h *
+ * scale_head_stride + s], v_scales alike.  q, k, v, q_out and the weights are
+ * fp16 or bf16 (dtype_code).  Codes as there. */
+int kv_paged_append_e4m3(const uint16_t* q, const uint16_t* k, const uint16_t* v, const uint16_t* q_norm_weight,
+                         const uint16_t* k_norm_weight, uint16_t* q_out, uint8_t* k_cache, uint8_t* v_cache,
+                         float* k_scales, float* v_scales, const int* page_table, const int* lengths,
+                         const int* row_starts, const double* rope_frequencies, int* rejected, int64_t rows,
+                         int64_t sequences, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t rope_pairs,
+                         int interleaved, int64_t q_row_stride, int64_t q_head_stride, int64_t k_row_stride,
+                         int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride, int64_t table_cols,
+                         int64_t num_pages, int64_t page_size, int64_t page_stride, int64_t slot_stride,
+                         int64_t head_stride, int64_t scale_page_stride, int64_t scale_head_stride, float rms_eps,
+                         int dtype_code);
+
+/* kv_paged_attention_decode_u16 over such a cache: a key or value is its byte
+ * times its position's scale.  q and out are fp16 or bf16 (dtype_code); scratch
+ * of kv_paged_attention_scratch_bytes serves here too.  Codes as there. */
+int kv_paged_attention_decode_e4m3(const uint16_t* q, const uint8_t* k_cache, const uint8_t* v_cache,
+                                   const float* k_scales, const float* v_scales, const int* page_table,
+                                   const int* lengths, uint16_t* out, void* scratch, int64_t scratch_bytes,
+                                   int64_t sequences, int64_t rows, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                   int64_t q_seq_stride, int64_t q_row_stride, int64_t q_head_stride,
+                                   int64_t table_cols, int64_t num_pages, int64_t page_size, int64_t page_stride,
+                                   int64_t slot_stride, int64_t head_stride, int64_t scale_page_stride,
+                                   int64_t scale_head_stride, float softmax_scale, int dtype_code);
+
+/* Attention of any number of new rows of each sequence over its pages, after
+ * the append of the same rows with the same lengths and row_starts: row i of
+ * sequence b sees positions 0 .. lengths[b] + i, so a prompt into an empty
+ * sequence (length 0) is causal attention, and chunks of it and single tokens
+ * may share a call.
+ *   out[r][h] = softmax(q[r][h] . K * softmax_scale) V
+ * with the key-value head h / (heads / kv_heads).  q [rows][heads][head_dim]
+ * with strides in values (multiples of 8), out contiguous; sequence b has rows
+ * [row_starts[b], row_starts[b + 1]) (int32 [sequences + 1], ascending, on the
+ * device).  Rows of no sequence or of an idle one are zero, as is a row that
+ * sees nothing; positions without a page are left out, those past the table
+ * too.  What a row does not see never reaches it, NaN or not.  Softmax weights
+ * are rounded once to the cache's type (bf16 for e4m3 caches).  scratch: device
+ * memory of kv_paged_attention_chunk_scratch_bytes, 16-byte aligned, or NULL
+ * for the library's own; capacity is table_cols * page_size.  rows * heads <
+ * 2^31.  Codes -1 null, -2 bad dimensions, -3 scratch. */
+int kv_paged_attention_chunk_u16(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,
+                                 const int* page_table, const int* lengths, const int* row_starts, uint16_t* out,
+                                 void* scratch, int64_t scratch_bytes, int64_t rows, int64_t sequences, int64_t heads,
+                                 int64_t kv_heads, int64_t head_dim, int64_t q_row_stride, int64_t q_head_stride,
+                                 int64_t table_cols, int64_t num_pages, int64_t page_size, int64_t page_stride,
+                                 int64_t slot_stride, int64_t head_stride, float softmax_scale, int dtype_code);
+/* The same over an e4m3 cache. */
+int kv_paged_attention_chunk_e4m3(const uint16_t* q, const uint8_t* k_cache, const uint8_t* v_cache,
+                                  const float* k_scales, const float* v_scales, const int* page_table,
+                                  const int* lengths, const int* row_starts, uint16_t* out, void* scratch,
+                                  int64_t scratch_bytes, int64_t rows, int64_t sequences, int64_t heads,
+                                  int64_t kv_heads, int64_t head_dim, int64_t q_row_stride, int64_t q_head_stride,
+                                  int64_t table_cols, int64_t num_pages, int64_t page_size, int64_t page_stride,
+                                  int64_t slot_stride, int64_t head_stride, int64_t scale_page_stride,
+                                  int64_t scale_head_stride, float softmax_scale, int dtype_code);
+int64_t kv_paged_attention_chunk_scratch_bytes(int64_t sequences, int64_t rows, int64_t heads, int64_t kv_heads,
+                                               int64_t head_dim, int64_t capacity);
+
 #ifdef __cplusplus
 }
 #endif

@@ -150,6 +150,12 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "kv_paged_append_u16": (_i32, [_vp] * 11 + [_i64] * 6 + [_i32] + [_i64] * 12 + [_i32]),
     "kv_paged_attention_decode_u16": (_i32, [_vp] * 7 + [_i64] * 15 + [_f32, _i32]),
     "kv_paged_attention_scratch_bytes": (_i64, [_i64] * 6),
+    "kv_paged_norm_append_u16": (_i32, [_vp] * 13 + [_i64] * 6 + [_i32] + [_i64] * 12 + [_f32, _i32]),
+    "kv_paged_append_e4m3": (_i32, [_vp] * 15 + [_i64] * 6 + [_i32] + [_i64] * 14 + [_f32, _i32]),
+    "kv_paged_attention_decode_e4m3": (_i32, [_vp] * 9 + [_i64] * 17 + [_f32, _i32]),
+    "kv_paged_attention_chunk_u16": (_i32, [_vp] * 8 + [_i64] * 14 + [_f32, _i32]),
+    "kv_paged_attention_chunk_e4m3": (_i32, [_vp] * 10 + [_i64] * 16 + [_f32, _i32]),
+    "kv_paged_attention_chunk_scratch_bytes": (_i64, [_i64] * 6),
 }
 
 _LIB: ctypes.CDLL | None = None

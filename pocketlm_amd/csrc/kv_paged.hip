@@ -10,76 +10,11 @@
 #include <cmath>
 #include <type_traits>
 
-#include "common.h"
+#include "kv_paged.h"
 
 namespace {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef float f32x8 __attribute__((ext_vector_type(8)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-    const f32x2 v = {a, b};
-    if constexpr (BF16)
-        return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
-    else
-        return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
-}
-
-template <bool BF16>
-__device__ __forceinline__ f32x8 widen8(u32x4 v) {
-    if constexpr (BF16)
-        return __builtin_convertvector(__builtin_bit_cast(bf16x8, v), f32x8);
-    else
-        return __builtin_convertvector(__builtin_bit_cast(f16x8, v), f32x8);
-}
-
-template <bool BF16>
-__device__ __forceinline__ u32x4 narrow8(const f32x8 v) {
-    if constexpr (BF16)
-        return __builtin_bit_cast(u32x4, __builtin_convertvector(v, bf16x8));
-    else
-        return __builtin_bit_cast(u32x4, __builtin_convertvector(v, f16x8));
-}
-
-template <bool BF16>
-__device__ __forceinline__ float widen1(uint16_t v) {
-    if constexpr (BF16)
-        return __uint_as_float(static_cast<uint32_t>(v) << 16);
-    else
-        return static_cast<float>(__builtin_bit_cast(_Float16, v));
-}
-
-template <bool BF16>
-__device__ __forceinline__ uint16_t narrow1(float v) {
-    if constexpr (BF16)
-        return __builtin_bit_cast(uint16_t, static_cast<__bf16>(v));
-    else
-        return __builtin_bit_cast(uint16_t, static_cast<_Float16>(v));
-}
-
-// Where the pages are.  Strides in pieces of 8 values (16 bytes): 32 bits
-// reach 64 GiB; the head's offset is added in 64 bits.
-struct Pages {
-    uint16_t* k;
-    uint16_t* v;
-    const int* table;    // [sequences][table_cols]
-    const int* lengths;  // [sequences]
-    int64_t head_stride;  // values
-    uint32_t page_stride;
-    uint32_t slot_stride;
-    uint32_t page_size;
-    uint32_t num_pages;
-    int table_cols;
-    int sequences;
-};
+using namespace plm_paged;
 
 // ---------------------------------------------------------------- append
 
@@ -138,38 +73,11 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(const Appe
         if constexpr (!ANY) x1 = *reinterpret_cast<const u32x4*>(src + at1);
     }
 
-    // the row's sequence and position
-    int seq;
-    int64_t in_seq;
-    if (a.row_starts != nullptr) {
-        int count = 0;  // starts at or before the row
-        for (int base = 0; base <= a.p.sequences; base += 64) {
-            const int i = base + lane;
-            const bool before = i <= a.p.sequences && a.row_starts[min(i, a.p.sequences)] <= row;
-            count += __popcll(__ballot(before));
-        }
-        seq = count - 1;
-        in_seq = seq >= 0 ? row - a.row_starts[min(seq, a.p.sequences)] : 0;
-    } else {
-        seq = static_cast<int>(row / a.rows_per_sequence);
-        in_seq = row - static_cast<int64_t>(seq) * a.rows_per_sequence;
-    }
-    const bool in_batch = seq >= 0 && seq < a.p.sequences;
-    const int length = in_batch ? a.p.lengths[seq] : -1;
-    const int64_t pos = length >= 0 ? length + in_seq : -1;
-    const bool placed = pos >= 0;
-    bool stored = false;
-    uint32_t off = 0;
-    if (placed) {
-        const int64_t index = pos / a.p.page_size;
-        if (index < a.p.table_cols) {
-            const int page = a.p.table[static_cast<int64_t>(seq) * a.p.table_cols + index];
-            stored = page >= 0 && static_cast<uint32_t>(page) < a.p.num_pages;
-            off = static_cast<uint32_t>(page) * a.p.page_stride +
-                  static_cast<uint32_t>(pos - index * a.p.page_size) * a.p.slot_stride;
-        }
-        if (!stored && a.rejected != nullptr && threadIdx.x == 0 && blockIdx.y == 0) atomicAdd(a.rejected, 1);
-    }
+    const Place at = place_of(a.p, a.row_starts, a.rows_per_sequence, row, lane);
+    const int64_t pos = at.pos;
+    const bool placed = pos >= 0, stored = at.stored;
+    const uint32_t off = at.page * a.p.page_stride + at.slot * a.p.slot_stride;
+    if (placed && !stored && a.rejected != nullptr && threadIdx.x == 0 && blockIdx.y == 0) atomicAdd(a.rejected, 1);
     if constexpr (MODE != kCopy) {
         for (int i = threadIdx.x; i < a.pairs; i += blockDim.x) {
             constexpr double kTurn = 6.283185307179586476925286766559;
@@ -269,6 +177,7 @@ constexpr uint32_t kUnevenHalves = 3, kUnevenUnits = 12, kUnevenUnitsHalf = 8;
 
 struct AttnArgs {
     Pages p;
+    Scales s;          // of e4m3 caches
     const uint16_t* q;
     uint16_t* out;     // [sequences][rows][heads][head_dim]
     float* part;       // [slot][head and column block][column][head_dim], then the maxima and sums
@@ -420,33 +329,6 @@ __device__ __forceinline__ bool find_plan(const AttnArgs& a, int lane, uint32_t 
     return false;
 }
 
-__device__ __forceinline__ float swap_max(float v) {
-    // over the four lanes l, l ^ 16, l ^ 32, l ^ 48
-    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = fmaxf(__uint_as_float(h[0]), __uint_as_float(h[1]));
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float swap_sum(float v) {
-    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(h[0]) + __uint_as_float(h[1]);
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
-template <bool BF16>
-__device__ __forceinline__ f32x4 mfma16(const u32x4 a, const u32x4 b, const f32x4 c) {
-    if constexpr (BF16)
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
-                                                       0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
-                                                      0, 0);
-}
-
-// exp2(x - m) for a running maximum that may be -inf (nothing seen yet).
-__device__ __forceinline__ float exp2_from(float x, float m) { return exp2f(x - (m == -INFINITY ? 0.0f : m)); }
-
 // Two weights as sums of two values of the cache's type each: cut off, so that
 // the rest is not negative, and the rest, rounded; together they keep 15 bits
 // (fp16 21) of each weight.  The rest of a weight above 0 is not 0: times an
@@ -504,14 +386,24 @@ constexpr uint32_t kNoRow = 0xFFFFFFFFu;
 // through an L2 that they share: with 4 in a workgroup, one wave a SIMD, 8 rows
 // of 7 heads took 29 us for 700 positions and 137 for 50 sequences of 4000, now
 // 17 and 108.
-template <bool BF16, int DP, bool EXACT, int CT>
+//
+// E8: caches of e4m3 values.  A value is exact in fp16 and bf16, so keys become
+// the queries' type in registers, a score is multiplied by its position's key
+// scale, a weight by the value scale in fp32 before it is halved, and values
+// and weights are bf16 whatever the queries' type, whose range a weight times a
+// scale may leave.  A lane's keys are 16 adjacent values (32 s + 8 g of the
+// 16-bit caches become 64 (s / 2) + 16 g + 8 (s % 2), of the queries as well).
+// Each lane holds a scale of the tile: lanes 0 to 31 the keys', the others the
+// values'.
+template <bool BF16, bool E8, int DP, bool EXACT, int CT>
 __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void paged_attention_kernel(
     const AttnArgs a) {
+    constexpr bool VBF16 = BF16 || E8;        // the values' type
     constexpr int KS = DP / 32;               // score steps of 32 head values
     constexpr int NV = DP / 16;               // value instructions
     constexpr int PV = DP == 64 ? 4 : 8;      // adjacent head values of a lane
     constexpr int SETS = NV / PV;             // pieces of a lane per position
-    constexpr float kBias = BF16 ? 0.0f : 15.0f;
+    constexpr float kBias = VBF16 ? 0.0f : 15.0f;
     __shared__ float meet[2][CT * (NV * 4 + 2)][64];  // at most 35 KB
     __shared__ uint32_t held[kHeld];
     const int lane = threadIdx.x & 63;
@@ -572,14 +464,19 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void paged_atten
             limit[t] = col < a.columns ? static_cast<int>(seen_of(length, r + 1, a.capacity)) : 0;
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
-                const int d = 32 * s + 8 * g;
+                const int d = E8 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g;
                 q[t][s] = *reinterpret_cast<const u32x4*>(src + (EXACT || d < a.head_dim ? d : 0));
                 if (col >= a.columns || (!EXACT && d >= a.head_dim)) q[t][s] = u32x4{0, 0, 0, 0};
             }
         }
         const int least = static_cast<int>(seen_of(length, 1, a.capacity));  // what every row sees
-        const uint16_t* kbase = a.p.k + kvh * a.p.head_stride;
-        const uint16_t* vbase = a.p.v + kvh * a.p.head_stride;
+        // (rows in pieces of 16 bytes behind them)
+        const uint16_t* kbase = E8 ? reinterpret_cast<const uint16_t*>(reinterpret_cast<const uint8_t*>(a.p.k) +
+                                                                       kvh * a.p.head_stride)
+                                   : a.p.k + kvh * a.p.head_stride;
+        const uint16_t* vbase = E8 ? reinterpret_cast<const uint16_t*>(reinterpret_cast<const uint8_t*>(a.p.v) +
+                                                                       kvh * a.p.head_stride)
+                                   : a.p.v + kvh * a.p.head_stride;
         const int* table = a.p.table + static_cast<int64_t>(seq) * a.p.table_cols;
 
         float m[CT], l[CT];
@@ -603,19 +500,37 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void paged_atten
             const bool there = pos < end && page >= 0 && static_cast<uint32_t>(page) < a.p.num_pages;
             return there ? static_cast<uint32_t>(page) * a.p.page_stride + slot * a.p.slot_stride : kNoRow;
         };
-        u32x4 k[2][KS];
-        u32x4 v[8][SETS];
+        // this lane's scale of a tile (of a position that is not there: 0)
+        auto scale_of = [&](int page, int t0) {
+            const int pos = t0 + (lane & 31);
+            const uint32_t slot = static_cast<uint32_t>(pos) % a.p.page_size;
+            const bool there = pos < end && page >= 0 && static_cast<uint32_t>(page) < a.p.num_pages;
+            const float* from = lane < 32 ? a.s.k : a.s.v;
+            return there ? from[page * a.s.page_stride + kvh * a.s.head_stride + slot] : 0.0f;
+        };
+        u32x4 k[2][E8 ? KS / 2 : KS];
+        std::conditional_t<E8, u32x2, u32x4> v[8][SETS];
         auto load_k = [&](uint32_t row) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const uint32_t o = __shfl(row, 16 * i + li);
                 // a position that is not there reads the cache's first row; its score is replaced
                 const uint16_t* src = kbase + static_cast<int64_t>(o == kNoRow ? 0u : o) * 8;
+                if constexpr (E8) {
 #pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    const int d = 32 * s + 8 * g;
-                    k[i][s] = *reinterpret_cast<const u32x4*>(src + (EXACT || d < a.head_dim ? d : 0));
-                    if (!EXACT && d >= a.head_dim) k[i][s] = u32x4{0, 0, 0, 0};
+                    for (int s = 0; s < KS / 2; ++s) {
+                        const int d = 64 * s + 16 * g;
+                        k[i][s] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint8_t*>(src) +
+                                                                  (EXACT || d < a.head_dim ? d : 0));
+                        if (!EXACT && d >= a.head_dim) k[i][s] = u32x4{0, 0, 0, 0};
+                    }
+                } else {
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) {
+                        const int d = 32 * s + 8 * g;
+                        k[i][s] = *reinterpret_cast<const u32x4*>(src + (EXACT || d < a.head_dim ? d : 0));
+                        if (!EXACT && d >= a.head_dim) k[i][s] = u32x4{0, 0, 0, 0};
+                    }
                 }
             }
         };
@@ -630,14 +545,25 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void paged_atten
                 for (int s = 0; s < SETS; ++s) {
                     const int d = PV * li + 128 * s;
                     const uint16_t* at = src + (EXACT || d < a.head_dim ? d : 0);
-                    if constexpr (PV == 8) {
+                    if constexpr (E8) {
+                        const uint8_t* at8 =
+                            reinterpret_cast<const uint8_t*>(src) + (EXACT || d < a.head_dim ? d : 0);
+                        if constexpr (PV == 8)
+                            v[j][s] = past ? __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(at8))
+                                           : *reinterpret_cast<const u32x2*>(at8);
+                        else
+                            v[j][s] = u32x2{*reinterpret_cast<const uint32_t*>(at8), 0};
+                        if (!EXACT && d >= a.head_dim) v[j][s] = u32x2{0, 0};
+                        continue;
+                    } else if constexpr (PV == 8) {
                         v[j][s] = past ? __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at))
                                        : *reinterpret_cast<const u32x4*>(at);
                     } else {
                         const u32x2 two = *reinterpret_cast<const u32x2*>(at);
                         v[j][s] = u32x4{two.x, two.y, 0, 0};
                     }
-                    if (!EXACT && d >= a.head_dim) v[j][s] = u32x4{0, 0, 0, 0};
+                    if constexpr (!E8)
+                        if (!EXACT && d >= a.head_dim) v[j][s] = u32x4{0, 0, 0, 0};
                 }
             }
         };
@@ -646,19 +572,30 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void paged_atten
             const uint32_t pick = (i & 1) ? 0x07060302u : 0x05040100u;
             u32x4 t;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) t[j] = __builtin_amdgcn_perm(v[2 * j + 1][s][i >> 1], v[2 * j][s][i >> 1], pick);
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (E8)
+                    t[j] = __builtin_amdgcn_perm(pair_of<true>(v[2 * j + 1][s][i >> 2], (i >> 1) & 1),
+                                                 pair_of<true>(v[2 * j][s][i >> 2], (i >> 1) & 1), pick);
+                else
+                    t[j] = __builtin_amdgcn_perm(v[2 * j + 1][s][i >> 1], v[2 * j][s][i >> 1], pick);
+            }
             return t;
         };
 
         int t0 = begin + 32 * wave;
         if (t0 < end) {
-            uint32_t row = row_of(page_of(t0), t0);
+            int page = page_of(t0);
+            uint32_t row = row_of(page, t0);
+            float held_scale = 0.0f;
+            if constexpr (E8) held_scale = scale_of(page, t0);
             load_k(row);
             load_v(row, std::false_type{});
-            int page = page_of(t0 + kUnit);
+            page = page_of(t0 + kUnit);
             for (; t0 < end; t0 += kUnit) {
                 // past the range: no position is there, every lane reads the cache's first row
                 const uint32_t next = row_of(page, t0 + kUnit);
+                float next_scale = 0.0f;
+                if constexpr (E8) next_scale = scale_of(page, t0 + kUnit);
                 page = page_of(t0 + 2 * kUnit);
                 f32x4 s[CT][2];
 #pragma unroll
@@ -667,12 +604,29 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void paged_atten
                     for (int i = 0; i < 2; ++i) {
                         s[t][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                        for (int x = 0; x < KS; ++x) s[t][i] = mfma16<BF16>(k[i][x], q[t][x], s[t][i]);
+                        for (int x = 0; x < KS; ++x) {
+                            if constexpr (E8)
+                                s[t][i] = mfma16<BF16>(eight_of<BF16>(k[i][x >> 1], x & 1), q[t][x], s[t][i]);
+                            else
+                                s[t][i] = mfma16<BF16>(k[i][x], q[t][x], s[t][i]);
+                        }
                     }
+                float vscale[8];
+                if constexpr (E8) {
 #pragma unroll
-                for (int t = 0; t < CT; ++t)
+                    for (int j = 0; j < 8; ++j) {
+                        const int at = (j < 4 ? 0 : 12) + 4 * g + j;
+                        const float kscale = __shfl(held_scale, at) * a.scale;
+                        vscale[j] = __shfl(held_scale, 32 + at);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) s[t][i] = s[t][i] * a.scale;
+                        for (int t = 0; t < CT; ++t) s[t][j >> 2][j & 3] *= kscale;
+                    }
+                } else {
+#pragma unroll
+                    for (int t = 0; t < CT; ++t)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) s[t][i] = s[t][i] * a.scale;
+                }
                 __builtin_amdgcn_sched_barrier(0);
                 load_k(next);
                 const bool full = t0 + 32 <= least && __all(row != kNoRow);
@@ -692,6 +646,13 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void paged_atten
                             else
                                 floor[t] = -FLT_MAX;
                         }
+                }
+                if constexpr (E8) {
+                    // of what some row does not see: its scale may be anything, its values are cleared below
+                    if (!full)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (t0 + (j < 4 ? 0 : 12) + 4 * g + j >= least || vrow[j] == kNoRow) vscale[j] = 0.0f;
                 }
                 u32x4 w[CT], w_low[CT];
 #pragma unroll
@@ -716,7 +677,9 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void paged_atten
                     for (int i = 0; i < NV; ++i) acc[t][i] = acc[t][i] * fade;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const Halves x = halves<BF16>(s[t][i >> 1][2 * (i & 1)], s[t][i >> 1][2 * (i & 1) + 1]);
+                        float w0 = s[t][i >> 1][2 * (i & 1)], w1 = s[t][i >> 1][2 * (i & 1) + 1];
+                        if constexpr (E8) w0 *= vscale[2 * i], w1 *= vscale[2 * i + 1];
+                        const Halves x = halves<VBF16>(w0, w1);
                         w[t][i] = x.high;
                         w_low[t][i] = x.low;
                     }
@@ -740,7 +703,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void paged_atten
 #pragma unroll
                         for (int t = 0; t < CT; ++t)
                             acc[t][PV * x + i] =
-                                mfma16<BF16>(values, w_low[t], mfma16<BF16>(values, w[t], acc[t][PV * x + i]));
+                                mfma16<VBF16>(values, w_low[t], mfma16<VBF16>(values, w[t], acc[t][PV * x + i]));
                     }
                 // the positions that some of the rows see, at most rows - 1 of them, one at a time
                 for (int pos = max(least, t0); pos < min(t0 + 32, seen); ++pos) {
@@ -748,6 +711,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void paged_atten
                     if (there == kNoRow) continue;
                     const int at = pos - t0, from = (at & 12) * 4 + li;  // the lane that has this column's weight of it
                     u32x4 value[SETS][4];
+                    float by = 1.0f;
+                    if constexpr (E8) by = __shfl(held_scale, 32 + pos - t0);
                     const uint16_t* src = vbase + static_cast<int64_t>(there) * 8;
 #pragma unroll
                     for (int x = 0; x < SETS; ++x)
@@ -755,7 +720,11 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void paged_atten
                         for (int j = 0; j < 4; ++j) {
                             const int d = PV * (4 * g + j) + 128 * x;
                             const uint16_t* piece = src + (EXACT || d < a.head_dim ? d : 0);
-                            if constexpr (PV == 8) {
+                            if constexpr (E8) {
+                                const uint32_t* piece8 = reinterpret_cast<const uint32_t*>(
+                                    reinterpret_cast<const uint8_t*>(src) + (EXACT || d < a.head_dim ? d : 0));
+                                value[x][j] = eight_of<true>(u32x4{piece8[0], PV == 8 ? piece8[1] : 0, 0, 0}, 0);
+                            } else if constexpr (PV == 8) {
                                 value[x][j] = *reinterpret_cast<const u32x4*>(piece);
                             } else {
                                 const u32x2 two = *reinterpret_cast<const u32x2*>(piece);
@@ -767,13 +736,13 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void paged_atten
                         float p = s[t][0][0];
 #pragma unroll
                         for (int j = 1; j < 8; ++j) p = (at >> 4) * 4 + (at & 3) == j ? s[t][j >> 2][j & 3] : p;
-                        p = __shfl(p, from);
+                        p = __shfl(p, from) * by;
                         const bool sees = pos < limit[t];
 #pragma unroll
                         for (int x = 0; x < SETS; ++x)
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
-                                const f32x8 f = widen8<BF16>(value[x][j]);
+                                const f32x8 f = widen8<VBF16>(value[x][j]);
 #pragma unroll
                                 for (int i = 0; i < PV; ++i) {
                                     const float was = acc[t][PV * x + i][j];
@@ -791,6 +760,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void paged_atten
                     load_v(next, std::false_type{});
                 }
                 row = next;
+                held_scale = next_scale;
             }
         }
 #pragma unroll
@@ -983,42 +953,6 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(const AttnArgs
 
 // ---------------------------------------------------------------- host side
 
-constexpr int64_t kMostInt = 0x7FFFFFFF;
-// Positions are ints, and the attention looks two units ahead of its last one.
-constexpr int64_t kMostPositions = kMostInt - 1023;
-
-// The checks and layout that both calls share; 0, or the code of the failure.
-int pages_of(Pages& p, void* k_cache, void* v_cache, const int* page_table, const int* lengths, int64_t sequences,
-             int64_t table_cols, int64_t num_pages, int64_t page_size, int64_t kv_heads, int64_t head_dim,
-             int64_t page_stride, int64_t slot_stride, int64_t head_stride, int dtype_code) {
-    if (k_cache == nullptr || v_cache == nullptr || page_table == nullptr || lengths == nullptr)
-        return plm::fail(-1, "null pointer");
-    if (sequences <= 0 || table_cols <= 0 || num_pages <= 0 || page_size <= 0 || kv_heads <= 0 || head_dim <= 0 ||
-        sequences > 65535 || kv_heads > 65535 || num_pages > kMostInt || page_size > kMostInt ||
-        table_cols > kMostPositions / page_size || (dtype_code != 0 && dtype_code != 1))
-        return plm::fail(-2, "bad dimensions");
-    if (head_dim % 8 != 0 || head_dim > 256) return plm::fail(-2, "head_dim must be a multiple of 8 up to 256");
-    if (page_stride < 0 || slot_stride < 0 || head_stride < 0 || page_stride % 8 != 0 || slot_stride % 8 != 0 ||
-        head_stride % 8 != 0 || !plm::aligned16(k_cache) || !plm::aligned16(v_cache))
-        return plm::fail(-2, "cache strides and addresses must be multiples of 16 bytes");
-    const double last = static_cast<double>(num_pages - 1) * static_cast<double>(page_stride / 8) +
-                        static_cast<double>(page_size - 1) * static_cast<double>(slot_stride / 8);
-    if (last >= 4294967295.0 || head_stride > (static_cast<int64_t>(1) << 40))
-        return plm::fail(-2, "a cache spans at most 64 GiB");
-    p = Pages{static_cast<uint16_t*>(k_cache),
-              static_cast<uint16_t*>(v_cache),
-              page_table,
-              lengths,
-              head_stride,
-              static_cast<uint32_t>(page_stride / 8),
-              static_cast<uint32_t>(slot_stride / 8),
-              static_cast<uint32_t>(page_size),
-              static_cast<uint32_t>(num_pages),
-              static_cast<int>(table_cols),
-              static_cast<int>(sequences)};
-    return 0;
-}
-
 template <bool BF16>
 void launch_append(const AppendArgs& a, int mode, dim3 grid, dim3 block, hipStream_t st) {
     switch (mode) {
@@ -1078,11 +1012,12 @@ AttnShape shape_of(int64_t sequences, int64_t rows, int64_t heads, int64_t kv_he
     return s;
 }
 
-template <bool BF16>
+template <bool BF16, bool E8>
 void launch_attention(const AttnArgs& a, const AttnShape& s, hipStream_t st) {
     const dim3 grid(static_cast<unsigned>(s.runs * a.kv_heads * a.column_blocks)), block(64 * kAttnWaves);
     const int d = a.head_dim;
-#define PLM_ATTN(DP, EXACT, CT) hipLaunchKernelGGL((paged_attention_kernel<BF16, DP, EXACT, CT>), grid, block, 0, st, a)
+#define PLM_ATTN(DP, EXACT, CT) \
+    hipLaunchKernelGGL((paged_attention_kernel<BF16, E8, DP, EXACT, CT>), grid, block, 0, st, a)
     if (s.ct == 2) {
         if (d == 64)
             PLM_ATTN(64, true, 2);
@@ -1115,6 +1050,59 @@ void launch_attention(const AttnArgs& a, const AttnShape& s, hipStream_t st) {
 
 bool bad_heads(int64_t rows, int64_t heads, int64_t kv_heads) {
     return rows <= 0 || rows > kMaxQueryRows || heads <= 0 || heads > 65535 || kv_heads <= 0 || heads % kv_heads != 0;
+}
+
+// What both entry points check and launch once the caches are known.
+template <bool E8>
+int run_decode(AttnArgs& a, const uint16_t* q, uint16_t* out, void* scratch, int64_t scratch_bytes, int64_t sequences,
+               int64_t rows, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t q_seq_stride,
+               int64_t q_row_stride, int64_t q_head_stride, float softmax_scale, int dtype_code, const char* name) {
+    if (bad_heads(rows, heads, kv_heads)) return plm::fail(-2, "bad dimensions");
+    if (!plm::aligned16(q) || !plm::aligned16(out) || q_seq_stride < 0 || q_row_stride < 0 || q_head_stride < 0 ||
+        q_seq_stride % 8 != 0 || q_row_stride % 8 != 0 || q_head_stride % 8 != 0)
+        return plm::fail(-2, "query strides and addresses must be multiples of 16 bytes");
+    a.capacity = static_cast<int64_t>(a.p.table_cols) * a.p.page_size;
+    const AttnShape s = shape_of(sequences, rows, heads, kv_heads, head_dim, a.capacity);
+    if (sequences * plm::ceil_div(a.capacity, kUnit) > kMostInt / 4 ||
+        s.runs * kv_heads * s.column_blocks > kMostInt || sequences * rows * heads > kMostInt)
+        return plm::fail(-2, "too many sequences, heads or pages");
+    void* part = scratch;
+    if (s.bytes > 0) {
+        if (scratch == nullptr) {
+            part = plm::workspace(s.bytes);
+            if (part == nullptr) return -3;
+        } else if (scratch_bytes < static_cast<int64_t>(s.bytes) || !plm::aligned16(scratch)) {
+            return plm::fail(-3, "scratch must hold kv_paged_attention_scratch_bytes, 16-byte aligned");
+        }
+    }
+    a.q = q;
+    a.out = out;
+    a.q_seq = q_seq_stride;
+    a.q_row = q_row_stride;
+    a.q_head = q_head_stride;
+    a.rows = static_cast<int>(rows);
+    a.heads = static_cast<int>(heads);
+    a.kv_heads = static_cast<int>(kv_heads);
+    a.group = static_cast<int>(heads / kv_heads);
+    a.head_dim = static_cast<int>(head_dim);
+    a.columns = a.rows * a.group;
+    a.column_blocks = s.column_blocks;
+    a.budget = static_cast<uint32_t>(s.budget);
+    a.short_runs = static_cast<uint32_t>(s.short_runs);
+    a.single = s.single ? 1 : 0;
+    a.uneven = s.uneven;
+    a.streamed = static_cast<uint32_t>(kStreamedBytes / (kUnit * (E8 ? 2 : 4) * kv_heads * head_dim));
+    a.scale = softmax_scale * 1.44269504088896340736f;
+    a.part = static_cast<float*>(part);
+    a.part_ml = a.part + s.slots * kv_heads * s.column_blocks * s.ct * 16 * head_dim;
+    // whole vectors of 16 bytes before it: 16 columns or more of head_dim + 2 values
+    a.plan = s.joined ? reinterpret_cast<uint4*>(a.part_ml + s.slots * kv_heads * s.column_blocks * s.ct * 32) : nullptr;
+    const hipStream_t st = plm::current_stream();
+    if (dtype_code == 1)
+        launch_attention<true, E8>(a, s, st);
+    else
+        launch_attention<false, E8>(a, s, st);
+    return plm::check_launch(name);
 }
 
 }  // namespace
@@ -1201,50 +1189,28 @@ PLM_EXPORT int kv_paged_attention_decode_u16(const uint16_t* q, const uint16_t* 
                               sequences, table_cols, num_pages, page_size, kv_heads, head_dim, page_stride, slot_stride,
                               head_stride, dtype_code);
     if (code != 0) return code;
-    if (bad_heads(rows, heads, kv_heads)) return plm::fail(-2, "bad dimensions");
-    if (!plm::aligned16(q) || !plm::aligned16(out) || q_seq_stride < 0 || q_row_stride < 0 || q_head_stride < 0 ||
-        q_seq_stride % 8 != 0 || q_row_stride % 8 != 0 || q_head_stride % 8 != 0)
-        return plm::fail(-2, "query strides and addresses must be multiples of 16 bytes");
-    a.capacity = table_cols * page_size;
-    const AttnShape s = shape_of(sequences, rows, heads, kv_heads, head_dim, a.capacity);
-    if (sequences * plm::ceil_div(a.capacity, kUnit) > kMostInt / 4 ||
-        s.runs * kv_heads * s.column_blocks > kMostInt || sequences * rows * heads > kMostInt)
-        return plm::fail(-2, "too many sequences, heads or pages");
-    void* part = scratch;
-    if (s.bytes > 0) {
-        if (scratch == nullptr) {
-            part = plm::workspace(s.bytes);
-            if (part == nullptr) return -3;
-        } else if (scratch_bytes < static_cast<int64_t>(s.bytes) || !plm::aligned16(scratch)) {
-            return plm::fail(-3, "scratch must hold kv_paged_attention_scratch_bytes, 16-byte aligned");
-        }
-    }
-    a.q = q;
-    a.out = out;
-    a.q_seq = q_seq_stride;
-    a.q_row = q_row_stride;
-    a.q_head = q_head_stride;
-    a.rows = static_cast<int>(rows);
-    a.heads = static_cast<int>(heads);
-    a.kv_heads = static_cast<int>(kv_heads);
-    a.group = static_cast<int>(heads / kv_heads);
-    a.head_dim = static_cast<int>(head_dim);
-    a.columns = a.rows * a.group;
-    a.column_blocks = s.column_blocks;
-    a.budget = static_cast<uint32_t>(s.budget);
-    a.short_runs = static_cast<uint32_t>(s.short_runs);
-    a.single = s.single ? 1 : 0;
-    a.uneven = s.uneven;
-    a.streamed = static_cast<uint32_t>(kStreamedBytes / (kUnit * 4 * kv_heads * head_dim));
-    a.scale = softmax_scale * 1.44269504088896340736f;
-    a.part = static_cast<float*>(part);
-    a.part_ml = a.part + s.slots * kv_heads * s.column_blocks * s.ct * 16 * head_dim;
-    // whole vectors of 16 bytes before it: 16 columns or more of head_dim + 2 values
-    a.plan = s.joined ? reinterpret_cast<uint4*>(a.part_ml + s.slots * kv_heads * s.column_blocks * s.ct * 32) : nullptr;
-    const hipStream_t st = plm::current_stream();
-    if (dtype_code == 1)
-        launch_attention<true>(a, s, st);
-    else
-        launch_attention<false>(a, s, st);
-    return plm::check_launch("kv_paged_attention_decode_u16");
+    return run_decode<false>(a, q, out, scratch, scratch_bytes, sequences, rows, heads, kv_heads, head_dim, q_seq_stride,
+                             q_row_stride, q_head_stride, softmax_scale, dtype_code, "kv_paged_attention_decode_u16");
+}
+
+PLM_EXPORT int kv_paged_attention_decode_e4m3(const uint16_t* q, const uint8_t* k_cache, const uint8_t* v_cache,
+                                              const float* k_scales, const float* v_scales, const int* page_table,
+                                              const int* lengths, uint16_t* out, void* scratch, int64_t scratch_bytes,
+                                              int64_t sequences, int64_t rows, int64_t heads, int64_t kv_heads,
+                                              int64_t head_dim, int64_t q_seq_stride, int64_t q_row_stride,
+                                              int64_t q_head_stride, int64_t table_cols, int64_t num_pages,
+                                              int64_t page_size, int64_t page_stride, int64_t slot_stride,
+                                              int64_t head_stride, int64_t scale_page_stride, int64_t scale_head_stride,
+                                              float softmax_scale, int dtype_code) {
+    if (q == nullptr || out == nullptr) return plm::fail(-1, "null pointer");
+    AttnArgs a = {};
+    int code = pages_of<16>(a.p, const_cast<uint8_t*>(k_cache), const_cast<uint8_t*>(v_cache), page_table, lengths,
+                            sequences, table_cols, num_pages, page_size, kv_heads, head_dim, page_stride, slot_stride,
+                            head_stride, dtype_code);
+    if (code != 0) return code;
+    code = scales_of(a.s, const_cast<float*>(k_scales), const_cast<float*>(v_scales), scale_page_stride,
+                     scale_head_stride);
+    if (code != 0) return code;
+    return run_decode<true>(a, q, out, scratch, scratch_bytes, sequences, rows, heads, kv_heads, head_dim, q_seq_stride,
+                            q_row_stride, q_head_stride, softmax_scale, dtype_code, "kv_paged_attention_decode_e4m3");
 }

@@ -2059,6 +2059,10 @@ def _check_pages(what: str, k_cache, v_cache, page_table, lengths):
         raise TypeError(f"{what} requires torch.float16 or torch.bfloat16 caches")
     if v_cache.dtype != dtype:
         raise TypeError(f"{what} requires caches to share dtype")
+    return (dtype, code, *_check_page_shapes(k_cache, v_cache, page_table, lengths))
+
+
+def _check_page_shapes(k_cache, v_cache, page_table, lengths):
     if page_table.dtype != torch.int32 or lengths.dtype != torch.int32:
         raise TypeError("page_table and lengths must be torch.int32")
     shape, stride = tuple(k_cache.shape), k_cache.stride()
@@ -2069,7 +2073,63 @@ def _check_pages(what: str, k_cache, v_cache, page_table, lengths):
         raise ValueError("page_table must have shape [sequences, pages], lengths one entry per sequence")
     if not page_table.is_contiguous() or not lengths.is_contiguous():
         raise ValueError("page_table and lengths must be contiguous")
-    return dtype, code, shape, stride
+    return shape, stride
+
+
+def _check_e4m3_pages(what: str, rows, k_cache, v_cache, k_scales, v_scales, page_table, lengths):
+    """As _check_pages, for e4m3 caches: (the rows' dtype, its code, the caches' sizes and strides, the scales')."""
+    if k_cache.dtype not in _FP8_DTYPES or v_cache.dtype != k_cache.dtype:
+        raise TypeError(f"{what} requires caches of torch.float8_e4m3fn or of torch.uint8 raw e4m3 bytes")
+    if k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32:
+        raise TypeError("FP8 scales must be torch.float32")
+    dtype = rows.dtype
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"{what} requires torch.float16 or torch.bfloat16 rows")
+    shape, stride = _check_page_shapes(k_cache, v_cache, page_table, lengths)
+    pages, page_size, kv_heads, _ = shape
+    scale_stride = k_scales.stride()
+    if (k_scales.shape != (pages, kv_heads, page_size) or v_scales.shape != k_scales.shape
+            or v_scales.stride() != scale_stride or (scale_stride[2] != 1 and page_size != 1)):
+        raise ValueError("scales must have shape [pages, kv_heads, page_size], the same strides and adjacent slots")
+    return dtype, _ROW_CODES[dtype], shape, stride, scale_stride
+
+
+def _check_append(what: str, dtype, q, k, v, shape, page_table, row_starts, rope_frequencies, rejected):
+    """Checks of the appends' rows; (rows, query heads, rotated pairs)."""
+    if k.dtype != dtype or v.dtype != dtype or (q is not None and q.dtype != dtype):
+        raise TypeError(f"{what} requires {dtype} rows")
+    _, _, kv_heads, head_dim = shape
+    k_shape = k.shape
+    if len(k_shape) != 3 or k_shape[1] != kv_heads or k_shape[2] != head_dim or v.shape != k_shape:
+        raise ValueError("k and v must have shape [rows, kv_heads, head_dim]")
+    rows, sequences, heads = k_shape[0], page_table.shape[0], 0
+    if q is not None:
+        q_shape = q.shape
+        if len(q_shape) != 3 or q_shape[0] != rows or q_shape[2] != head_dim:
+            raise ValueError("q must have shape [rows, heads, head_dim]")
+        heads = q_shape[1]
+    if row_starts is None:
+        if rows % sequences if sequences else rows:
+            raise ValueError("rows must be a multiple of the sequences (or give row_starts)")
+    else:
+        _check_row_starts(row_starts, sequences)
+    pairs = 0
+    if rope_frequencies is not None:
+        if rope_frequencies.dtype != torch.float64:
+            raise TypeError("rope_frequencies must be torch.float64")
+        pairs = rope_frequencies.numel()
+        if rope_frequencies.ndim != 1 or not rope_frequencies.is_contiguous() or 2 * pairs > head_dim:
+            raise ValueError("rope_frequencies must hold at most head_dim / 2 values")
+    if rejected is not None and (rejected.dtype != torch.int32 or rejected.numel() != 1):
+        raise TypeError("rejected must be one torch.int32 value")
+    return rows, heads, pairs
+
+
+def _check_row_starts(row_starts, sequences: int) -> None:
+    if row_starts.dtype != torch.int32:
+        raise TypeError("row_starts must be torch.int32")
+    if row_starts.shape != (sequences + 1,) or not row_starts.is_contiguous():
+        raise ValueError("row_starts must hold sequences + 1 entries")
 
 
 def kv_paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
@@ -2092,35 +2152,11 @@ def kv_paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_
     advanced."""
     lib = _paged_lib()
     dtype, code, shape, stride = _check_pages("kv_paged_append", k_cache, v_cache, page_table, lengths)
-    if k.dtype != dtype or v.dtype != dtype or (q is not None and q.dtype != dtype):
-        raise TypeError(f"kv_paged_append requires {dtype} rows")
+    rows, heads, pairs = _check_append("kv_paged_append", dtype, q, k, v, shape, page_table, row_starts,
+                                       rope_frequencies, rejected)
     pages, page_size, kv_heads, head_dim = shape
-    k_shape = k.shape
-    if len(k_shape) != 3 or k_shape[1] != kv_heads or k_shape[2] != head_dim or v.shape != k_shape:
-        raise ValueError("k and v must have shape [rows, kv_heads, head_dim]")
-    rows, (sequences, table_cols) = k_shape[0], page_table.shape
-    q_out, heads, qs = None, 0, (0, 0)
-    if q is not None:
-        q_shape = q.shape
-        if len(q_shape) != 3 or q_shape[0] != rows or q_shape[2] != head_dim:
-            raise ValueError("q must have shape [rows, heads, head_dim]")
-        heads = q_shape[1]
-    if row_starts is None:
-        if rows % sequences if sequences else rows:
-            raise ValueError("rows must be a multiple of the sequences (or give row_starts)")
-    elif row_starts.dtype != torch.int32:
-        raise TypeError("row_starts must be torch.int32")
-    elif row_starts.shape != (sequences + 1,) or not row_starts.is_contiguous():
-        raise ValueError("row_starts must hold sequences + 1 entries")
-    pairs = 0
-    if rope_frequencies is not None:
-        if rope_frequencies.dtype != torch.float64:
-            raise TypeError("rope_frequencies must be torch.float64")
-        pairs = rope_frequencies.numel()
-        if rope_frequencies.ndim != 1 or not rope_frequencies.is_contiguous() or 2 * pairs > head_dim:
-            raise ValueError("rope_frequencies must hold at most head_dim / 2 values")
-    if rejected is not None and (rejected.dtype != torch.int32 or rejected.numel() != 1):
-        raise TypeError("rejected must be one torch.int32 value")
+    sequences, table_cols = page_table.shape
+    q_out, qs = None, (0, 0)
     index = _on_device("kv_paged_append", k_cache, v_cache, q, k, v, page_table, lengths, row_starts, rope_frequencies,
                        rejected)
     k, v = _rows_of_heads(k), _rows_of_heads(v)
@@ -2182,4 +2218,222 @@ def kv_paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: t
               nbytes, sequences, rows, heads, kv_heads, head_dim, qs[0], qs[1] if len(q_shape) == 4 else 0, qs[-2],
               table_cols, pages, page_size, stride[0], stride[1], stride[2],
               head_dim ** -0.5 if softmax_scale is None else softmax_scale, code)
+    return out
+
+
+def _check_norm_weight(what: str, weight, dtype, head_dim: int):
+    """A norm's weight in place where the kernels can read it, else a copy."""
+    if weight is None:
+        return None
+    if weight.dtype != dtype:
+        raise TypeError(f"{what} requires {dtype} norm weights")
+    if weight.shape != (head_dim,):
+        raise ValueError("norm weights must hold one value per head value")
+    if weight.data_ptr() & 15 or not weight.is_contiguous():
+        weight = weight.clone(memory_format=torch.contiguous_format)
+    return weight
+
+
+def kv_paged_norm_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, q_norm_weight: torch.Tensor | None,
+                         k_norm_weight: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                         page_table: torch.Tensor, lengths: torch.Tensor, *, rms_eps: float,
+                         row_starts: torch.Tensor | None = None, rope_frequencies: torch.Tensor | None = None,
+                         interleaved: bool = False, rejected: torch.Tensor | None = None) -> torch.Tensor | None:
+    """kv_paged_append with the RMS norm of each query and key head before its
+    rotation, in the same pass: x * rsqrt(mean(x^2) + rms_eps) * weight in fp32,
+    rounded once, after the rotation.  Weights [head_dim] share the rows' dtype
+    (q_norm_weight may be None without q); values are not normed."""
+    what = "kv_paged_norm_append"
+    lib = _paged_lib()
+    dtype, code, shape, stride = _check_pages(what, k_cache, v_cache, page_table, lengths)
+    rows, heads, pairs = _check_append(what, dtype, q, k, v, shape, page_table, row_starts, rope_frequencies, rejected)
+    pages, page_size, kv_heads, head_dim = shape
+    sequences, table_cols = page_table.shape
+    if k_norm_weight is None or (heads and q_norm_weight is None):
+        raise TypeError(f"{what} requires norm weights (kv_paged_append is the call without)")
+    if not rms_eps >= 0.0:
+        raise ValueError("rms_eps must not be negative")
+    index = _on_device(what, k_cache, v_cache, q, k, v, q_norm_weight, k_norm_weight, page_table, lengths, row_starts,
+                       rope_frequencies, rejected)
+    q_weight = _check_norm_weight(what, q_norm_weight, dtype, head_dim)
+    k_weight = _check_norm_weight(what, k_norm_weight, dtype, head_dim)
+    k, v = _rows_of_heads(k), _rows_of_heads(v)
+    ks, vs = k.stride(), v.stride()
+    q_out, qs = None, (0, 0)
+    if q is not None:
+        q = _rows_of_heads(q)
+        qs = q.stride()
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if rows:
+        _call(lib, index, "kv_paged_norm_append_u16", q.data_ptr() if heads else None, k.data_ptr(), v.data_ptr(),
+              _p(q_weight), k_weight.data_ptr(), q_out.data_ptr() if heads else None, k_cache.data_ptr(),
+              v_cache.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), _p(row_starts),
+              _p(rope_frequencies) if pairs else None, _p(rejected), rows, sequences, heads, kv_heads, head_dim, pairs,
+              1 if interleaved else 0, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], table_cols, pages, page_size, stride[0],
+              stride[1], stride[2], rms_eps, code)
+    return q_out
+
+
+def kv_paged_append_e4m3(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
+                         v_cache: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
+                         page_table: torch.Tensor, lengths: torch.Tensor, *, q_norm_weight: torch.Tensor | None = None,
+                         k_norm_weight: torch.Tensor | None = None, rms_eps: float = 0.0,
+                         row_starts: torch.Tensor | None = None, rope_frequencies: torch.Tensor | None = None,
+                         interleaved: bool = False, rejected: torch.Tensor | None = None) -> torch.Tensor | None:
+    """kv_paged_append (or, with norm weights, kv_paged_norm_append) into caches
+    of e4m3 values [pages, page_size, kv_heads, head_dim] (float8_e4m3fn, or
+    uint8 bytes) with a scale for each position and head, float32 [pages,
+    kv_heads, page_size]: max|z| / 448 of the head's fp32 values z, which are
+    not rounded before.  head_dim is a multiple of 16; q, k, v and the weights
+    are fp16 or bf16, the queries returned too."""
+    what = "kv_paged_append_e4m3"
+    lib = _paged_lib()
+    dtype, code, shape, stride, scale_stride = _check_e4m3_pages(what, k, k_cache, v_cache, k_scales, v_scales, page_table,
+                                                                 lengths)
+    rows, heads, pairs = _check_append(what, dtype, q, k, v, shape, page_table, row_starts, rope_frequencies, rejected)
+    pages, page_size, kv_heads, head_dim = shape
+    sequences, table_cols = page_table.shape
+    if not rms_eps >= 0.0:
+        raise ValueError("rms_eps must not be negative")
+    index = _on_device(what, k_cache, v_cache, k_scales, v_scales, q, k, v, q_norm_weight, k_norm_weight, page_table,
+                       lengths, row_starts, rope_frequencies, rejected)
+    q_weight = _check_norm_weight(what, q_norm_weight, dtype, head_dim)
+    k_weight = _check_norm_weight(what, k_norm_weight, dtype, head_dim)
+    k, v = _rows_of_heads(k), _rows_of_heads(v)
+    ks, vs = k.stride(), v.stride()
+    q_out, qs = None, (0, 0)
+    if q is not None:
+        q = _rows_of_heads(q)
+        qs = q.stride()
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if rows:
+        _call(lib, index, "kv_paged_append_e4m3", q.data_ptr() if heads else None, k.data_ptr(), v.data_ptr(),
+              _p(q_weight), _p(k_weight), q_out.data_ptr() if heads else None, k_cache.data_ptr(), v_cache.data_ptr(),
+              k_scales.data_ptr(), v_scales.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), _p(row_starts),
+              _p(rope_frequencies) if pairs else None, _p(rejected), rows, sequences, heads, kv_heads, head_dim, pairs,
+              1 if interleaved else 0, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], table_cols, pages, page_size, stride[0],
+              stride[1], stride[2], scale_stride[0], scale_stride[1], rms_eps, code)
+    return q_out
+
+
+def kv_paged_attention_decode_e4m3(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                                   k_scales: torch.Tensor, v_scales: torch.Tensor, page_table: torch.Tensor,
+                                   lengths: torch.Tensor, *, softmax_scale: float | None = None) -> torch.Tensor:
+    """kv_paged_attention_decode over the caches and scales of
+    kv_paged_append_e4m3; q fp16 or bf16, as the result."""
+    what = "kv_paged_attention_decode_e4m3"
+    lib = _paged_lib()
+    _, code, shape, stride, scale_stride = _check_e4m3_pages(what, q, k_cache, v_cache, k_scales, v_scales, page_table,
+                                                             lengths)
+    pages, page_size, kv_heads, head_dim = shape
+    sequences, table_cols = page_table.shape
+    q_shape = q.shape
+    if len(q_shape) not in (3, 4) or q_shape[0] != sequences or q_shape[-1] != head_dim:
+        raise ValueError("q must have shape [sequences, heads, head_dim] or [sequences, rows, heads, head_dim]")
+    rows = 1 if len(q_shape) == 3 else q_shape[1]
+    heads = q_shape[-2]
+    if not 1 <= rows <= 8:
+        raise ValueError(f"{what} takes 1 to 8 rows of a sequence")
+    if kv_heads == 0 or heads % kv_heads or not heads:
+        raise ValueError("heads must be a multiple of kv_heads")
+    index = _on_device(what, k_cache, v_cache, k_scales, v_scales, q, page_table, lengths)
+    q = _rows_of_heads(q)
+    qs, device = q.stride(), q.device
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if sequences:
+        nbytes = _attention_scratch(sequences, rows, heads, kv_heads, head_dim, table_cols * page_size, index)
+        scratch = torch.empty((nbytes,), dtype=torch.uint8, device=device) if nbytes > 0 else None
+        _call(lib, index, "kv_paged_attention_decode_e4m3", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+              k_scales.data_ptr(), v_scales.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), out.data_ptr(),
+              None if scratch is None else scratch.data_ptr(), nbytes, sequences, rows, heads, kv_heads, head_dim, qs[0],
+              qs[1] if len(q_shape) == 4 else 0, qs[-2], table_cols, pages, page_size, stride[0], stride[1], stride[2],
+              scale_stride[0], scale_stride[1], head_dim ** -0.5 if softmax_scale is None else softmax_scale, code)
+    return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _chunk_scratch(sequences: int, rows: int, heads: int, kv_heads: int, head_dim: int, capacity: int,
+                   device_index: int) -> int:
+    with torch.cuda.device(device_index):
+        return int(_lib.load().kv_paged_attention_chunk_scratch_bytes(sequences, rows, heads, kv_heads, head_dim,
+                                                                      capacity))
+
+
+def _check_chunk(q, shape, page_table, row_starts) -> int:
+    """Checks of a chunk's queries; their heads."""
+    _, _, kv_heads, head_dim = shape
+    q_shape = q.shape
+    if len(q_shape) != 3 or q_shape[2] != head_dim:
+        raise ValueError("q must have shape [rows, heads, head_dim]")
+    heads = q_shape[1]
+    if kv_heads == 0 or heads % kv_heads or not heads:
+        raise ValueError("heads must be a multiple of kv_heads")
+    _check_row_starts(row_starts, page_table.shape[0])
+    return heads
+
+
+def kv_paged_attention_chunk(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                             lengths: torch.Tensor, row_starts: torch.Tensor, *,
+                             softmax_scale: float | None = None) -> torch.Tensor:
+    """Attention of any number of new rows of each sequence over its pages, after
+    kv_paged_append (or kv_paged_norm_append) of the same rows with the same
+    page_table, lengths and row_starts: row i of sequence b sees the positions up
+    to lengths[b] + i.  Whole prompts (lengths 0), chunks of them and single
+    tokens may share a call.
+
+    q [rows, heads, head_dim], row_starts int32 [sequences + 1]; the result has
+    q's shape.  softmax_scale: head_dim ** -0.5 by default.  Rows of idle
+    sequences (negative lengths) and of none get zeros."""
+    what = "kv_paged_attention_chunk"
+    lib = _paged_lib()
+    dtype, code, shape, stride = _check_pages(what, k_cache, v_cache, page_table, lengths)
+    if q.dtype != dtype:
+        raise TypeError(f"{what} requires {dtype} queries")
+    heads = _check_chunk(q, shape, page_table, row_starts)
+    pages, page_size, kv_heads, head_dim = shape
+    sequences, table_cols = page_table.shape
+    index = _on_device(what, k_cache, v_cache, q, page_table, lengths, row_starts)
+    q = _rows_of_heads(q)
+    rows, qs, device = q.shape[0], q.stride(), q.device
+    if not sequences:
+        return torch.zeros_like(q, memory_format=torch.contiguous_format)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if rows:
+        nbytes = _chunk_scratch(sequences, rows, heads, kv_heads, head_dim, table_cols * page_size, index)
+        scratch = torch.empty((nbytes,), dtype=torch.uint8, device=device) if nbytes > 0 else None
+        _call(lib, index, "kv_paged_attention_chunk_u16", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+              page_table.data_ptr(), lengths.data_ptr(), row_starts.data_ptr(), out.data_ptr(),
+              None if scratch is None else scratch.data_ptr(), nbytes, rows, sequences, heads, kv_heads, head_dim, qs[0],
+              qs[1], table_cols, pages, page_size, stride[0], stride[1], stride[2],
+              head_dim ** -0.5 if softmax_scale is None else softmax_scale, code)
+    return out
+
+
+def kv_paged_attention_chunk_e4m3(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                                  k_scales: torch.Tensor, v_scales: torch.Tensor, page_table: torch.Tensor,
+                                  lengths: torch.Tensor, row_starts: torch.Tensor, *,
+                                  softmax_scale: float | None = None) -> torch.Tensor:
+    """kv_paged_attention_chunk over the caches and scales of
+    kv_paged_append_e4m3; q fp16 or bf16, as the result."""
+    what = "kv_paged_attention_chunk_e4m3"
+    lib = _paged_lib()
+    _, code, shape, stride, scale_stride = _check_e4m3_pages(what, q, k_cache, v_cache, k_scales, v_scales, page_table,
+                                                             lengths)
+    heads = _check_chunk(q, shape, page_table, row_starts)
+    pages, page_size, kv_heads, head_dim = shape
+    sequences, table_cols = page_table.shape
+    index = _on_device(what, k_cache, v_cache, k_scales, v_scales, q, page_table, lengths, row_starts)
+    q = _rows_of_heads(q)
+    rows, qs, device = q.shape[0], q.stride(), q.device
+    if not sequences:
+        return torch.zeros_like(q, memory_format=torch.contiguous_format)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if rows:
+        nbytes = _chunk_scratch(sequences, rows, heads, kv_heads, head_dim, table_cols * page_size, index)
+        scratch = torch.empty((nbytes,), dtype=torch.uint8, device=device) if nbytes > 0 else None
+        _call(lib, index, "kv_paged_attention_chunk_e4m3", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+              k_scales.data_ptr(), v_scales.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), row_starts.data_ptr(),
+              out.data_ptr(), None if scratch is None else scratch.data_ptr(), nbytes, rows, sequences, heads, kv_heads,
+              head_dim, qs[0], qs[1], table_cols, pages, page_size, stride[0], stride[1], stride[2], scale_stride[0],
+              scale_stride[1], head_dim ** -0.5 if softmax_scale is None else softmax_scale, code)
     return out
