@@ -223,10 +223,15 @@ __device__ __forceinline__ float both_sum(float v) {
     return __uint_as_float(h[0]) + __uint_as_float(h[1]);
 }
 
-// A 16-byte piece of a row of LDS is kept at piece ^ swizzle(row): the eight
-// rows whose pieces are read together as keys lie in eight groups of banks, and
-// the four whose 32 bytes are read together, transposed, as values in four.
-__device__ __forceinline__ int swizzle(int row) { return (row & 3) << 1 | (row >> 2 & 1); }
+// A 16-byte piece of a row of LDS is kept at piece ^ swizzle(row), so that what is
+// read together touches every group of banks (a line of 256 bytes) once: the same
+// piece of 16 adjacent rows for keys, four adjacent pieces of four rows,
+// transposed, for values.  Where a line holds two rows, their lowest bit is one
+// of the line's.
+template <int DP>
+__device__ __forceinline__ int swizzle(int row) {
+    return DP == 64 ? (row >> 1 & 1) << 2 | (row >> 2 & 3) : (row & 3) << 2 | (row >> 2 & 3);
+}
 
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
@@ -370,6 +375,8 @@ __global__ __launch_bounds__(64 * kWaves, (DP >= 128 && CB == 2) || DP > 128 ? 1
     constexpr int COLS = 32 * CB * kWaves;
     constexpr int KS = DP / 16;   // score steps
     constexpr int DB = DP / 32;   // blocks of head values
+    constexpr int kLines = KS < 8 ? KS : 8;  // score steps whose pieces lie in one line of 256 bytes
+    constexpr int kAhead = 6;
     constexpr float kBias = bias_of(VBF16);
     extern __shared__ char lds_raw[];
     lds_char* const lds = (lds_char*)lds_raw;
@@ -386,14 +393,17 @@ __global__ __launch_bounds__(64 * kWaves, (DP >= 128 && CB == 2) || DP > 128 ? 1
 
     const int columns = piece.rows * a.group;
     const int col0 = piece.tile * COLS;
-    const int seen = seen_by(a, piece.length, (min(col0 + COLS, columns) - 1) / a.group);
-    const int least = seen_by(a, piece.length, col0 / a.group);  // what every column sees
+    auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    const int seen = uniform(seen_by(a, piece.length, (min(col0 + COLS, columns) - 1) / a.group));
+    const int least = uniform(seen_by(a, piece.length, col0 / a.group));  // what every column sees
     const uint32_t units = tiles_of(seen, kTile);
-    const int begin = static_cast<int>(static_cast<uint64_t>(units) * piece.split / piece.splits) * kTile;
-    const int end = min(seen, static_cast<int>(static_cast<uint64_t>(units) * (piece.split + 1) / piece.splits) * kTile);
+    const int begin = uniform(static_cast<int>(static_cast<uint64_t>(units) * piece.split / piece.splits) * kTile);
+    const int end = uniform(
+        min(seen, static_cast<int>(static_cast<uint64_t>(units) * (piece.split + 1) / piece.splits) * kTile));
     const int wave0 = col0 + 32 * CB * wave;
-    const int wave_least = seen_by(a, piece.length, min(wave0, columns - 1) / a.group);
-    const int wave_seen = wave0 < columns ? seen_by(a, piece.length, (min(wave0 + 32 * CB, columns) - 1) / a.group) : 0;
+    const int wave_least = uniform(seen_by(a, piece.length, min(wave0, columns - 1) / a.group));
+    const int wave_seen =
+        wave0 < columns ? uniform(seen_by(a, piece.length, (min(wave0 + 32 * CB, columns) - 1) / a.group)) : 0;
 
     u32x4 q[CB][KS];
     int limit[CB];
@@ -426,18 +436,20 @@ __global__ __launch_bounds__(64 * kWaves, (DP >= 128 && CB == 2) || DP > 128 ? 1
     };
     auto page_of = [&](int t0) { return table[index_of(min(t0 + lane, seen - 1))]; };
 
-    // LDS addresses of this lane's reads
-    int kat[4], vat[2];
+    // LDS addresses of this lane's reads: keys by score step, values by block and half
+    constexpr int kMask = DP == 64 ? 7 : 15;
+    constexpr int kBlocks = DB < 4 ? DB : 4;  // blocks whose pieces lie in one line
+    int kat[kLines], vat[kBlocks][2];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) kat[s] = li * St::kRow + (((2 * s + half) ^ swizzle(li)) & 7) * 16;
-    {
-        const int i16 = lane & 15, row = 4 * half + (i16 >> 2);
+    for (int x = 0; x < kLines; ++x) kat[x] = li * St::kRow + (((2 * x + half) ^ swizzle<DP>(li)) & kMask) * 16;
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+            const int i16 = lane & 15, row = 8 * z + 4 * half + (i16 >> 2);
             const int chunk = 4 * b + 2 * (lane >> 4 & 1) + (i16 >> 1 & 1);
-            vat[b] = St::kV + row * St::kRow + ((chunk ^ swizzle(row)) & 7) * 16 + (i16 & 1) * 8;
+            vat[b][z] = St::kV + row * St::kRow + ((chunk ^ swizzle<DP>(row)) & kMask) * 16 + (i16 & 1) * 8;
         }
-    }
 
     float m[CB], l[CB];  // weights are exp2(score - m): m is the maximum less the bias, up to kLate behind
     f32x16 acc[CB][DB];
@@ -474,17 +486,29 @@ __global__ __launch_bounds__(64 * kWaves, (DP >= 128 && CB == 2) || DP > 128 ? 1
         auto load = [&](int stage) {
             constexpr int kPerRow = St::kRow / 16;       // pieces of a row
             constexpr int kLoads = kTile * St::kRow / 1024 / kWaves;
+            int64_t from[kLoads];
+            bool in[kLoads];
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                const int block = wave * kLoads + i;
-                const int r = block * (64 / kPerRow) + lane / kPerRow;
-                const int chunk = (lane % kPerRow) ^ swizzle(r);
-                const int64_t from = static_cast<int64_t>(__shfl(row, r)) * 16 + chunk * 16;
-                const uint32_t to = __builtin_amdgcn_readfirstlane(lds_at + stage * St::kBytes + block * 1024);
-                if (chunk * 8 < a.head_dim) {
-                    load_to_lds(kbase + from, to);
-                    load_to_lds(vbase + from, to + St::kV);
+                const int r = (wave * kLoads + i) * (64 / kPerRow) + lane / kPerRow;
+                const int chunk = (lane % kPerRow) ^ swizzle<DP>(r);
+                from[i] = static_cast<int64_t>(__shfl(row, r)) * 16 + chunk * 16;
+                in[i] = chunk * 8 < a.head_dim;
+            }
+            const uint32_t to = __builtin_amdgcn_readfirstlane(lds_at + stage * St::kBytes + wave * kLoads * 1024);
+            if (a.head_dim == DP) {
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) {
+                    load_to_lds(kbase + from[i], to + i * 1024);
+                    load_to_lds(vbase + from[i], to + St::kV + i * 1024);
                 }
+            } else {
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i)
+                    if (in[i]) {
+                        load_to_lds(kbase + from[i], to + i * 1024);
+                        load_to_lds(vbase + from[i], to + St::kV + i * 1024);
+                    }
             }
         };
         // e4m3 caches: to registers first
@@ -512,7 +536,7 @@ __global__ __launch_bounds__(64 * kWaves, (DP >= 128 && CB == 2) || DP > 128 ? 1
                 if (16 * c < a.head_dim) {
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const int where = r * St::kRow + ((2 * c + x) ^ swizzle(r)) * 16;
+                        const int where = r * St::kRow + ((2 * c + x) ^ swizzle<DP>(r)) * 16;
                         *(__attribute__((address_space(3))) u32x4*)(to + where) = eight_of<BF16>(kraw[i], x);
                         *(__attribute__((address_space(3))) u32x4*)(to + St::kV + where) = eight_of<true>(vraw[i], x);
                     }
@@ -554,18 +578,27 @@ __global__ __launch_bounds__(64 * kWaves, (DP >= 128 && CB == 2) || DP > 128 ? 1
             if (t0 < wave_seen && gone != ~0ull) {
                 f32x16 s[CB][2];
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
+                for (int t = 0; t < CB; ++t)
 #pragma unroll
-                    for (int t = 0; t < CB; ++t)
+                    for (int b = 0; b < 2; ++b)
 #pragma unroll
                         for (int j = 0; j < 16; ++j) s[t][b][j] = 0.0f;
 #pragma unroll
-                    for (int x = 0; x < KS; ++x) {
-                        const u32x4 k = lds16(tile, kat[x & 3] + (x >> 2) * 128 + b * 32 * St::kRow);
+                for (int x = 0; x < KS; ++x)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        const u32x4 k = lds16(tile, kat[x % kLines] + x / kLines * 256 + b * 32 * St::kRow);
 #pragma unroll
                         for (int t = 0; t < CB; ++t) s[t][b] = mfma32<BF16>(k, q[t][x], s[t][b]);
                     }
+                // keys kAhead reads in front of their matrix instructions (without this each is waited for)
+                __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+                for (int i = 0; i < 2 * KS - kAhead; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x8, CB, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
                 }
+                __builtin_amdgcn_sched_group_barrier(0x8, kAhead * CB, 0);
                 if constexpr (E8) {
 #pragma unroll
                     for (int b = 0; b < 2; ++b)
@@ -586,6 +619,7 @@ __global__ __launch_bounds__(64 * kWaves, (DP >= 128 && CB == 2) || DP > 128 ? 1
 #pragma unroll
                 for (int t = 0; t < CB; ++t) floor[t] = full ? -FLT_MAX : -INFINITY;
                 if (!full) {
+                    asm volatile("");  // a branch, not selects in every tile
 #pragma unroll
                     for (int t = 0; t < CB; ++t)
 #pragma unroll
@@ -672,8 +706,9 @@ __global__ __launch_bounds__(64 * kWaves, (DP >= 128 && CB == 2) || DP > 128 ? 1
                 for (int x = 0; x < 4; ++x)
 #pragma unroll
                     for (int b = 0; b < DB; ++b) {
-                        const int from = vat[b & 1] + (b >> 1) * 128 + 16 * x * St::kRow;
-                        const u32x2 lo = lds_transposed(tile, from), hi = lds_transposed(tile, from + 8 * St::kRow);
+                        const int from = b / kBlocks * 256 + 16 * x * St::kRow;
+                        const u32x2 lo = lds_transposed(tile, vat[b % kBlocks][0] + from);
+                        const u32x2 hi = lds_transposed(tile, vat[b % kBlocks][1] + from);
                         const u32x4 v = {lo[0], lo[1], hi[0], hi[1]};
 #pragma unroll
                         for (int t = 0; t < CB; ++t) acc[t][b] = mfma32<VBF16>(v, w[t][x], acc[t][b]);
@@ -807,7 +842,7 @@ ChunkShape shape_of(int64_t sequences, int64_t rows, int64_t heads, int64_t kv_h
                     int64_t capacity) {
     ChunkShape s;
     const int64_t group = heads / kv_heads, cus = plm::cu_count();
-    s.blocks = head_dim <= 128 && rows * heads >= 256 * cus ? 2 : 1;
+    s.blocks = head_dim <= 128 && false ? 2 : 1;
     const int64_t cols = 32 * kWaves * s.blocks;
     s.tiles = rows * group / cols + sequences + 2;
     s.budget = cus * ((head_dim > 64 && s.blocks == 2) || head_dim > 128 ? 1 : 2);
