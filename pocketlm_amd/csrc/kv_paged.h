@@ -141,6 +141,20 @@ __device__ __forceinline__ Place place_of(const Pages& p, const int* row_starts,
     return at;
 }
 
+// Inclusive prefix sum over the lanes of a wave (DPP, no LDS).
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t v) {
+#define PLM_PREFIX(ctrl, rows) \
+    v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), ctrl, rows, 0xF, false))
+    PLM_PREFIX(0x111, 0xF);  // row_shr:1, 2, 4, 8
+    PLM_PREFIX(0x112, 0xF);
+    PLM_PREFIX(0x114, 0xF);
+    PLM_PREFIX(0x118, 0xF);
+    PLM_PREFIX(0x142, 0xA);  // row_bcast:15 into rows 1 and 3
+    PLM_PREFIX(0x143, 0xC);  // row_bcast:31 into rows 2 and 3
+#undef PLM_PREFIX
+    return v;
+}
+
 __device__ __forceinline__ float swap_max(float v) {
     // over the four lanes l, l ^ 16, l ^ 32, l ^ 48
     const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);

@@ -23,6 +23,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
+constexpr int kColumns = 32 * kWaves;  // of a tile
 constexpr int kTile = 64;  // positions, one for each lane that looks up their pages
 // A running maximum is only moved once a score is more than 2^kLate above it: weights grow to 2^kLate, the
 // accumulators are multiplied in a few tiles instead of all.
@@ -38,7 +39,7 @@ struct ChunkArgs {
     const int* row_starts; // [sequences + 1]
     float* part;           // [slot][kv head][column of a tile][head_dim], then the maxima and sums
     float* part_ml;
-    uint2* plan;           // {slot of the first piece, splits} of each place; null: no tile is split
+    int* plan;             // {the run that begins it, the one that ends it} of each tile; null: no tile is split
     int64_t q_row, q_head; // strides, values
     int64_t capacity;      // positions of a table row
     int rows;
@@ -46,10 +47,8 @@ struct ChunkArgs {
     int kv_heads;
     int group;
     int head_dim;
-    int pieces;            // of a head, at most
-    int slots;             // of partials, at most
-    uint32_t budget;       // pieces that the device takes at once
-    uint32_t least_span;   // tiles of a piece, at least
+    int pieces;            // tiles of a head, or runs, at most
+    uint32_t work_shift;   // so that a head's work stays in 32 bits
     uint32_t divide;       // position / page_size: position * divide >> 31 + shift
     uint32_t shift;
     uint32_t flip;         // sign bits of the queries, where the softmax scale is negative
@@ -67,6 +66,10 @@ __device__ __forceinline__ int length_of(const ChunkArgs& a, int place) {
     return place == 0 || place > a.p.sequences ? -1 : a.p.lengths[place - 1];
 }
 
+__device__ __forceinline__ int rows_of(const ChunkArgs& a, int place) {
+    return max(start_of(a, place + 1) - start_of(a, place), 0);
+}
+
 // Tiles of `count` positions or columns.
 __device__ __forceinline__ uint32_t tiles_of(int64_t count, int tile) {
     return static_cast<uint32_t>((count + tile - 1) / tile);
@@ -76,119 +79,156 @@ __device__ __forceinline__ int seen_by(const ChunkArgs& a, int length, int row) 
     return length < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(length) + row + 1, a.capacity));
 }
 
+// Part of a tile's positions, in tiles of kTile: a workgroup's work until its next one.
 struct Piece {
     int place;
     int first;    // row
     int rows;
     int length;
-    int tile;     // of the place's columns
-    int split;
-    int splits;
-    int slot;     // of this place's partials, the first
+    int tiles;    // of the place's columns
+    int tile;
+    int seen;     // positions that its last column sees
+    int least;    // and that every one sees
+    int begin;    // this piece's
+    int end;
+    bool whole;   // all that the tile sees
+    int slot;     // of its partial, where it is not
 };
 
-// The place of a tile where no tile is split: place i's tiles begin at
-// floor(start * group / COLS) + i, which leaves room for each place's last,
-// partly filled one.  A search 64 wide.
-template <int COLS>
-__device__ __forceinline__ int place_of_tile(const ChunkArgs& a, int at, int lane, int& begin) {
+// A tile of a place, whole.
+__device__ __forceinline__ Piece piece_of(const ChunkArgs& a, int place, int tile) {
+    auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    Piece p;
+    p.place = place;
+    p.first = uniform(start_of(a, place));
+    p.rows = uniform(rows_of(a, place));
+    p.length = uniform(length_of(a, place));
+    const int columns = p.rows * a.group;
+    p.tiles = static_cast<int>(tiles_of(columns, kColumns));
+    p.tile = tile;
+    p.seen = uniform(seen_by(a, p.length, (min((tile + 1) * kColumns, columns) - 1) / a.group));
+    p.least = uniform(seen_by(a, p.length, tile * kColumns / a.group));
+    p.begin = 0;
+    p.end = p.seen;
+    p.whole = true;
+    p.slot = 0;
+    return p;
+}
+
+// Place i's tiles begin at floor(start * group / kColumns) + i, which leaves
+// room for each place's last, partly filled one.
+__device__ __forceinline__ int first_tile_of(const ChunkArgs& a, int place) {
+    return static_cast<int>(static_cast<int64_t>(start_of(a, place)) * a.group / kColumns) + place;
+}
+// The place of tile `at`, by a search 64 wide; every lane calls it.
+__device__ __forceinline__ int place_of_tile(const ChunkArgs& a, int at, int lane, int& first) {
     int lo = 0, hi = a.p.sequences + 2;
-    auto begin_of = [&](int i) { return static_cast<int>(static_cast<int64_t>(start_of(a, i)) * a.group / COLS) + i; };
     while (hi - lo > 1) {
         const int step = (hi - lo + 63) / 64;
         const int i = lo + lane * step;
-        const int count = __popcll(__ballot(i < hi && begin_of(min(i, hi - 1)) <= at));
+        const int count = __popcll(__ballot(i < hi && first_tile_of(a, min(i, hi - 1)) <= at));
         lo += (max(count, 1) - 1) * step;
         hi = min(hi, lo + step);
     }
     lo = __builtin_amdgcn_readfirstlane(lo);
-    begin = begin_of(lo);
+    first = __builtin_amdgcn_readfirstlane(first_tile_of(a, lo));
     return lo;
 }
 
-// Piece `at` of a head; false: there is none.  Every lane calls it.
-//
-// Where tiles are few for the device their positions are split: the places'
-// tiles times their middle number of position tiles are the work, a piece of a
-// place is to hold about a `budget`th of it.
-template <int COLS>
-__device__ __forceinline__ bool find_piece(const ChunkArgs& a, int at, int lane, Piece& piece) {
-    if (a.plan == nullptr) {
-        int begin;
-        piece.place = place_of_tile<COLS>(a, at, lane, begin);
-        piece.first = start_of(a, piece.place);
-        piece.rows = max(start_of(a, piece.place + 1) - piece.first, 0);
-        const int tiles = static_cast<int>(tiles_of(static_cast<int64_t>(piece.rows) * a.group, COLS));
-        if (at - begin >= tiles) return false;
-        piece.tile = tiles - 1 - (at - begin);  // the longest first
-        piece.split = 0;
-        piece.splits = 1;
-        piece.slot = 0;
-    } else {
-        const int places = a.p.sequences + 2;
-        auto tiles_at = [&](int i, uint32_t& most, float& work) {
-            const int first = i < places ? start_of(a, i) : 0;
-            const int rows = i < places ? max(start_of(a, i + 1) - first, 0) : 0;
-            const int length = i < places ? length_of(a, i) : -1;
-            const uint32_t tiles = tiles_of(static_cast<int64_t>(rows) * a.group, COLS);
-            most = tiles_of(seen_by(a, length, rows - 1), kTile);
-            work = static_cast<float>(tiles) * 0.5f * static_cast<float>(most + tiles_of(seen_by(a, length, 0), kTile));
-            return tiles;
-        };
-        float work = 0.0f;
-        uint32_t most;
-        for (int base = 0; base < places; base += 64) {
-            float w;
-            tiles_at(base + lane, most, w);
-            work += w;
-        }
-        work = __shfl(plm_wave_sum(work), kSumLane);
-        const uint32_t span = max(a.least_span, static_cast<uint32_t>(work * static_cast<float>(a.kv_heads) /
-                                                                      static_cast<float>(a.budget)) + 1u);
-        uint32_t before = 0, slots = 0;
-        bool found = false;
-        for (int base = 0; base < places && !found; base += 64) {
-            float w;
-            const uint32_t tiles = tiles_at(base + lane, most, w);
-            const uint32_t splits = max(1u, most / span);
-            const uint32_t mine = tiles * splits, parts = splits > 1 ? mine : 0;
-            uint32_t upto = mine, part_upto = parts;
-            for (int off = 1; off < 64; off <<= 1) {
-                const uint32_t u = __shfl_up(upto, off), v = __shfl_up(part_upto, off);
-                if (lane >= off) upto += u, part_upto += v;
-            }
-            const unsigned long long past = __ballot(before + upto > static_cast<uint32_t>(at));
-            if (past != 0) {
-                const int l = __ffsll(past) - 1;
-                const uint32_t n = __shfl(tiles, l), s = __shfl(splits, l);
-                const uint32_t begin = before + __shfl(upto, l) - n * s;
-                const uint32_t in = static_cast<uint32_t>(at) - begin;
-                piece.place = base + l;
-                piece.tile = static_cast<int>(n - 1 - in / s);
-                piece.split = static_cast<int>(in % s);
-                piece.splits = static_cast<int>(s);
-                piece.slot = static_cast<int>(slots + __shfl(part_upto, l) - (s > 1 ? n * s : 0));
-                found = true;
-            }
-            before += __shfl(upto, 63);
-            slots += __shfl(part_upto, 63);
-        }
-        if (!found) return false;
-        piece.place = __builtin_amdgcn_readfirstlane(piece.place);
-        piece.split = __builtin_amdgcn_readfirstlane(piece.split);
-        piece.splits = __builtin_amdgcn_readfirstlane(piece.splits);
-        piece.slot = __builtin_amdgcn_readfirstlane(piece.slot);
-        piece.first = start_of(a, piece.place);
-        piece.rows = max(start_of(a, piece.place + 1) - piece.first, 0);
+// Where tiles are few for the device, runs: the places' tiles in their order, a
+// tile's work its position tiles (taken to grow evenly from a place's first tile
+// to its last) and kTileWork for its queries and results, dealt in equal parts
+// whatever the tiles' borders.  A run writes the results of the tiles that it
+// holds whole; of the others it leaves two partials at most: of the tile that
+// it goes on with (slot 2 run) and of the one that it begins and does not end
+// (slot 2 run + 1).
+constexpr uint32_t kTileWork = 2;
+constexpr uint32_t kLeastWork = 4;  // of a run
+
+struct Work {
+    int tiles;
+    uint32_t first, last;  // position tiles of its first and last tile
+
+    // Work of the tiles before `tile`, times 2 max(tiles - 1, 1).
+    __device__ __forceinline__ double before(int tile) const {
+        const double t = tile, n = max(tiles - 1, 1);
+        return 2.0 * n * static_cast<double>(first + kTileWork) * t +
+               (static_cast<double>(last) - static_cast<double>(first)) * t * (t - 1.0);
     }
-    piece.tile = __builtin_amdgcn_readfirstlane(piece.tile);
-    piece.first = __builtin_amdgcn_readfirstlane(piece.first);
-    piece.rows = __builtin_amdgcn_readfirstlane(piece.rows);
-    piece.length = __builtin_amdgcn_readfirstlane(length_of(a, piece.place));
+    __device__ __forceinline__ uint32_t total(uint32_t shift) const {
+        const uint64_t twice = static_cast<uint64_t>(tiles) * (static_cast<uint64_t>(first) + last + 2 * kTileWork);
+        return tiles > 0 ? max(1u, static_cast<uint32_t>(twice >> (shift + 1))) : 0u;
+    }
+};
+
+__device__ __forceinline__ Work work_of(const ChunkArgs& a, int place) {
+    Work w = {0, 0, 0};
+    if (place >= a.p.sequences + 2) return w;
+    const int rows = rows_of(a, place);
+    const int length = length_of(a, place);
+    w.tiles = static_cast<int>(tiles_of(static_cast<int64_t>(rows) * a.group, kColumns));
+    w.first = tiles_of(seen_by(a, length, min(kColumns / a.group, rows) - 1), kTile);
+    w.last = tiles_of(seen_by(a, length, rows - 1), kTile);
+    return w;
+}
+
+// A border between runs: a place, a tile of it and the share of the tile before the border (of 1).
+struct Border {
+    int place;
+    int tile;
+    float share;
+};
+
+// The borders of run `run`; false: there is no such run.  Every lane calls it.
+__device__ __forceinline__ bool find_run(const ChunkArgs& a, int run, int lane, Border& from, Border& to) {
+    const int places = a.p.sequences + 2;
+    const Work mine = work_of(a, lane);
+    uint32_t all = 0;
+    for (int base = 0; base < places; base += 64)
+        all += (base == 0 ? mine : work_of(a, base + lane)).total(a.work_shift);
+    all = __builtin_amdgcn_readlane(wave_prefix(all), 63);
+    const uint32_t runs = min(static_cast<uint32_t>(a.pieces), max(1u, all / kLeastWork));
+    if (static_cast<uint32_t>(run) >= runs) return false;
+    const uint32_t each = all / runs, rest = all - each * runs;
+    const uint32_t u = static_cast<uint32_t>(run);
+    const uint32_t begin = u * each + static_cast<uint32_t>(static_cast<uint64_t>(u) * rest / runs);
+    const uint32_t end = (u + 1) * each + static_cast<uint32_t>(static_cast<uint64_t>(u + 1) * rest / runs);
+    from.place = to.place = places;
+    from.tile = to.tile = 0;
+    from.share = to.share = 0.0f;
+    uint32_t before = 0;
+    for (int base = 0; base < places; base += 64) {
+        const Work w = base == 0 ? mine : work_of(a, base + lane);
+        const uint32_t total = w.total(a.work_shift), upto = before + wave_prefix(total);
+        auto place = [&](uint32_t x, Border& b) {
+            const unsigned long long past = __ballot(upto > x);
+            if (past == 0 || b.place < places) return;
+            const int l = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
+            Work of;
+            of.tiles = __builtin_amdgcn_readlane(w.tiles, l);
+            of.first = __builtin_amdgcn_readlane(w.first, l);
+            of.last = __builtin_amdgcn_readlane(w.last, l);
+            const uint32_t size = __builtin_amdgcn_readlane(total, l);
+            const uint32_t in = x - (__builtin_amdgcn_readlane(upto, l) - size);
+            const double z = static_cast<double>(in) / static_cast<double>(size) * of.before(of.tiles);
+            int lo = 0, hi = of.tiles;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                (of.before(mid) <= z ? lo : hi) = mid;
+            }
+            b.place = base + l;
+            b.tile = __builtin_amdgcn_readfirstlane(lo);
+            b.share = in == 0 ? 0.0f
+                              : static_cast<float>((z - of.before(lo)) / (of.before(lo + 1) - of.before(lo)));
+        };
+        place(begin, from);
+        place(end, to);
+        before = __builtin_amdgcn_readlane(upto, 63);
+    }
     return true;
 }
 
-// Workgroup -> (piece, head).  Workgroups are dealt to the 8 XCDs in turn: a
+// Workgroup -> (tile or run, head).  They are dealt to the 8 XCDs in turn: a
 // head's are kept on as few of them as there are heads for, so that its keys
 // and values lie in few L2s.
 __device__ __forceinline__ void block_of(const ChunkArgs& a, int& at, int& kvh) {
@@ -248,14 +288,14 @@ __device__ __forceinline__ void loads_barrier() {
 // the column does not see: a lane has a position's score, then the values d =
 // lane + 64 i of the sum.  For columns that meet infinities or NaN, so only right,
 // not fast.
-template <bool BF16, bool E8, int COLS>
-__device__ void careful_column(const ChunkArgs& a, const Piece& piece, int kvh, int col, int begin, int end, int lane) {
+template <bool BF16, bool E8>
+__device__ void careful_column(const ChunkArgs& a, const Piece& piece, int kvh, int col, int lane) {
     const int r = col / a.group, h = col - r * a.group;
     const uint16_t* q = a.q + (piece.first + r) * a.q_row + (kvh * a.group + h) * a.q_head;
     const int* table = a.p.table + static_cast<int64_t>(piece.place - 1) * a.p.table_cols;
     const uint8_t* kbase = reinterpret_cast<const uint8_t*>(a.p.k) + (E8 ? 1 : 2) * kvh * a.p.head_stride;
     const uint8_t* vbase = reinterpret_cast<const uint8_t*>(a.p.v) + (E8 ? 1 : 2) * kvh * a.p.head_stride;
-    const int last = min(end, seen_by(a, piece.length, r));
+    const int last = min(piece.end, seen_by(a, piece.length, r));
     auto value = [&](const uint8_t* row, int d) {
         if constexpr (E8)
             return __uint_as_float(pair_of<true>(row[d], false) << 16);
@@ -264,7 +304,7 @@ __device__ void careful_column(const ChunkArgs& a, const Piece& piece, int kvh, 
     };
     float m = -INFINITY, l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
-    for (int t0 = begin; t0 < last; t0 += kTile) {
+    for (int t0 = piece.begin; t0 < last; t0 += kTile) {
         const int pos = t0 + lane;
         int page = -1;
         uint32_t slot = 0;
@@ -314,10 +354,8 @@ __device__ void careful_column(const ChunkArgs& a, const Piece& piece, int kvh, 
             }
         }
     }
-    if (piece.splits > 1) {
-        const int slot = piece.slot + piece.tile * piece.splits + piece.split;
-        if (slot >= a.slots) return;
-        const int64_t to = (static_cast<int64_t>(slot) * a.kv_heads + kvh) * COLS + (col - piece.tile * COLS);
+    if (!piece.whole) {
+        const int64_t to = (static_cast<int64_t>(piece.slot) * a.kv_heads + kvh) * kColumns + (col - piece.tile * kColumns);
         if (lane == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * to) = f32x2{m, l};
         for (int i = 0; i < 4; ++i)
             if (lane + 64 * i < a.head_dim) a.part[to * a.head_dim + lane + 64 * i] = acc[i];
@@ -346,8 +384,8 @@ struct Stage {
     static constexpr int kLds = 2 * kBytes;
 };
 
-// Workgroup (piece, key-value head): 4 waves of 32 CB columns each over the
-// piece's positions, 64 at a time through LDS, two tiles deep.
+// A piece by a workgroup: 4 waves of 32 columns each over the piece's positions,
+// 64 at a time through LDS, two tiles deep.
 //
 //   scores  S^T = K Q^T (32 x 32 x 16): a lane has, of column l & 31, the positions
 //           8 (j / 4) + 4 (l / 32) + j % 4, so that a column's maximum and sum are
@@ -367,65 +405,41 @@ struct Stage {
 // finite and met positions that not every column sees does its columns again, one at
 // a time (careful_column).  Positions behind the last one seen, or without a page, are
 // never read.
-template <bool BF16, bool E8, int DP, int CB>
-__global__ __launch_bounds__(64 * kWaves, (DP >= 128 && CB == 2) || DP > 128 ? 1 : 2) void paged_chunk_kernel(
-    const ChunkArgs a) {
+template <bool BF16, bool E8, int DP>
+__device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, int kvh, lds_char* lds) {
     using St = Stage<DP, E8>;
     constexpr bool VBF16 = BF16 || E8;
-    constexpr int COLS = 32 * CB * kWaves;
     constexpr int KS = DP / 16;   // score steps
     constexpr int DB = DP / 32;   // blocks of head values
     constexpr int kLines = KS < 8 ? KS : 8;  // score steps whose pieces lie in one line of 256 bytes
     constexpr int kAhead = 6;
     constexpr float kBias = bias_of(VBF16);
-    extern __shared__ char lds_raw[];
-    lds_char* const lds = (lds_char*)lds_raw;
     const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int li = lane & 31, half = lane >> 5;
-    int at, kvh;
-    block_of(a, at, kvh);
-    Piece piece;
-    if (at >= a.pieces || !find_piece<COLS>(a, at, lane, piece)) return;
-    if (a.plan != nullptr && kvh == 0 && piece.tile == 0 && piece.split == 0 && threadIdx.x == 0)
-        a.plan[piece.place] = make_uint2(piece.slot, piece.splits);
-
-    const int columns = piece.rows * a.group;
-    const int col0 = piece.tile * COLS;
+    const int columns = piece.rows * a.group, col0 = piece.tile * kColumns;
+    const int seen = piece.seen, least = piece.least, begin = piece.begin, end = piece.end;
     auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-    const int seen = uniform(seen_by(a, piece.length, (min(col0 + COLS, columns) - 1) / a.group));
-    const int least = uniform(seen_by(a, piece.length, col0 / a.group));  // what every column sees
-    const uint32_t units = tiles_of(seen, kTile);
-    const int begin = uniform(static_cast<int>(static_cast<uint64_t>(units) * piece.split / piece.splits) * kTile);
-    const int end = uniform(
-        min(seen, static_cast<int>(static_cast<uint64_t>(units) * (piece.split + 1) / piece.splits) * kTile));
-    const int wave0 = col0 + 32 * CB * wave;
+    const int wave0 = col0 + 32 * wave;
     const int wave_least = uniform(seen_by(a, piece.length, min(wave0, columns - 1) / a.group));
     const int wave_seen =
-        wave0 < columns ? uniform(seen_by(a, piece.length, (min(wave0 + 32 * CB, columns) - 1) / a.group)) : 0;
+        wave0 < columns ? uniform(seen_by(a, piece.length, (min(wave0 + 32, columns) - 1) / a.group)) : 0;
 
-    u32x4 q[CB][KS];
-    int limit[CB];
-#pragma unroll
-    for (int t = 0; t < CB; ++t) {
-        const int col = wave0 + 32 * t + li;
+    u32x4 q[KS];
+    int limit;
+    {
+        const int col = wave0 + li;
         const int r = min(col, columns - 1) / a.group, h = min(col, columns - 1) - r * a.group;
         const uint16_t* src = a.q + (piece.first + r) * a.q_row + (kvh * a.group + h) * a.q_head;
-        limit[t] = col < columns ? seen_by(a, piece.length, r) : 0;
+        limit = col < columns ? seen_by(a, piece.length, r) : 0;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int d = 16 * s + 8 * half;
-            q[t][s] = *reinterpret_cast<const u32x4*>(src + (d < a.head_dim ? d : 0)) ^ a.flip;
-            if (col >= columns || d >= a.head_dim) q[t][s] = u32x4{0, 0, 0, 0};
+            q[s] = *reinterpret_cast<const u32x4*>(src + (d < a.head_dim ? d : 0)) ^ a.flip;
+            if (col >= columns || d >= a.head_dim) q[s] = u32x4{0, 0, 0, 0};
         }
     }
-    if (a.head_dim != DP) {  // the loads leave out what is behind a head's end
-        for (int i = threadIdx.x; i < St::kLds / 16; i += 64 * kWaves)
-            *(__attribute__((address_space(3))) u32x4*)(lds + 16 * i) = u32x4{0, 0, 0, 0};
-        __syncthreads();
-    }
-
     const int* table = a.p.table + static_cast<int64_t>(max(piece.place - 1, 0)) * a.p.table_cols;
     const uint8_t* kbase = reinterpret_cast<const uint8_t*>(a.p.k) + (E8 ? 1 : 2) * kvh * a.p.head_stride;
     const uint8_t* vbase = reinterpret_cast<const uint8_t*>(a.p.v) + (E8 ? 1 : 2) * kvh * a.p.head_stride;
@@ -451,19 +465,14 @@ __global__ __launch_bounds__(64 * kWaves, (DP >= 128 && CB == 2) || DP > 128 ? 1
             vat[b][z] = St::kV + row * St::kRow + ((chunk ^ swizzle<DP>(row)) & kMask) * 16 + (i16 & 1) * 8;
         }
 
-    float m[CB], l[CB];  // weights are exp2(score - m): m is the maximum less the bias, up to kLate behind
-    f32x16 acc[CB][DB];
+    float m = -INFINITY, l = 0.0f;  // weights are exp2(score - m): m is the maximum less the bias, up to kLate behind
+    f32x16 acc[DB];
 
     bool masked = false;  // there was a position that some column does not see
 #pragma unroll
-        for (int t = 0; t < CB; ++t) {
-            m[t] = -INFINITY;
-            l[t] = 0.0f;
+    for (int b = 0; b < DB; ++b)
 #pragma unroll
-            for (int b = 0; b < DB; ++b)
-#pragma unroll
-                for (int j = 0; j < 16; ++j) acc[t][b][j] = 0.0f;
-        }
+        for (int j = 0; j < 16; ++j) acc[b][j] = 0.0f;
     if (begin < end) {
         // rows of a tile, in pieces of 16 bytes; a position without a page reads one that has one, a tile of none
         // is left out
@@ -576,29 +585,26 @@ __global__ __launch_bounds__(64 * kWaves, (DP >= 128 && CB == 2) || DP > 128 ? 1
             lds_char* const tile = lds + stage * St::kBytes;
             masked |= t0 + kTile > least || gone != 0;
             if (t0 < wave_seen && gone != ~0ull) {
-                f32x16 s[CB][2];
+                f32x16 s[2];
 #pragma unroll
-                for (int t = 0; t < CB; ++t)
+                for (int b = 0; b < 2; ++b)
 #pragma unroll
-                    for (int b = 0; b < 2; ++b)
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) s[t][b][j] = 0.0f;
+                    for (int j = 0; j < 16; ++j) s[b][j] = 0.0f;
 #pragma unroll
                 for (int x = 0; x < KS; ++x)
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
                         const u32x4 k = lds16(tile, kat[x % kLines] + x / kLines * 256 + b * 32 * St::kRow);
-#pragma unroll
-                        for (int t = 0; t < CB; ++t) s[t][b] = mfma32<BF16>(k, q[t][x], s[t][b]);
+                        s[b] = mfma32<BF16>(k, q[x], s[b]);
                     }
                 // keys kAhead reads in front of their matrix instructions (without this each is waited for)
                 __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
                 for (int i = 0; i < 2 * KS - kAhead; ++i) {
-                    __builtin_amdgcn_sched_group_barrier(0x8, CB, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
                     __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
                 }
-                __builtin_amdgcn_sched_group_barrier(0x8, kAhead * CB, 0);
+                __builtin_amdgcn_sched_group_barrier(0x8, kAhead, 0);
                 if constexpr (E8) {
 #pragma unroll
                     for (int b = 0; b < 2; ++b)
@@ -607,83 +613,60 @@ __global__ __launch_bounds__(64 * kWaves, (DP >= 128 && CB == 2) || DP > 128 ? 1
                             const f32x4 by = a.scale *
                                 __builtin_bit_cast(f32x4, lds16(tile, St::kScales + (32 * b + 2 * j + 4 * half) * 4));
 #pragma unroll
-                            for (int t = 0; t < CB; ++t)
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) s[t][b][j + i] *= by[i];
+                            for (int i = 0; i < 4; ++i) s[b][j + i] *= by[i];
                         }
                 }
                 const bool full = t0 + kTile <= wave_least && gone == 0;
                 // A row that sees a position has a maximum of at least the lowest number, one that sees none keeps
                 // -inf: its result is 0, while scores that are all -inf give 0 / 0.
-                float floor[CB];
-#pragma unroll
-                for (int t = 0; t < CB; ++t) floor[t] = full ? -FLT_MAX : -INFINITY;
+                float floor = full ? -FLT_MAX : -INFINITY;
                 if (!full) {
                     asm volatile("");  // a branch, not selects in every tile
 #pragma unroll
-                    for (int t = 0; t < CB; ++t)
-#pragma unroll
                         for (int b = 0; b < 2; ++b) {
                             // bit i: position 32 b + 4 half + i of the tile is hidden
-                            const int left = limit[t] - t0 - 32 * b - 4 * half;
+                            const int left = limit - t0 - 32 * b - 4 * half;
                             const uint32_t hidden = static_cast<uint32_t>(gone >> 32 * b) >> 4 * half |
                                                     (left >= 32 ? 0u : ~0u << max(left, 0));
-                            if ((~hidden & 0x0F0F0F0Fu) != 0) floor[t] = -FLT_MAX;
+                            if ((~hidden & 0x0F0F0F0Fu) != 0) floor = -FLT_MAX;
 #pragma unroll
                             for (int j = 0; j < 16; ++j)
-                                if (hidden >> (8 * (j >> 2) + (j & 3)) & 1) s[t][b][j] = -INFINITY;
+                                if (hidden >> (8 * (j >> 2) + (j & 3)) & 1) s[b][j] = -INFINITY;
                         }
                 }
                 // 16-bit caches: the scale goes into the weights' exponents as they are formed, in one instruction.
                 // The maximum is rounded there and the scores are not, which all weights of a column share, but from
                 // 2^22 on it might be large: such scores are multiplied first.
                 float times = E8 ? 1.0f : a.scale;
-                float top[CB];
-                bool late = false, large = false;
+                float top = s[0][0];
 #pragma unroll
-                for (int t = 0; t < CB; ++t) {
-                    float v = s[t][0][0];
-#pragma unroll
-                    for (int j = 1; j < 32; ++j) v = fmaxf(v, s[t][j >> 4][j & 15]);
-                    top[t] = both_max(fmaxf(v * times, floor[t])) - kBias;
-                    late |= top[t] > m[t] + kLate;
-                    const float to = fmaxf(top[t], m[t]);
-                    large |= fabsf(to) > 0x1p22f && to > -0x1p127f;
-                }
-                if (!E8 && __any(large)) {
+                for (int j = 1; j < 32; ++j) top = fmaxf(top, s[j >> 4][j & 15]);
+                top = fmaxf(m, both_max(fmaxf(top * times, floor)) - kBias);
+                if (!E8 && __any(fabsf(top) > 0x1p22f && top > -0x1p127f)) {
                     times = 1.0f;
 #pragma unroll
-                    for (int t = 0; t < CB; ++t)
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) s[t][j >> 4][j & 15] *= a.scale;
+                    for (int j = 0; j < 32; ++j) s[j >> 4][j & 15] *= a.scale;
                 }
-                if (__any(late)) {
+                if (__any(top > m + kLate)) {
+                    const float fade = exp2_from(m, top);
+                    m = top;
+                    l *= fade;
 #pragma unroll
-                    for (int t = 0; t < CB; ++t) {
-                        const float to = fmaxf(m[t], top[t]);
-                        const float fade = exp2_from(m[t], to);
-                        m[t] = to;
-                        l[t] *= fade;
+                    for (int b = 0; b < DB; ++b)
 #pragma unroll
-                        for (int b = 0; b < DB; ++b)
+                        for (int j = 0; j < 16; ++j) acc[b][j] *= fade;
+                }
+                u32x4 w[4];
+                const float from = m == -INFINITY ? 0.0f : m;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) acc[t][b][j] *= fade;
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        s[b][j] = __builtin_amdgcn_exp2f(fmaf(s[b][j], times, -from));
+                        sum[j & 3] += s[b][j];
                     }
-                }
-                u32x4 w[CB][4];
-#pragma unroll
-                for (int t = 0; t < CB; ++t) {
-                    const float from = m[t] == -INFINITY ? 0.0f : m[t];
-                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int b = 0; b < 2; ++b)
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            s[t][b][j] = __builtin_amdgcn_exp2f(fmaf(s[t][b][j], times, -from));
-                            sum[j & 3] += s[t][b][j];
-                        }
-                    l[t] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -692,15 +675,12 @@ __global__ __launch_bounds__(64 * kWaves, (DP >= 128 && CB == 2) || DP > 128 ? 1
                         if constexpr (E8) {
                             by = __builtin_bit_cast(f32x4, lds16(tile, St::kScales + kTile * 4 + (32 * b + 2 * j + 4 * half) * 4));
                         }
+                        f32x4 v = {s[b][j], s[b][j + 1], s[b][j + 2], s[b][j + 3]};
+                        if constexpr (E8)
 #pragma unroll
-                        for (int t = 0; t < CB; ++t) {
-                            f32x4 v = {s[t][b][j], s[t][b][j + 1], s[t][b][j + 2], s[t][b][j + 3]};
-                            if constexpr (E8)
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) v[i] *= by[i];
-                            w[t][2 * b + (j >> 3)][(j & 4) / 2] = pack2<VBF16>(v[0], v[1]);
-                            w[t][2 * b + (j >> 3)][(j & 4) / 2 + 1] = pack2<VBF16>(v[2], v[3]);
-                        }
+                            for (int i = 0; i < 4; ++i) v[i] *= by[i];
+                        w[2 * b + (j >> 3)][(j & 4) / 2] = pack2<VBF16>(v[0], v[1]);
+                        w[2 * b + (j >> 3)][(j & 4) / 2 + 1] = pack2<VBF16>(v[2], v[3]);
                     }
 #pragma unroll
                 for (int x = 0; x < 4; ++x)
@@ -710,8 +690,7 @@ __global__ __launch_bounds__(64 * kWaves, (DP >= 128 && CB == 2) || DP > 128 ? 1
                         const u32x2 lo = lds_transposed(tile, vat[b % kBlocks][0] + from);
                         const u32x2 hi = lds_transposed(tile, vat[b % kBlocks][1] + from);
                         const u32x4 v = {lo[0], lo[1], hi[0], hi[1]};
-#pragma unroll
-                        for (int t = 0; t < CB; ++t) acc[t][b] = mfma32<VBF16>(v, w[t][x], acc[t][b]);
+                        acc[b] = mfma32<VBF16>(v, w[x], acc[b]);
                     }
             }
             if constexpr (E8)
@@ -719,175 +698,250 @@ __global__ __launch_bounds__(64 * kWaves, (DP >= 128 && CB == 2) || DP > 128 ? 1
             gone = next_gone;
         }
     }
-#pragma unroll
-    for (int t = 0; t < CB; ++t) l[t] = both_sum(l[t]);
+    l = both_sum(l);
 
     bool odd = false;
 #pragma unroll
-    for (int t = 0; t < CB; ++t)
+    for (int b = 0; b < DB; ++b)
 #pragma unroll
-        for (int b = 0; b < DB; ++b)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) odd |= !(fabsf(acc[t][b][j]) < INFINITY);
+        for (int j = 0; j < 16; ++j) odd |= !(fabsf(acc[b][j]) < INFINITY);
     if (__any(masked && odd)) {
-        const int most = min(wave0 + 32 * CB, columns);
-        for (int col = wave0; col < most; ++col) careful_column<BF16, E8, COLS>(a, piece, kvh, col, begin, end, lane);
+        const int most = min(wave0 + 32, columns);
+        for (int col = wave0; col < most; ++col) careful_column<BF16, E8>(a, piece, kvh, col, lane);
         return;
     }
 
-#pragma unroll
-    for (int t = 0; t < CB; ++t) {
-        const int in = wave * 32 * CB + 32 * t + li;
-        const int col = col0 + in;
-        if (col >= columns) continue;
-        if (piece.splits > 1) {
-            const int slot = piece.slot + piece.tile * piece.splits + piece.split;
-            if (slot >= a.slots) continue;
-            const int64_t to = (static_cast<int64_t>(slot) * a.kv_heads + kvh) * COLS + in;
-            if (half == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * to) = f32x2{m[t], l[t]};
-#pragma unroll
-            for (int b = 0; b < DB; ++b)
-#pragma unroll
-                for (int j = 0; j < 16; j += 4) {
-                    const int d = 32 * b + 2 * j + 4 * half;
-                    if (d < a.head_dim)
-                        *reinterpret_cast<f32x4*>(a.part + to * a.head_dim + d) =
-                            f32x4{acc[t][b][j], acc[t][b][j + 1], acc[t][b][j + 2], acc[t][b][j + 3]};
-                }
-            continue;
-        }
-        // a row that sees nothing is zero
-        const int r = col / a.group, h = col - r * a.group;
-        const bool empty = m[t] == -INFINITY;
-        const float inv = 1.0f / l[t];
-        uint16_t* to = a.out + (static_cast<int64_t>(piece.first + r) * a.heads + kvh * a.group + h) * a.head_dim;
+    const int in = 32 * wave + li;
+    const int col = col0 + in;
+    if (col >= columns) return;
+    if (!piece.whole) {
+        const int64_t to = (static_cast<int64_t>(piece.slot) * a.kv_heads + kvh) * kColumns + in;
+        if (half == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * to) = f32x2{m, l};
 #pragma unroll
         for (int b = 0; b < DB; ++b)
 #pragma unroll
             for (int j = 0; j < 16; j += 4) {
                 const int d = 32 * b + 2 * j + 4 * half;
-                u32x2 o;
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
-                    o[x] = pack2<BF16>(empty ? 0.0f : acc[t][b][j + 2 * x] * inv,
-                                       empty ? 0.0f : acc[t][b][j + 2 * x + 1] * inv);
-                if (d < a.head_dim) *reinterpret_cast<u32x2*>(to + d) = o;
+                if (d < a.head_dim)
+                    *reinterpret_cast<f32x4*>(a.part + to * a.head_dim + d) =
+                        f32x4{acc[b][j], acc[b][j + 1], acc[b][j + 2], acc[b][j + 3]};
             }
+        return;
+    }
+    // a row that sees nothing is zero
+    const int r = col / a.group, h = col - r * a.group;
+    const bool empty = m == -INFINITY;
+    const float inv = 1.0f / l;
+    uint16_t* to = a.out + (static_cast<int64_t>(piece.first + r) * a.heads + kvh * a.group + h) * a.head_dim;
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+            const int d = 32 * b + 2 * j + 4 * half;
+            u32x2 o;
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+                o[x] = pack2<BF16>(empty ? 0.0f : acc[b][j + 2 * x] * inv,
+                                   empty ? 0.0f : acc[b][j + 2 * x + 1] * inv);
+            if (d < a.head_dim) *reinterpret_cast<u32x2*>(to + d) = o;
+        }
+}
+
+// Workgroup -> (tile or run, key-value head).
+template <bool BF16, bool E8, int DP>
+__global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void paged_chunk_kernel(const ChunkArgs a) {
+    using St = Stage<DP, E8>;
+    extern __shared__ char lds_raw[];
+    lds_char* const lds = (lds_char*)lds_raw;
+    const int lane = threadIdx.x & 63;
+    int at, kvh;
+    block_of(a, at, kvh);
+    if (at >= a.pieces) return;
+    if (a.head_dim != DP)  // the loads leave out what is behind a head's end
+        for (int i = threadIdx.x; i < St::kLds / 16; i += 64 * kWaves)
+            *(__attribute__((address_space(3))) u32x4*)(lds + 16 * i) = u32x4{0, 0, 0, 0};
+    Border next, last;
+    if (a.plan == nullptr) {
+        int first;
+        const int place = place_of_tile(a, at, lane, first);
+        const int tiles = static_cast<int>(tiles_of(rows_of(a, place) * static_cast<int64_t>(a.group), kColumns));
+        if (at - first >= tiles) return;
+        next = Border{place, tiles - 1 - (at - first), 0.0f};  // the longest first
+        last = Border{place, next.tile + 1, 0.0f};
+    } else if (!find_run(a, at, lane, next, last)) {
+        return;
+    }
+    int place = next.place, tile = next.tile;
+    while (place < last.place || (place == last.place && tile <= last.tile)) {
+        Piece piece = piece_of(a, place, tile);
+        if (tile >= piece.tiles) {
+            if (++place > a.p.sequences + 1) return;
+            tile = 0;
+            continue;
+        }
+        const int units = static_cast<int>(tiles_of(piece.seen, kTile));
+        auto unit_at = [&](float share) {
+            return __builtin_amdgcn_readfirstlane(min(units, static_cast<int>(share * static_cast<float>(units))));
+        };
+        const bool goes_on = place == next.place && tile == next.tile && next.share > 0.0f;
+        const bool ends_here = place == last.place && tile == last.tile;
+        if (ends_here && last.share == 0.0f) return;
+        const int from = goes_on ? unit_at(next.share) : 0, to = ends_here ? unit_at(last.share) : units;
+        if (units > 0 && to == 0) return;  // the next run begins it
+        // (not what the run before has ended)
+        if (units > 0 ? from < units : !goes_on) {
+            if (a.plan != nullptr && kvh == 0 && threadIdx.x == 0) {
+                int* const noted = a.plan + 2 * (first_tile_of(a, place) + tile);
+                if (from == 0) noted[0] = at;
+                if (to == units) noted[1] = at;
+            }
+            piece.whole = from == 0 && to == units;
+            piece.slot = 2 * at + (from == 0 ? 1 : 0);
+            piece.begin = from * kTile;
+            piece.end = min(piece.seen, to * kTile);
+            __syncthreads();  // the tile before has been read
+            attend<BF16, E8, DP>(a, piece, kvh, lds);
+        }
+        ++tile;
     }
 }
 
-// Joins the pieces of split tiles: a workgroup for 32 columns of a tile, 8
-// threads a column, each every eighth quad of head values.
+// Joins the partials of the tiles that several runs hold: a workgroup for 16
+// columns of a tile, 16 threads a column, which first weigh the partials (every
+// sixteenth each), then take every sixteenth quad of head values.
 constexpr int kJoinThreads = 256;
-constexpr int kJoinColumns = 32;
+constexpr int kJoinColumns = 16;
+constexpr int kJoinPartials = 64;  // at a time
 
-template <bool BF16, int COLS>
+template <bool BF16>
 __global__ __launch_bounds__(kJoinThreads) void paged_chunk_join_kernel(const ChunkArgs a) {
+    __shared__ float weights[kJoinColumns][kJoinPartials + 1];
     const int lane = threadIdx.x & 63;
     int begin;
-    const int place = place_of_tile<COLS>(a, blockIdx.x, lane, begin);
+    const int place = place_of_tile(a, blockIdx.x, lane, begin);
     const int first = start_of(a, place);
-    const int columns = max(start_of(a, place + 1) - first, 0) * a.group;
+    const int columns = rows_of(a, place) * a.group;
     const int tile = blockIdx.x - begin;
-    const int in = blockIdx.z * kJoinColumns + threadIdx.x / 8;
-    const int col = tile * COLS + in;
-    if (tile >= static_cast<int>(tiles_of(columns, COLS))) return;
-    const uint2 noted = a.plan[place];
-    const int splits = static_cast<int>(noted.y);
-    const int slot = static_cast<int>(noted.x) + tile * splits;
-    if (splits <= 1 || slot + splits > a.slots || col >= columns) return;
+    if (tile >= static_cast<int>(tiles_of(columns, kColumns))) return;
+    // (within the runs also where the lengths were changed under the first kernel)
+    const int run = min(max(a.plan[2 * blockIdx.x], 0), a.pieces - 1);
+    const int parts = min(a.plan[2 * blockIdx.x + 1], a.pieces - 1) - run + 1;
+    if (parts <= 1) return;
+    const int c = threadIdx.x >> 4, j = threadIdx.x & 15;
+    const int in = blockIdx.z * kJoinColumns + c, col = tile * kColumns + in;
     const int kvh = blockIdx.y;
-    const int64_t stride = static_cast<int64_t>(a.kv_heads) * COLS;
-    const int64_t from = (static_cast<int64_t>(slot) * a.kv_heads + kvh) * COLS + in;
+    // partial i: the first is its run's second
+    auto slot = [](int i) { return max(2 * i, 1); };
+    const int64_t stride = static_cast<int64_t>(a.kv_heads) * kColumns;
+    const int64_t from = (static_cast<int64_t>(2 * run) * a.kv_heads + kvh) * kColumns + in;
     const f32x2* ml = reinterpret_cast<const f32x2*>(a.part_ml) + from;
+    auto over16 = [](float v, auto op) {
+#pragma unroll
+        for (int off = 1; off < 16; off <<= 1) v = op(v, __shfl_xor(v, off));
+        return v;
+    };
     float m = -INFINITY;
-    for (int s = 0; s < splits; ++s) m = fmaxf(m, ml[s * stride][0]);
+    for (int i = j; i < parts; i += 16) m = fmaxf(m, ml[slot(i) * stride][0]);
+    m = over16(m, [](float u, float v) { return fmaxf(u, v); });
+    const float* part = a.part + from * a.head_dim + 4 * j;
     float sum = 0.0f;
-    for (int s = 0; s < splits; ++s) sum = fmaf(ml[s * stride][1], exp2_from(ml[s * stride][0], m), sum);
+    f32x4 acc[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) acc[x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int base = 0; base < parts; base += kJoinPartials) {
+        const int n = min(kJoinPartials, parts - base);
+        __syncthreads();
+        for (int i = j; i < n; i += 16) {
+            const f32x2 v = ml[slot(base + i) * stride];
+            const float w = exp2_from(v[0], m);
+            weights[c][i] = w;
+            sum = fmaf(v[1], w, sum);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            if (4 * j + 64 * x < a.head_dim) {
+#pragma unroll 4
+                for (int i = 0; i < n; ++i) {
+                    const f32x4 v = *reinterpret_cast<const f32x4*>(part + slot(base + i) * stride * a.head_dim + 64 * x);
+                    const float w = weights[c][i];
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) acc[x][y] = fmaf(v[y], w, acc[x][y]);
+                }
+            }
+    }
+    sum = over16(sum, [](float u, float v) { return u + v; });
+    if (col >= columns) return;
     const bool empty = m == -INFINITY;
     const float inv = 1.0f / sum;
     const int r = col / a.group, h = col - r * a.group;
-    uint16_t* to = a.out + (static_cast<int64_t>(first + r) * a.heads + kvh * a.group + h) * a.head_dim;
-    for (int d = 4 * (threadIdx.x & 7); d < a.head_dim; d += 32) {
-        f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int s = 0; s < splits; ++s) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(a.part + (from + s * stride) * a.head_dim + d);
-            const float w = exp2_from(ml[s * stride][0], m);
+    uint16_t* to = a.out + (static_cast<int64_t>(first + r) * a.heads + kvh * a.group + h) * a.head_dim + 4 * j;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i] = fmaf(x[i], w, acc[i]);
+    for (int x = 0; x < 4; ++x)
+        if (4 * j + 64 * x < a.head_dim) {
+            u32x2 o;
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+                o[y] = empty ? 0u : pack2<BF16>(acc[x][2 * y] * inv, acc[x][2 * y + 1] * inv);
+            *reinterpret_cast<u32x2*>(to + 64 * x) = o;
         }
-        u32x2 o;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) o[x] = empty ? 0u : pack2<BF16>(acc[2 * x] * inv, acc[2 * x + 1] * inv);
-        *reinterpret_cast<u32x2*>(to + d) = o;
-    }
 }
 
 // ---------------------------------------------------------------- host side
 
 struct ChunkShape {
-    int blocks;        // of 32 columns of a wave
     int64_t tiles;     // of a head, at most
-    int64_t pieces;    // of a head, at most
-    int64_t slots;     // of partials, at most
-    int64_t budget;
+    int64_t pieces;    // of a head, at most: tiles or runs
     bool split;
+    uint32_t work_shift;
     size_t bytes;
 };
 
-constexpr int kMostSplitSequences = 256;  // every workgroup reads all their lengths
-constexpr int kLeastSpan = 4;
+constexpr int64_t kMostSplitSequences = 256;  // every workgroup reads all their lengths
+constexpr int64_t kFewTiles = 4;              // for each workgroup that the device holds
 
 ChunkShape shape_of(int64_t sequences, int64_t rows, int64_t heads, int64_t kv_heads, int64_t head_dim,
                     int64_t capacity) {
     ChunkShape s;
-    const int64_t group = heads / kv_heads, cus = plm::cu_count();
-    s.blocks = head_dim <= 128 && false ? 2 : 1;
-    const int64_t cols = 32 * kWaves * s.blocks;
-    s.tiles = rows * group / cols + sequences + 2;
-    s.budget = cus * ((head_dim > 64 && s.blocks == 2) || head_dim > 128 ? 1 : 2);
-    s.split = sequences <= kMostSplitSequences && rows * heads / cols < 4 * s.budget &&
-              capacity >= 2 * kLeastSpan * kTile;
+    const int64_t group = heads / kv_heads;
+    const int64_t resident = plm::cu_count() * (head_dim > 128 ? 1 : 2);
+    s.tiles = rows * group / kColumns + sequences + 2;
+    s.split = sequences <= kMostSplitSequences && rows * heads / kColumns < kFewTiles * resident;
     s.pieces = s.tiles;
-    s.slots = 0;
+    s.work_shift = 0;
     s.bytes = 0;
     if (s.split) {
-        // splits of a place are at most its position tiles over the span, which twice the work bounds
-        const int64_t most = std::min(s.tiles * (plm::ceil_div(capacity, kTile) / kLeastSpan),
-                                      2 * s.budget / kv_heads + s.budget / 32 + 2);
-        s.pieces = s.tiles + most;
-        s.slots = most;
-        s.bytes = static_cast<size_t>(s.slots) * kv_heads * cols * (head_dim + 2) * sizeof(float) +
-                  sizeof(uint2) * (sequences + 2);
+        s.pieces = std::max<int64_t>(1, resident / kv_heads);
+        while (s.tiles * (plm::ceil_div(capacity, kTile) + kTileWork) >> s.work_shift > kMostInt / 2) ++s.work_shift;
+        s.bytes = static_cast<size_t>(2 * s.pieces) * kv_heads * kColumns * (head_dim + 2) * sizeof(float) +
+                  2 * sizeof(int) * s.tiles;
     }
     return s;
 }
 
-template <bool BF16, bool E8, int DP, int CB>
+template <bool BF16, bool E8, int DP>
 int launch_kernel(const ChunkArgs& a, const ChunkShape& s, hipStream_t st) {
     constexpr int bytes = Stage<DP, E8>::kLds;
     if (bytes > 64 * 1024) {
-        const int code = plm::allow_large_lds(reinterpret_cast<const void*>(&paged_chunk_kernel<BF16, E8, DP, CB>), bytes);
+        const int code = plm::allow_large_lds(reinterpret_cast<const void*>(&paged_chunk_kernel<BF16, E8, DP>), bytes);
         if (code != 0) return code;
     }
     const int64_t g = 8 % a.kv_heads == 0 ? 8 / a.kv_heads : 1;
     const int64_t blocks = plm::ceil_div(s.pieces, g) * g * a.kv_heads;
-    hipLaunchKernelGGL((paged_chunk_kernel<BF16, E8, DP, CB>), dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves),
+    hipLaunchKernelGGL((paged_chunk_kernel<BF16, E8, DP>), dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves),
                        bytes, st, a);
     if (s.split)
-        hipLaunchKernelGGL((paged_chunk_join_kernel<BF16, 32 * CB * kWaves>),
+        hipLaunchKernelGGL((paged_chunk_join_kernel<BF16>),
                            dim3(static_cast<unsigned>(s.tiles), static_cast<unsigned>(a.kv_heads),
-                                32 * CB * kWaves / kJoinColumns),
+                                kColumns / kJoinColumns),
                            dim3(kJoinThreads), 0, st, a);
     return 0;
 }
 
 template <bool BF16, bool E8>
 int launch_chunk(const ChunkArgs& a, const ChunkShape& s, hipStream_t st) {
-    if (a.head_dim > 128) return launch_kernel<BF16, E8, 256, 1>(a, s, st);
-    if (a.head_dim > 64)
-        return s.blocks == 2 ? launch_kernel<BF16, E8, 128, 2>(a, s, st) : launch_kernel<BF16, E8, 128, 1>(a, s, st);
-    return s.blocks == 2 ? launch_kernel<BF16, E8, 64, 2>(a, s, st) : launch_kernel<BF16, E8, 64, 1>(a, s, st);
+    if (a.head_dim > 128) return launch_kernel<BF16, E8, 256>(a, s, st);
+    return a.head_dim > 64 ? launch_kernel<BF16, E8, 128>(a, s, st) : launch_kernel<BF16, E8, 64>(a, s, st);
 }
 
 bool bad_heads(int64_t rows, int64_t heads, int64_t kv_heads) {
@@ -926,13 +980,10 @@ int run_chunk(ChunkArgs& a, const uint16_t* q, uint16_t* out, const int* row_sta
     a.group = static_cast<int>(heads / kv_heads);
     a.head_dim = static_cast<int>(head_dim);
     a.pieces = static_cast<int>(s.pieces);
-    a.slots = static_cast<int>(s.slots);
-    a.budget = static_cast<uint32_t>(s.budget);
-    a.least_span = kLeastSpan;
-    const int64_t cols = 32 * kWaves * s.blocks;
+    a.work_shift = s.work_shift;
     a.part = static_cast<float*>(part);
-    a.part_ml = a.part + s.slots * kv_heads * cols * head_dim;
-    a.plan = s.split ? reinterpret_cast<uint2*>(a.part_ml + s.slots * kv_heads * cols * 2) : nullptr;
+    a.part_ml = a.part + 2 * s.pieces * kv_heads * kColumns * head_dim;
+    a.plan = s.split ? reinterpret_cast<int*>(a.part_ml + 2 * s.pieces * kv_heads * kColumns * 2) : nullptr;
     // position / page_size of positions below 2^31: 2^(31 + shift) / page_size rounded up, 2^shift >= page_size
     a.shift = 0;
     while ((static_cast<uint64_t>(1) << a.shift) < a.p.page_size) ++a.shift;
