@@ -22,9 +22,7 @@ using namespace plm_paged;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kWaves = 4;
-constexpr int kColumns = 32 * kWaves;  // of a tile
-constexpr int kTile = 64;  // positions, one for each lane that looks up their pages
+constexpr int kTile = 64;  // positions that work is counted in
 // A running maximum is only moved once a score is more than 2^kLate above it: weights grow to 2^kLate, the
 // accumulators are multiplied in a few tiles instead of all.
 constexpr float kLate = 8.0f;
@@ -47,6 +45,7 @@ struct ChunkArgs {
     int kv_heads;
     int group;
     int head_dim;
+    int columns;           // of a tile
     int pieces;            // tiles of a head, or runs, at most
     uint32_t work_shift;   // so that a head's work stays in 32 bits
     uint32_t divide;       // position / page_size: position * divide >> 31 + shift
@@ -104,10 +103,10 @@ __device__ __forceinline__ Piece piece_of(const ChunkArgs& a, int place, int til
     p.rows = uniform(rows_of(a, place));
     p.length = uniform(length_of(a, place));
     const int columns = p.rows * a.group;
-    p.tiles = static_cast<int>(tiles_of(columns, kColumns));
+    p.tiles = static_cast<int>(tiles_of(columns, a.columns));
     p.tile = tile;
-    p.seen = uniform(seen_by(a, p.length, (min((tile + 1) * kColumns, columns) - 1) / a.group));
-    p.least = uniform(seen_by(a, p.length, tile * kColumns / a.group));
+    p.seen = uniform(seen_by(a, p.length, (min((tile + 1) * a.columns, columns) - 1) / a.group));
+    p.least = uniform(seen_by(a, p.length, tile * a.columns / a.group));
     p.begin = 0;
     p.end = p.seen;
     p.whole = true;
@@ -115,10 +114,10 @@ __device__ __forceinline__ Piece piece_of(const ChunkArgs& a, int place, int til
     return p;
 }
 
-// Place i's tiles begin at floor(start * group / kColumns) + i, which leaves
+// Place i's tiles begin at floor(start * group / a.columns) + i, which leaves
 // room for each place's last, partly filled one.
 __device__ __forceinline__ int first_tile_of(const ChunkArgs& a, int place) {
-    return static_cast<int>(static_cast<int64_t>(start_of(a, place)) * a.group / kColumns) + place;
+    return static_cast<int>(static_cast<int64_t>(start_of(a, place)) * a.group / a.columns) + place;
 }
 // The place of tile `at`, by a search 64 wide; every lane calls it.
 __device__ __forceinline__ int place_of_tile(const ChunkArgs& a, int at, int lane, int& first) {
@@ -166,8 +165,8 @@ __device__ __forceinline__ Work work_of(const ChunkArgs& a, int place) {
     if (place >= a.p.sequences + 2) return w;
     const int rows = rows_of(a, place);
     const int length = length_of(a, place);
-    w.tiles = static_cast<int>(tiles_of(static_cast<int64_t>(rows) * a.group, kColumns));
-    w.first = tiles_of(seen_by(a, length, min(kColumns / a.group, rows) - 1), kTile);
+    w.tiles = static_cast<int>(tiles_of(static_cast<int64_t>(rows) * a.group, a.columns));
+    w.first = tiles_of(seen_by(a, length, min(a.columns / a.group, rows) - 1), kTile);
     w.last = tiles_of(seen_by(a, length, rows - 1), kTile);
     return w;
 }
@@ -263,14 +262,13 @@ __device__ __forceinline__ float both_sum(float v) {
     return __uint_as_float(h[0]) + __uint_as_float(h[1]);
 }
 
-// A 16-byte piece of a row of LDS is kept at piece ^ swizzle(row), so that what is
-// read together touches every group of banks (a line of 256 bytes) once: the same
-// piece of 16 adjacent rows for keys, four adjacent pieces of four rows,
-// transposed, for values.  Where a line holds two rows, their lowest bit is one
-// of the line's.
-template <int DP>
-__device__ __forceinline__ int swizzle(int row) {
-    return DP == 64 ? (row >> 1 & 1) << 2 | (row >> 2 & 3) : (row & 3) << 2 | (row >> 2 & 3);
+// A tile lies in LDS in blocks of 64 head values, a position's 128 bytes after the
+// other's, each 16-byte piece at piece ^ swizzle(position), so that what is read
+// together touches every group of banks (a line of 256 bytes) once: the same piece
+// of 16 adjacent positions for keys, four adjacent pieces of four positions,
+// transposed, for values.
+__device__ __forceinline__ int swizzle(int position) {
+    return (position >> 1 & 1) << 2 | (position >> 2 & 3);
 }
 
 #pragma clang diagnostic push
@@ -279,10 +277,11 @@ __device__ __forceinline__ int swizzle(int row) {
 __device__ __forceinline__ void load_to_lds(const void* from, uint32_t to) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(to) : "m0", "memory");
 }
-#pragma clang diagnostic pop
-__device__ __forceinline__ void loads_barrier() {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+// 4 bytes a lane.
+__device__ __forceinline__ void load4_to_lds(const void* from, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(from), "s"(to) : "m0", "memory");
 }
+#pragma clang diagnostic pop
 
 // One column over positions [begin, end) by a wave, in fp32, reading nothing that
 // the column does not see: a lane has a position's score, then the values d =
@@ -355,7 +354,7 @@ __device__ void careful_column(const ChunkArgs& a, const Piece& piece, int kvh, 
         }
     }
     if (!piece.whole) {
-        const int64_t to = (static_cast<int64_t>(piece.slot) * a.kv_heads + kvh) * kColumns + (col - piece.tile * kColumns);
+        const int64_t to = (static_cast<int64_t>(piece.slot) * a.kv_heads + kvh) * a.columns + (col - piece.tile * a.columns);
         if (lane == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * to) = f32x2{m, l};
         for (int i = 0; i < 4; ++i)
             if (lane + 64 * i < a.head_dim) a.part[to * a.head_dim + lane + 64 * i] = acc[i];
@@ -375,17 +374,27 @@ __device__ __forceinline__ u32x2 lds_transposed(lds_char* base, int at) {
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(base + at)));
 }
 
+// LDS of a workgroup: kStages tiles of keys and values (and scales), then for each
+// wave the page table's entries of eight tiles.
 template <int DP, bool E8>
-struct Stage {
-    static constexpr int kRow = 2 * DP;                     // bytes
-    static constexpr int kV = kTile * kRow;                 // values behind the keys
-    static constexpr int kScales = 2 * kTile * kRow;        // then the scales
-    static constexpr int kBytes = kScales + (E8 ? 2 * kTile * 4 : 0);
-    static constexpr int kLds = 2 * kBytes;
+struct Layout {
+    static constexpr int kWaves = DP > 128 ? 4 : 8;
+    static constexpr int kColumns = 32 * kWaves;
+    static constexpr int kPositions = DP > 128 ? 32 : 64;   // of a tile
+    static constexpr int kBlocks = DP / 64;
+    static constexpr int kBlock = kPositions * 128;         // bytes
+    static constexpr int kV = kBlocks * kBlock;             // values behind the keys
+    static constexpr int kScales = 2 * kV;                  // then the scales
+    static constexpr int kStage = kScales + (E8 ? 2 * kPositions * 4 : 0);
+    static constexpr int kStages = 4;
+    static constexpr int kEntries = kStages * kStage;
+    static constexpr int kRing = 8;
+    static constexpr int kBytes = kEntries + kWaves * kRing * 256;
+    static_assert(kPositions == 8 * kWaves, "a wave loads eight positions of a tile");
 };
 
-// A piece by a workgroup: 4 waves of 32 columns each over the piece's positions,
-// 64 at a time through LDS, two tiles deep.
+// A piece by a workgroup: waves of 32 columns each over the piece's positions, a
+// tile at a time through LDS.
 //
 //   scores  S^T = K Q^T (32 x 32 x 16): a lane has, of column l & 31, the positions
 //           8 (j / 4) + 4 (l / 32) + j % 4, so that a column's maximum and sum are
@@ -394,6 +403,15 @@ struct Stage {
 //           values' eight positions are chosen to match, by two transposed reads
 //
 // Weights are rounded to the values' type once.
+//
+// Each wave alternates between the matrix cores (the scores of tile i + 1, then the
+// values of tile i) and the vector units (the weights of tile i + 1); the second four
+// waves are one step behind the first, so that of the two waves of a SIMD one is in
+// each.  A barrier a step keeps them so.  Tile t's keys are read in steps 2 t - 1
+// and 2 t (first and second waves), its values in 2 t + 1 and 2 t + 2; a wave loads its
+// part of tile t + 3 in the step of tile t's products, when tile t - 1, which lay
+// there, has been read.  Loads past the piece's end repeat its last row, so that
+// their count is always the same.
 //
 // E8: keys and values become 16-bit (exactly) on their way to LDS, values and
 // weights bf16 whatever the queries' type, scores and weights are multiplied by
@@ -407,296 +425,360 @@ struct Stage {
 // never read.
 template <bool BF16, bool E8, int DP>
 __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, int kvh, lds_char* lds) {
-    using St = Stage<DP, E8>;
+    using L = Layout<DP, E8>;
     constexpr bool VBF16 = BF16 || E8;
+    constexpr int KT = L::kPositions;
+    constexpr int KB = KT / 32;   // blocks of 32 positions
     constexpr int KS = DP / 16;   // score steps
     constexpr int DB = DP / 32;   // blocks of head values
-    constexpr int kLines = KS < 8 ? KS : 8;  // score steps whose pieces lie in one line of 256 bytes
-    constexpr int kAhead = 6;
     constexpr float kBias = bias_of(VBF16);
+    constexpr bool kDotSum = BF16 && !E8;  // the weights are summed as they were rounded, two an instruction
+    constexpr int kOutstanding = 1 + 2 * L::kBlocks;  // loads of a step
+    typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+    typedef __attribute__((address_space(3))) const int lds_int;
     const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool second = wave >= 4;
     const int li = lane & 31, half = lane >> 5;
-    const int columns = piece.rows * a.group, col0 = piece.tile * kColumns;
-    const int seen = piece.seen, least = piece.least, begin = piece.begin, end = piece.end;
     auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-    const int wave0 = col0 + 32 * wave;
+    const int columns = piece.rows * a.group;
+    const int wave0 = piece.tile * L::kColumns + 32 * wave;
+    const int col = wave0 + li;
     const int wave_least = uniform(seen_by(a, piece.length, min(wave0, columns - 1) / a.group));
     const int wave_seen =
         wave0 < columns ? uniform(seen_by(a, piece.length, (min(wave0 + 32, columns) - 1) / a.group)) : 0;
-
-    u32x4 q[KS];
-    int limit;
-    {
-        const int col = wave0 + li;
-        const int r = min(col, columns - 1) / a.group, h = min(col, columns - 1) - r * a.group;
-        const uint16_t* src = a.q + (piece.first + r) * a.q_row + (kvh * a.group + h) * a.q_head;
-        limit = col < columns ? seen_by(a, piece.length, r) : 0;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const int d = 16 * s + 8 * half;
-            q[s] = *reinterpret_cast<const u32x4*>(src + (d < a.head_dim ? d : 0)) ^ a.flip;
-            if (col >= columns || d >= a.head_dim) q[s] = u32x4{0, 0, 0, 0};
-        }
-    }
-    const int* table = a.p.table + static_cast<int64_t>(max(piece.place - 1, 0)) * a.p.table_cols;
-    const uint8_t* kbase = reinterpret_cast<const uint8_t*>(a.p.k) + (E8 ? 1 : 2) * kvh * a.p.head_stride;
-    const uint8_t* vbase = reinterpret_cast<const uint8_t*>(a.p.v) + (E8 ? 1 : 2) * kvh * a.p.head_stride;
-
-    // lane l looks up position t0 + l of a tile; past the last one it is the last
-    auto index_of = [&](int pos) {
-        return static_cast<uint32_t>(static_cast<uint64_t>(pos) * a.divide >> 31 >> a.shift);
-    };
-    auto page_of = [&](int t0) { return table[index_of(min(t0 + lane, seen - 1))]; };
-
-    // LDS addresses of this lane's reads: keys by score step, values by block and half
-    constexpr int kMask = DP == 64 ? 7 : 15;
-    constexpr int kBlocks = DB < 4 ? DB : 4;  // blocks whose pieces lie in one line
-    int kat[kLines], vat[kBlocks][2];
-#pragma unroll
-    for (int x = 0; x < kLines; ++x) kat[x] = li * St::kRow + (((2 * x + half) ^ swizzle<DP>(li)) & kMask) * 16;
-#pragma unroll
-    for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-            const int i16 = lane & 15, row = 8 * z + 4 * half + (i16 >> 2);
-            const int chunk = 4 * b + 2 * (lane >> 4 & 1) + (i16 >> 1 & 1);
-            vat[b][z] = St::kV + row * St::kRow + ((chunk ^ swizzle<DP>(row)) & kMask) * 16 + (i16 & 1) * 8;
-        }
+    const int begin = piece.begin, end = piece.end;
 
     float m = -INFINITY, l = 0.0f;  // weights are exp2(score - m): m is the maximum less the bias, up to kLate behind
     f32x16 acc[DB];
-
     bool masked = false;  // there was a position that some column does not see
 #pragma unroll
     for (int b = 0; b < DB; ++b)
 #pragma unroll
         for (int j = 0; j < 16; ++j) acc[b][j] = 0.0f;
+
     if (begin < end) {
-        // rows of a tile, in pieces of 16 bytes; a position without a page reads one that has one, a tile of none
-        // is left out
-        uint32_t row, slot;
-        int page;
-        bool there;
-        auto find_rows = [&](int t0) {
-            const uint32_t pos = static_cast<uint32_t>(min(t0 + lane, seen - 1));
-            slot = pos - index_of(static_cast<int>(pos)) * a.p.page_size;
-            there = page >= 0 && static_cast<uint32_t>(page) < a.p.num_pages;
-            row = static_cast<uint32_t>(page) * a.p.page_stride + slot * a.p.slot_stride;
-            const unsigned long long gone = __ballot(!there);
-            if (gone != 0 && gone != ~0ull) {
-                const uint32_t other = __shfl(row, __ffsll(~gone) - 1);
-                if (!there) row = other;
+        u32x4 q[KS];
+        int limit;
+        {
+            const int r = min(col, columns - 1) / a.group, h = min(col, columns - 1) - r * a.group;
+            const uint16_t* src = a.q + (piece.first + r) * a.q_row + (kvh * a.group + h) * a.q_head;
+            limit = col < columns ? seen_by(a, piece.length, r) : 0;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const int d = 16 * s + 8 * half;
+                q[s] = *reinterpret_cast<const u32x4*>(src + (d < a.head_dim ? d : 0)) ^ a.flip;
+                if (col >= columns || d >= a.head_dim) q[s] = u32x4{0, 0, 0, 0};
             }
-            return gone;
+        }
+        const int* table = a.p.table + static_cast<int64_t>(piece.place - 1) * a.p.table_cols;
+        const uint8_t* kbase = reinterpret_cast<const uint8_t*>(a.p.k) + (E8 ? 1 : 2) * kvh * a.p.head_stride;
+        const uint8_t* vbase = reinterpret_cast<const uint8_t*>(a.p.v) + (E8 ? 1 : 2) * kvh * a.p.head_stride;
+
+        // LDS addresses of this lane's reads: keys by score step, values by block of 32 and half
+        int kat[4], vat[2][2];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) kat[x] = li * 128 + ((2 * x + half) ^ swizzle(li)) * 16;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+                const int i16 = lane & 15, row = 8 * z + 4 * half + (i16 >> 2);
+                const int chunk = 4 * b + 2 * (lane >> 4 & 1) + (i16 >> 1 & 1);
+                vat[b][z] = L::kV + row * 128 + (chunk ^ swizzle(row)) * 16 + (i16 & 1) * 8;
+            }
+
+        auto index_of = [&](uint32_t pos) {
+            return __umulhi(2 * pos, a.divide) >> a.shift;
         };
-        // 16-bit caches: straight to LDS
-        auto load = [&](int stage) {
-            constexpr int kPerRow = St::kRow / 16;       // pieces of a row
-            constexpr int kLoads = kTile * St::kRow / 1024 / kWaves;
-            int64_t from[kLoads];
-            bool in[kLoads];
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                const int r = (wave * kLoads + i) * (64 / kPerRow) + lane / kPerRow;
-                const int chunk = (lane % kPerRow) ^ swizzle<DP>(r);
-                from[i] = static_cast<int64_t>(__shfl(row, r)) * 16 + chunk * 16;
-                in[i] = chunk * 8 < a.head_dim;
+        // position r of tile t; past the piece's end its last one
+        auto position = [&](int t, int r) { return static_cast<uint32_t>(min(begin + KT * t + r, end - 1)); };
+        auto row_at = [&](int page, uint32_t pos) {
+            return static_cast<uint32_t>(page) * a.p.page_stride + (pos - index_of(pos) * a.p.page_size) * a.p.slot_stride;
+        };
+        auto is_page = [&](int page) { return page >= 0 && static_cast<uint32_t>(page) < a.p.num_pages; };
+        const uint32_t ring = L::kEntries + wave * L::kRing * 256;
+        // the page table's entries of tile t, to LDS
+        auto load_entries = [&](int t) {
+            load4_to_lds(table + index_of(position(t, lane & (KT - 1))), lds_at + ring + (t & (L::kRing - 1)) * 256);
+        };
+        auto entry = [&](int t, int r) { return *(lds_int*)(lds + ring + (t & (L::kRing - 1)) * 256 + r * 4); };
+        // bit r: position r of a tile, whose entries the lanes hold, has no page
+        auto gone_of = [&](int page) {
+            const unsigned long long gone = __ballot(!is_page(page));
+            return KT == 64 ? gone : gone & 0xFFFFFFFFull;
+        };
+        // what a position without a page reads instead: one of the tile that has one, the cache's first row where none has
+        auto other_row = [&](int t, unsigned long long gone) {
+            const unsigned long long there = KT == 64 ? ~gone : ~gone & 0xFFFFFFFFull;
+            if (there == 0) return 0u;
+            const int f = __ffsll(there) - 1;
+            return row_at(entry(t, f), position(t, f));
+        };
+        // 16-bit caches: this wave's eight positions of tile t straight to LDS, eight lanes each
+        const int own = 8 * wave + (lane >> 3), chunk = (lane & 7) ^ swizzle(own);
+        int own_page = 0;
+        const uint8_t *ksrc = nullptr, *vsrc = nullptr;
+        auto find_own = [&](int t) {
+            uint32_t row = row_at(own_page, position(t, own));
+            if (__any(!is_page(own_page))) {
+                const uint32_t instead = other_row(t, gone_of(entry(t, lane)));
+                if (!is_page(own_page)) row = instead;
             }
-            const uint32_t to = __builtin_amdgcn_readfirstlane(lds_at + stage * St::kBytes + wave * kLoads * 1024);
-            if (a.head_dim == DP) {
-#pragma unroll
-                for (int i = 0; i < kLoads; ++i) {
-                    load_to_lds(kbase + from[i], to + i * 1024);
-                    load_to_lds(vbase + from[i], to + St::kV + i * 1024);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < kLoads; ++i)
-                    if (in[i]) {
-                        load_to_lds(kbase + from[i], to + i * 1024);
-                        load_to_lds(vbase + from[i], to + St::kV + i * 1024);
-                    }
+            const int64_t from = static_cast<int64_t>(row) * 16 + chunk * 16;
+            ksrc = kbase + from;
+            vsrc = vbase + from;
+        };
+        auto load_block = [&](int t, int i) {
+            const uint32_t to = uniform(lds_at + (t & (L::kStages - 1)) * L::kStage + i * L::kBlock + wave * 1024);
+            if (a.head_dim == DP || 64 * i + 8 * chunk < a.head_dim) {  // (some lanes of every load)
+                load_to_lds(ksrc + 128 * i, to);
+                load_to_lds(vsrc + 128 * i, to + L::kV);
             }
         };
-        // e4m3 caches: to registers first
-        constexpr int kUnits = E8 ? DP / 64 : 1;
+        // e4m3 caches: to registers first, to LDS a step of weights later
+        constexpr int kThreads = 64 * L::kWaves;
+        constexpr int kUnits = (KT * DP / 16 + kThreads - 1) / kThreads;
+        constexpr bool kSome = KT * DP / 16 % kThreads != 0;  // threads without a last unit
         u32x4 kraw[kUnits], vraw[kUnits];
         float scale_raw = 0.0f;
-        auto load8 = [&] {
+        auto load8 = [&](int t) {
+            const unsigned long long gone = gone_of(entry(t, lane));
+            const uint32_t instead = gone != 0 ? other_row(t, gone) : 0u;
 #pragma unroll
             for (int i = 0; i < kUnits; ++i) {
-                const int u = threadIdx.x + 64 * kWaves * i;
-                const int r = u / (DP / 16), c = u % (DP / 16);
-                const int64_t from = static_cast<int64_t>(__shfl(row, r)) * 16 + (16 * c < a.head_dim ? 16 * c : 0);
+                const int u = threadIdx.x + kThreads * i;
+                const int r = u / (DP / 16) & (KT - 1), c = u % (DP / 16);
+                const int page = entry(t, r);
+                const uint32_t row = is_page(page) ? row_at(page, position(t, r)) : instead;
+                const int64_t from = static_cast<int64_t>(row) * 16 + (16 * c < a.head_dim ? 16 * c : 0);
                 kraw[i] = *reinterpret_cast<const u32x4*>(kbase + from);
                 vraw[i] = *reinterpret_cast<const u32x4*>(vbase + from);
             }
-            if (wave < 2)
-                scale_raw = there ? (wave == 0 ? a.s.k : a.s.v)[page * a.s.page_stride + kvh * a.s.head_stride + slot] : 0.0f;
+            if (wave < 2) {
+                const int r = lane & (KT - 1), page = entry(t, r);
+                const uint32_t pos = position(t, r);
+                scale_raw = 0.0f;
+                if (is_page(page))
+                    scale_raw = (wave == 0 ? a.s.k : a.s.v)[page * a.s.page_stride + kvh * a.s.head_stride +
+                                                            (pos - index_of(pos) * a.p.page_size)];
+            }
         };
-        auto store8 = [&](int stage) {
-            lds_char* const to = lds + stage * St::kBytes;
+        auto store8 = [&](int t) {
+            lds_char* const to = lds + (t & (L::kStages - 1)) * L::kStage;
 #pragma unroll
             for (int i = 0; i < kUnits; ++i) {
-                const int u = threadIdx.x + 64 * kWaves * i;
+                const int u = threadIdx.x + kThreads * i;
                 const int r = u / (DP / 16), c = u % (DP / 16);
-                if (16 * c < a.head_dim) {
+                if (16 * c < a.head_dim && (!kSome || r < KT)) {
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const int where = r * St::kRow + ((2 * c + x) ^ swizzle<DP>(r)) * 16;
-                        *(__attribute__((address_space(3))) u32x4*)(to + where) = eight_of<BF16>(kraw[i], x);
-                        *(__attribute__((address_space(3))) u32x4*)(to + St::kV + where) = eight_of<true>(vraw[i], x);
+                        const int where = c / 4 * L::kBlock + r * 128 + (((2 * c + x) & 7) ^ swizzle(r)) * 16;
+                        *(lds_u32x4*)(to + where) = eight_of<BF16>(kraw[i], x);
+                        *(lds_u32x4*)(to + L::kV + where) = eight_of<true>(vraw[i], x);
                     }
                 }
             }
-            if (wave < 2) *(__attribute__((address_space(3))) float*)(to + St::kScales + wave * kTile * 4 + lane * 4) = scale_raw;
+            if (wave < 2 && lane < KT)
+                *(__attribute__((address_space(3))) float*)(to + L::kScales + wave * KT * 4 + lane * 4) = scale_raw;
         };
 
-        page = page_of(begin);
-        unsigned long long gone = find_rows(begin), next_gone = 0;
-        if (gone != ~0ull) {
+        f32x16 s[KB];
+        u32x4 w[2 * KB];
+        u32x4 ahead_v[DB];
+        auto value_piece = [&](lds_char* tile, int x, int b) {
+            const int from = b / 2 * L::kBlock + 16 * x * 128;
+            const u32x2 lo = lds_transposed(tile, vat[b % 2][0] + from);
+            const u32x2 hi = lds_transposed(tile, vat[b % 2][1] + from);
+            return u32x4{lo[0], lo[1], hi[0], hi[1]};
+        };
+        // Scores of tile t + 1, and the first values of tile t for what follows.  Reads of LDS are kept kAhead in
+        // front of their matrix instructions: as the compiler orders them each is waited for.  Between them (LOAD) the
+        // loads of tile t + 3, in the matrix instructions' shade.
+        int tile_page = 0;  // this lane's entry of the tile that is weighed next
+        auto scores = [&](int t, auto with_loads) {
+            constexpr bool LOAD = decltype(with_loads)::value;
+            const lds_char* const tile = lds + ((t + 1) & (L::kStages - 1)) * L::kStage;
+            lds_char* const vtile = lds + (t & (L::kStages - 1)) * L::kStage;
+            constexpr int kAhead = DB > 6 ? DB : 6, kSteps = KB * KS;
+            u32x4 k[kAhead];
+            auto key_piece = [&](int i) {
+                const int x = i / KB, b = i % KB;
+                return lds16(tile, kat[x % 4] + x / 4 * L::kBlock + b * 32 * 128);
+            };
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) s[b][j] = 0.0f;
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) k[i] = key_piece(i);
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                __builtin_amdgcn_sched_barrier(0);
+                s[i % KB] = mfma32<BF16>(k[i % kAhead], q[i / KB], s[i % KB]);
+                if (i + kAhead < kSteps)
+                    k[i % kAhead] = key_piece(i + kAhead);
+                else if (i + kAhead - kSteps < DB)
+                    ahead_v[i + kAhead - kSteps] = value_piece(vtile, 0, i + kAhead - kSteps);
+                if constexpr (LOAD && E8) {
+                    if (i == 1) store8(t + 3);
+                    if (i == 3) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the entries of the step before
+                    if (i == 3) load8(t + 4);
+                    if (i == 5) load_entries(t + 5);
+                } else if constexpr (LOAD) {
+                    if (i == 0) own_page = entry(t + 3, own);
+                    if (i == 1) load_entries(t + 5);
+                    if (i == 4) find_own(t + 3);
+                    if (i >= 5 && i - 5 < L::kBlocks) load_block(t + 3, i - 5);
+                }
+                if (i == kSteps - 1) tile_page = entry(t + 1, lane);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        // the values of tile t, after scores(t)
+        auto values = [&](int t) {
+            lds_char* const tile = lds + (t & (L::kStages - 1)) * L::kStage;
+#pragma unroll
+            for (int x = 0; x < 2 * KB; ++x)
+#pragma unroll
+                for (int b = 0; b < DB; ++b) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    acc[b] = mfma32<VBF16>(ahead_v[b], w[x], acc[b]);
+                    if (x + 1 < 2 * KB) ahead_v[b] = value_piece(tile, x + 1, b);
+                }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        // the weights of tile t's scores; false: the wave's columns see none of it
+        auto weigh = [&](int t) {
+            const int t0 = begin + KT * t;
+            const unsigned long long gone = gone_of(tile_page);
+            masked |= t0 + KT > piece.least || gone != 0;
+            if (t0 >= wave_seen || gone == (KT == 64 ? ~0ull : 0xFFFFFFFFull)) return false;
+            const lds_char* const tile = lds + (t & (L::kStages - 1)) * L::kStage;
             if constexpr (E8) {
-                load8();
-                store8(0);
-            } else {
-                load(0);
-            }
-        }
-        page = page_of(begin + kTile);
-        int stage = 0;
-        for (int t0 = begin; t0 < end; t0 += kTile, stage ^= 1) {
-            if constexpr (E8)
-                __syncthreads();
-            else
-                loads_barrier();
-            const bool more = t0 + kTile < end;
-            if (more) {
-                next_gone = find_rows(t0 + kTile);
-                if (next_gone != ~0ull) {
-                    if constexpr (E8)
-                        load8();
-                    else
-                        load(stage ^ 1);
-                }
-                page = page_of(t0 + 2 * kTile);
-            }
-            lds_char* const tile = lds + stage * St::kBytes;
-            masked |= t0 + kTile > least || gone != 0;
-            if (t0 < wave_seen && gone != ~0ull) {
-                f32x16 s[2];
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) s[b][j] = 0.0f;
-#pragma unroll
-                for (int x = 0; x < KS; ++x)
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        const u32x4 k = lds16(tile, kat[x % kLines] + x / kLines * 256 + b * 32 * St::kRow);
-                        s[b] = mfma32<BF16>(k, q[x], s[b]);
-                    }
-                // keys kAhead reads in front of their matrix instructions (without this each is waited for)
-                __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
-#pragma unroll
-                for (int i = 0; i < 2 * KS - kAhead; ++i) {
-                    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                }
-                __builtin_amdgcn_sched_group_barrier(0x8, kAhead, 0);
-                if constexpr (E8) {
-#pragma unroll
-                    for (int b = 0; b < 2; ++b)
-#pragma unroll
-                        for (int j = 0; j < 16; j += 4) {
-                            const f32x4 by = a.scale *
-                                __builtin_bit_cast(f32x4, lds16(tile, St::kScales + (32 * b + 2 * j + 4 * half) * 4));
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) s[b][j + i] *= by[i];
-                        }
-                }
-                const bool full = t0 + kTile <= wave_least && gone == 0;
-                // A row that sees a position has a maximum of at least the lowest number, one that sees none keeps
-                // -inf: its result is 0, while scores that are all -inf give 0 / 0.
-                float floor = full ? -FLT_MAX : -INFINITY;
-                if (!full) {
-                    asm volatile("");  // a branch, not selects in every tile
-#pragma unroll
-                        for (int b = 0; b < 2; ++b) {
-                            // bit i: position 32 b + 4 half + i of the tile is hidden
-                            const int left = limit - t0 - 32 * b - 4 * half;
-                            const uint32_t hidden = static_cast<uint32_t>(gone >> 32 * b) >> 4 * half |
-                                                    (left >= 32 ? 0u : ~0u << max(left, 0));
-                            if ((~hidden & 0x0F0F0F0Fu) != 0) floor = -FLT_MAX;
-#pragma unroll
-                            for (int j = 0; j < 16; ++j)
-                                if (hidden >> (8 * (j >> 2) + (j & 3)) & 1) s[b][j] = -INFINITY;
-                        }
-                }
-                // 16-bit caches: the scale goes into the weights' exponents as they are formed, in one instruction.
-                // The maximum is rounded there and the scores are not, which all weights of a column share, but from
-                // 2^22 on it might be large: such scores are multiplied first.
-                float times = E8 ? 1.0f : a.scale;
-                float top = s[0][0];
-#pragma unroll
-                for (int j = 1; j < 32; ++j) top = fmaxf(top, s[j >> 4][j & 15]);
-                top = fmaxf(m, both_max(fmaxf(top * times, floor)) - kBias);
-                if (!E8 && __any(fabsf(top) > 0x1p22f && top > -0x1p127f)) {
-                    times = 1.0f;
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) s[j >> 4][j & 15] *= a.scale;
-                }
-                if (__any(top > m + kLate)) {
-                    const float fade = exp2_from(m, top);
-                    m = top;
-                    l *= fade;
-#pragma unroll
-                    for (int b = 0; b < DB; ++b)
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) acc[b][j] *= fade;
-                }
-                u32x4 w[4];
-                const float from = m == -INFINITY ? 0.0f : m;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        s[b][j] = __builtin_amdgcn_exp2f(fmaf(s[b][j], times, -from));
-                        sum[j & 3] += s[b][j];
-                    }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
+                for (int b = 0; b < KB; ++b)
 #pragma unroll
                     for (int j = 0; j < 16; j += 4) {
-                        f32x4 by = {1.0f, 1.0f, 1.0f, 1.0f};
-                        if constexpr (E8) {
-                            by = __builtin_bit_cast(f32x4, lds16(tile, St::kScales + kTile * 4 + (32 * b + 2 * j + 4 * half) * 4));
-                        }
-                        f32x4 v = {s[b][j], s[b][j + 1], s[b][j + 2], s[b][j + 3]};
-                        if constexpr (E8)
+                        const f32x4 by = a.scale *
+                            __builtin_bit_cast(f32x4, lds16(tile, L::kScales + (32 * b + 2 * j + 4 * half) * 4));
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) v[i] *= by[i];
-                        w[2 * b + (j >> 3)][(j & 4) / 2] = pack2<VBF16>(v[0], v[1]);
-                        w[2 * b + (j >> 3)][(j & 4) / 2 + 1] = pack2<VBF16>(v[2], v[3]);
-                    }
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-#pragma unroll
-                    for (int b = 0; b < DB; ++b) {
-                        const int from = b / kBlocks * 256 + 16 * x * St::kRow;
-                        const u32x2 lo = lds_transposed(tile, vat[b % kBlocks][0] + from);
-                        const u32x2 hi = lds_transposed(tile, vat[b % kBlocks][1] + from);
-                        const u32x4 v = {lo[0], lo[1], hi[0], hi[1]};
-                        acc[b] = mfma32<VBF16>(v, w[x], acc[b]);
+                        for (int i = 0; i < 4; ++i) s[b][j + i] *= by[i];
                     }
             }
-            if constexpr (E8)
-                if (more && next_gone != ~0ull) store8(stage ^ 1);
-            gone = next_gone;
+            const bool full = t0 + KT <= wave_least && gone == 0;
+            // A row that sees a position has a maximum of at least the lowest number, one that sees none keeps
+            // -inf: its result is 0, while scores that are all -inf give 0 / 0.
+            float floor = full ? -FLT_MAX : -INFINITY;
+            if (!full) {
+                asm volatile("");  // a branch, not selects in every tile
+#pragma unroll
+                for (int b = 0; b < KB; ++b) {
+                    // bit i: position 32 b + 4 half + i of the tile is hidden
+                    const int left = limit - t0 - 32 * b - 4 * half;
+                    const uint32_t hidden = static_cast<uint32_t>(gone >> 32 * b) >> 4 * half |
+                                            (left >= 32 ? 0u : ~0u << max(left, 0));
+                    if ((~hidden & 0x0F0F0F0Fu) != 0) floor = -FLT_MAX;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (hidden >> (8 * (j >> 2) + (j & 3)) & 1) s[b][j] = -INFINITY;
+                }
+            }
+            // 16-bit caches: the scale goes into the weights' exponents as they are formed, in one instruction.
+            // The maximum is rounded there and the scores are not, which all weights of a column share, but from
+            // 2^22 on it might be large: such scores are multiplied first.
+            float times = E8 ? 1.0f : a.scale;
+            float top = s[0][0];
+#pragma unroll
+            for (int j = 1; j < 16 * KB; ++j) top = fmaxf(top, s[j >> 4][j & 15]);
+            top = fmaxf(m, both_max(fmaxf(top * times, floor)) - kBias);
+            if (!E8 && __any(fabsf(top) > 0x1p22f && top > -0x1p127f)) {
+                times = 1.0f;
+#pragma unroll
+                for (int j = 0; j < 16 * KB; ++j) s[j >> 4][j & 15] *= a.scale;
+            }
+            if (__any(top > m + kLate)) {
+                const float fade = exp2_from(m, top);
+                m = top;
+                l *= fade;
+#pragma unroll
+                for (int b = 0; b < DB; ++b)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) acc[b][j] *= fade;
+            }
+            const float from = m == -INFINITY ? 0.0f : m;
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                    f32x4 v;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        v[i] = __builtin_amdgcn_exp2f(fmaf(s[b][j + i], times, -from));
+                        if constexpr (!kDotSum) sum[i] += v[i];
+                    }
+                    if constexpr (E8)
+                        v = v * __builtin_bit_cast(f32x4, lds16(tile, L::kScales + KT * 4 + (32 * b + 2 * j + 4 * half) * 4));
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t two = pack2<VBF16>(v[2 * i], v[2 * i + 1]);
+                        w[2 * b + (j >> 3)][(j & 4) / 2 + i] = two;
+                        if constexpr (kDotSum)
+                            sum[2 * (j >> 2 & 1) + i] = __builtin_amdgcn_fdot2_f32_bf16(
+                                __builtin_bit_cast(bf16x2, two), __builtin_bit_cast(bf16x2, 0x3F803F80u),
+                                sum[2 * (j >> 2 & 1) + i], false);
+                    }
+                }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            return true;
+        };
+        // until this wave's loads but the last step's are there (the first waves after their weights, the second
+        // after their products), and every wave is here
+        auto step_end = [&](bool wait) {
+            if constexpr (E8) {
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            } else {
+                if (wait)
+                    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kOutstanding) : "memory");
+                else
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                asm volatile("s_barrier" ::: "memory");
+            }
+        };
+
+        const int tiles = (end - begin + KT - 1) / KT;
+        for (int t = 0; t < 5; ++t) load_entries(t);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        for (int t = 0; t < 3; ++t) {
+            if constexpr (E8) {
+                load8(t);
+                store8(t);
+            } else {
+                own_page = entry(t, own);
+                find_own(t);
+#pragma unroll
+                for (int i = 0; i < L::kBlocks; ++i) load_block(t, i);
+            }
         }
+        if constexpr (E8) load8(3);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (second) asm volatile("s_barrier" ::: "memory");
+        scores(-1, std::false_type{});
+        step_end(false);
+        for (int t = 0; t < tiles; ++t) {
+            const bool live = weigh(t);
+            step_end(!second);
+            __builtin_amdgcn_s_setprio(1);
+            scores(t, std::true_type{});
+            if (live) values(t);
+            __builtin_amdgcn_s_setprio(0);
+            step_end(second);
+        }
+        if (!second) asm volatile("s_barrier" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what was loaded past the end
     }
     l = both_sum(l);
 
@@ -707,15 +789,13 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
         for (int j = 0; j < 16; ++j) odd |= !(fabsf(acc[b][j]) < INFINITY);
     if (__any(masked && odd)) {
         const int most = min(wave0 + 32, columns);
-        for (int col = wave0; col < most; ++col) careful_column<BF16, E8>(a, piece, kvh, col, lane);
+        for (int c = wave0; c < most; ++c) careful_column<BF16, E8>(a, piece, kvh, c, lane);
         return;
     }
-
-    const int in = 32 * wave + li;
-    const int col = col0 + in;
     if (col >= columns) return;
     if (!piece.whole) {
-        const int64_t to = (static_cast<int64_t>(piece.slot) * a.kv_heads + kvh) * kColumns + in;
+        const int64_t to =
+            (static_cast<int64_t>(piece.slot) * a.kv_heads + kvh) * L::kColumns + (col - piece.tile * L::kColumns);
         if (half == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * to) = f32x2{m, l};
 #pragma unroll
         for (int b = 0; b < DB; ++b)
@@ -749,8 +829,8 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
 
 // Workgroup -> (tile or run, key-value head).
 template <bool BF16, bool E8, int DP>
-__global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void paged_chunk_kernel(const ChunkArgs a) {
-    using St = Stage<DP, E8>;
+__global__ __launch_bounds__(DP > 128 ? 256 : 512, 1) void paged_chunk_kernel(const ChunkArgs a) {
+    using L = Layout<DP, E8>;
     extern __shared__ char lds_raw[];
     lds_char* const lds = (lds_char*)lds_raw;
     const int lane = threadIdx.x & 63;
@@ -758,13 +838,13 @@ __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void paged_chunk_ker
     block_of(a, at, kvh);
     if (at >= a.pieces) return;
     if (a.head_dim != DP)  // the loads leave out what is behind a head's end
-        for (int i = threadIdx.x; i < St::kLds / 16; i += 64 * kWaves)
+        for (int i = threadIdx.x; i < L::kStages * L::kStage / 16; i += 64 * L::kWaves)
             *(__attribute__((address_space(3))) u32x4*)(lds + 16 * i) = u32x4{0, 0, 0, 0};
     Border next, last;
     if (a.plan == nullptr) {
         int first;
         const int place = place_of_tile(a, at, lane, first);
-        const int tiles = static_cast<int>(tiles_of(rows_of(a, place) * static_cast<int64_t>(a.group), kColumns));
+        const int tiles = static_cast<int>(tiles_of(rows_of(a, place) * static_cast<int64_t>(a.group), L::kColumns));
         if (at - first >= tiles) return;
         next = Border{place, tiles - 1 - (at - first), 0.0f};  // the longest first
         last = Border{place, next.tile + 1, 0.0f};
@@ -822,18 +902,18 @@ __global__ __launch_bounds__(kJoinThreads) void paged_chunk_join_kernel(const Ch
     const int first = start_of(a, place);
     const int columns = rows_of(a, place) * a.group;
     const int tile = blockIdx.x - begin;
-    if (tile >= static_cast<int>(tiles_of(columns, kColumns))) return;
+    if (tile >= static_cast<int>(tiles_of(columns, a.columns))) return;
     // (within the runs also where the lengths were changed under the first kernel)
     const int run = min(max(a.plan[2 * blockIdx.x], 0), a.pieces - 1);
     const int parts = min(a.plan[2 * blockIdx.x + 1], a.pieces - 1) - run + 1;
     if (parts <= 1) return;
     const int c = threadIdx.x >> 4, j = threadIdx.x & 15;
-    const int in = blockIdx.z * kJoinColumns + c, col = tile * kColumns + in;
+    const int in = blockIdx.z * kJoinColumns + c, col = tile * a.columns + in;
     const int kvh = blockIdx.y;
     // partial i: the first is its run's second
     auto slot = [](int i) { return max(2 * i, 1); };
-    const int64_t stride = static_cast<int64_t>(a.kv_heads) * kColumns;
-    const int64_t from = (static_cast<int64_t>(2 * run) * a.kv_heads + kvh) * kColumns + in;
+    const int64_t stride = static_cast<int64_t>(a.kv_heads) * a.columns;
+    const int64_t from = (static_cast<int64_t>(2 * run) * a.kv_heads + kvh) * a.columns + in;
     const f32x2* ml = reinterpret_cast<const f32x2*>(a.part_ml) + from;
     auto over16 = [](float v, auto op) {
 #pragma unroll
@@ -890,6 +970,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_chunk_join_kernel(const Ch
 // ---------------------------------------------------------------- host side
 
 struct ChunkShape {
+    int64_t columns;   // of a tile
     int64_t tiles;     // of a head, at most
     int64_t pieces;    // of a head, at most: tiles or runs
     bool split;
@@ -904,16 +985,17 @@ ChunkShape shape_of(int64_t sequences, int64_t rows, int64_t heads, int64_t kv_h
                     int64_t capacity) {
     ChunkShape s;
     const int64_t group = heads / kv_heads;
-    const int64_t resident = plm::cu_count() * (head_dim > 128 ? 1 : 2);
-    s.tiles = rows * group / kColumns + sequences + 2;
-    s.split = sequences <= kMostSplitSequences && rows * heads / kColumns < kFewTiles * resident;
+    const int64_t resident = plm::cu_count();
+    s.columns = head_dim > 128 ? Layout<256, false>::kColumns : Layout<128, false>::kColumns;
+    s.tiles = rows * group / s.columns + sequences + 2;
+    s.split = sequences <= kMostSplitSequences && rows * heads / s.columns < kFewTiles * resident;
     s.pieces = s.tiles;
     s.work_shift = 0;
     s.bytes = 0;
     if (s.split) {
         s.pieces = std::max<int64_t>(1, resident / kv_heads);
         while (s.tiles * (plm::ceil_div(capacity, kTile) + kTileWork) >> s.work_shift > kMostInt / 2) ++s.work_shift;
-        s.bytes = static_cast<size_t>(2 * s.pieces) * kv_heads * kColumns * (head_dim + 2) * sizeof(float) +
+        s.bytes = static_cast<size_t>(2 * s.pieces) * kv_heads * s.columns * (head_dim + 2) * sizeof(float) +
                   2 * sizeof(int) * s.tiles;
     }
     return s;
@@ -921,26 +1003,28 @@ ChunkShape shape_of(int64_t sequences, int64_t rows, int64_t heads, int64_t kv_h
 
 template <bool BF16, bool E8, int DP>
 int launch_kernel(const ChunkArgs& a, const ChunkShape& s, hipStream_t st) {
-    constexpr int bytes = Stage<DP, E8>::kLds;
+    using L = Layout<DP, E8>;
+    constexpr int bytes = L::kBytes;
     if (bytes > 64 * 1024) {
         const int code = plm::allow_large_lds(reinterpret_cast<const void*>(&paged_chunk_kernel<BF16, E8, DP>), bytes);
         if (code != 0) return code;
     }
     const int64_t g = 8 % a.kv_heads == 0 ? 8 / a.kv_heads : 1;
     const int64_t blocks = plm::ceil_div(s.pieces, g) * g * a.kv_heads;
-    hipLaunchKernelGGL((paged_chunk_kernel<BF16, E8, DP>), dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves),
+    hipLaunchKernelGGL((paged_chunk_kernel<BF16, E8, DP>), dim3(static_cast<unsigned>(blocks)), dim3(64 * L::kWaves),
                        bytes, st, a);
     if (s.split)
         hipLaunchKernelGGL((paged_chunk_join_kernel<BF16>),
                            dim3(static_cast<unsigned>(s.tiles), static_cast<unsigned>(a.kv_heads),
-                                kColumns / kJoinColumns),
+                                L::kColumns / kJoinColumns),
                            dim3(kJoinThreads), 0, st, a);
     return 0;
 }
 
 template <bool BF16, bool E8>
 int launch_chunk(const ChunkArgs& a, const ChunkShape& s, hipStream_t st) {
-    if (a.head_dim > 128) return launch_kernel<BF16, E8, 256>(a, s, st);
+    if (a.head_dim > 192) return launch_kernel<BF16, E8, 256>(a, s, st);
+    if (a.head_dim > 128) return launch_kernel<BF16, E8, 192>(a, s, st);
     return a.head_dim > 64 ? launch_kernel<BF16, E8, 128>(a, s, st) : launch_kernel<BF16, E8, 64>(a, s, st);
 }
 
@@ -979,11 +1063,12 @@ int run_chunk(ChunkArgs& a, const uint16_t* q, uint16_t* out, const int* row_sta
     a.kv_heads = static_cast<int>(kv_heads);
     a.group = static_cast<int>(heads / kv_heads);
     a.head_dim = static_cast<int>(head_dim);
+    a.columns = static_cast<int>(s.columns);
     a.pieces = static_cast<int>(s.pieces);
     a.work_shift = s.work_shift;
     a.part = static_cast<float*>(part);
-    a.part_ml = a.part + 2 * s.pieces * kv_heads * kColumns * head_dim;
-    a.plan = s.split ? reinterpret_cast<int*>(a.part_ml + 2 * s.pieces * kv_heads * kColumns * 2) : nullptr;
+    a.part_ml = a.part + 2 * s.pieces * kv_heads * s.columns * head_dim;
+    a.plan = s.split ? reinterpret_cast<int*>(a.part_ml + 2 * s.pieces * kv_heads * s.columns * 2) : nullptr;
     // position / page_size of positions below 2^31: 2^(31 + shift) / page_size rounded up, 2^shift >= page_size
     a.shift = 0;
     while ((static_cast<uint64_t>(1) << a.shift) < a.p.page_size) ++a.shift;
