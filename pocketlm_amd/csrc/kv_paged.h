@@ -91,12 +91,16 @@ struct Pages {
 };
 
 // The scales of e4m3 caches: a position's and head's at page * page_stride +
-// head * head_stride + slot.
+// head * head_stride + slot, which 32 bits reach.
 struct Scales {
     float* k;
     float* v;
-    int64_t page_stride;
-    int64_t head_stride;
+    uint32_t page_stride;
+    uint32_t head_stride;
+
+    __device__ __forceinline__ uint32_t at(int page, int head, uint32_t slot) const {
+        return static_cast<uint32_t>(page) * page_stride + static_cast<uint32_t>(head) * head_stride + slot;
+    }
 };
 
 // Where row `row` of a call goes.  Every lane of a wave calls it.
@@ -221,13 +225,15 @@ inline int pages_of(Pages& p, void* k_cache, void* v_cache, const int* page_tabl
     return 0;
 }
 
-// The scales of e4m3 caches; 0, or the code of the failure.
-inline int scales_of(Scales& s, float* k_scales, float* v_scales, int64_t page_stride, int64_t head_stride) {
+// The scales of e4m3 caches whose pages are known; 0, or the code of the failure.
+inline int scales_of(Scales& s, const Pages& p, int64_t kv_heads, float* k_scales, float* v_scales, int64_t page_stride,
+                     int64_t head_stride) {
     if (k_scales == nullptr || v_scales == nullptr) return plm::fail(-1, "null pointer");
-    if (page_stride < 0 || head_stride < 0 || page_stride > (static_cast<int64_t>(1) << 40) ||
-        head_stride > (static_cast<int64_t>(1) << 40))
-        return plm::fail(-2, "bad strides of the scales");
-    s = Scales{k_scales, v_scales, page_stride, head_stride};
+    if (page_stride < 0 || head_stride < 0) return plm::fail(-2, "bad strides of the scales");
+    const double last = static_cast<double>(p.num_pages - 1) * static_cast<double>(page_stride) +
+                        static_cast<double>(kv_heads - 1) * static_cast<double>(head_stride) + p.page_size;
+    if (last >= 4294967296.0) return plm::fail(-2, "scales span at most 16 GiB");
+    s = Scales{k_scales, v_scales, static_cast<uint32_t>(page_stride), static_cast<uint32_t>(head_stride)};
     return 0;
 }
 

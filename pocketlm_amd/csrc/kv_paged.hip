@@ -492,7 +492,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void paged_atten
             const uint32_t slot = static_cast<uint32_t>(pos) % a.p.page_size;
             const bool there = pos < end && page >= 0 && static_cast<uint32_t>(page) < a.p.num_pages;
             const float* from = lane < 32 ? a.s.k : a.s.v;
-            return there ? from[page * a.s.page_stride + kvh * a.s.head_stride + slot] : 0.0f;
+            return there ? from[a.s.at(page, kvh, slot)] : 0.0f;
         };
         u32x4 k[2][E8 ? KS / 2 : KS];
         std::conditional_t<E8, u32x2, u32x4> v[8][SETS];
@@ -1194,7 +1194,7 @@ PLM_EXPORT int kv_paged_attention_decode_e4m3(const uint16_t* q, const uint8_t* 
                             sequences, table_cols, num_pages, page_size, kv_heads, head_dim, page_stride, slot_stride,
                             head_stride, dtype_code);
     if (code != 0) return code;
-    code = scales_of(a.s, const_cast<float*>(k_scales), const_cast<float*>(v_scales), scale_page_stride,
+    code = scales_of(a.s, a.p, kv_heads, const_cast<float*>(k_scales), const_cast<float*>(v_scales), scale_page_stride,
                      scale_head_stride);
     if (code != 0) return code;
     return run_decode<true>(a, q, out, scratch, scratch_bytes, sequences, rows, heads, kv_heads, head_dim, q_seq_stride,

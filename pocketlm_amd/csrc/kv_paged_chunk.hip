@@ -323,7 +323,7 @@ __device__ void careful_column(const ChunkArgs& a, const Piece& piece, int kvh, 
 #pragma unroll 1
             for (int d = 0; d < a.head_dim; ++d) s = fmaf(widen1<BF16>(q[d] ^ static_cast<uint16_t>(a.flip)), value(k, d), s);
             if constexpr (E8) {
-                const int64_t scale = page * a.s.page_stride + kvh * a.s.head_stride + slot;
+                const uint32_t scale = a.s.at(page, kvh, slot);
                 s *= a.s.k[scale];
                 by = a.s.v[scale];
             }
@@ -494,8 +494,9 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
         };
         // position r of tile t; past the piece's end its last one
         auto position = [&](int t, int r) { return static_cast<uint32_t>(min(begin + KT * t + r, end - 1)); };
-        auto row_at = [&](int page, uint32_t pos) {
-            return static_cast<uint32_t>(page) * a.p.page_stride + (pos - index_of(pos) * a.p.page_size) * a.p.slot_stride;
+        auto slot_of = [&](uint32_t pos) { return pos - index_of(pos) * a.p.page_size; };
+        auto row_at = [&](int page, uint32_t slot) {
+            return static_cast<uint32_t>(page) * a.p.page_stride + slot * a.p.slot_stride;
         };
         auto is_page = [&](int page) { return page >= 0 && static_cast<uint32_t>(page) < a.p.num_pages; };
         const uint32_t ring = L::kEntries + wave * L::kRing * 256;
@@ -514,22 +515,25 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
             const unsigned long long there = KT == 64 ? ~gone : ~gone & 0xFFFFFFFFull;
             if (there == 0) return 0u;
             const int f = __ffsll(there) - 1;
-            return row_at(entry(t, f), position(t, f));
+            return row_at(entry(t, f), slot_of(position(t, f)));
         };
-        // 16-bit caches: this wave's eight positions of tile t straight to LDS, eight lanes each
-        const int own = 8 * wave + (lane >> 3), chunk = (lane & 7) ^ swizzle(own);
+        // A wave loads eight positions of a tile, eight lanes each: this lane's, its page and where it lies.
+        const int own = 8 * wave + (lane >> 3), piece8 = lane & 7, chunk = piece8 ^ swizzle(own);
         int own_page = 0;
+        uint32_t own_slot = 0;
         const uint8_t *ksrc = nullptr, *vsrc = nullptr;
         auto find_own = [&](int t) {
-            uint32_t row = row_at(own_page, position(t, own));
+            own_slot = slot_of(position(t, own));
+            uint32_t row = row_at(own_page, own_slot);
             if (__any(!is_page(own_page))) {
                 const uint32_t instead = other_row(t, gone_of(entry(t, lane)));
                 if (!is_page(own_page)) row = instead;
             }
-            const int64_t from = static_cast<int64_t>(row) * 16 + chunk * 16;
+            const int64_t from = static_cast<int64_t>(row) * 16 + (E8 ? (16 * piece8 < a.head_dim ? piece8 : 0) : chunk) * 16;
             ksrc = kbase + from;
             vsrc = vbase + from;
         };
+        // 16-bit caches: straight to LDS
         auto load_block = [&](int t, int i) {
             const uint32_t to = uniform(lds_at + (t & (L::kStages - 1)) * L::kStage + i * L::kBlock + wave * 1024);
             if (a.head_dim == DP || 64 * i + 8 * chunk < a.head_dim) {  // (some lanes of every load)
@@ -537,51 +541,41 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
                 load_to_lds(vsrc + 128 * i, to + L::kV);
             }
         };
-        // e4m3 caches: to registers first, to LDS a step of weights later
-        constexpr int kThreads = 64 * L::kWaves;
-        constexpr int kUnits = (KT * DP / 16 + kThreads - 1) / kThreads;
-        constexpr bool kSome = KT * DP / 16 % kThreads != 0;  // threads without a last unit
+        // e4m3 caches: to registers first, 16 values a lane and piece, to LDS a step of products later; the first lane of
+        // a position has its key scale (times the softmax's), the second its value scale
+        // (every lane loads something: a branch around a load is a wait for the ones before it)
+        constexpr int kUnits = (DP + 127) / 128;
         u32x4 kraw[kUnits], vraw[kUnits];
         float scale_raw = 0.0f;
-        auto load8 = [&](int t) {
-            const unsigned long long gone = gone_of(entry(t, lane));
-            const uint32_t instead = gone != 0 ? other_row(t, gone) : 0u;
+        bool scale_there = false;
+        const float* const scales = (piece8 == 0 ? a.s.k : a.s.v) + static_cast<uint32_t>(kvh) * a.s.head_stride;
+        const int further = 16 * piece8 + 128 < a.head_dim ? 128 : 0;
+        auto load8 = [&] {
+            scale_there = is_page(own_page);
+            const uint32_t at = scale_there ? static_cast<uint32_t>(own_page) * a.s.page_stride + own_slot : 0u;
 #pragma unroll
             for (int i = 0; i < kUnits; ++i) {
-                const int u = threadIdx.x + kThreads * i;
-                const int r = u / (DP / 16) & (KT - 1), c = u % (DP / 16);
-                const int page = entry(t, r);
-                const uint32_t row = is_page(page) ? row_at(page, position(t, r)) : instead;
-                const int64_t from = static_cast<int64_t>(row) * 16 + (16 * c < a.head_dim ? 16 * c : 0);
-                kraw[i] = *reinterpret_cast<const u32x4*>(kbase + from);
-                vraw[i] = *reinterpret_cast<const u32x4*>(vbase + from);
+                kraw[i] = *reinterpret_cast<const u32x4*>(ksrc + (i > 0 ? further : 0));
+                vraw[i] = *reinterpret_cast<const u32x4*>(vsrc + (i > 0 ? further : 0));
             }
-            if (wave < 2) {
-                const int r = lane & (KT - 1), page = entry(t, r);
-                const uint32_t pos = position(t, r);
-                scale_raw = 0.0f;
-                if (is_page(page))
-                    scale_raw = (wave == 0 ? a.s.k : a.s.v)[page * a.s.page_stride + kvh * a.s.head_stride +
-                                                            (pos - index_of(pos) * a.p.page_size)];
-            }
+            scale_raw = scales[at];
         };
         auto store8 = [&](int t) {
             lds_char* const to = lds + (t & (L::kStages - 1)) * L::kStage;
 #pragma unroll
-            for (int i = 0; i < kUnits; ++i) {
-                const int u = threadIdx.x + kThreads * i;
-                const int r = u / (DP / 16), c = u % (DP / 16);
-                if (16 * c < a.head_dim && (!kSome || r < KT)) {
+            for (int i = 0; i < kUnits; ++i)
+                if (16 * piece8 + 128 * i < a.head_dim) {
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const int where = c / 4 * L::kBlock + r * 128 + (((2 * c + x) & 7) ^ swizzle(r)) * 16;
+                        const int where = (piece8 / 4 + 2 * i) * L::kBlock + own * 128 +
+                                          (((2 * piece8 + x) & 7) ^ swizzle(own)) * 16;
                         *(lds_u32x4*)(to + where) = eight_of<BF16>(kraw[i], x);
                         *(lds_u32x4*)(to + L::kV + where) = eight_of<true>(vraw[i], x);
                     }
                 }
-            }
-            if (wave < 2 && lane < KT)
-                *(__attribute__((address_space(3))) float*)(to + L::kScales + wave * KT * 4 + lane * 4) = scale_raw;
+            if (piece8 < 2)
+                *(__attribute__((address_space(3))) float*)(to + L::kScales + (piece8 * KT + own) * 4) =
+                    scale_there ? (piece8 == 0 ? scale_raw * a.scale : scale_raw) : 0.0f;
         };
 
         f32x16 s[KB];
@@ -623,10 +617,16 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
                 else if (i + kAhead - kSteps < DB)
                     ahead_v[i + kAhead - kSteps] = value_piece(vtile, 0, i + kAhead - kSteps);
                 if constexpr (LOAD && E8) {
-                    if (i == 1) store8(t + 3);
-                    if (i == 3) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the entries of the step before
-                    if (i == 3) load8(t + 4);
-                    if (i == 5) load_entries(t + 5);
+                    if (i == 1) {
+                        store8(t + 3);
+                        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the entries of the step before
+                        own_page = entry(t + 4, own);
+                    }
+                    if (i == 3) load_entries(t + 5);
+                    if (i == 5) {
+                        find_own(t + 4);
+                        load8();
+                    }
                 } else if constexpr (LOAD) {
                     if (i == 0) own_page = entry(t + 3, own);
                     if (i == 1) load_entries(t + 5);
@@ -657,16 +657,20 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
             masked |= t0 + KT > piece.least || gone != 0;
             if (t0 >= wave_seen || gone == (KT == 64 ? ~0ull : 0xFFFFFFFFull)) return false;
             const lds_char* const tile = lds + (t & (L::kStages - 1)) * L::kStage;
+            // scales of this lane's positions, each kind read at once (as the compiler orders them each is waited for)
+            f32x4 scale[E8 ? 4 * KB : 1];
+            auto read_scales = [&](int kind) {
+#pragma unroll
+                for (int i = 0; i < 4 * KB; ++i)
+                    scale[i] = __builtin_bit_cast(f32x4, lds16(tile, L::kScales + (kind * KT + 8 * i + 4 * half) * 4));
+                __builtin_amdgcn_sched_barrier(0);
+            };
             if constexpr (E8) {
+                read_scales(0);
 #pragma unroll
-                for (int b = 0; b < KB; ++b)
-#pragma unroll
-                    for (int j = 0; j < 16; j += 4) {
-                        const f32x4 by = a.scale *
-                            __builtin_bit_cast(f32x4, lds16(tile, L::kScales + (32 * b + 2 * j + 4 * half) * 4));
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) s[b][j + i] *= by[i];
-                    }
+                for (int j = 0; j < 16 * KB; ++j) s[j >> 4][j & 15] *= scale[j >> 2][j & 3];
+                __builtin_amdgcn_sched_barrier(0);
+                read_scales(1);
             }
             const bool full = t0 + KT <= wave_least && gone == 0;
             // A row that sees a position has a maximum of at least the lowest number, one that sees none keeps
@@ -721,7 +725,7 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
                         if constexpr (!kDotSum) sum[i] += v[i];
                     }
                     if constexpr (E8)
-                        v = v * __builtin_bit_cast(f32x4, lds16(tile, L::kScales + KT * 4 + (32 * b + 2 * j + 4 * half) * 4));
+                        v = v * scale[4 * b + j / 4];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const uint32_t two = pack2<VBF16>(v[2 * i], v[2 * i + 1]);
@@ -753,17 +757,21 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
         for (int t = 0; t < 5; ++t) load_entries(t);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         for (int t = 0; t < 3; ++t) {
+            own_page = entry(t, own);
+            find_own(t);
             if constexpr (E8) {
-                load8(t);
+                load8();
                 store8(t);
             } else {
-                own_page = entry(t, own);
-                find_own(t);
 #pragma unroll
                 for (int i = 0; i < L::kBlocks; ++i) load_block(t, i);
             }
         }
-        if constexpr (E8) load8(3);
+        if constexpr (E8) {
+            own_page = entry(3, own);
+            find_own(3);
+            load8();
+        }
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (second) asm volatile("s_barrier" ::: "memory");
         scores(-1, std::false_type{});
@@ -1126,7 +1134,7 @@ PLM_EXPORT int kv_paged_attention_chunk_e4m3(const uint16_t* q, const uint8_t* k
                             sequences, table_cols, num_pages, page_size, kv_heads, head_dim, page_stride, slot_stride,
                             head_stride, dtype_code);
     if (code != 0) return code;
-    code = scales_of(a.s, const_cast<float*>(k_scales), const_cast<float*>(v_scales), scale_page_stride,
+    code = scales_of(a.s, a.p, kv_heads, const_cast<float*>(k_scales), const_cast<float*>(v_scales), scale_page_stride,
                      scale_head_stride);
     if (code != 0) return code;
     return run_chunk<true>(a, q, out, row_starts, scratch, scratch_bytes, rows, sequences, heads, kv_heads, head_dim,

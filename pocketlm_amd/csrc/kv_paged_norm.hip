@@ -246,7 +246,7 @@ __global__ __launch_bounds__(kThreads) void norm_append_kernel(const NormArgs a)
 #pragma unroll
         for (int i = 0; i < N; ++i)
             *reinterpret_cast<u32x2*>(out + at[i]) = finite ? pack8_e4m3(y[i], s, inv) : u32x2{0x7F7F7F7Fu, 0x7F7F7F7Fu};
-        if (c == 0) (is_k ? a.s.k : a.s.v)[to.page * a.s.page_stride + kvh * a.s.head_stride + to.slot] = s;
+        if (c == 0) (is_k ? a.s.k : a.s.v)[a.s.at(static_cast<int>(to.page), kvh, to.slot)] = s;
     } else {
         uint16_t* out = (is_k ? a.p.k : a.p.v) + piece * 8 + kvh * a.p.head_stride;
 #pragma unroll
@@ -357,7 +357,7 @@ PLM_EXPORT int kv_paged_append_e4m3(const uint16_t* q, const uint16_t* k, const 
     int code = pages_of<16>(a.p, k_cache, v_cache, page_table, lengths, sequences, table_cols, num_pages, page_size,
                             kv_heads, head_dim, page_stride, slot_stride, head_stride, dtype_code);
     if (code != 0) return code;
-    code = scales_of(a.s, k_scales, v_scales, scale_page_stride, scale_head_stride);
+    code = scales_of(a.s, a.p, kv_heads, k_scales, v_scales, scale_page_stride, scale_head_stride);
     if (code != 0) return code;
     a.q = q, a.k = k, a.v = v;
     a.q_weight = heads > 0 ? q_norm_weight : nullptr;
