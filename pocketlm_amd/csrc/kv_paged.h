@@ -159,6 +159,20 @@ __device__ __forceinline__ uint32_t wave_prefix(uint32_t v) {
     return v;
 }
 
+// The maximum over the lanes of a wave.
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+#define PLM_MAX(ctrl, rows) \
+    v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), ctrl, rows, 0xF, false)))
+    PLM_MAX(0x111, 0xF);
+    PLM_MAX(0x112, 0xF);
+    PLM_MAX(0x114, 0xF);
+    PLM_MAX(0x118, 0xF);
+    PLM_MAX(0x142, 0xA);
+    PLM_MAX(0x143, 0xC);
+#undef PLM_MAX
+    return __builtin_amdgcn_readlane(v, 63);
+}
+
 __device__ __forceinline__ float swap_max(float v) {
     // over the four lanes l, l ^ 16, l ^ 32, l ^ 48
     const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);

@@ -234,20 +234,6 @@ struct Plan {
     }
 };
 
-// Of the lanes of a wave (lane 63 has it).
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-#define PLM_MAX(ctrl, rows) \
-    v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), ctrl, rows, 0xF, false)))
-    PLM_MAX(0x111, 0xF);
-    PLM_MAX(0x112, 0xF);
-    PLM_MAX(0x114, 0xF);
-    PLM_MAX(0x118, 0xF);
-    PLM_MAX(0x142, 0xA);
-    PLM_MAX(0x143, 0xC);
-#undef PLM_MAX
-    return __builtin_amdgcn_readlane(v, 63);
-}
-
 // The plan, at the sequence that holds the first unit of run `run`.  Every
 // thread of a workgroup calls it; false for a run past the last.  (Kept short:
 // a small call waits for its instructions as for its data.)

@@ -29,6 +29,16 @@ constexpr float kLate = 8.0f;
 // fp16 weights are kept times 2^7, so that with kLate they end at 2^15 and begin at 2^-31.
 __host__ __device__ constexpr float bias_of(bool bf16) { return bf16 ? 0.0f : 7.0f; }
 
+// n / d of n < 2^31 without a division: n * times >> 31 + shift, where times is
+// 2^(31 + shift) / d rounded up and 2^shift >= d, so that its error, less than d,
+// times n stays below 2^(31 + shift).
+struct Divider {
+    uint32_t times;
+    uint32_t shift;
+
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return __umulhi(2 * n, times) >> shift; }
+};
+
 struct ChunkArgs {
     Pages p;
     Scales s;              // of e4m3 caches
@@ -45,11 +55,12 @@ struct ChunkArgs {
     int kv_heads;
     int group;
     int head_dim;
-    int columns;           // of a tile
-    int pieces;            // tiles of a head, or runs, at most
+    int columns_log2;      // of a tile
+    int pieces;            // tiles of a head, and runs, at most
+    int runs;              // at most
     uint32_t work_shift;   // so that a head's work stays in 32 bits
-    uint32_t divide;       // position / page_size: position * divide >> 31 + shift
-    uint32_t shift;
+    Divider by_page;       // positions by page_size
+    Divider by_group;      // columns by group
     uint32_t flip;         // sign bits of the queries, where the softmax scale is negative
     float scale;           // |softmax scale| * log2(e)
 };
@@ -69,9 +80,11 @@ __device__ __forceinline__ int rows_of(const ChunkArgs& a, int place) {
     return max(start_of(a, place + 1) - start_of(a, place), 0);
 }
 
-// Tiles of `count` positions or columns.
-__device__ __forceinline__ uint32_t tiles_of(int64_t count, int tile) {
-    return static_cast<uint32_t>((count + tile - 1) / tile);
+// Tiles of `count` positions, and of the columns of `rows` rows (rows * heads is below 2^31).
+__device__ __forceinline__ uint32_t position_tiles(int count) { return (static_cast<uint32_t>(count) + kTile - 1) / kTile; }
+__device__ __forceinline__ int column_tiles(const ChunkArgs& a, int rows) {
+    const uint32_t columns = static_cast<uint32_t>(rows) * static_cast<uint32_t>(a.group);
+    return static_cast<int>((columns + (1u << a.columns_log2) - 1) >> a.columns_log2);
 }
 // Positions that row `row` of a sequence sees.
 __device__ __forceinline__ int seen_by(const ChunkArgs& a, int length, int row) {
@@ -103,10 +116,10 @@ __device__ __forceinline__ Piece piece_of(const ChunkArgs& a, int place, int til
     p.rows = uniform(rows_of(a, place));
     p.length = uniform(length_of(a, place));
     const int columns = p.rows * a.group;
-    p.tiles = static_cast<int>(tiles_of(columns, a.columns));
+    p.tiles = column_tiles(a, p.rows);
     p.tile = tile;
-    p.seen = uniform(seen_by(a, p.length, (min((tile + 1) * a.columns, columns) - 1) / a.group));
-    p.least = uniform(seen_by(a, p.length, tile * a.columns / a.group));
+    p.seen = uniform(seen_by(a, p.length, a.by_group(max(min((tile + 1) << a.columns_log2, columns), 1) - 1)));
+    p.least = uniform(seen_by(a, p.length, a.by_group(min(tile << a.columns_log2, columns))));
     p.begin = 0;
     p.end = p.seen;
     p.whole = true;
@@ -114,10 +127,10 @@ __device__ __forceinline__ Piece piece_of(const ChunkArgs& a, int place, int til
     return p;
 }
 
-// Place i's tiles begin at floor(start * group / a.columns) + i, which leaves
-// room for each place's last, partly filled one.
+// Place i's tiles begin at floor(start * group / columns of a tile) + i, which
+// leaves room for each place's last, partly filled one.
 __device__ __forceinline__ int first_tile_of(const ChunkArgs& a, int place) {
-    return static_cast<int>(static_cast<int64_t>(start_of(a, place)) * a.group / a.columns) + place;
+    return static_cast<int>(static_cast<uint32_t>(start_of(a, place) * a.group) >> a.columns_log2) + place;
 }
 // The place of tile `at`, by a search 64 wide; every lane calls it.
 __device__ __forceinline__ int place_of_tile(const ChunkArgs& a, int at, int lane, int& first) {
@@ -141,18 +154,27 @@ __device__ __forceinline__ int place_of_tile(const ChunkArgs& a, int at, int lan
 // holds whole; of the others it leaves two partials at most: of the tile that
 // it goes on with (slot 2 run) and of the one that it begins and does not end
 // (slot 2 run + 1).
+//
+// Unless whole tiles take no longer.  They take as many position tiles as the
+// longest of them has, or where there are more than the device holds their share
+// of the work and half of the longest; runs take their share, kStart for each tile
+// that they hold a part of, kJoin, and kJoinRuns where every workgroup leaves
+// partials of full tiles (67 MB at a head of 128).  28 and 4 heads of 128, whole / in runs: a prompt
+// of 500 rows 25 / 41 us, of 1500 62 / 67, 16 of up to 200 rows 33 / 56; 37 rows
+// behind 700 positions 34 / 27, 64 times 2 rows behind up to 4000 128 / 110.
 constexpr uint32_t kTileWork = 2;
 constexpr uint32_t kLeastWork = 4;  // of a run
+constexpr float kStart = 3.0f, kJoin = 3.0f, kJoinRuns = 11.0f;
 
 struct Work {
     int tiles;
     uint32_t first, last;  // position tiles of its first and last tile
 
-    // Work of the tiles before `tile`, times 2 max(tiles - 1, 1).
-    __device__ __forceinline__ double before(int tile) const {
-        const double t = tile, n = max(tiles - 1, 1);
-        return 2.0 * n * static_cast<double>(first + kTileWork) * t +
-               (static_cast<double>(last) - static_cast<double>(first)) * t * (t - 1.0);
+    // Work of the tiles before `tile`, times 2 max(tiles - 1, 1); about, which every run takes alike.
+    __device__ __forceinline__ float before(int tile) const {
+        const float t = tile, n = max(tiles - 1, 1);
+        return t * (2.0f * n * static_cast<float>(first + kTileWork) +
+                    (static_cast<float>(last) - static_cast<float>(first)) * (t - 1.0f));
     }
     __device__ __forceinline__ uint32_t total(uint32_t shift) const {
         const uint64_t twice = static_cast<uint64_t>(tiles) * (static_cast<uint64_t>(first) + last + 2 * kTileWork);
@@ -165,9 +187,9 @@ __device__ __forceinline__ Work work_of(const ChunkArgs& a, int place) {
     if (place >= a.p.sequences + 2) return w;
     const int rows = rows_of(a, place);
     const int length = length_of(a, place);
-    w.tiles = static_cast<int>(tiles_of(static_cast<int64_t>(rows) * a.group, a.columns));
-    w.first = tiles_of(seen_by(a, length, min(a.columns / a.group, rows) - 1), kTile);
-    w.last = tiles_of(seen_by(a, length, rows - 1), kTile);
+    w.tiles = column_tiles(a, rows);
+    w.first = position_tiles(seen_by(a, length, min(static_cast<int>(a.by_group(1u << a.columns_log2)), rows) - 1));
+    w.last = position_tiles(seen_by(a, length, rows - 1));
     return w;
 }
 
@@ -178,30 +200,50 @@ struct Border {
     float share;
 };
 
-// The borders of run `run`; false: there is no such run.  Every lane calls it.
-__device__ __forceinline__ bool find_run(const ChunkArgs& a, int run, int lane, Border& from, Border& to) {
+// What workgroup `run` of a head does: kRun and its borders, kTiles (tile `run`, whole) or kNone.  Every lane calls
+// it.
+// (Kept short, as all that a call does once: a small call waits for its
+// instructions.)
+enum Dealt { kNone, kTiles, kRun };
+__device__ __forceinline__ Dealt find_run(const ChunkArgs& a, int run, int lane, Border (&border)[2]) {
     const int places = a.p.sequences + 2;
-    const Work mine = work_of(a, lane);
-    uint32_t all = 0;
-    for (int base = 0; base < places; base += 64)
-        all += (base == 0 ? mine : work_of(a, base + lane)).total(a.work_shift);
-    all = __builtin_amdgcn_readlane(wave_prefix(all), 63);
-    const uint32_t runs = min(static_cast<uint32_t>(a.pieces), max(1u, all / kLeastWork));
-    if (static_cast<uint32_t>(run) >= runs) return false;
-    const uint32_t each = all / runs, rest = all - each * runs;
-    const uint32_t u = static_cast<uint32_t>(run);
-    const uint32_t begin = u * each + static_cast<uint32_t>(static_cast<uint64_t>(u) * rest / runs);
-    const uint32_t end = (u + 1) * each + static_cast<uint32_t>(static_cast<uint64_t>(u + 1) * rest / runs);
-    from.place = to.place = places;
-    from.tile = to.tile = 0;
-    from.share = to.share = 0.0f;
-    uint32_t before = 0;
+    uint32_t all = 0, longest = 0, tiles = 0;
+#pragma unroll 1
     for (int base = 0; base < places; base += 64) {
-        const Work w = base == 0 ? mine : work_of(a, base + lane);
+        const Work w = work_of(a, base + lane);
+        all += w.total(a.work_shift);
+        longest = max(longest, w.last);
+        tiles += w.tiles;
+    }
+    all = __builtin_amdgcn_readlane(wave_prefix(all), 63);
+    longest = wave_max(longest);
+    tiles = __builtin_amdgcn_readlane(wave_prefix(tiles), 63);
+    const uint32_t runs = min(static_cast<uint32_t>(a.runs), max(1u, all / kLeastWork));
+    // (what is only about right is the same for both runs of a border)
+    const float each = __builtin_amdgcn_rcpf(static_cast<float>(runs)), per_run = static_cast<float>(all) * each;
+    const float filled = static_cast<float>(a.rows) * static_cast<float>(a.group) *
+                         __builtin_amdgcn_rcpf(static_cast<float>(tiles << a.columns_log2));
+    const float share = __builtin_amdgcn_rcpf(static_cast<float>(a.runs)), scale = static_cast<float>(1u << a.work_shift);
+    const float in_runs = per_run * scale + kStart * static_cast<float>(tiles) * each + kJoin +
+                          kJoinRuns * static_cast<float>(runs) * share * filled;
+    float whole = static_cast<float>(longest);
+    if (tiles > static_cast<uint32_t>(a.runs)) whole = fmaxf(whole, static_cast<float>(all) * share * scale + whole * 0.5f);
+    if (whole <= in_runs) return kTiles;
+    if (static_cast<uint32_t>(run) >= runs) return kNone;
+    auto border_at = [&](uint32_t r) { return r == runs ? all : static_cast<uint32_t>(static_cast<float>(r) * per_run); };
+    border[0].place = border[1].place = places;
+    border[0].tile = border[1].tile = 0;
+    border[0].share = border[1].share = 0.0f;
+    uint32_t before = 0;
+#pragma unroll 1
+    for (int base = 0; base < places && border[1].place == places; base += 64) {
+        const Work w = work_of(a, base + lane);
         const uint32_t total = w.total(a.work_shift), upto = before + wave_prefix(total);
-        auto place = [&](uint32_t x, Border& b) {
+#pragma unroll 1
+        for (int k = 0; k < 2; ++k) {
+            const uint32_t x = border_at(static_cast<uint32_t>(run + k));
             const unsigned long long past = __ballot(upto > x);
-            if (past == 0 || b.place < places) return;
+            if (past == 0 || (k == 0 && border[0].place < places)) continue;
             const int l = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
             Work of;
             of.tiles = __builtin_amdgcn_readlane(w.tiles, l);
@@ -209,22 +251,23 @@ __device__ __forceinline__ bool find_run(const ChunkArgs& a, int run, int lane, 
             of.last = __builtin_amdgcn_readlane(w.last, l);
             const uint32_t size = __builtin_amdgcn_readlane(total, l);
             const uint32_t in = x - (__builtin_amdgcn_readlane(upto, l) - size);
-            const double z = static_cast<double>(in) / static_cast<double>(size) * of.before(of.tiles);
+            const float z = static_cast<float>(in) * __builtin_amdgcn_rcpf(static_cast<float>(size)) * of.before(of.tiles);
             int lo = 0, hi = of.tiles;
+#pragma unroll 1
             while (hi - lo > 1) {
                 const int mid = (lo + hi) / 2;
                 (of.before(mid) <= z ? lo : hi) = mid;
             }
-            b.place = base + l;
-            b.tile = __builtin_amdgcn_readfirstlane(lo);
-            b.share = in == 0 ? 0.0f
-                              : static_cast<float>((z - of.before(lo)) / (of.before(lo + 1) - of.before(lo)));
-        };
-        place(begin, from);
-        place(end, to);
+            lo = __builtin_amdgcn_readfirstlane(lo);
+            const float from = of.before(lo);
+            const float share = in == 0 ? 0.0f : (z - from) * __builtin_amdgcn_rcpf(of.before(lo + 1) - from);
+            const Border found = {base + l, lo, share};
+            if (k == 0) border[0] = found;
+            if (k == 1) border[1] = found;
+        }
         before = __builtin_amdgcn_readlane(upto, 63);
     }
-    return true;
+    return kRun;
 }
 
 // Workgroup -> (tile or run, head).  They are dealt to the 8 XCDs in turn: a
@@ -289,7 +332,7 @@ __device__ __forceinline__ void load4_to_lds(const void* from, uint32_t to) {
 // not fast.
 template <bool BF16, bool E8>
 __device__ void careful_column(const ChunkArgs& a, const Piece& piece, int kvh, int col, int lane) {
-    const int r = col / a.group, h = col - r * a.group;
+    const int r = a.by_group(col), h = col - r * a.group;
     const uint16_t* q = a.q + (piece.first + r) * a.q_row + (kvh * a.group + h) * a.q_head;
     const int* table = a.p.table + static_cast<int64_t>(piece.place - 1) * a.p.table_cols;
     const uint8_t* kbase = reinterpret_cast<const uint8_t*>(a.p.k) + (E8 ? 1 : 2) * kvh * a.p.head_stride;
@@ -308,7 +351,7 @@ __device__ void careful_column(const ChunkArgs& a, const Piece& piece, int kvh, 
         int page = -1;
         uint32_t slot = 0;
         if (pos < last) {
-            const uint32_t index = static_cast<uint32_t>(pos) / a.p.page_size;
+            const uint32_t index = a.by_page(pos);
             page = table[index];
             slot = static_cast<uint32_t>(pos) - index * a.p.page_size;
         }
@@ -354,7 +397,7 @@ __device__ void careful_column(const ChunkArgs& a, const Piece& piece, int kvh, 
         }
     }
     if (!piece.whole) {
-        const int64_t to = (static_cast<int64_t>(piece.slot) * a.kv_heads + kvh) * a.columns + (col - piece.tile * a.columns);
+        const int64_t to = (static_cast<int64_t>(piece.slot) * a.kv_heads + kvh) * (1 << a.columns_log2) + (col - (piece.tile << a.columns_log2));
         if (lane == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * to) = f32x2{m, l};
         for (int i = 0; i < 4; ++i)
             if (lane + 64 * i < a.head_dim) a.part[to * a.head_dim + lane + 64 * i] = acc[i];
@@ -445,9 +488,9 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
     const int columns = piece.rows * a.group;
     const int wave0 = piece.tile * L::kColumns + 32 * wave;
     const int col = wave0 + li;
-    const int wave_least = uniform(seen_by(a, piece.length, min(wave0, columns - 1) / a.group));
+    const int wave_least = uniform(seen_by(a, piece.length, a.by_group(min(wave0, columns - 1))));
     const int wave_seen =
-        wave0 < columns ? uniform(seen_by(a, piece.length, (min(wave0 + 32, columns) - 1) / a.group)) : 0;
+        wave0 < columns ? uniform(seen_by(a, piece.length, a.by_group(min(wave0 + 32, columns) - 1))) : 0;
     const int begin = piece.begin, end = piece.end;
 
     float m = -INFINITY, l = 0.0f;  // weights are exp2(score - m): m is the maximum less the bias, up to kLate behind
@@ -462,7 +505,7 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
         u32x4 q[KS];
         int limit;
         {
-            const int r = min(col, columns - 1) / a.group, h = min(col, columns - 1) - r * a.group;
+            const int r = a.by_group(min(col, columns - 1)), h = min(col, columns - 1) - r * a.group;
             const uint16_t* src = a.q + (piece.first + r) * a.q_row + (kvh * a.group + h) * a.q_head;
             limit = col < columns ? seen_by(a, piece.length, r) : 0;
 #pragma unroll
@@ -489,9 +532,7 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
                 vat[b][z] = L::kV + row * 128 + (chunk ^ swizzle(row)) * 16 + (i16 & 1) * 8;
             }
 
-        auto index_of = [&](uint32_t pos) {
-            return __umulhi(2 * pos, a.divide) >> a.shift;
-        };
+        auto index_of = [&](uint32_t pos) { return a.by_page(pos); };
         // position r of tile t; past the piece's end its last one
         auto position = [&](int t, int r) { return static_cast<uint32_t>(min(begin + KT * t + r, end - 1)); };
         auto slot_of = [&](uint32_t pos) { return pos - index_of(pos) * a.p.page_size; };
@@ -754,8 +795,10 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
         };
 
         const int tiles = (end - begin + KT - 1) / KT;
+#pragma unroll 1
         for (int t = 0; t < 5; ++t) load_entries(t);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll 1
         for (int t = 0; t < 3; ++t) {
             own_page = entry(t, own);
             find_own(t);
@@ -790,49 +833,44 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
     }
     l = both_sum(l);
 
-    bool odd = false;
+    if (masked) {
+        float odd = 0.0f;  // 0 times what is not finite is NaN
 #pragma unroll
-    for (int b = 0; b < DB; ++b)
+        for (int b = 0; b < DB; ++b)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) odd |= !(fabsf(acc[b][j]) < INFINITY);
-    if (__any(masked && odd)) {
-        const int most = min(wave0 + 32, columns);
-        for (int c = wave0; c < most; ++c) careful_column<BF16, E8>(a, piece, kvh, c, lane);
-        return;
+            for (int j = 0; j < 16; ++j) odd = fmaf(acc[b][j], 0.0f, odd);
+        if (__any(odd != odd)) {
+            const int most = min(wave0 + 32, columns);
+            for (int c = wave0; c < most; ++c) careful_column<BF16, E8>(a, piece, kvh, c, lane);
+            return;
+        }
     }
     if (col >= columns) return;
     if (!piece.whole) {
         const int64_t to =
             (static_cast<int64_t>(piece.slot) * a.kv_heads + kvh) * L::kColumns + (col - piece.tile * L::kColumns);
         if (half == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * to) = f32x2{m, l};
+        float* const at = a.part + to * a.head_dim + 4 * half;
 #pragma unroll
         for (int b = 0; b < DB; ++b)
 #pragma unroll
-            for (int j = 0; j < 16; j += 4) {
-                const int d = 32 * b + 2 * j + 4 * half;
-                if (d < a.head_dim)
-                    *reinterpret_cast<f32x4*>(a.part + to * a.head_dim + d) =
+            for (int j = 0; j < 16; j += 4)
+                if (32 * b + 2 * j < a.head_dim)
+                    *reinterpret_cast<f32x4*>(at + 32 * b + 2 * j) =
                         f32x4{acc[b][j], acc[b][j + 1], acc[b][j + 2], acc[b][j + 3]};
-            }
         return;
     }
     // a row that sees nothing is zero
-    const int r = col / a.group, h = col - r * a.group;
-    const bool empty = m == -INFINITY;
-    const float inv = 1.0f / l;
-    uint16_t* to = a.out + (static_cast<int64_t>(piece.first + r) * a.heads + kvh * a.group + h) * a.head_dim;
+    const int r = a.by_group(col), h = col - r * a.group;
+    const float inv = m == -INFINITY ? 0.0f : __builtin_amdgcn_rcpf(l);  // (the accumulators are 0 there too)
+    uint16_t* const to = a.out + (static_cast<int64_t>(piece.first + r) * a.heads + kvh * a.group + h) * a.head_dim + 4 * half;
 #pragma unroll
     for (int b = 0; b < DB; ++b)
 #pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-            const int d = 32 * b + 2 * j + 4 * half;
-            u32x2 o;
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-                o[x] = pack2<BF16>(empty ? 0.0f : acc[b][j + 2 * x] * inv,
-                                   empty ? 0.0f : acc[b][j + 2 * x + 1] * inv);
-            if (d < a.head_dim) *reinterpret_cast<u32x2*>(to + d) = o;
-        }
+        for (int j = 0; j < 16; j += 4)
+            if (32 * b + 2 * j < a.head_dim)
+                *reinterpret_cast<u32x2*>(to + 32 * b + 2 * j) =
+                    u32x2{pack2<BF16>(acc[b][j] * inv, acc[b][j + 1] * inv), pack2<BF16>(acc[b][j + 2] * inv, acc[b][j + 3] * inv)};
 }
 
 // Workgroup -> (tile or run, key-value head).
@@ -848,17 +886,18 @@ __global__ __launch_bounds__(DP > 128 ? 256 : 512, 1) void paged_chunk_kernel(co
     if (a.head_dim != DP)  // the loads leave out what is behind a head's end
         for (int i = threadIdx.x; i < L::kStages * L::kStage / 16; i += 64 * L::kWaves)
             *(__attribute__((address_space(3))) u32x4*)(lds + 16 * i) = u32x4{0, 0, 0, 0};
-    Border next, last;
-    if (a.plan == nullptr) {
+    Border border[2];  // of the run: where it goes on, where it ends
+    const Dealt dealt = a.plan == nullptr ? kTiles : find_run(a, at, lane, border);
+    if (dealt == kNone) return;
+    if (dealt == kTiles) {
         int first;
         const int place = place_of_tile(a, at, lane, first);
-        const int tiles = static_cast<int>(tiles_of(rows_of(a, place) * static_cast<int64_t>(a.group), L::kColumns));
-        if (at - first >= tiles) return;
-        next = Border{place, tiles - 1 - (at - first), 0.0f};  // the longest first
-        last = Border{place, next.tile + 1, 0.0f};
-    } else if (!find_run(a, at, lane, next, last)) {
-        return;
+        const int longest_first = column_tiles(a, rows_of(a, place)) - 1 - (at - first);
+        if (longest_first < 0) return;
+        border[0] = Border{place, longest_first, 0.0f};
+        border[1] = Border{place, longest_first + 1, 0.0f};
     }
+    const Border &next = border[0], &last = border[1];
     int place = next.place, tile = next.tile;
     while (place < last.place || (place == last.place && tile <= last.tile)) {
         Piece piece = piece_of(a, place, tile);
@@ -867,7 +906,7 @@ __global__ __launch_bounds__(DP > 128 ? 256 : 512, 1) void paged_chunk_kernel(co
             tile = 0;
             continue;
         }
-        const int units = static_cast<int>(tiles_of(piece.seen, kTile));
+        const int units = static_cast<int>(position_tiles(piece.seen));
         auto unit_at = [&](float share) {
             return __builtin_amdgcn_readfirstlane(min(units, static_cast<int>(share * static_cast<float>(units))));
         };
@@ -894,79 +933,74 @@ __global__ __launch_bounds__(DP > 128 ? 256 : 512, 1) void paged_chunk_kernel(co
     }
 }
 
-// Joins the partials of the tiles that several runs hold: a workgroup for 16
-// columns of a tile, 16 threads a column, which first weigh the partials (every
-// sixteenth each), then take every sixteenth quad of head values.
+// Joins the partials of the tiles that several runs hold.  GROUPS of 16 lanes for a
+// column: a lane takes four head values of every GROUPS-th partial.  One group
+// where partials are few, a wave's four where they are many (64 partials of 112
+// columns of 4 heads: 50 us with one, 16 with four; 4 partials of 10500 columns 13
+// and 28).
 constexpr int kJoinThreads = 256;
-constexpr int kJoinColumns = 16;
-constexpr int kJoinPartials = 64;  // at a time
+constexpr int kJoinColumns = 4;  // of a workgroup, one a wave; 16 where partials are few
+constexpr int kFewPartials = 8;
 
-template <bool BF16>
-__global__ __launch_bounds__(kJoinThreads) void paged_chunk_join_kernel(const ChunkArgs a) {
-    __shared__ float weights[kJoinColumns][kJoinPartials + 1];
-    const int lane = threadIdx.x & 63;
-    int begin;
-    const int place = place_of_tile(a, blockIdx.x, lane, begin);
-    const int first = start_of(a, place);
-    const int columns = rows_of(a, place) * a.group;
-    const int tile = blockIdx.x - begin;
-    if (tile >= static_cast<int>(tiles_of(columns, a.columns))) return;
-    // (within the runs also where the lengths were changed under the first kernel)
-    const int run = min(max(a.plan[2 * blockIdx.x], 0), a.pieces - 1);
-    const int parts = min(a.plan[2 * blockIdx.x + 1], a.pieces - 1) - run + 1;
-    if (parts <= 1) return;
-    const int c = threadIdx.x >> 4, j = threadIdx.x & 15;
-    const int in = blockIdx.z * kJoinColumns + c, col = tile * a.columns + in;
-    const int kvh = blockIdx.y;
+template <bool BF16, int GROUPS>
+__device__ __forceinline__ void join_column(const ChunkArgs& a, int run, int parts, int kvh, int first, int in, int col,
+                                            int lane) {
+    constexpr int LANES = 16 * GROUPS;
+    const int part_lane = lane & (LANES - 1), g = part_lane >> 4, j = lane & 15;
     // partial i: the first is its run's second
     auto slot = [](int i) { return max(2 * i, 1); };
-    const int64_t stride = static_cast<int64_t>(a.kv_heads) * a.columns;
-    const int64_t from = (static_cast<int64_t>(2 * run) * a.kv_heads + kvh) * a.columns + in;
+    const int64_t stride = static_cast<int64_t>(a.kv_heads) << a.columns_log2;
+    const int64_t from = ((static_cast<int64_t>(2 * run) * a.kv_heads + kvh) << a.columns_log2) + in;
     const f32x2* ml = reinterpret_cast<const f32x2*>(a.part_ml) + from;
-    auto over16 = [](float v, auto op) {
-#pragma unroll
-        for (int off = 1; off < 16; off <<= 1) v = op(v, __shfl_xor(v, off));
-        return v;
-    };
     float m = -INFINITY;
-    for (int i = j; i < parts; i += 16) m = fmaxf(m, ml[slot(i) * stride][0]);
-    m = over16(m, [](float u, float v) { return fmaxf(u, v); });
+    for (int i = part_lane; i < parts; i += LANES) m = fmaxf(m, ml[slot(i) * stride][0]);
+#pragma unroll
+    for (int off = 1; off < LANES; off <<= 1) m = fmaxf(m, __shfl_xor(m, off));
     const float* part = a.part + from * a.head_dim + 4 * j;
     float sum = 0.0f;
     f32x4 acc[4];
 #pragma unroll
     for (int x = 0; x < 4; ++x) acc[x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int base = 0; base < parts; base += kJoinPartials) {
-        const int n = min(kJoinPartials, parts - base);
-        __syncthreads();
-        for (int i = j; i < n; i += 16) {
-            const f32x2 v = ml[slot(base + i) * stride];
-            const float w = exp2_from(v[0], m);
-            weights[c][i] = w;
-            sum = fmaf(v[1], w, sum);
+    for (int base = 0; base < parts; base += LANES) {
+        const int n = min(LANES, parts - base);
+        float weight = 0.0f;
+        if (part_lane < n) {
+            const f32x2 v = ml[slot(base + part_lane) * stride];
+            weight = exp2_from(v[0], m);
+            sum = fmaf(v[1], weight, sum);
         }
-        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            if (64 * x >= a.head_dim) break;
+            const bool in_head = 4 * j + 64 * x < a.head_dim;
+#pragma unroll 4
+            for (int i = g; i < n + g; i += GROUPS) {  // as often in every lane
+                const float w = __shfl(weight, (lane & ~(LANES - 1)) + min(i, n - 1));
+                const f32x4 v = *reinterpret_cast<const f32x4*>(part + slot(base + min(i, n - 1)) * stride * a.head_dim +
+                                                                (in_head ? 64 * x : -4 * j));
+#pragma unroll
+                for (int y = 0; y < 4; ++y) acc[x][y] = i < n ? fmaf(v[y], w, acc[x][y]) : acc[x][y];
+            }
+        }
+    }
+#pragma unroll
+    for (int off = 1; off < LANES; off <<= 1) sum += __shfl_xor(sum, off);
+    if constexpr (GROUPS == 4) {
 #pragma unroll
         for (int x = 0; x < 4; ++x)
-            if (4 * j + 64 * x < a.head_dim) {
-#pragma unroll 4
-                for (int i = 0; i < n; ++i) {
-                    const f32x4 v = *reinterpret_cast<const f32x4*>(part + slot(base + i) * stride * a.head_dim + 64 * x);
-                    const float w = weights[c][i];
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) acc[x][y] = fmaf(v[y], w, acc[x][y]);
-                }
+            for (int y = 0; y < 4; ++y) {
+                acc[x][y] += __shfl_xor(acc[x][y], 16);
+                acc[x][y] += __shfl_xor(acc[x][y], 32);
             }
     }
-    sum = over16(sum, [](float u, float v) { return u + v; });
-    if (col >= columns) return;
     const bool empty = m == -INFINITY;
     const float inv = 1.0f / sum;
-    const int r = col / a.group, h = col - r * a.group;
+    const int r = a.by_group(col), h = col - r * a.group;
     uint16_t* to = a.out + (static_cast<int64_t>(first + r) * a.heads + kvh * a.group + h) * a.head_dim + 4 * j;
 #pragma unroll
     for (int x = 0; x < 4; ++x)
-        if (4 * j + 64 * x < a.head_dim) {
+        if (g == 0 && 4 * j + 64 * x < a.head_dim) {
             u32x2 o;
 #pragma unroll
             for (int y = 0; y < 2; ++y)
@@ -975,12 +1009,36 @@ __global__ __launch_bounds__(kJoinThreads) void paged_chunk_join_kernel(const Ch
         }
 }
 
+template <bool BF16>
+__global__ __launch_bounds__(kJoinThreads) void paged_chunk_join_kernel(const ChunkArgs a) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // (within the runs also where the lengths were changed under the first kernel)
+    const int run = max(a.plan[2 * blockIdx.x], 0);
+    const int parts = min(a.plan[2 * blockIdx.x + 1], a.runs - 1) - run + 1;
+    if (parts <= 1) return;
+    int begin;
+    const int place = place_of_tile(a, blockIdx.x, lane, begin);
+    const int first = start_of(a, place), rows = rows_of(a, place);
+    const int tile = blockIdx.x - begin;
+    if (tile >= column_tiles(a, rows)) return;
+    const int col0 = tile << a.columns_log2, columns = rows * a.group;
+    if (parts > kFewPartials) {
+        const int in = blockIdx.z * kJoinColumns + wave;
+        if (col0 + in < columns) join_column<BF16, 4>(a, run, parts, blockIdx.y, first, in, col0 + in, lane);
+    } else if (blockIdx.z % 4 == 0) {
+        // a lane without a column joins the last one again
+        const int in = min(blockIdx.z * kJoinColumns + 4 * wave + (lane >> 4), columns - 1 - col0);
+        if (blockIdx.z * kJoinColumns < columns - col0)
+            join_column<BF16, 1>(a, run, parts, blockIdx.y, first, in, col0 + in, lane);
+    }
+}
+
 // ---------------------------------------------------------------- host side
 
 struct ChunkShape {
     int64_t columns;   // of a tile
     int64_t tiles;     // of a head, at most
-    int64_t pieces;    // of a head, at most: tiles or runs
+    int64_t runs;      // of a head, at most
     bool split;
     uint32_t work_shift;
     size_t bytes;
@@ -996,17 +1054,26 @@ ChunkShape shape_of(int64_t sequences, int64_t rows, int64_t heads, int64_t kv_h
     const int64_t resident = plm::cu_count();
     s.columns = head_dim > 128 ? Layout<256, false>::kColumns : Layout<128, false>::kColumns;
     s.tiles = rows * group / s.columns + sequences + 2;
-    s.split = sequences <= kMostSplitSequences && rows * heads / s.columns < kFewTiles * resident;
-    s.pieces = s.tiles;
+    s.split = sequences <= kMostSplitSequences && rows * heads / s.columns < kFewTiles * resident &&
+              capacity > kTile * (static_cast<int64_t>(kStart + kJoin) + 1);
+    s.runs = 0;
     s.work_shift = 0;
     s.bytes = 0;
     if (s.split) {
-        s.pieces = std::max<int64_t>(1, resident / kv_heads);
+        s.runs = std::max<int64_t>(1, resident / kv_heads);
         while (s.tiles * (plm::ceil_div(capacity, kTile) + kTileWork) >> s.work_shift > kMostInt / 2) ++s.work_shift;
-        s.bytes = static_cast<size_t>(2 * s.pieces) * kv_heads * s.columns * (head_dim + 2) * sizeof(float) +
+        s.bytes = static_cast<size_t>(2 * s.runs) * kv_heads * s.columns * (head_dim + 2) * sizeof(float) +
                   2 * sizeof(int) * s.tiles;
     }
     return s;
+}
+
+Divider divider_of(uint32_t d) {
+    Divider by = {0, 0};
+    while ((static_cast<uint64_t>(1) << by.shift) < d) ++by.shift;
+    const uint64_t whole = static_cast<uint64_t>(1) << (31 + by.shift);
+    by.times = static_cast<uint32_t>(whole / d + (whole % d != 0 ? 1 : 0));
+    return by;
 }
 
 template <bool BF16, bool E8, int DP>
@@ -1018,7 +1085,7 @@ int launch_kernel(const ChunkArgs& a, const ChunkShape& s, hipStream_t st) {
         if (code != 0) return code;
     }
     const int64_t g = 8 % a.kv_heads == 0 ? 8 / a.kv_heads : 1;
-    const int64_t blocks = plm::ceil_div(s.pieces, g) * g * a.kv_heads;
+    const int64_t blocks = plm::ceil_div(a.pieces, g) * g * a.kv_heads;
     hipLaunchKernelGGL((paged_chunk_kernel<BF16, E8, DP>), dim3(static_cast<unsigned>(blocks)), dim3(64 * L::kWaves),
                        bytes, st, a);
     if (s.split)
@@ -1051,7 +1118,7 @@ int run_chunk(ChunkArgs& a, const uint16_t* q, uint16_t* out, const int* row_sta
         return plm::fail(-2, "query strides and addresses must be multiples of 16 bytes");
     a.capacity = static_cast<int64_t>(a.p.table_cols) * a.p.page_size;
     const ChunkShape s = shape_of(sequences, rows, heads, kv_heads, head_dim, a.capacity);
-    if ((s.pieces + 8) * kv_heads > kMostInt) return plm::fail(-2, "too many rows, heads or sequences");
+    if ((std::max(s.tiles, s.runs) + 8) * kv_heads > kMostInt) return plm::fail(-2, "too many rows, heads or sequences");
     void* part = scratch;
     if (s.bytes > 0) {
         if (scratch == nullptr) {
@@ -1071,17 +1138,16 @@ int run_chunk(ChunkArgs& a, const uint16_t* q, uint16_t* out, const int* row_sta
     a.kv_heads = static_cast<int>(kv_heads);
     a.group = static_cast<int>(heads / kv_heads);
     a.head_dim = static_cast<int>(head_dim);
-    a.columns = static_cast<int>(s.columns);
-    a.pieces = static_cast<int>(s.pieces);
+    a.columns_log2 = 0;
+    while ((1 << a.columns_log2) < s.columns) ++a.columns_log2;
+    a.pieces = static_cast<int>(std::max(s.tiles, s.runs));
+    a.runs = static_cast<int>(s.runs);
     a.work_shift = s.work_shift;
     a.part = static_cast<float*>(part);
-    a.part_ml = a.part + 2 * s.pieces * kv_heads * s.columns * head_dim;
-    a.plan = s.split ? reinterpret_cast<int*>(a.part_ml + 2 * s.pieces * kv_heads * s.columns * 2) : nullptr;
-    // position / page_size of positions below 2^31: 2^(31 + shift) / page_size rounded up, 2^shift >= page_size
-    a.shift = 0;
-    while ((static_cast<uint64_t>(1) << a.shift) < a.p.page_size) ++a.shift;
-    a.divide = static_cast<uint32_t>((static_cast<uint64_t>(1) << (31 + a.shift)) / a.p.page_size +
-                                     ((static_cast<uint64_t>(1) << (31 + a.shift)) % a.p.page_size != 0 ? 1 : 0));
+    a.part_ml = a.part + 2 * s.runs * kv_heads * s.columns * head_dim;
+    a.plan = s.split ? reinterpret_cast<int*>(a.part_ml + 2 * s.runs * kv_heads * s.columns * 2) : nullptr;
+    a.by_page = divider_of(a.p.page_size);
+    a.by_group = divider_of(static_cast<uint32_t>(a.group));
     // a scale of 0 would make NaN of hidden scores
     a.scale = std::fabs(softmax_scale) * 1.44269504088896340736f;
     if (a.scale == 0.0f) a.scale = 1.4e-45f;
