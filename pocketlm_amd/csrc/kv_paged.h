@@ -110,6 +110,25 @@ struct Place {
     uint32_t slot;
     bool stored;   // there is a page for it
 };
+// (row `in_seq` of the call's rows of sequence `seq`)
+__device__ __forceinline__ Place place_in(const Pages& p, int seq, int64_t in_seq) {
+    const bool in_batch = seq >= 0 && seq < p.sequences;
+    const int length = in_batch ? p.lengths[seq] : -1;
+    Place at;
+    at.pos = length >= 0 ? length + in_seq : -1;
+    at.stored = false;
+    at.page = at.slot = 0;
+    if (at.pos >= 0) {
+        const int64_t index = at.pos / p.page_size;
+        if (index < p.table_cols) {
+            const int page = p.table[static_cast<int64_t>(seq) * p.table_cols + index];
+            at.stored = page >= 0 && static_cast<uint32_t>(page) < p.num_pages;
+            at.page = static_cast<uint32_t>(page);
+            at.slot = static_cast<uint32_t>(at.pos - index * p.page_size);
+        }
+    }
+    return at;
+}
 __device__ __forceinline__ Place place_of(const Pages& p, const int* row_starts, int rows_per_sequence, int64_t row,
                                           int lane) {
     int seq;
@@ -127,22 +146,32 @@ __device__ __forceinline__ Place place_of(const Pages& p, const int* row_starts,
         seq = static_cast<int>(row / rows_per_sequence);
         in_seq = row - static_cast<int64_t>(seq) * rows_per_sequence;
     }
-    const bool in_batch = seq >= 0 && seq < p.sequences;
-    const int length = in_batch ? p.lengths[seq] : -1;
-    Place at;
-    at.pos = length >= 0 ? length + in_seq : -1;
-    at.stored = false;
-    at.page = at.slot = 0;
-    if (at.pos >= 0) {
-        const int64_t index = at.pos / p.page_size;
-        if (index < p.table_cols) {
-            const int page = p.table[static_cast<int64_t>(seq) * p.table_cols + index];
-            at.stored = page >= 0 && static_cast<uint32_t>(page) < p.num_pages;
-            at.page = static_cast<uint32_t>(page);
-            at.slot = static_cast<uint32_t>(at.pos - index * p.page_size);
+    return place_in(p, seq, in_seq);
+}
+
+// The same of `count` rows from `row` on, lane r having row r's (the lanes behind them the last one's).
+__device__ __forceinline__ Place places_of(const Pages& p, const int* row_starts, int rows_per_sequence, int64_t row,
+                                           int count, int lane) {
+    int seq;
+    int64_t in_seq;
+    const int mine = min(lane, count - 1);
+    if (row_starts != nullptr) {
+        int starts = 0;
+        for (int base = 0; base <= p.sequences; base += 64) {
+            const int i = base + lane;
+            const int start = row_starts[min(i, p.sequences)];
+            for (int r = 0; r < count; ++r) {
+                const int before = __popcll(__ballot(i <= p.sequences && start <= row + r));
+                starts += mine == r ? before : 0;
+            }
         }
+        seq = starts - 1;
+        in_seq = seq >= 0 ? row + mine - row_starts[min(seq, p.sequences)] : 0;
+    } else {
+        seq = static_cast<int>((row + mine) / rows_per_sequence);
+        in_seq = row + mine - static_cast<int64_t>(seq) * rows_per_sequence;
     }
-    return at;
+    return place_in(p, seq, in_seq);
 }
 
 // Inclusive prefix sum over the lanes of a wave (DPP, no LDS).

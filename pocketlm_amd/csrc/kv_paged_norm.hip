@@ -9,6 +9,8 @@
 //
 // The scale's lower bound keeps 1 / scale finite; a head that holds an infinity
 // or a NaN gets the scale NaN and bytes 0x7F, as in fp8_rows.hip.
+#include <algorithm>
+
 #include "kv_paged.h"
 
 namespace {
@@ -17,7 +19,14 @@ using namespace plm_paged;
 
 constexpr float kE4m3Max = 448.0f;
 constexpr float kSmallestScale = 1.17549435e-38f;  // 2^-126
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
+constexpr int kMostRows = 8;  // of a workgroup
+
+// Workgroups of a compute unit before they take more rows than one: three or
+// four are resident (102 registers), and more rows than one pay once all have work
+// (5 x 1700 rows of 28 and 4 heads of 128: 30 us with 8 rows a workgroup, 34
+// with 4, 55 with 2, 58 with 1; 1 x 512 rows 6.0 us with 1).
+constexpr int kBlocks = 4;
 
 struct NormArgs {
     Pages p;
@@ -32,6 +41,8 @@ struct NormArgs {
     const int* row_starts;  // null: every sequence has rows_per_sequence rows
     const double* freq;     // [pairs]
     int* rejected;
+    int rows;
+    int block_rows;         // rows of a workgroup
     int rows_per_sequence;
     int heads;              // 0 without q
     int kv_heads;
@@ -85,17 +96,26 @@ __device__ __forceinline__ u32x2 pack8_e4m3(const f32x8 y, float scale, float in
     return o;
 }
 
-// Workgroup (row, part of the row's heads); a head has 2^lanes_log2 lanes of a
+// Workgroup (rows, part of a row's heads); a head has 2^lanes_log2 lanes of a
 // wave, `pieces` of which hold 16 values each (c and c + half a head, or
 // adjacent ones), or 8 in the modes for any size, so that a head's sum and
 // maximum are a few register permutes and every value is read once (kAny*: the
-// partner of a rotated pair is read again, from the first cache).
+// partner of a rotated pair is read again, from the first cache).  The places
+// and the angles of all of a workgroup's rows are found at once and the next
+// row's values are read while one is at work: a row by itself waits for row
+// starts, lengths and page table one after the other.
+//
+// Bound by memory where rows are many: 125 MB of 5 x 1700 rows (28 and 4 heads
+// of 128, fp16) in 30 us, 4.2 TB/s (e4m3 pages 119 MB in 35 us: the quotients
+// and the head's maximum come on top); one row takes 3.6 us, which is its chain of loads.
 template <bool BF16, int MODE, bool E8>
 __global__ __launch_bounds__(kThreads) void norm_append_kernel(const NormArgs a) {
-    __shared__ float cs[128], sn[128];
     constexpr bool ANY = MODE == kAny || MODE == kAnyAdjacent;
     constexpr int N = ANY ? 1 : 2;  // pieces of 8 values
-    const int64_t row = blockIdx.x;
+    constexpr int kPairs = 128;
+    __shared__ __attribute__((aligned(16))) float cs[kMostRows][kPairs], sn[kMostRows][kPairs];
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.block_rows;
+    const int count = min(static_cast<int64_t>(a.block_rows), a.rows - row0);
     const int lane = threadIdx.x & 63;
     const int all = a.heads + 2 * a.kv_heads;
     const int head = (blockIdx.y * blockDim.x + threadIdx.x) >> a.lanes_log2;
@@ -103,155 +123,188 @@ __global__ __launch_bounds__(kThreads) void norm_append_kernel(const NormArgs a)
     const bool live = head < all && c < a.pieces;
     const bool is_q = head < a.heads, is_k = !is_q && head < a.heads + a.kv_heads;
     const int kvh = is_q ? 0 : is_k ? head - a.heads : head - a.heads - a.kv_heads;
-    const uint16_t* src = is_q   ? a.q + row * a.q_row + head * a.q_head
-                          : is_k ? a.k + row * a.k_row + kvh * a.k_head
-                                 : a.v + row * a.v_row + kvh * a.v_head;
+    const int64_t src_row = is_q ? a.q_row : is_k ? a.k_row : a.v_row;
+    const uint16_t* src = (is_q   ? a.q + head * a.q_head
+                           : is_k ? a.k + kvh * a.k_head
+                                  : a.v + kvh * a.v_head) + row0 * src_row;
     const uint16_t* weight = is_q ? a.q_weight : is_k ? a.k_weight : nullptr;
     const bool turned = is_q || is_k;
     int at[2];
     at[0] = ANY || (MODE == kHalves && turned) ? 8 * c : 16 * c;
     at[1] = MODE == kHalves && turned ? a.head_dim / 2 + 8 * c : at[0] + 8;
-    u32x4 x[N], w[N];
+    u32x4 x[N], ahead[N], w[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        x[i] = w[i] = u32x4{0, 0, 0, 0};
+        ahead[i] = w[i] = u32x4{0, 0, 0, 0};
         if (live) {
-            x[i] = *reinterpret_cast<const u32x4*>(src + at[i]);
+            ahead[i] = *reinterpret_cast<const u32x4*>(src + at[i]);
             if (weight != nullptr) w[i] = *reinterpret_cast<const u32x4*>(weight + at[i]);
         }
     }
-    const Place to = place_of(a.p, a.row_starts, a.rows_per_sequence, row, lane);
-    const bool placed = to.pos >= 0;
-    if (placed && !to.stored && a.rejected != nullptr && threadIdx.x == 0 && blockIdx.y == 0) atomicAdd(a.rejected, 1);
-    for (int i = threadIdx.x; i < a.pairs; i += blockDim.x) {
-        constexpr double kTurn = 6.283185307179586476925286766559;
-        const double angle = static_cast<double>(placed ? to.pos : 0) * a.freq[i];
-        const float r = static_cast<float>(angle - kTurn * rint(angle / kTurn));
-        cs[i] = cosf(r);
-        sn[i] = sinf(r);
+    const Place places = places_of(a.p, a.row_starts, a.rows_per_sequence, row0, count, lane);
+    if (a.rejected != nullptr && threadIdx.x < 64 && blockIdx.y == 0) {
+        const int lost = __popcll(__ballot(lane < count && places.pos >= 0 && !places.stored));
+        if (lost > 0 && lane == 0) atomicAdd(a.rejected, lost);
     }
-    f32x8 y[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) y[i] = widen8<BF16>(x[i]);
-
-    // the norm; every lane of the head takes part
-    float scale = 1.0f;
-    int shift = 0;
-    if (a.q_weight != nullptr || a.k_weight != nullptr) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sum = fmaf(y[i][j], y[i][j], sum);
-        auto add = [](float u, float v) { return u + v; };
-        sum = over_head(sum, a.lanes_log2, add);
-        scale = 1.0f / sqrtf(sum / static_cast<float>(a.head_dim) + a.eps);
-        if (__builtin_expect(__any(weight != nullptr && beyond(sum, a.eps, a.head_dim)), 0)) {
-            double wide = 0.0;
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const double v = y[i][j];
-                    wide = fma(v, v, wide);
-                }
-            for (int off = 1; off < 1 << a.lanes_log2; off <<= 1) wide += __shfl_xor(wide, off);
-            if (beyond(sum, a.eps, a.head_dim)) {
-                // the root's power of two goes to the values, which it leaves exact, so that both stay in range
-                const double mean = wide / static_cast<double>(a.head_dim) + static_cast<double>(a.eps);
-                shift = -(__builtin_amdgcn_frexp_exp(mean) >> 1);
-                scale = 1.0f / sqrtf(static_cast<float>(__builtin_ldexp(mean, 2 * shift)));
-            }
-        }
-        if (weight != nullptr) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const f32x8 wf = widen8<BF16>(w[i]);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) y[i][j] = ldexpf(y[i][j], shift) * scale * wf[j];
-            }
+    const int low = static_cast<int>(places.pos), high = static_cast<int>(places.pos >> 32);
+    for (int base = 0; base < count * a.pairs; base += blockDim.x) {
+        // (every lane takes part in the shuffles)
+        const int i = base + threadIdx.x;
+        const int r = min(static_cast<int>(static_cast<unsigned>(i) / static_cast<unsigned>(a.pairs)), count - 1);
+        const int pair = i - r * a.pairs;
+        const int64_t pos = static_cast<int64_t>(__shfl(high, r)) << 32 | static_cast<uint32_t>(__shfl(low, r));
+        if (pair < a.pairs) {
+            constexpr double kTurn = 6.283185307179586476925286766559;
+            const double angle = static_cast<double>(max(pos, static_cast<int64_t>(0))) * a.freq[pair];
+            const float turn = static_cast<float>(angle - kTurn * rint(angle / kTurn));
+            cs[r][pair] = cosf(turn);
+            sn[r][pair] = sinf(turn);
         }
     }
     __syncthreads();
-    if (turned) {
-        if constexpr (MODE == kHalves) {
+#pragma unroll 1
+    for (int r = 0; r < count; ++r) {
+        const int64_t row = row0 + r;
+        const bool placed = __builtin_amdgcn_readlane(high, r) >= 0;
+        const bool stored = __builtin_amdgcn_readlane(places.stored ? 1 : 0, r) != 0;
+        const uint32_t page = __builtin_amdgcn_readlane(places.page, r);
+        const uint32_t slot = __builtin_amdgcn_readlane(places.slot, r);
+        f32x8 y[N];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                // (a mode of whole heads without a rotation has no pairs)
-                const bool on = a.pairs > 0;
-                const float cc = on ? cs[(8 * c + j) & 127] : 1.0f, ss = on ? sn[(8 * c + j) & 127] : 0.0f;
-                const float u = y[0][j], v = y[1][j];
-                if (on) {
-                    y[0][j] = u * cc - v * ss;
-                    y[1][j] = v * cc + u * ss;
-                }
-            }
-        } else if constexpr (MODE == kAdjacent) {
+        for (int i = 0; i < N; ++i) {
+            x[i] = ahead[i];
+            y[i] = widen8<BF16>(x[i]);
+        }
+        const uint16_t* const here = src;
+        src += src_row;
+        if (live && r + 1 < count)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < N; ++i) ahead[i] = *reinterpret_cast<const u32x4*>(src + at[i]);
+
+        // the norm; every lane of the head takes part
+        float scale = 1.0f;
+        int shift = 0;
+        if (a.q_weight != nullptr || a.k_weight != nullptr) {
+            float sum = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 8; j += 2) {
-                    const int pair = (8 * c + 4 * i + j / 2) & 127;
-                    const float u = y[i][j], v = y[i][j + 1];
-                    y[i][j] = u * cs[pair] - v * sn[pair];
-                    y[i][j + 1] = v * cs[pair] + u * sn[pair];
-                }
-        } else {
-            const f32x8 mine = y[0];
+            for (int i = 0; i < N; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int d = 8 * c + j;
-                if (live && d < 2 * a.pairs) {
-                    const bool first = MODE == kAnyAdjacent ? (d & 1) == 0 : d < a.pairs;
-                    const int pair = MODE == kAnyAdjacent ? d >> 1 : first ? d : d - a.pairs;
-                    float o;
-                    if constexpr (MODE == kAnyAdjacent) {
-                        o = mine[j ^ 1];
-                    } else {
-                        const int other = first ? d + a.pairs : d - a.pairs;
-                        o = widen1<BF16>(src[other]);
-                        if (weight != nullptr) o = ldexpf(o, shift) * scale * widen1<BF16>(weight[other]);
+                for (int j = 0; j < 8; ++j) sum = fmaf(y[i][j], y[i][j], sum);
+            auto add = [](float u, float v) { return u + v; };
+            sum = over_head(sum, a.lanes_log2, add);
+            scale = 1.0f / sqrtf(sum / static_cast<float>(a.head_dim) + a.eps);
+            if (__builtin_expect(__any(weight != nullptr && beyond(sum, a.eps, a.head_dim)), 0)) {
+                double wide = 0.0;
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const double v = y[i][j];
+                        wide = fma(v, v, wide);
                     }
-                    y[0][j] = first ? mine[j] * cs[pair] - o * sn[pair] : mine[j] * cs[pair] + o * sn[pair];
+                for (int off = 1; off < 1 << a.lanes_log2; off <<= 1) wide += __shfl_xor(wide, off);
+                if (weight != nullptr && beyond(sum, a.eps, a.head_dim)) {
+                    // the root's power of two goes to the values, which it leaves exact, so that both stay in range
+                    const double mean = wide / static_cast<double>(a.head_dim) + static_cast<double>(a.eps);
+                    shift = -(__builtin_amdgcn_frexp_exp(mean) >> 1);
+                    scale = 1.0f / sqrtf(static_cast<float>(__builtin_ldexp(mean, 2 * shift)));
+                }
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) y[i][j] = ldexpf(y[i][j], shift);
+            }
+            if (weight != nullptr) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const f32x8 wf = widen8<BF16>(w[i]);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) y[i][j] = y[i][j] * scale * wf[j];
                 }
             }
         }
-    }
-    float largest = 0.0f;
-    bool finite = true;
-    if constexpr (E8) {
-        // as integers: a NaN is the largest
-        uint32_t m = 0;
+        if (turned && a.pairs > 0) {
+            if constexpr (MODE == kHalves) {
+                // (a head has twice as many values as pairs)
+                const float* const cc = &cs[r][min(8 * c, kPairs - 8)];
+                const float* const ss = &sn[r][min(8 * c, kPairs - 8)];
 #pragma unroll
-        for (int i = 0; i < N; ++i)
+                for (int j = 0; j < 8; ++j) {
+                    const float u = y[0][j], v = y[1][j];
+                    y[0][j] = u * cc[j] - v * ss[j];
+                    y[1][j] = v * cc[j] + u * ss[j];
+                }
+            } else if constexpr (MODE == kAdjacent) {
+                const float* const cc = &cs[r][min(8 * c, kPairs - 8)];
+                const float* const ss = &sn[r][min(8 * c, kPairs - 8)];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(y[i][j]) & 0x7FFFFFFFu);
-        auto most = [](float u, float v) { return __uint_as_float(max(__float_as_uint(u), __float_as_uint(v))); };
-        largest = over_head(__uint_as_float(m), a.lanes_log2, most);
-        finite = __float_as_uint(largest) < 0x7F800000u;
-    }
-    if (!live || (!is_q && !to.stored)) return;
-    if (is_q) {
-        uint16_t* out = a.q_out + (row * a.heads + head) * a.head_dim;
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            *reinterpret_cast<u32x4*>(out + at[i]) = placed ? narrow8<BF16>(y[i]) : u32x4{0, 0, 0, 0};
-        return;
-    }
-    const int64_t piece = to.page * a.p.page_stride + to.slot * a.p.slot_stride;
-    if constexpr (E8) {
-        uint8_t* out = reinterpret_cast<uint8_t*>(is_k ? a.p.k : a.p.v) + piece * 16 + kvh * a.p.head_stride;
-        const float s = finite ? fmaxf(largest / kE4m3Max, kSmallestScale) : __uint_as_float(0x7FC00000u);
-        const float inv = 1.0f / s;
+                    for (int j = 0; j < 8; j += 2) {
+                        const int pair = 4 * i + j / 2;
+                        const float u = y[i][j], v = y[i][j + 1];
+                        y[i][j] = u * cc[pair] - v * ss[pair];
+                        y[i][j + 1] = v * cc[pair] + u * ss[pair];
+                    }
+            } else {
+                const f32x8 mine = y[0];
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            *reinterpret_cast<u32x2*>(out + at[i]) = finite ? pack8_e4m3(y[i], s, inv) : u32x2{0x7F7F7F7Fu, 0x7F7F7F7Fu};
-        if (c == 0) (is_k ? a.s.k : a.s.v)[a.s.at(static_cast<int>(to.page), kvh, to.slot)] = s;
-    } else {
-        uint16_t* out = (is_k ? a.p.k : a.p.v) + piece * 8 + kvh * a.p.head_stride;
+                for (int j = 0; j < 8; ++j) {
+                    const int d = 8 * c + j;
+                    if (live && d < 2 * a.pairs) {
+                        const bool first = MODE == kAnyAdjacent ? (d & 1) == 0 : d < a.pairs;
+                        const int pair = MODE == kAnyAdjacent ? d >> 1 : first ? d : d - a.pairs;
+                        float o;
+                        if constexpr (MODE == kAnyAdjacent) {
+                            o = mine[j ^ 1];
+                        } else {
+                            const int other = first ? d + a.pairs : d - a.pairs;
+                            o = widen1<BF16>(here[other]);
+                            if (weight != nullptr) o = ldexpf(o, shift) * scale * widen1<BF16>(weight[other]);
+                        }
+                        y[0][j] = first ? mine[j] * cs[r][pair] - o * sn[r][pair] : mine[j] * cs[r][pair] + o * sn[r][pair];
+                    }
+                }
+            }
+        }
+        float largest = 0.0f;
+        bool finite = true;
+        if constexpr (E8) {
+            // as integers: a NaN is the largest
+            uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i)  // values v as they are
-            *reinterpret_cast<u32x4*>(out + at[i]) = is_k ? narrow8<BF16>(y[i]) : x[i];
+            for (int i = 0; i < N; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(y[i][j]) & 0x7FFFFFFFu);
+            auto most = [](float u, float v) { return __uint_as_float(max(__float_as_uint(u), __float_as_uint(v))); };
+            largest = over_head(__uint_as_float(m), a.lanes_log2, most);
+            finite = __float_as_uint(largest) < 0x7F800000u;
+        }
+        if (!live || (!is_q && !stored)) continue;
+        if (is_q) {
+            uint16_t* out = a.q_out + (row * a.heads + head) * a.head_dim;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                *reinterpret_cast<u32x4*>(out + at[i]) = placed ? narrow8<BF16>(y[i]) : u32x4{0, 0, 0, 0};
+            continue;
+        }
+        // (32 bits hold a place's piece of 16 bytes: see Pages)
+        const int64_t piece = page * a.p.page_stride + slot * a.p.slot_stride;
+        if constexpr (E8) {
+            uint8_t* out = reinterpret_cast<uint8_t*>(is_k ? a.p.k : a.p.v) + piece * 16 + kvh * a.p.head_stride;
+            const float s = finite ? fmaxf(largest / kE4m3Max, kSmallestScale) : __uint_as_float(0x7FC00000u);
+            const float inv = 1.0f / s;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                *reinterpret_cast<u32x2*>(out + at[i]) =
+                    finite ? pack8_e4m3(y[i], s, inv) : u32x2{0x7F7F7F7Fu, 0x7F7F7F7Fu};
+            if (c == 0) (is_k ? a.s.k : a.s.v)[a.s.at(static_cast<int>(page), kvh, slot)] = s;
+        } else {
+            uint16_t* out = (is_k ? a.p.k : a.p.v) + piece * 8 + kvh * a.p.head_stride;
+#pragma unroll
+            for (int i = 0; i < N; ++i)  // values v as they are
+                *reinterpret_cast<u32x4*>(out + at[i]) = is_k ? narrow8<BF16>(y[i]) : x[i];
+        }
     }
 }
 
@@ -295,7 +348,10 @@ int run(NormArgs& a, int64_t rows, int64_t sequences, int64_t heads, int64_t kv_
     const int64_t threads = (heads + 2 * kv_heads) << a.lanes_log2;
     const int64_t parts = plm::ceil_div(threads, kThreads);
     if (parts > 65535) return plm::fail(-2, "too many heads");
-    const dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>(parts));
+    a.rows = static_cast<int>(rows);
+    a.block_rows = static_cast<int>(
+        std::clamp<int64_t>(rows * parts / (kBlocks * plm::cu_count()), 1, kMostRows));
+    const dim3 grid(static_cast<unsigned>(plm::ceil_div(rows, a.block_rows)), static_cast<unsigned>(parts));
     const dim3 block(static_cast<unsigned>(plm::ceil_div(plm::ceil_div(threads, parts), 64) * 64));
     if (dtype_code == 1)
         launch<true, E8>(a, mode, grid, block, plm::current_stream());
