@@ -157,10 +157,10 @@ __device__ __forceinline__ int place_of_tile(const ChunkArgs& a, int at, int lan
 //
 // Unless whole tiles take no longer.  They take as many position tiles as the
 // longest of them has, or where there are more than the device holds their share
-// of the work and half of the longest; runs take their share, kStart for each tile
+// of the work and a fifth of the longest; runs take their share, kStart for each tile
 // that they hold a part of, kJoin, and kJoinRuns where every workgroup leaves
 // partials of full tiles (67 MB at a head of 128).  28 and 4 heads of 128, whole / in runs: a prompt
-// of 500 rows 25 / 41 us, of 1500 62 / 67, 16 of up to 200 rows 33 / 56; 37 rows
+// of 500 rows 28 / 41 us, of 1500 56 / 67, of 2500 81 / 108, 16 of up to 200 rows 33 / 56; 37 rows
 // behind 700 positions 34 / 27, 64 times 2 rows behind up to 4000 128 / 110.
 constexpr uint32_t kTileWork = 2;
 constexpr uint32_t kLeastWork = 4;  // of a run
@@ -227,7 +227,7 @@ __device__ __forceinline__ Dealt find_run(const ChunkArgs& a, int run, int lane,
     const float in_runs = per_run * scale + kStart * static_cast<float>(tiles) * each + kJoin +
                           kJoinRuns * static_cast<float>(runs) * share * filled;
     float whole = static_cast<float>(longest);
-    if (tiles > static_cast<uint32_t>(a.runs)) whole = fmaxf(whole, static_cast<float>(all) * share * scale + whole * 0.5f);
+    if (tiles > static_cast<uint32_t>(a.runs)) whole = fmaxf(whole, static_cast<float>(all) * share * scale + whole * 0.2f);
     if (whole <= in_runs) return kTiles;
     if (static_cast<uint32_t>(run) >= runs) return kNone;
     auto border_at = [&](uint32_t r) { return r == runs ? all : static_cast<uint32_t>(static_cast<float>(r) * per_run); };
@@ -908,12 +908,12 @@ __global__ __launch_bounds__(DP > 128 ? 256 : 512, 1) void paged_chunk_kernel(co
         }
         const int units = static_cast<int>(position_tiles(piece.seen));
         auto unit_at = [&](float share) {
-            return __builtin_amdgcn_readfirstlane(min(units, static_cast<int>(share * static_cast<float>(units))));
+            return __builtin_amdgcn_readfirstlane(min(units, max(0, static_cast<int>(share * static_cast<float>(units)))));
         };
         const bool goes_on = place == next.place && tile == next.tile && next.share > 0.0f;
         const bool ends_here = place == last.place && tile == last.tile;
         if (ends_here && last.share == 0.0f) return;
-        const int from = goes_on ? unit_at(next.share) : 0, to = ends_here ? unit_at(last.share) : units;
+        const int from = goes_on ? unit_at(next.share) : 0, to = ends_here ? max(from, unit_at(last.share)) : units;
         if (units > 0 && to == 0) return;  // the next run begins it
         // (not what the run before has ended)
         if (units > 0 ? from < units : !goes_on) {
@@ -1020,7 +1020,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_chunk_join_kernel(const Ch
     const int place = place_of_tile(a, blockIdx.x, lane, begin);
     const int first = start_of(a, place), rows = rows_of(a, place);
     const int tile = blockIdx.x - begin;
-    if (tile >= column_tiles(a, rows)) return;
+    if (tile < 0 || tile >= column_tiles(a, rows)) return;  // (below 0 where row starts do not ascend)
     const int col0 = tile << a.columns_log2, columns = rows * a.group;
     if (parts > kFewPartials) {
         const int in = blockIdx.z * kJoinColumns + wave;

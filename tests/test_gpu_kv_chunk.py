@@ -108,6 +108,15 @@ def test_many_rows(nat, e4m3, heads, kvh, dim, rows):
     check(nat, [0, 321], [rows, rows // 7], 64, heads, kvh, dim, BF16, e4m3=e4m3)
 
 
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("lengths,rows", [([0], [500]), ([0], [1500]), ([0, 0, 0], [900, 3, 860]), ([700], [37]), ([300] * 16, [150] * 16),
+                                          ([0, 3800], [300, 2])])
+def test_calls_that_whole_tiles_or_runs_take(nat, e4m3, lengths, rows):
+    """Sizes on both sides of what decides between whole tiles and runs, with tables that reach further."""
+    check(nat, lengths, rows, 16, 14, 2, 128, BF16, e4m3=e4m3, seed=sum(rows))
+    check(nat, [*lengths, 5000], [*rows, 1], 16, 14, 2, 128, BF16, e4m3=e4m3, seed=sum(rows))
+
+
 def test_many_rows_fp16(nat):
     check(nat, [77, 0], [2500, 300], 16, 32, 8, 128, F16)
 
@@ -540,3 +549,18 @@ def test_empty_calls(nat):
     q = torch.ones((3, 1, 64), dtype=F16, device="cuda")
     got = nat.kv_paged_attention_chunk_e4m3(q, *caches, *scales, table.cuda()[:0], i32([]), i32([0]))
     assert torch.equal(got, torch.zeros_like(q))
+
+
+def test_row_starts_that_do_not_ascend(nat):
+    """No promise about their rows, but the call ends and the next one is right."""
+    heads, kvh, dim = 14, 2, 128
+    caches, _, table = pref.make_pages([3000, 700, 40], 16, kvh, dim, BF16, 3)
+    table_d = table.cuda()
+    q = torch.randn((60, heads, dim), generator=torch.Generator().manual_seed(3)).to(BF16).cuda()
+    want = nat.kv_paged_attention_chunk(q, *caches, table_d, i32([2970, 680, 30]), i32([0, 30, 50, 60]))
+    for starts in ([0, 50, 20, 60], [60, 0, 60, 0], [-5, 1000, -7, 30]):
+        got = nat.kv_paged_attention_chunk(q, *caches, table_d, i32([2970, 680, 30]), i32(starts))
+        torch.cuda.synchronize()
+        assert got.shape == q.shape
+    again = nat.kv_paged_attention_chunk(q, *caches, table_d, i32([2970, 680, 30]), i32([0, 30, 50, 60]))
+    assert torch.equal(again, want)

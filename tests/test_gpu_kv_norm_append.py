@@ -144,6 +144,22 @@ def test_prompts_of_ragged_lengths(nat, e4m3, page):
     check(nat, e4m3, [0, 3, 31, 0, -2, 8], rows, page, 4, 2, 64, torch.bfloat16, starts=starts, seed=page)
 
 
+@pytest.mark.parametrize("e4m3,dim,total", [(False, 16, 8400), (True, 16, 8400), (False, 24, 2500), (True, 48, 5003)])
+def test_many_rows(nat, e4m3, dim, total):
+    """Calls whose workgroups take several rows, across the borders of many short
+    sequences, idle ones and ones without rows, and of a long one."""
+    rows = [(7 * i) % 23 for i in range(90)]
+    rows.append(total - sum(rows))
+    lengths = [-1 if i % 13 == 5 else (31 * i) % 40 for i in range(91)]
+    starts = [sum(rows[:i]) for i in range(92)]
+
+    def spoil(table):
+        table[3] = -1
+        table[90, 7] = 10 ** 6
+
+    assert check(nat, e4m3, lengths, rows, 16, 2, 1, dim, torch.bfloat16, starts=starts, seed=dim, spoil=spoil) > 0
+
+
 @pytest.mark.parametrize("e4m3", [False, True])
 def test_rows_without_a_page(nat, e4m3):
     def spoil(table):
