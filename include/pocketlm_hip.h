@@ -902,7 +902,8 @@ int kv_paged_norm_append_u16(const uint16_t* q, const uint16_t* k, const uint16_
  * scale NaN and bytes 0x7F.  k_cache and v_cache are laid out as the 16-bit
  * caches, with head_dim and the strides (in values) multiples of 16; the scale
  * of slot s of page p and head h is k_scales[p * scale_page_stride + h *
- * scale_head_stride + s], v_scales alike.  q, k, v, q_out and the weights are
+ * scale_head_stride + s], v_scales alike, 16 GiB of each at most.  Rows of a call
+ * take different slots.  q, k, v, q_out and the weights are
  * fp16 or bf16 (dtype_code).  Codes as there. */
 int kv_paged_append_e4m3(const uint16_t* q, const uint16_t* k, const uint16_t* v, const uint16_t* q_norm_weight,
                          const uint16_t* k_norm_weight, uint16_t* q_out, uint8_t* k_cache, uint8_t* v_cache,
@@ -939,7 +940,9 @@ int kv_paged_attention_decode_e4m3(const uint16_t* q, const uint8_t* k_cache, co
  * device).  Rows of no sequence or of an idle one are zero, as is a row that
  * sees nothing; positions without a page are left out, those past the table
  * too.  What a row does not see never reaches it, NaN or not.  Softmax weights
- * are rounded once to the cache's type (bf16 for e4m3 caches).  scratch: device
+ * are rounded once to the cache's type; over an e4m3 cache, times the values'
+ * scales, to bf16, for fp16 rows and those that see few positions to the sum of
+ * two bf16 values.  scratch: device
  * memory of kv_paged_attention_chunk_scratch_bytes, 16-byte aligned, or NULL
  * for the library's own; capacity is table_cols * page_size.  rows * heads <
  * 2^31.  Codes -1 null, -2 bad dimensions, -3 scratch. */

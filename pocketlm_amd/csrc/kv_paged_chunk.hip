@@ -26,6 +26,7 @@ constexpr int kTile = 64;  // positions that work is counted in
 // A running maximum is only moved once a score is more than 2^kLate above it: weights grow to 2^kLate, the
 // accumulators are multiplied in a few tiles instead of all.
 constexpr float kLate = 8.0f;
+constexpr int kFewPositions = 512;  // see attend
 // fp16 weights are kept times 2^7, so that with kLate they end at 2^15 and begin at 2^-31.
 __host__ __device__ constexpr float bias_of(bool bf16) { return bf16 ? 0.0f : 7.0f; }
 
@@ -445,7 +446,13 @@ struct Layout {
 //   values  O^T = V^T P^T: the weights go in as they lie, eight registers a step; the
 //           values' eight positions are chosen to match, by two transposed reads
 //
-// Weights are rounded to the values' type once.
+// Weights are rounded to the values' type once.  But over e4m3 pages they are
+// multiplied by their values' scales, need bf16's range and are not summed as
+// they were rounded: so they go in as two values, the second the rest, for fp16
+// rows (results within 2.1e-4 of their size, 1.7e-3 with one value, 1.26 ms and
+// 0.99 for 2048 rows behind 30000 positions), and for bf16 rows that see few
+// positions, where one weight's rounding is the whole result's (a first prompt's
+// rows were off by up to 2.1 times the output's rounding, later ones by 1.4).
 //
 // Each wave alternates between the matrix cores (the scores of tile i + 1, then the
 // values of tile i) and the vector units (the weights of tile i + 1); the second four
@@ -475,6 +482,7 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
     constexpr int KS = DP / 16;   // score steps
     constexpr int DB = DP / 32;   // blocks of head values
     constexpr float kBias = bias_of(VBF16);
+    constexpr bool kTwo = E8 && !BF16;     // weights of two values
     constexpr bool kDotSum = BF16 && !E8;  // the weights are summed as they were rounded, two an instruction
     constexpr int kOutstanding = 1 + 2 * L::kBlocks;  // loads of a step
     typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
@@ -492,6 +500,7 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
     const int wave_seen =
         wave0 < columns ? uniform(seen_by(a, piece.length, a.by_group(min(wave0 + 32, columns) - 1))) : 0;
     const int begin = piece.begin, end = piece.end;
+    [[maybe_unused]] const bool few = wave_least < kFewPositions;
 
     float m = -INFINITY, l = 0.0f;  // weights are exp2(score - m): m is the maximum less the bias, up to kLate behind
     f32x16 acc[DB];
@@ -620,7 +629,7 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
         };
 
         f32x16 s[KB];
-        u32x4 w[2 * KB];
+        u32x4 w[2 * KB], rest[kTwo ? 2 * KB : 1];
         u32x4 ahead_v[DB];
         auto value_piece = [&](lds_char* tile, int x, int b) {
             const int from = b / 2 * L::kBlock + 16 * x * 128;
@@ -636,7 +645,8 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
             constexpr bool LOAD = decltype(with_loads)::value;
             const lds_char* const tile = lds + ((t + 1) & (L::kStages - 1)) * L::kStage;
             lds_char* const vtile = lds + (t & (L::kStages - 1)) * L::kStage;
-            constexpr int kAhead = DB > 6 ? DB : 6, kSteps = KB * KS;
+            constexpr int kLeast = kTwo ? 4 : 6;  // (registers)
+            constexpr int kAhead = DB > kLeast ? DB : kLeast, kSteps = KB * KS;
             u32x4 k[kAhead];
             auto key_piece = [&](int i) {
                 const int x = i / KB, b = i % KB;
@@ -687,6 +697,7 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
                 for (int b = 0; b < DB; ++b) {
                     __builtin_amdgcn_sched_barrier(0);
                     acc[b] = mfma32<VBF16>(ahead_v[b], w[x], acc[b]);
+                    if constexpr (kTwo) acc[b] = mfma32<VBF16>(ahead_v[b], rest[x], acc[b]);
                     if (x + 1 < 2 * KB) ahead_v[b] = value_piece(tile, x + 1, b);
                 }
             __builtin_amdgcn_sched_barrier(0);
@@ -769,7 +780,15 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
                         v = v * scale[4 * b + j / 4];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const uint32_t two = pack2<VBF16>(v[2 * i], v[2 * i + 1]);
+                        uint32_t two;
+                        if constexpr (kTwo) {
+                            const uint32_t lo = __float_as_uint(v[2 * i]), hi = __float_as_uint(v[2 * i + 1]) & 0xFFFF0000u;
+                            two = hi | lo >> 16;
+                            rest[2 * b + (j >> 3)][(j & 4) / 2 + i] =
+                                pack2<true>(v[2 * i] - __uint_as_float(lo & 0xFFFF0000u), v[2 * i + 1] - __uint_as_float(hi));
+                        } else {
+                            two = pack2<VBF16>(v[2 * i], v[2 * i + 1]);
+                        }
                         w[2 * b + (j >> 3)][(j & 4) / 2 + i] = two;
                         if constexpr (kDotSum)
                             sum[2 * (j >> 2 & 1) + i] = __builtin_amdgcn_fdot2_f32_bf16(
@@ -778,6 +797,29 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
                     }
                 }
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            if constexpr (E8 && BF16) {
+                // what the rounding left, formed again: its products at once
+                if (few) {
+#pragma unroll
+                    for (int x = 0; x < 2 * KB; ++x) {
+                        u32x4 left;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float v[2];
+#pragma unroll
+                            for (int y = 0; y < 2; ++y) {
+                                const int j = 8 * (x & 1) + 2 * i + y;
+                                v[y] = __builtin_amdgcn_exp2f(s[x >> 1][j] - from) * scale[4 * (x >> 1) + j / 4][j & 3];
+                            }
+                            left[i] = pack2<true>(v[0] - __uint_as_float(w[x][i] << 16),
+                                                  v[1] - __uint_as_float(w[x][i] & 0xFFFF0000u));
+                        }
+#pragma unroll
+                        for (int b = 0; b < DB; ++b)
+                            acc[b] = mfma32<true>(value_piece(const_cast<lds_char*>(tile), x, b), left, acc[b]);
+                    }
+                }
+            }
             return true;
         };
         // until this wave's loads but the last step's are there (the first waves after their weights, the second

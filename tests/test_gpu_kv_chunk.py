@@ -14,6 +14,9 @@ import paged_refs as pref
 pytestmark = pytest.mark.gpu
 
 BF16, F16, E4M3 = torch.bfloat16, torch.float16, torch.float8_e4m3fn
+# how far off the weights over e4m3 pages are: rounded to bf16; of fp16 rows the upper 8 bits, which leave less than 2^-7,
+# and that rest rounded to bf16
+E4M3_WEIGHT = {BF16: ref.HALF[BF16], F16: 2.0 ** -7 * ref.HALF[BF16]}
 
 
 @pytest.fixture(scope="module")
@@ -56,7 +59,7 @@ def check(nat, lengths, rows, page, heads, kvh, dim, dtype, *, e4m3=False, seed=
     kw = {} if scale is None else {"softmax_scale": scale}
     got = attend(nat, q, caches, scales, table, lengths, starts, **kw)
     want, bound = pref.chunk(q, *caches, table, lengths, starts, dim ** -0.5 if scale is None else scale, scales=scales,
-                             weight=ref.HALF[BF16] if e4m3 else None)
+                             weight=E4M3_WEIGHT[dtype] if e4m3 else None)
     assert got.shape == q.shape and got.dtype == dtype
     pref.agree(got, want, bound)
     return got
@@ -95,6 +98,20 @@ def test_rows_at_tiles_borders(nat, e4m3, rows):
 def test_few_rows_of_long_sequences(nat, dtype, e4m3, heads, kvh, dim):
     """Positions split over workgroups, in pieces of different numbers for each sequence."""
     check(nat, [5000, 700, 0, 2111], [3, 40, 9, 1], 64, heads, kvh, dim, dtype, e4m3=e4m3, behind=1)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads,kvh,dim", [(12, 2, 128), (16, 16, 64), (3, 1, 256), (4, 2, 96), (2, 1, 192)])
+@pytest.mark.parametrize("lengths,rows", [([0], [2]), ([0, 0], [3, 40]), ([40, 0], [2, 300]), ([500], [9])])
+def test_few_positions_over_e4m3_pages(nat, dtype, heads, kvh, dim, lengths, rows):
+    """Where a weight may be the whole result its rounding must not show: bounds as of a weight rounded to 15 bits."""
+    lens = [x + r for x, r in zip(lengths, rows)]
+    caches, scales, table = pref.make_pages(lens, 16, kvh, dim, E4M3, dim)
+    starts = starts_of(rows)
+    q = (torch.randn((starts[-1], heads, dim), generator=torch.Generator().manual_seed(dim)) * 2).to(dtype).cuda()
+    got = attend(nat, q, caches, scales, table, lengths, starts)
+    want, bound = pref.chunk(q, *caches, table, lengths, starts, dim ** -0.5, scales=scales, weight=2.0 ** -15)
+    pref.agree(got, want, bound)
 
 
 def test_one_row_of_a_very_long_sequence(nat):
@@ -428,7 +445,7 @@ def test_prompts_in_chunks_then_tokens(nat, dtype, e4m3):
         q = append(qkv, caches, scales, i32(lengths), i32(starts))
         got = attend(nat, q, caches, scales, table, lengths, starts)
         want, bound = pref.chunk(q, *caches, table, lengths, starts, dim ** -0.5, scales=scales,
-                                 weight=ref.HALF[BF16] if e4m3 else None)
+                                 weight=E4M3_WEIGHT[dtype] if e4m3 else None)
         pref.agree(got, want, bound)
         if rows == [1, 1]:
             if e4m3:
