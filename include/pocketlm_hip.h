@@ -902,9 +902,9 @@ int kv_paged_norm_append_u16(const uint16_t* q, const uint16_t* k, const uint16_
  * scale NaN and bytes 0x7F.  k_cache and v_cache are laid out as the 16-bit
  * caches, with head_dim and the strides (in values) multiples of 16; the scale
  * of slot s of page p and head h is k_scales[p * scale_page_stride + h *
- * scale_head_stride + s], v_scales alike, 16 GiB of each at most.  Rows of a call
- * take different slots.  q, k, v, q_out and the weights are
- * fp16 or bf16 (dtype_code).  Codes as there. */
+ * scale_head_stride + s], v_scales alike, 16 GiB of each at most.  Rows of a
+ * call take different slots.  q, k, v, q_out and the weights are fp16 or bf16
+ * (dtype_code).  Codes as there. */
 int kv_paged_append_e4m3(const uint16_t* q, const uint16_t* k, const uint16_t* v, const uint16_t* q_norm_weight,
                          const uint16_t* k_norm_weight, uint16_t* q_out, uint8_t* k_cache, uint8_t* v_cache,
                          float* k_scales, float* v_scales, const int* page_table, const int* lengths,

@@ -223,7 +223,7 @@ __global__ __launch_bounds__(kThreads) void norm_append_kernel(const NormArgs a)
                 }
             }
         }
-        if (turned && a.pairs > 0) {
+        if (live && turned && a.pairs > 0) {  // (lanes without values stay 0: there are no angles for them)
             if constexpr (MODE == kHalves) {
                 // (a head has twice as many values as pairs)
                 const float* const cc = &cs[r][min(8 * c, kPairs - 8)];

@@ -161,6 +161,19 @@ def test_many_rows(nat, e4m3, dim, total):
 
 
 @pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("dim,interleaved", [(48, False), (48, True), (80, False), (96, True), (208, False), (240, False)])
+def test_heads_with_lanes_to_spare_after_nan_in_lds(nat, e4m3, dim, interleaved):
+    """Head sizes that leave lanes without values, whose angles nobody wrote: what an attention over NaN left in LDS
+    must not reach the head's maximum."""
+    pages = torch.full((64, 64, 4, 128), float("nan"), dtype=torch.bfloat16, device="cuda")
+    table = torch.arange(64, dtype=torch.int32, device="cuda")[None]
+    q = torch.ones((4096, 4, 128), dtype=torch.bfloat16, device="cuda")
+    nat.kv_paged_attention_chunk(q, pages, pages, table, i32([0]), i32([0, 4096]))
+    check(nat, e4m3, [0, 17, -1, 403], [40, 900, 3, 300], 16, 4, 2, dim, torch.bfloat16, interleaved=interleaved,
+          starts=[0, 40, 940, 943, 1243], seed=dim)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
 def test_rows_without_a_page(nat, e4m3):
     def spoil(table):
         table[0, 0] = -1
