@@ -473,6 +473,13 @@ struct Layout {
 // finite and met positions that not every column sees does its columns again, one at
 // a time (careful_column).  Positions behind the last one seen, or without a page, are
 // never read.
+//
+// Bound by the matrix cores' power and by the exponentials between them: two
+// prompts of up to 8191 rows of 28 and 4 heads of 128, 752 GFLOP, in 726 us, 1.03 PFLOP/s
+// (a library product of 8192^3 1.05 to 1.2); in step, with tiles three deep, the waves
+// took 818.  Over e4m3 pages 2048 rows behind 30000 positions, 911 GFLOP, in 952
+// us (1065 with each lane's page and scale found anew for each load).  Small calls wait for
+// memory and for the code: 37 rows behind 700 positions 20 us of kernel.
 template <bool BF16, bool E8, int DP>
 __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, int kvh, lds_char* lds) {
     using L = Layout<DP, E8>;

@@ -106,10 +106,14 @@ __device__ __forceinline__ u32x2 pack8_e4m3(const f32x8 y, float scale, float in
 // starts, lengths and page table one after the other.
 //
 // Bound by memory where rows are many: 125 MB of 5 x 1700 rows (28 and 4 heads
-// of 128, fp16) in 30 us, 4.2 TB/s (e4m3 pages 119 MB in 35 us: the quotients
+// of 128, fp16) in 30 us, 4.2 TB/s (e4m3 pages 119 MB in 29 us: the quotients
 // and the head's maximum come on top); one row takes 3.6 us, which is its chain of loads.
+//
+// Five waves a SIMD for e4m3 pages (5 x 1700 rows 29 us, 36 with the four that 102
+// registers allow), where more arithmetic stands between loads and stores; four
+// for 16-bit ones (39 with five, 31).
 template <bool BF16, int MODE, bool E8>
-__global__ __launch_bounds__(kThreads) void norm_append_kernel(const NormArgs a) {
+__global__ __launch_bounds__(kThreads, E8 ? 5 : 1) void norm_append_kernel(const NormArgs a) {
     constexpr bool ANY = MODE == kAny || MODE == kAnyAdjacent;
     constexpr int N = ANY ? 1 : 2;  // pieces of 8 values
     constexpr int kPairs = 128;
