@@ -366,8 +366,8 @@ constexpr uint32_t kNoRow = 0xFFFFFFFFu;
 // scale may leave.  A lane's keys are 16 adjacent values (32 s + 8 g of the
 // 16-bit caches become 64 (s / 2) + 16 g + 8 (s % 2), of the queries as well).
 // Each lane holds a scale of the tile: lanes 0 to 31 the keys', the others the
-// values'.  48 sequences of up to 16381 positions, 628 MB, in 124 us with the
-// join, 5.1 TB/s (212 of 16 bits); 700 positions 7.2 + 4.3 us.
+// values'.  48 sequences of up to 16381 positions, 628 MB, in 119 us and 8 of the
+// join, 5.3 TB/s (212 of 16 bits); 700 positions 7.1 + 4.6 us.
 template <bool BF16, bool E8, int DP, bool EXACT, int CT>
 __global__ __launch_bounds__(64 * kAttnWaves, DP > 128 ? 1 : 2) void paged_attention_kernel(
     const AttnArgs a) {

@@ -106,8 +106,8 @@ __device__ __forceinline__ u32x2 pack8_e4m3(const f32x8 y, float scale, float in
 // starts, lengths and page table one after the other.
 //
 // Bound by memory where rows are many: 125 MB of 5 x 1700 rows (28 and 4 heads
-// of 128, fp16) in 30 us, 4.2 TB/s (e4m3 pages 119 MB in 29 us: the quotients
-// and the head's maximum come on top); one row takes 3.6 us, which is its chain of loads.
+// of 128, fp16) in 30 us, 4.2 TB/s, 119 MB into e4m3 pages in 29 us; one row takes
+// 3.6 us, which is its chain of loads.
 //
 // Five waves a SIMD for e4m3 pages (5 x 1700 rows 29 us, 36 with the four that 102
 // registers allow), where more arithmetic stands between loads and stores; four
