@@ -602,22 +602,25 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
         // a position has its key scale (times the softmax's), the second its value scale
         // (every lane loads something: a branch around a load is a wait for the ones before it)
         constexpr int kUnits = (DP + 127) / 128;
-        u32x4 kraw[kUnits], vraw[kUnits];
-        float scale_raw = 0.0f;
-        bool scale_there = false;
+        struct Raw {
+            u32x4 k[kUnits], v[kUnits];
+            float scale;
+            bool there;
+        };
+        Raw raw = {};
         const float* const scales = (piece8 == 0 ? a.s.k : a.s.v) + static_cast<uint32_t>(kvh) * a.s.head_stride;
         const int further = 16 * piece8 + 128 < a.head_dim ? 128 : 0;
-        auto load8 = [&] {
-            scale_there = is_page(own_page);
-            const uint32_t at = scale_there ? static_cast<uint32_t>(own_page) * a.s.page_stride + own_slot : 0u;
+        auto load8 = [&](Raw& to) {
+            to.there = is_page(own_page);
+            const uint32_t at = to.there ? static_cast<uint32_t>(own_page) * a.s.page_stride + own_slot : 0u;
 #pragma unroll
             for (int i = 0; i < kUnits; ++i) {
-                kraw[i] = *reinterpret_cast<const u32x4*>(ksrc + (i > 0 ? further : 0));
-                vraw[i] = *reinterpret_cast<const u32x4*>(vsrc + (i > 0 ? further : 0));
+                to.k[i] = *reinterpret_cast<const u32x4*>(ksrc + (i > 0 ? further : 0));
+                to.v[i] = *reinterpret_cast<const u32x4*>(vsrc + (i > 0 ? further : 0));
             }
-            scale_raw = scales[at];
+            to.scale = scales[at];
         };
-        auto store8 = [&](int t) {
+        auto store8 = [&](int t, const Raw& from) {
             lds_char* const to = lds + (t & (L::kStages - 1)) * L::kStage;
 #pragma unroll
             for (int i = 0; i < kUnits; ++i)
@@ -626,13 +629,13 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
                     for (int x = 0; x < 2; ++x) {
                         const int where = (piece8 / 4 + 2 * i) * L::kBlock + own * 128 +
                                           (((2 * piece8 + x) & 7) ^ swizzle(own)) * 16;
-                        *(lds_u32x4*)(to + where) = eight_of<BF16>(kraw[i], x);
-                        *(lds_u32x4*)(to + L::kV + where) = eight_of<true>(vraw[i], x);
+                        *(lds_u32x4*)(to + where) = eight_of<BF16>(from.k[i], x);
+                        *(lds_u32x4*)(to + L::kV + where) = eight_of<true>(from.v[i], x);
                     }
                 }
             if (piece8 < 2)
                 *(__attribute__((address_space(3))) float*)(to + L::kScales + (piece8 * KT + own) * 4) =
-                    scale_there ? (piece8 == 0 ? scale_raw * a.scale : scale_raw) : 0.0f;
+                    from.there ? (piece8 == 0 ? from.scale * a.scale : from.scale) : 0.0f;
         };
 
         f32x16 s[KB];
@@ -676,14 +679,14 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
                     ahead_v[i + kAhead - kSteps] = value_piece(vtile, 0, i + kAhead - kSteps);
                 if constexpr (LOAD && E8) {
                     if (i == 1) {
-                        store8(t + 3);
+                        store8(t + 3, raw);
                         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the entries of the step before
                         own_page = entry(t + 4, own);
                     }
                     if (i == 3) load_entries(t + 5);
                     if (i == 5) {
                         find_own(t + 4);
-                        load8();
+                        load8(raw);
                     }
                 } else if constexpr (LOAD) {
                     if (i == 0) own_page = entry(t + 3, own);
@@ -847,22 +850,24 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
 #pragma unroll 1
         for (int t = 0; t < 5; ++t) load_entries(t);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if constexpr (E8) {
+            Raw first[3];  // all on their way at once
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                own_page = entry(t, own);
+                find_own(t);
+                load8(t < 3 ? first[t] : raw);
+            }
+#pragma unroll
+            for (int t = 0; t < 3; ++t) store8(t, first[t]);
+        } else {
 #pragma unroll 1
-        for (int t = 0; t < 3; ++t) {
-            own_page = entry(t, own);
-            find_own(t);
-            if constexpr (E8) {
-                load8();
-                store8(t);
-            } else {
+            for (int t = 0; t < 3; ++t) {
+                own_page = entry(t, own);
+                find_own(t);
 #pragma unroll
                 for (int i = 0; i < L::kBlocks; ++i) load_block(t, i);
             }
-        }
-        if constexpr (E8) {
-            own_page = entry(3, own);
-            find_own(3);
-            load8();
         }
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (second) asm volatile("s_barrier" ::: "memory");
