@@ -295,6 +295,30 @@ def test_without_weights_an_e4m3_append_quantizes_what_the_16_bit_one_rounds(nat
             assert bool(((x - y).abs() <= (2.0 ** -4 + 2.0 ** -8) * x.abs() + 2.0 ** -9 * top / 448 + 2.0 ** -8 * x.abs()).all())
 
 
+@pytest.mark.parametrize("size", [1.0, 2.0 ** 70])
+def test_e4m3_norms_of_queries_or_keys_alone(nat, size):
+    """A weight norms its own heads: the rest is as without any, also where a head's squares leave fp32."""
+    kvh, dim, page, dtype = 2, 128, 16, torch.bfloat16
+    g = torch.Generator().manual_seed(3)
+    q, k, v = ((torch.randn((40, h, dim), generator=g) * size).to(dtype).cuda() for h in (6, kvh, kvh))
+    w = (1 + 0.2 * torch.randn(dim, generator=g)).to(dtype).cuda()
+    freq = nat.kv_rope_frequencies(dim, 1e6)
+    starts, lengths = i32([0, 33, 40]), i32([5, 0])
+
+    def run(wq, wk):
+        caches, scales, table = pref.make_pages([38, 7], page, kvh, dim, torch.float8_e4m3fn, 1)
+        out = nat.kv_paged_append_e4m3(q, k, v, *caches, *scales, table.cuda(), lengths, q_norm_weight=wq, k_norm_weight=wk,
+                                       rms_eps=EPS, row_starts=starts, rope_frequencies=freq)
+        return [out] + [t.view(torch.uint8) if t.dtype != torch.float32 else t.view(torch.int32) for t in (*caches, *scales)]
+
+    none, both, queries, keys = run(None, None), run(w, w), run(w, None), run(None, w)
+    assert torch.equal(queries[0], both[0]) and torch.equal(keys[0], none[0])
+    for i in (1, 3):  # keys and their scales
+        assert torch.equal(queries[i], none[i]) and torch.equal(keys[i], both[i])
+    for i in (2, 4):
+        assert all(torch.equal(x[i], none[i]) for x in (both, queries, keys))
+
+
 def test_an_empty_call(nat):
     (dk, dv), (ks, vs), table = pref.make_pages([4], 4, 1, 64, torch.float8_e4m3fn, 0)
     x = torch.empty((0, 1, 64), dtype=torch.float16, device="cuda")
