@@ -193,6 +193,8 @@ struct AttnArgs {
     int columns;       // rows * group: column r * group + h is row r, head h of the group
     int column_blocks;
     uint32_t budget;      // runs of long sequences
+    uint32_t budget_many; // and where their units are `many`
+    uint32_t many;
     uint32_t short_runs;  // runs of short ones, about
     int single;           // no table row holds more than a few units: each sequence has a workgroup
     uint32_t uneven;      // units of a sequence more than its share that a workgroup may take; 0: never
@@ -267,10 +269,11 @@ __device__ __forceinline__ bool find_plan(const AttnArgs& a, int lane, uint32_t 
     plan.align = 1;
     plan.total = sum();
     longest = wave_max(longest);
-    const uint64_t most = 2 * a.uneven * a.budget + kUnevenHalves * static_cast<uint64_t>(plan.total);
-    plan.single = longest <= kFewUnits || (a.uneven > 0 && 2 * static_cast<uint64_t>(longest) * a.budget <= most);
-    plan.runs = plan.single ? a.p.sequences : a.budget;
-    if (!plan.single && plan.total < kShortRuns * a.budget) {
+    const uint32_t budget = plan.total >= a.many ? a.budget_many : a.budget;
+    const uint64_t most = 2 * a.uneven * budget + kUnevenHalves * static_cast<uint64_t>(plan.total);
+    plan.single = longest <= kFewUnits || (a.uneven > 0 && 2 * static_cast<uint64_t>(longest) * budget <= most);
+    plan.runs = plan.single ? a.p.sequences : budget;
+    if (!plan.single && plan.total < kShortRuns * budget) {
         plan.align = max(1u, (plan.total + a.short_runs - 1) / a.short_runs);
         if (plan.align > 1) plan.total = sum();
         plan.runs = plan.total / plan.align;
@@ -943,17 +946,19 @@ void launch_append(const AppendArgs& a, int mode, dim3 grid, dim3 block, hipStre
 constexpr int64_t kStreamedBytes = static_cast<int64_t>(128) << 20;
 constexpr double kLittleBytes = 64.0 * (1 << 20);
 
-// e4m3 caches: workgroups of three to a compute unit, where registers allow them
-// and the tables reach more than this of 16-bit values, half of it in bytes: a wave has
+// e4m3 caches: three workgroups to a compute unit, where registers allow them and
+// the sequences hold more than this of 16-bit values, half of it in bytes: a wave has
 // half as many bytes in flight (48 sequences of up to 16381 positions, 4 heads of
 // 128, 133 us against 141 with two, 64 of 8000, 8 heads of 64 144 and 148; but 32
-// of 3000 with 2 rows, 4 heads of 128 37 and 31).
+// of 3000 with 2 rows, 4 heads of 128 37 and 31; head sizes below 128 that are not 64
+// or less take more registers: 48 of 16000, 5 heads of 96 193 and 177).
 constexpr double kManyBytes = 512.0 * (1 << 20);
 
 struct AttnShape {
     int ct;             // blocks of 16 columns in a workgroup
     int column_blocks;
     int64_t budget;     // runs of long sequences
+    int64_t budget_many;
     int64_t short_runs; // of short ones, about
     int64_t runs;       // at most
     bool single;        // a run for each sequence
@@ -977,13 +982,15 @@ AttnShape shape_of(int64_t sequences, int64_t rows, int64_t heads, int64_t kv_he
     const int64_t hc = kv_heads * s.column_blocks;
     const int64_t units = std::max<int64_t>(1, plm::ceil_div(capacity, kUnit));
     // as many workgroups as the compute units hold at once, and as there are compute units
-    const int resident = head_dim > 128 ? 1 : e8 && s.ct == 1 && reach > kManyBytes ? 3 : 2;
+    const int resident = head_dim > 128 ? 1 : 2;
     s.budget = std::max<int64_t>(1, resident * plm::cu_count() / hc);
+    s.budget_many = e8 && (head_dim <= 64 || head_dim == 128) && s.ct == 1 && reach > kManyBytes
+                        ? std::max<int64_t>(1, 3 * plm::cu_count() / hc) : s.budget;
     s.short_runs = std::max<int64_t>(1, plm::cu_count() / hc);
     s.single = units <= kFewUnits;
     const int64_t groups = sequences * hc;
     s.uneven = groups >= plm::cu_count() ? kUnevenUnits : 2 * groups >= plm::cu_count() ? kUnevenUnitsHalf : 0;
-    const int64_t shared = std::min(sequences * units, s.budget + std::min(sequences, kShortRuns * s.budget));
+    const int64_t shared = std::min(sequences * units, s.budget_many + std::min(sequences, kShortRuns * s.budget_many));
     s.runs = s.single ? sequences : std::max(sequences, shared);
     s.joined = !s.single;
     s.slots = s.joined ? 2 * shared : 0;
@@ -1068,6 +1075,8 @@ int run_decode(AttnArgs& a, const uint16_t* q, uint16_t* out, void* scratch, int
     a.columns = a.rows * a.group;
     a.column_blocks = s.column_blocks;
     a.budget = static_cast<uint32_t>(s.budget);
+    a.budget_many = static_cast<uint32_t>(s.budget_many);
+    a.many = static_cast<uint32_t>(kManyBytes / static_cast<double>(kUnit * 4 * kv_heads * head_dim));
     a.short_runs = static_cast<uint32_t>(s.short_runs);
     a.single = s.single ? 1 : 0;
     a.uneven = s.uneven;
