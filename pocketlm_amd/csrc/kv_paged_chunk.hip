@@ -187,6 +187,7 @@ __device__ __forceinline__ Work work_of(const ChunkArgs& a, int place) {
     Work w = {0, 0, 0};
     if (place >= a.p.sequences + 2) return w;
     const int rows = rows_of(a, place);
+    if (rows == 0) return w;  // whatever its length
     const int length = length_of(a, place);
     w.tiles = column_tiles(a, rows);
     w.first = position_tiles(seen_by(a, length, min(static_cast<int>(a.by_group(1u << a.columns_log2)), rows) - 1));
