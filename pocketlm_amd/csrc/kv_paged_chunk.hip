@@ -27,8 +27,10 @@ constexpr int kTile = 64;  // positions that work is counted in
 // accumulators are multiplied in a few tiles instead of all.
 constexpr float kLate = 8.0f;
 constexpr int kFewPositions = 512;  // see attend
-// fp16 weights are kept times 2^7, so that with kLate they end at 2^15 and begin at 2^-31.
-__host__ __device__ constexpr float bias_of(bool bf16) { return bf16 ? 0.0f : 7.0f; }
+// So bf16 weights are kept times 2^-kLate, which ends them at 1: their sum with values at the end of the range
+// leaves fp32 no sooner than the decode kernel's.  fp16 weights are kept times 2^7, so that they end at 2^15 and
+// begin at 2^-31.
+__host__ __device__ constexpr float bias_of(bool bf16) { return bf16 ? -kLate : 7.0f; }
 
 // n / d of n < 2^31 without a division: n * times >> 31 + shift, where times is
 // 2^(31 + shift) / d rounded up and 2^shift >= d, so that its error, less than d,
