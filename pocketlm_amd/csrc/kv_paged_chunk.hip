@@ -330,89 +330,6 @@ __device__ __forceinline__ void load4_to_lds(const void* from, uint32_t to) {
 }
 #pragma clang diagnostic pop
 
-// One column over positions [begin, end) by a wave, in fp32, reading nothing that
-// the column does not see: a lane has a position's score, then the values d =
-// lane + 64 i of the sum.  For columns that meet infinities or NaN, so only right,
-// not fast.
-template <bool BF16, bool E8>
-__device__ void careful_column(const ChunkArgs& a, const Piece& piece, int kvh, int col, int lane) {
-    const int r = a.by_group(col), h = col - r * a.group;
-    const uint16_t* q = a.q + (piece.first + r) * a.q_row + (kvh * a.group + h) * a.q_head;
-    const int* table = a.p.table + static_cast<int64_t>(piece.place - 1) * a.p.table_cols;
-    const uint8_t* kbase = reinterpret_cast<const uint8_t*>(a.p.k) + (E8 ? 1 : 2) * kvh * a.p.head_stride;
-    const uint8_t* vbase = reinterpret_cast<const uint8_t*>(a.p.v) + (E8 ? 1 : 2) * kvh * a.p.head_stride;
-    const int last = min(piece.end, seen_by(a, piece.length, r));
-    auto value = [&](const uint8_t* row, int d) {
-        if constexpr (E8)
-            return __uint_as_float(pair_of<true>(row[d], false) << 16);
-        else
-            return widen1<BF16>(reinterpret_cast<const uint16_t*>(row)[d]);
-    };
-    float m = -INFINITY, l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 1
-    for (int t0 = piece.begin; t0 < last; t0 += kTile) {
-        const int pos = t0 + lane;
-        int page = -1;
-        uint32_t slot = 0;
-        if (pos < last) {
-            const uint32_t index = a.by_page(pos);
-            page = table[index];
-            slot = static_cast<uint32_t>(pos) - index * a.p.page_size;
-        }
-        const bool there = page >= 0 && static_cast<uint32_t>(page) < a.p.num_pages;
-        const uint32_t row = there ? static_cast<uint32_t>(page) * a.p.page_stride + slot * a.p.slot_stride : 0u;
-        unsigned long long left = __ballot(there);
-        if (left == 0) continue;
-        float s = -INFINITY, by = 1.0f;
-        if (there) {
-            const uint8_t* k = kbase + static_cast<int64_t>(row) * 16;
-            s = 0.0f;
-#pragma unroll 1
-            for (int d = 0; d < a.head_dim; ++d) s = fmaf(widen1<BF16>(q[d] ^ static_cast<uint16_t>(a.flip)), value(k, d), s);
-            if constexpr (E8) {
-                const uint32_t scale = a.s.at(page, kvh, slot);
-                s *= a.s.k[scale];
-                by = a.s.v[scale];
-            }
-            s *= a.scale;
-        }
-        float top = fmaxf(s, there ? -FLT_MAX : -INFINITY);
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
-        top = fmaxf(top - bias_of(BF16 || E8), m);  // weights of the sizes that they have elsewhere
-        const float fade = exp2_from(m, top);
-        m = top;
-        const float p = there ? exp2f(s - m) : 0.0f;
-        float sum = p;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off);
-        l = fmaf(l, fade, sum);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] *= fade;
-        for (; left != 0; left &= left - 1) {
-            const int at = __ffsll(left) - 1;
-            const uint8_t* v = vbase + static_cast<int64_t>(__shfl(row, at)) * 16;
-            const float w = __shfl(p, at) * __shfl(by, at);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int d = lane + 64 * i;
-                if (d < a.head_dim) acc[i] = fmaf(w, value(v, d), acc[i]);
-            }
-        }
-    }
-    if (!piece.whole) {
-        const int64_t to = (static_cast<int64_t>(piece.slot) * a.kv_heads + kvh) * (1 << a.columns_log2) + (col - (piece.tile << a.columns_log2));
-        if (lane == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * to) = f32x2{m, l};
-        for (int i = 0; i < 4; ++i)
-            if (lane + 64 * i < a.head_dim) a.part[to * a.head_dim + lane + 64 * i] = acc[i];
-        return;
-    }
-    uint16_t* out = a.out + (static_cast<int64_t>(piece.first + r) * a.heads + kvh * a.group + h) * a.head_dim;
-    for (int i = 0; i < 4; ++i)
-        if (lane + 64 * i < a.head_dim)
-            out[lane + 64 * i] = m == -INFINITY ? static_cast<uint16_t>(0) : narrow1<BF16>(acc[i] * (1.0f / l));
-}
-
 typedef __attribute__((address_space(3))) char lds_char;
 __device__ __forceinline__ u32x4 lds16(const lds_char* base, int at) {
     return *(const __attribute__((address_space(3))) u32x4*)(base + at);
@@ -422,7 +339,9 @@ __device__ __forceinline__ u32x2 lds_transposed(lds_char* base, int at) {
 }
 
 // LDS of a workgroup: kStages tiles of keys and values (and scales), then for each
-// wave the page table's entries of eight tiles.
+// wave the page table's entries of eight tiles, then what has been cleared (see
+// attend): the first position of each head value that is NaN, inf or -inf, and
+// whether there is any.
 template <int DP, bool E8>
 struct Layout {
     static constexpr int kWaves = DP > 128 ? 4 : 8;
@@ -436,9 +355,18 @@ struct Layout {
     static constexpr int kStages = 4;
     static constexpr int kEntries = kStages * kStage;
     static constexpr int kRing = 8;
-    static constexpr int kBytes = kEntries + kWaves * kRing * 256;
+    static constexpr int kCleared = kEntries + kWaves * kRing * 256;
+    static constexpr int kAnyCleared = kCleared + 3 * DP * 4;
+    static constexpr int kBytes = kAnyCleared + 16;
     static_assert(kPositions == 8 * kWaves, "a wave loads eight positions of a tile");
 };
+
+template <int DP, bool E8>
+__device__ __forceinline__ void reset_cleared(lds_char* lds) {
+    using L = Layout<DP, E8>;
+    for (int i = threadIdx.x; i <= 3 * DP; i += 64 * L::kWaves)
+        *(__attribute__((address_space(3))) int*)(lds + L::kCleared + 4 * i) = i < 3 * DP ? 0x7FFFFFFF : 0;
+}
 
 // A piece by a workgroup: waves of 32 columns each over the piece's positions, a
 // tile at a time through LDS.
@@ -471,11 +399,11 @@ struct Layout {
 // their positions' scales in fp32.
 //
 // What a row does not see must not reach it, but a weight of 0 times an infinity or
-// a NaN left there is NaN.  That shows: such an accumulator stays NaN.  So the
-// first pass goes without care, and a wave that ends with a value that is not
-// finite and met positions that not every column sees does its columns again, one at
-// a time (careful_column).  Positions behind the last one seen, or without a page, are
-// never read.
+// a NaN left there is NaN.  So where some column of the workgroup does not see all
+// of a tile, each wave looks at the values that it has loaded of it (32 bytes a lane
+// at a head of 128), clears those that are not finite and notes their first positions;
+// at the end the columns that see one get it: whatever a cache holds, a call takes as
+// long as without it.  Positions behind the last one seen are never read.
 //
 // Bound by the matrix cores' power and by the exponentials between them: two
 // prompts of up to 8191 rows of 28 and 4 heads of 128, 752 GFLOP, in 726 us, 1.03 PFLOP/s
@@ -512,9 +440,10 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
     const int begin = piece.begin, end = piece.end;
     [[maybe_unused]] const bool few = wave_least < kFewPositions;
 
+    typedef __attribute__((address_space(3))) int lds_word;
+    bool cleared = false;
     float m = -INFINITY, l = 0.0f;  // weights are exp2(score - m): m is the maximum less the bias, up to kLate behind
     f32x16 acc[DB];
-    bool masked = false;  // there was a position that some column does not see
 #pragma unroll
     for (int b = 0; b < DB; ++b)
 #pragma unroll
@@ -581,11 +510,16 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
         const int own = 8 * wave + (lane >> 3), piece8 = lane & 7, chunk = piece8 ^ swizzle(own);
         int own_page = 0;
         uint32_t own_slot = 0;
+        const int tiles = (end - begin + KT - 1) / KT;
+        // the first tile that some column does not see all of, or where a position of the wave's has no page or a scale
+        // that is not finite (times which a weight has no two values)
+        int open = max(piece.least - begin, 0) / KT;
         const uint8_t *ksrc = nullptr, *vsrc = nullptr;
         auto find_own = [&](int t) {
             own_slot = slot_of(position(t, own));
             uint32_t row = row_at(own_page, own_slot);
             if (__any(!is_page(own_page))) {
+                open = min(open, t);
                 const uint32_t instead = other_row(t, gone_of(entry(t, lane)));
                 if (!is_page(own_page)) row = instead;
             }
@@ -636,9 +570,59 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
                         *(lds_u32x4*)(to + L::kV + where) = eight_of<true>(from.v[i], x);
                     }
                 }
+            if (__any(from.there && !(fabsf(from.scale) < INFINITY))) open = min(open, t);
             if (piece8 < 2)
                 *(__attribute__((address_space(3))) float*)(to + L::kScales + (piece8 * KT + own) * 4) =
                     from.there ? (piece8 == 0 ? from.scale * a.scale : from.scale) : 0.0f;
+        };
+
+        // The values of the wave's positions of tile t, which have been loaded, from the first open tile on: what is not
+        // finite is cleared and noted (not of a position without a page, which has another one's values).
+        auto clean = [&](int t) {
+            if (t < open || t >= tiles) return;
+            int here = lane;
+            asm volatile("" : "+v"(here));  // (nothing of this is kept in registers over the tiles)
+            lds_char* const tile = lds + (t & (L::kStages - 1)) * L::kStage;
+            const int at = L::kV + wave * 1024 + here * 16, position8 = 8 * wave + (here >> 3);
+            constexpr uint32_t kInf = VBF16 ? 0x7F80u : 0x7C00u;
+            uint32_t high = 0, low = 0;  // largest magnitudes
+#pragma unroll
+            for (int i = 0; i < L::kBlocks; ++i) {
+                const u32x4 piece16 = lds16(tile, at + i * L::kBlock);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    high = max(high, piece16[x] & 0x7FFF0000u);
+                    low = max(low, piece16[x] & 0x7FFFu);
+                }
+            }
+            bool odd = max(high >> 16, low) >= kInf;
+            float scale = 1.0f;
+            __attribute__((address_space(3))) float* const held =
+                (__attribute__((address_space(3))) float*)(tile + L::kScales + (KT + position8) * 4);
+            if constexpr (E8) {
+                scale = *held;
+                odd |= !(fabsf(scale) < INFINITY);
+            }
+            if (!__any(odd)) return;
+            const int pos = static_cast<int>(position(t, position8));
+            const bool there = is_page(entry(t, position8));
+            const int first = 8 * ((here & 7) ^ swizzle(position8));  // head value
+#pragma unroll 1
+            for (int j = 0; j < 8 * L::kBlocks; ++j) {
+                typedef __attribute__((address_space(3))) uint16_t lds_half;
+                lds_half* const one = (lds_half*)(tile + at + j / 8 * L::kBlock + j % 8 * 2);
+                const float value = widen1<VBF16>(*one);
+                if (fabsf(value) < INFINITY && fabsf(scale) < INFINITY) continue;
+                *one = 0;
+                const float seen = value * scale;
+                const int kind = seen != seen ? 0 : seen > 0.0f ? 1 : 2;
+                if (there)
+                    __hip_atomic_fetch_min((lds_word*)(lds + L::kCleared + (kind * DP + first + j / 8 * 64 + j % 8) * 4), pos,
+                                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            }
+            if constexpr (E8)
+                if (!(fabsf(scale) < INFINITY)) *held = 0.0f;
+            if (lane == 0) *(lds_word*)(lds + L::kAnyCleared) = 1;
         };
 
         f32x16 s[KB];
@@ -719,7 +703,6 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
         auto weigh = [&](int t) {
             const int t0 = begin + KT * t;
             const unsigned long long gone = gone_of(tile_page);
-            masked |= t0 + KT > piece.least || gone != 0;
             if (t0 >= wave_seen || gone == (KT == 64 ? ~0ull : 0xFFFFFFFFull)) return false;
             const lds_char* const tile = lds + (t & (L::kStages - 1)) * L::kStage;
             // scales of this lane's positions, each kind read at once (as the compiler orders them each is waited for)
@@ -835,21 +818,14 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
             }
             return true;
         };
-        // until this wave's loads but the last step's are there (the first waves after their weights, the second
-        // after their products), and every wave is here
-        auto step_end = [&](bool wait) {
-            if constexpr (E8) {
-                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            } else {
-                if (wait)
-                    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kOutstanding) : "memory");
-                else
-                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                asm volatile("s_barrier" ::: "memory");
-            }
+        // This wave's loads but the last step's are there, of tile t the last ones (16-bit caches: the first waves after
+        // their weights, the second after their products).
+        auto landed = [&](int t) {
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kOutstanding) : "memory");
+            clean(t);
         };
+        auto step_end = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
 
-        const int tiles = (end - begin + KT - 1) / KT;
 #pragma unroll 1
         for (int t = 0; t < 5; ++t) load_entries(t);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -872,40 +848,41 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
                 for (int i = 0; i < L::kBlocks; ++i) load_block(t, i);
             }
         }
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        for (int t = 0; t < 3; ++t) clean(t);
+        step_end();
         if (second) asm volatile("s_barrier" ::: "memory");
         scores(-1, std::false_type{});
-        step_end(false);
+        step_end();
         for (int t = 0; t < tiles; ++t) {
             const bool live = weigh(t);
-            step_end(!second);
+            if constexpr (!E8)
+                if (!second) landed(t + 1);
+            step_end();
             __builtin_amdgcn_s_setprio(1);
             scores(t, std::true_type{});
             if (live) values(t);
             __builtin_amdgcn_s_setprio(0);
-            step_end(second);
+            if constexpr (E8)
+                clean(t + 3);
+            else if (second)
+                landed(t + 2);
+            step_end();
         }
         if (!second) asm volatile("s_barrier" ::: "memory");
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what was loaded past the end
+        cleared = __builtin_amdgcn_readfirstlane(*(lds_int*)(lds + L::kAnyCleared)) != 0;
     }
     l = both_sum(l);
-
-    if (masked) {
-        float odd = 0.0f;  // 0 times what is not finite is NaN
-#pragma unroll
-        for (int b = 0; b < DB; ++b)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) odd = fmaf(acc[b][j], 0.0f, odd);
-        if (__any(odd != odd)) {
-            const int most = min(wave0 + 32, columns);
-            for (int c = wave0; c < most; ++c) careful_column<BF16, E8>(a, piece, kvh, c, lane);
-            return;
-        }
-    }
-    if (col >= columns) return;
-    if (!piece.whole) {
-        const int64_t to =
-            (static_cast<int64_t>(piece.slot) * a.kv_heads + kvh) * L::kColumns + (col - piece.tile * L::kColumns);
+    // where column c's results go: a partial's, or the output's
+    auto partial_of = [&](int c) {
+        return (static_cast<int64_t>(piece.slot) * a.kv_heads + kvh) * L::kColumns + (c - piece.tile * L::kColumns);
+    };
+    auto output_of = [&](int c, int r) {
+        return a.out + (static_cast<int64_t>(piece.first + r) * a.heads + kvh * a.group + c - r * a.group) * a.head_dim + 4 * half;
+    };
+    if (col < columns && !piece.whole) {
+        const int64_t to = partial_of(col);
         if (half == 0) *reinterpret_cast<f32x2*>(a.part_ml + 2 * to) = f32x2{m, l};
         float* const at = a.part + to * a.head_dim + 4 * half;
 #pragma unroll
@@ -915,19 +892,40 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
                 if (32 * b + 2 * j < a.head_dim)
                     *reinterpret_cast<f32x4*>(at + 32 * b + 2 * j) =
                         f32x4{acc[b][j], acc[b][j + 1], acc[b][j + 2], acc[b][j + 3]};
-        return;
+    } else if (col < columns) {
+        // a row that sees nothing is zero
+        const float inv = m == -INFINITY ? 0.0f : __builtin_amdgcn_rcpf(l);  // (the accumulators are 0 there too)
+        uint16_t* const to = output_of(col, a.by_group(col));
+#pragma unroll
+        for (int b = 0; b < DB; ++b)
+#pragma unroll
+            for (int j = 0; j < 16; j += 4)
+                if (32 * b + 2 * j < a.head_dim)
+                    *reinterpret_cast<u32x2*>(to + 32 * b + 2 * j) = u32x2{
+                        pack2<BF16>(acc[b][j] * inv, acc[b][j + 1] * inv), pack2<BF16>(acc[b][j + 2] * inv, acc[b][j + 3] * inv)};
     }
-    // a row that sees nothing is zero
-    const int r = a.by_group(col), h = col - r * a.group;
-    const float inv = m == -INFINITY ? 0.0f : __builtin_amdgcn_rcpf(l);  // (the accumulators are 0 there too)
-    uint16_t* const to = a.out + (static_cast<int64_t>(piece.first + r) * a.heads + kvh * a.group + h) * a.head_dim + 4 * half;
-#pragma unroll
-    for (int b = 0; b < DB; ++b)
-#pragma unroll
-        for (int j = 0; j < 16; j += 4)
-            if (32 * b + 2 * j < a.head_dim)
-                *reinterpret_cast<u32x2*>(to + 32 * b + 2 * j) =
-                    u32x2{pack2<BF16>(acc[b][j] * inv, acc[b][j + 1] * inv), pack2<BF16>(acc[b][j + 2] * inv, acc[b][j + 3] * inv)};
+    if (cleared) {
+        // what has been cleared, to the results of the columns that see it
+        int c = col;
+        asm volatile("" : "+v"(c));  // (nothing of this is kept in registers over the rest)
+        const int r = a.by_group(min(c, columns - 1));
+        const int limit = c < columns ? seen_by(a, piece.length, r) : 0;
+        float* const part = a.part + partial_of(c) * a.head_dim + 4 * half;
+        uint16_t* const out = output_of(c, r);
+#pragma unroll 1
+        for (int d = 0; d < a.head_dim - 4 * half; ++d) {
+            if (d % 8 >= 4) continue;  // the other half's
+            auto sees = [&](int kind) { return limit > *(lds_int*)(lds + L::kCleared + (kind * DP + d + 4 * half) * 4); };
+            const float add = (sees(0) ? NAN : 0.0f) + (sees(1) ? INFINITY : 0.0f) + (sees(2) ? -INFINITY : 0.0f);
+            if (add == 0.0f) continue;
+            if (piece.whole)
+                out[d] = narrow1<BF16>(widen1<BF16>(out[d]) + add);
+            else
+                part[d] += add;
+        }
+        __syncthreads();  // that has been read
+        reset_cleared<DP, E8>(lds);
+    }
 }
 
 // Workgroup -> (tile or run, key-value head).
@@ -943,6 +941,7 @@ __global__ __launch_bounds__(DP > 128 ? 256 : 512, 1) void paged_chunk_kernel(co
     if (a.head_dim != DP)  // the loads leave out what is behind a head's end
         for (int i = threadIdx.x; i < L::kStages * L::kStage / 16; i += 64 * L::kWaves)
             *(__attribute__((address_space(3))) u32x4*)(lds + 16 * i) = u32x4{0, 0, 0, 0};
+    reset_cleared<DP, E8>(lds);
     Border border[2];  // of the run: where it goes on, where it ends
     const Dealt dealt = a.plan == nullptr ? kTiles : find_run(a, at, lane, border);
     if (dealt == kNone) return;

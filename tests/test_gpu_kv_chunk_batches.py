@@ -2,14 +2,19 @@
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
+import batched_refs as ref
 import paged_refs as pref
 
 pytestmark = pytest.mark.gpu
 
 BF16, F16, E4M3 = torch.bfloat16, torch.float16, torch.float8_e4m3fn
+# how far off the weights over e4m3 pages are: rounded to bf16; of fp16 rows the upper 8 bits, and their rest rounded
+E4M3_WEIGHT = {BF16: ref.HALF[BF16], F16: 2.0 ** -7 * ref.HALF[BF16]}
 
 
 @pytest.fixture(scope="module")
@@ -75,3 +80,90 @@ def test_values_at_the_end_of_bf16(nat, e4m3, length, rows):
     want, bound = pref.chunk(q, *caches, table, [length], [0, rows], 1.0, scales=scales)
     assert bool(want.isfinite().all())
     pref.agree(got, want, bound)
+
+
+def milliseconds(call, times=5):
+    """The shortest of a few calls."""
+    call()
+    best = math.inf
+    for _ in range(times):
+        begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        begin.record()
+        call()
+        end.record()
+        end.synchronize()
+        best = min(best, begin.elapsed_time(end))
+    return best
+
+
+@pytest.mark.parametrize("dtype,e4m3", [(BF16, False), (F16, False), (BF16, True), (F16, True)])
+@pytest.mark.parametrize("heads,kvh,dim", [(14, 2, 128), (8, 8, 64), (4, 2, 256)])
+@pytest.mark.parametrize("what", ["value", "key", "query", "hidden"])
+def test_a_nan_that_rows_see(nat, dtype, e4m3, heads, kvh, dim, what):
+    """A prompt whose first position holds a NaN (or an infinity in fp16 values), one NaN query row, and a NaN of the last
+    position: the right rows get it, and the call takes no more than a few times as long as without."""
+    rows, page = 1400, 16
+    caches, scales, table = pref.make_pages([rows], page, kvh, dim, E4M3 if e4m3 else dtype, 5)
+    q = randn((rows, heads, dim), dtype, 6)
+
+    def call():
+        return attend(nat, q, caches, scales, table, [0], [0, rows])
+
+    usual = milliseconds(call)
+    first, last = (int(table[0, 0]), 0), (int(table[0, (rows - 1) // page]), (rows - 1) % page)
+    if what == "query":
+        q[700, 1, 3] = float("nan")
+    else:
+        cache = caches[0] if what == "key" else caches[1]
+        value = float("inf") if dtype == F16 and what == "value" else float("nan")
+        if e4m3:
+            cache.view(torch.uint8)[(*(last if what == "hidden" else first), slice(None), 5)] = 0x7F
+        else:
+            cache[(*(last if what == "hidden" else first), slice(None), 5)] = value
+    poisoned = milliseconds(call)
+    got = call()
+    want, bound = pref.chunk(q, *caches, table, [0], [0, rows], dim ** -0.5, scales=scales,
+                             weight=E4M3_WEIGHT[dtype] if e4m3 else None)
+    pref.agree(got, want, bound)
+    assert poisoned < 10 * usual + 0.2, (poisoned, usual)
+
+
+@pytest.mark.parametrize("dtype,e4m3", [(BF16, False), (F16, False), (BF16, True), (F16, True)])
+@pytest.mark.parametrize("heads,kvh,dim", [(14, 2, 128), (4, 4, 64), (2, 1, 248), (2, 1, 176)])
+@pytest.mark.parametrize("length,rows", [(0, 90), (3000, 70), (130, 1200)])
+def test_infinities_of_both_signs(nat, dtype, e4m3, heads, kvh, dim, length, rows):
+    """One that every row sees, then two of the other sign in the same and in another head value, then a NaN, that later
+    rows see; pages that are not there between them, for which rows that hold such values may be read."""
+    page = 16
+    if e4m3:
+        dim -= dim % 16
+    caches, scales, table = pref.make_pages([length + rows], page, kvh, dim, E4M3 if e4m3 else dtype, 9, dirt=float("nan"))
+
+    def put(pos, at, value):
+        where = (int(table[0, pos // page]), pos % page)
+        if not e4m3:
+            caches[1][(*where, slice(None), at)] = value
+            return
+        # a scale of infinity, whose sign is its byte's (and NaN where that is 0): head values of the other sign take one too
+        raw = caches[1].view(torch.uint8)
+        if math.isnan(value):
+            raw[(*where, slice(None), at)] = 0x7F
+            return
+        raw[where] = 0x38 if value > 0 else 0xB8
+        scales[1][where[0], :, where[1]] = math.inf
+
+    put(0, 5, math.inf)
+    put(length + rows // 3, 7, -math.inf)
+    put(length + rows // 2, 5, -math.inf)
+    put(length + rows - 2, dim - 1, math.nan)
+    for pos in (32, length + rows // 4):
+        if pos // page not in (0, (length + rows // 3) // page):
+            table[0, pos // page] = -7
+    q = randn((rows, heads, dim), dtype, 10)
+    got = attend(nat, q, caches, scales, table, [length], [0, rows])
+    want, bound = pref.chunk(q, *caches, table, [length], [0, rows], dim ** -0.5, scales=scales,
+                             weight=E4M3_WEIGHT[dtype] if e4m3 else None)
+    pref.agree(got, want, bound)
+    assert bool(want[0, :, 5].isinf().all()) and bool(want[-1, :, dim - 1].isnan().all())
+    if int(table[0, (length + rows // 2) // page]) >= 0:
+        assert bool(want[-1, :, 5].isnan().all())
