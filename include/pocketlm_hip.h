@@ -941,8 +941,8 @@ int kv_paged_attention_decode_e4m3(const uint16_t* q, const uint8_t* k_cache, co
  * sees nothing; positions without a page are left out, those past the table
  * too.  What a row does not see never reaches it, NaN or not.  Softmax weights
  * are rounded once to the cache's type; over an e4m3 cache, times the values'
- * scales, to bf16, for fp16 rows and those that see few positions to the sum of
- * two bf16 values.  scratch: device
+ * scales, to bf16, for fp16 rows, those that see few positions and weights that
+ * are much of their row's sum to the sum of two bf16 values.  scratch: device
  * memory of kv_paged_attention_chunk_scratch_bytes, 16-byte aligned, or NULL
  * for the library's own; capacity is table_cols * page_size.  rows * heads <
  * 2^31.  Codes -1 null, -2 bad dimensions, -3 scratch. */

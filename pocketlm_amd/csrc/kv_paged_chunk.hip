@@ -26,7 +26,8 @@ constexpr int kTile = 64;  // positions that work is counted in
 // A running maximum is only moved once a score is more than 2^kLate above it: weights grow to 2^kLate, the
 // accumulators are multiplied in a few tiles instead of all.
 constexpr float kLate = 8.0f;
-constexpr int kFewPositions = 512;  // see attend
+constexpr int kFewPositions = 512;    // see attend
+constexpr float kMuch = 1.0f / 3.0f;
 // So bf16 weights are kept times 2^-kLate, which ends them at 1: their sum with values at the end of the range
 // leaves fp32 no sooner than the decode kernel's.  fp16 weights are kept times 2^7, so that they end at 2^15 and
 // begin at 2^-31.
@@ -381,9 +382,14 @@ __device__ __forceinline__ void reset_cleared(lds_char* lds) {
 // multiplied by their values' scales, need bf16's range and are not summed as
 // they were rounded: so they go in as two values, the second the rest, for fp16
 // rows (results within 2.1e-4 of their size, 1.7e-3 with one value, 1.26 ms and
-// 0.99 for 2048 rows behind 30000 positions), and for bf16 rows that see few
-// positions, where one weight's rounding is the whole result's (a first prompt's
-// rows were off by up to 2.1 times the output's rounding, later ones by 1.4).
+// 0.99 for 2048 rows behind 30000 positions), and for bf16 rows where one weight's
+// rounding may be most of the result's: in tiles with a weight of more than kMuch of
+// its column's sum so far, and all of those of rows that see few positions (a
+// first prompt's rows were off by up to 2.1 times the output's rounding).  Rows of
+// 8000 positions whose scores spread by 2 and 4 were off by 1.4 times the output's
+// rounding, up to 1.7, and are by 1.02 and 1.00; evenly spread ones, of whose many weights
+// each is rounded, by 1.4 (kMuch of 1/8 1.25, but tiles of a call's first positions
+// exceed it: six turns of 24 rows behind 5000 50 us instead of 46, 46 with 1/3).
 //
 // Each wave alternates between the matrix cores (the scores of tile i + 1, then the
 // values of tile i) and the vector units (the weights of tile i + 1); the second four
@@ -745,7 +751,8 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
             float top = s[0][0];
 #pragma unroll
             for (int j = 1; j < 16 * KB; ++j) top = fmaxf(top, s[j >> 4][j & 15]);
-            top = fmaxf(m, both_max(fmaxf(top * times, floor)) - kBias);
+            const float best = both_max(fmaxf(top * times, floor));
+            top = fmaxf(m, best - kBias);
             if (!E8 && __any(fabsf(top) > 0x1p22f && top > -0x1p127f)) {
                 times = 1.0f;
 #pragma unroll
@@ -795,7 +802,7 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             if constexpr (E8 && BF16) {
                 // what the rounding left, formed again: its products at once
-                if (few) {
+                if (few || __any(__builtin_amdgcn_exp2f(best - from) > kMuch * both_sum(l))) {
 #pragma unroll
                     for (int x = 0; x < 2 * KB; ++x) {
                         u32x4 left;

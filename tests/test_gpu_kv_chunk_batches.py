@@ -167,3 +167,56 @@ def test_infinities_of_both_signs(nat, dtype, e4m3, heads, kvh, dim, length, row
     assert bool(want[0, :, 5].isinf().all()) and bool(want[-1, :, dim - 1].isnan().all())
     if int(table[0, (length + rows // 2) // page]) >= 0:
         assert bool(want[-1, :, 5].isnan().all())
+
+
+@pytest.mark.parametrize("heads,kvh,dim", [(28, 4, 128), (4, 2, 64), (3, 1, 256), (2, 2, 192)])
+@pytest.mark.parametrize("length,rows,place", [(5000, 3, 0), (5000, 3, 2900), (5000, 40, 4999), (1500, 1500, 700), (20000, 130, 12345)])
+def test_weight_on_one_of_many_e4m3_positions(nat, heads, kvh, dim, length, rows, place):
+    """A row whose weight lies on one position gets that position's value, rounded once: the weight's own rounding does
+    not show, however many positions there are.
+
+    The position's score is 24 above the others' bound of 3, so theirs are shares of exp(-21) each, 21500 of them
+    2^-15.9 in all; rounded to bf16, 2^-8 of that, of the largest value.  Its own weight has 15 bits."""
+    page = 64
+    caches, scales, table = pref.make_pages([length + rows], page, kvh, dim, E4M3, 7)
+    k = caches[0].view(torch.uint8)
+    g = torch.Generator().manual_seed(8)
+    # scores: head value 0 of every key at most 3 in size (the others 0), of the chosen one 24
+    k.zero_()
+    low = (torch.rand(k.shape[:3], generator=g) * 6 - 3).to(E4M3)
+    k[..., 0] = low.view(torch.uint8).cuda()
+    k[int(table[0, place // page]), place % page, :, 0] = torch.tensor(24.0).to(E4M3).view(torch.uint8).cuda()
+    scales[0].fill_(1.0)
+    q = torch.zeros((rows, heads, dim), dtype=BF16, device="cuda")
+    q[:, :, 0] = (1.0 + 0.25 * torch.rand((rows, heads), generator=g)).to(BF16).cuda()
+    got = attend(nat, q, caches, scales, table, [length], [0, rows], softmax_scale=1.0)
+    want, bound = pref.chunk(q, *caches, table, [length], [0, rows], 1.0, scales=scales, weight=2.0 ** -15)
+    rest = 2.0 ** -8 * (length + rows) * math.exp(-21.0) * 448.0 * float(scales[1].max())
+    # the output's own rounding: half a step at its size, not the most that is of any size
+    half = torch.exp2(torch.floor(torch.log2(want.abs() * (1 + 2.0 ** -9) + rest)) - 8)
+    pref.agree(got, want, bound + rest - ref.HALF[BF16] * want.abs() + half)
+
+
+@pytest.mark.parametrize("heads,kvh,dim", [(28, 4, 128), (4, 2, 64), (3, 1, 256)])
+@pytest.mark.parametrize("length,rows", [(6000, 40), (2500, 500)])
+def test_weight_on_a_few_of_many_e4m3_positions(nat, heads, kvh, dim, length, rows):
+    """Rows of which two positions, far apart, have a half of the weight each, and their values cancel but for a part.
+
+    Both are in tiles of weights of two values: 15 bits of each, beside 2^-8 of the others, 2 * 6040 exp(-21) at most."""
+    page = 32
+    caches, scales, table = pref.make_pages([length + rows], page, kvh, dim, E4M3, 11)
+    k, v = (c.view(torch.uint8) for c in caches)
+    g = torch.Generator().manual_seed(12)
+    k.zero_()
+    k[..., 0] = (torch.rand(k.shape[:3], generator=g) * 6 - 3).to(E4M3).view(torch.uint8).cuda()
+    pair = [(int(table[0, p // page]), p % page) for p in (length // 3, length - 5)]
+    for where in pair:
+        k[where[0], where[1], :, 0] = torch.tensor(24.0).to(E4M3).view(torch.uint8).cuda()
+    v[pair[1]] = v[pair[0]] ^ 0x80  # times its own scale, of up to 9 / 4 of the other
+    scales[0].fill_(1.0)
+    q = torch.zeros((rows, heads, dim), dtype=BF16, device="cuda")
+    q[:, :, 0] = (1.0 + 0.25 * torch.rand((rows, heads), generator=g)).to(BF16).cuda()
+    got = attend(nat, q, caches, scales, table, [length], [0, rows], softmax_scale=1.0)
+    want, bound = pref.chunk(q, *caches, table, [length], [0, rows], 1.0, scales=scales, weight=2.0 ** -15)
+    rest = 2.0 ** -8 * 2 * (length + rows) * math.exp(-21.0) * 448.0 * float(scales[1].max())
+    pref.agree(got, want, bound + rest)
