@@ -52,6 +52,9 @@ struct ChunkArgs {
     float* part;           // [slot][kv head][column of a tile][head_dim], then the maxima and sums
     float* part_ml;
     int* plan;             // {the run that begins it, the one that ends it} of each tile; null: no tile is split
+    struct Found* found;   // of each run, by a kernel of its own; null: each workgroup finds its run
+    int* begun;            // with found: the tile that each run begins and does not end, or -1
+    int tiles;             // of a head, at most
     int64_t q_row, q_head; // strides, values
     int64_t capacity;      // positions of a table row
     int rows;
@@ -205,11 +208,61 @@ struct Border {
     float share;
 };
 
+// The border at work x of a block of 64 places, which begins at work `before`; each lane has a place's work and
+// `upto`, the work up to its end, lane l the first place that ends past x.
+__device__ __forceinline__ Border border_in(const Work& w, uint32_t total, uint32_t upto, uint32_t x, int base, int l) {
+    Work of;
+    of.tiles = __builtin_amdgcn_readlane(w.tiles, l);
+    of.first = __builtin_amdgcn_readlane(w.first, l);
+    of.last = __builtin_amdgcn_readlane(w.last, l);
+    const uint32_t size = __builtin_amdgcn_readlane(total, l);
+    const uint32_t in = x - (__builtin_amdgcn_readlane(upto, l) - size);
+    const float z = static_cast<float>(in) * __builtin_amdgcn_rcpf(static_cast<float>(size)) * of.before(of.tiles);
+    int lo = 0, hi = of.tiles;
+#pragma unroll 1
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        (of.before(mid) <= z ? lo : hi) = mid;
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    const float from = of.before(lo);
+    const float share = in == 0 ? 0.0f : (z - from) * __builtin_amdgcn_rcpf(of.before(lo + 1) - from);
+    return Border{base + l, lo, share};
+}
+
 // What workgroup `run` of a head does: kRun and its borders, kTiles (tile `run`, whole) or kNone.  Every lane calls
 // it.
 // (Kept short, as all that a call does once: a small call waits for its
 // instructions.)
 enum Dealt { kNone, kTiles, kRun };
+
+// Of the work of all places: the runs, whether they take whole tiles instead, and the work before run r.
+struct Deal {
+    uint32_t all, runs;
+    float per_run;
+    bool whole;
+
+    __device__ __forceinline__ Deal(const ChunkArgs& a, uint32_t work, uint32_t longest, uint32_t tiles) : all(work) {
+        runs = min(static_cast<uint32_t>(a.runs), max(1u, all / kLeastWork));
+        // (what is only about right is the same for both runs of a border)
+        const float each = __builtin_amdgcn_rcpf(static_cast<float>(runs));
+        per_run = static_cast<float>(all) * each;
+        const float filled = static_cast<float>(a.rows) * static_cast<float>(a.group) *
+                             __builtin_amdgcn_rcpf(static_cast<float>(tiles << a.columns_log2));
+        const float share = __builtin_amdgcn_rcpf(static_cast<float>(a.runs));
+        const float scale = static_cast<float>(1u << a.work_shift);
+        const float in_runs = per_run * scale + kStart * static_cast<float>(tiles) * each + kJoin +
+                              kJoinRuns * static_cast<float>(runs) * share * filled;
+        float in_tiles = static_cast<float>(longest);
+        if (tiles > static_cast<uint32_t>(a.runs))
+            in_tiles = fmaxf(in_tiles, static_cast<float>(all) * share * scale + in_tiles * 0.2f);
+        whole = in_tiles <= in_runs;
+    }
+    __device__ __forceinline__ uint32_t border_at(uint32_t r) const {
+        return r == runs ? all : static_cast<uint32_t>(static_cast<float>(r) * per_run);
+    }
+};
+
 __device__ __forceinline__ Dealt find_run(const ChunkArgs& a, int run, int lane, Border (&border)[2]) {
     const int places = a.p.sequences + 2;
     uint32_t all = 0, longest = 0, tiles = 0;
@@ -223,19 +276,9 @@ __device__ __forceinline__ Dealt find_run(const ChunkArgs& a, int run, int lane,
     all = __builtin_amdgcn_readlane(wave_prefix(all), 63);
     longest = wave_max(longest);
     tiles = __builtin_amdgcn_readlane(wave_prefix(tiles), 63);
-    const uint32_t runs = min(static_cast<uint32_t>(a.runs), max(1u, all / kLeastWork));
-    // (what is only about right is the same for both runs of a border)
-    const float each = __builtin_amdgcn_rcpf(static_cast<float>(runs)), per_run = static_cast<float>(all) * each;
-    const float filled = static_cast<float>(a.rows) * static_cast<float>(a.group) *
-                         __builtin_amdgcn_rcpf(static_cast<float>(tiles << a.columns_log2));
-    const float share = __builtin_amdgcn_rcpf(static_cast<float>(a.runs)), scale = static_cast<float>(1u << a.work_shift);
-    const float in_runs = per_run * scale + kStart * static_cast<float>(tiles) * each + kJoin +
-                          kJoinRuns * static_cast<float>(runs) * share * filled;
-    float whole = static_cast<float>(longest);
-    if (tiles > static_cast<uint32_t>(a.runs)) whole = fmaxf(whole, static_cast<float>(all) * share * scale + whole * 0.2f);
-    if (whole <= in_runs) return kTiles;
-    if (static_cast<uint32_t>(run) >= runs) return kNone;
-    auto border_at = [&](uint32_t r) { return r == runs ? all : static_cast<uint32_t>(static_cast<float>(r) * per_run); };
+    const Deal deal(a, all, longest, tiles);
+    if (deal.whole) return kTiles;
+    if (static_cast<uint32_t>(run) >= deal.runs) return kNone;
     border[0].place = border[1].place = places;
     border[0].tile = border[1].tile = 0;
     border[0].share = border[1].share = 0.0f;
@@ -246,33 +289,81 @@ __device__ __forceinline__ Dealt find_run(const ChunkArgs& a, int run, int lane,
         const uint32_t total = w.total(a.work_shift), upto = before + wave_prefix(total);
 #pragma unroll 1
         for (int k = 0; k < 2; ++k) {
-            const uint32_t x = border_at(static_cast<uint32_t>(run + k));
+            const uint32_t x = deal.border_at(static_cast<uint32_t>(run + k));
             const unsigned long long past = __ballot(upto > x);
             if (past == 0 || (k == 0 && border[0].place < places)) continue;
-            const int l = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
-            Work of;
-            of.tiles = __builtin_amdgcn_readlane(w.tiles, l);
-            of.first = __builtin_amdgcn_readlane(w.first, l);
-            of.last = __builtin_amdgcn_readlane(w.last, l);
-            const uint32_t size = __builtin_amdgcn_readlane(total, l);
-            const uint32_t in = x - (__builtin_amdgcn_readlane(upto, l) - size);
-            const float z = static_cast<float>(in) * __builtin_amdgcn_rcpf(static_cast<float>(size)) * of.before(of.tiles);
-            int lo = 0, hi = of.tiles;
-#pragma unroll 1
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) / 2;
-                (of.before(mid) <= z ? lo : hi) = mid;
-            }
-            lo = __builtin_amdgcn_readfirstlane(lo);
-            const float from = of.before(lo);
-            const float share = in == 0 ? 0.0f : (z - from) * __builtin_amdgcn_rcpf(of.before(lo + 1) - from);
-            const Border found = {base + l, lo, share};
+            const Border found = border_in(w, total, upto, x, base, __builtin_amdgcn_readfirstlane(__ffsll(past) - 1));
             if (k == 0) border[0] = found;
             if (k == 1) border[1] = found;
         }
         before = __builtin_amdgcn_readlane(upto, 63);
     }
     return kRun;
+}
+
+// The same in a kernel of its own, a workgroup for each run, for calls of many sequences: each workgroup of the
+// attention would read all their lengths.  The waves share the places out, blocks of 64 whose work is kept in
+// LDS.  (us where calls of more than 256 sequences were never split, and now: 512 of 200 positions but one of 100000
+// 1986 and 170, 512 of up to 2000 262 and 277; two launches more, 9 and 5 us.)
+constexpr int kFewSequences = 256;  // that each workgroup reads itself
+constexpr int kFindThreads = 1024;
+struct Found {
+    int dealt;
+    Border border[2];
+};
+__global__ __launch_bounds__(kFindThreads) void paged_chunk_find_kernel(const ChunkArgs a) {
+    constexpr int kBlocks = (65535 + 2 + 63) / 64;  // of places, at most
+    __shared__ uint32_t block_work[kBlocks + 63];
+    __shared__ uint32_t sums[kFindThreads / 64][2];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int places = a.p.sequences + 2, blocks = (places + 63) / 64, run = blockIdx.x;
+    uint32_t longest = 0, tiles = 0;
+    for (int b = wave; b < blocks; b += kFindThreads / 64) {
+        const Work w = work_of(a, 64 * b + lane);
+        const uint32_t work = wave_prefix(w.total(a.work_shift));
+        if (lane == 63) block_work[b] = work;
+        longest = max(longest, w.last);
+        tiles += w.tiles;
+    }
+    longest = wave_max(longest);
+    tiles = __builtin_amdgcn_readlane(wave_prefix(tiles), 63);
+    if (lane == 0) sums[wave][0] = longest, sums[wave][1] = tiles;
+    __syncthreads();
+    if (wave > 0) return;
+    uint32_t all = 0;
+    for (int b = 0; b < blocks; b += 64) all += b + lane < blocks ? block_work[b + lane] : 0;
+    all = __builtin_amdgcn_readlane(wave_prefix(all), 63);
+    longest = wave_max(lane < kFindThreads / 64 ? sums[lane][0] : 0);
+    tiles = __builtin_amdgcn_readlane(wave_prefix(lane < kFindThreads / 64 ? sums[lane][1] : 0), 63);
+    const Deal deal(a, all, longest, tiles);
+    Found found = {deal.whole ? kTiles : static_cast<uint32_t>(run) < deal.runs ? kRun : kNone,
+                   {Border{places, 0, 0.0f}, Border{places, 0, 0.0f}}};
+    if (found.dealt == kRun)
+#pragma unroll 1
+        for (int k = 0; k < 2; ++k) {
+            const uint32_t x = deal.border_at(static_cast<uint32_t>(run + k));
+            uint32_t before = 0;
+            int block = -1;
+            for (int b = 0; b < blocks && block < 0; b += 64) {
+                const uint32_t work = b + lane < blocks ? block_work[b + lane] : 0;
+                const uint32_t upto = before + wave_prefix(work);
+                const unsigned long long past = __ballot(upto > x);
+                const int l = past == 0 ? 63 : __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
+                if (past != 0) block = b + l;
+                before = __builtin_amdgcn_readlane(upto, l) - (past == 0 ? 0 : __builtin_amdgcn_readlane(work, l));
+            }
+            if (block < 0) continue;  // the end
+            const Work w = work_of(a, 64 * block + lane);
+            const uint32_t total = w.total(a.work_shift), upto = before + wave_prefix(total);
+            const unsigned long long past = __ballot(upto > x);
+            if (past == 0) continue;  // (lengths changed under the kernel)
+            found.border[k] =
+                border_in(w, total, upto, x, 64 * block, __builtin_amdgcn_readfirstlane(__ffsll(past) - 1));
+        }
+    if (lane == 0) {
+        a.found[run] = found;
+        a.begun[run] = -1;
+    }
 }
 
 // Workgroup -> (tile or run, head).  They are dealt to the 8 XCDs in turn: a
@@ -950,7 +1041,19 @@ __global__ __launch_bounds__(DP > 128 ? 256 : 512, 1) void paged_chunk_kernel(co
             *(__attribute__((address_space(3))) u32x4*)(lds + 16 * i) = u32x4{0, 0, 0, 0};
     reset_cleared<DP, E8>(lds);
     Border border[2];  // of the run: where it goes on, where it ends
-    const Dealt dealt = a.plan == nullptr ? kTiles : find_run(a, at, lane, border);
+    Dealt dealt = kTiles;
+    if (a.found != nullptr) {
+        auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+        const Found found = a.found[min(at, a.runs - 1)];
+        dealt = static_cast<Dealt>(uniform(found.dealt));
+        if (dealt == kRun && at >= a.runs) dealt = kNone;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            border[k] = Border{uniform(found.border[k].place), uniform(found.border[k].tile),
+                               __int_as_float(uniform(__float_as_int(found.border[k].share)))};
+    } else if (a.plan != nullptr) {
+        dealt = find_run(a, at, lane, border);
+    }
     if (dealt == kNone) return;
     if (dealt == kTiles) {
         int first;
@@ -984,6 +1087,7 @@ __global__ __launch_bounds__(DP > 128 ? 256 : 512, 1) void paged_chunk_kernel(co
                 int* const noted = a.plan + 2 * (first_tile_of(a, place) + tile);
                 if (from == 0) noted[0] = at;
                 if (to == units) noted[1] = at;
+                if (a.begun != nullptr && from == 0 && to < units) a.begun[at] = first_tile_of(a, place) + tile;
             }
             piece.whole = from == 0 && to == units;
             piece.slot = 2 * at + (from == 0 ? 1 : 0);
@@ -996,7 +1100,9 @@ __global__ __launch_bounds__(DP > 128 ? 256 : 512, 1) void paged_chunk_kernel(co
     }
 }
 
-// Joins the partials of the tiles that several runs hold.  GROUPS of 16 lanes for a
+// Joins the partials of the tiles that several runs hold: of each tile, or with many
+// sequences of the one that each run begins and does not end (2048 sequences have
+// 530000 workgroups of tiles, which take 114 us to do nothing).  GROUPS of 16 lanes for a
 // column: a lane takes four head values of every GROUPS-th partial.  One group
 // where partials are few, a wave's four where they are many (64 partials of 112
 // columns of 4 heads: 50 us with one, 16 with four; 4 partials of 10500 columns 13
@@ -1075,14 +1181,19 @@ __device__ __forceinline__ void join_column(const ChunkArgs& a, int run, int par
 template <bool BF16>
 __global__ __launch_bounds__(kJoinThreads) void paged_chunk_join_kernel(const ChunkArgs a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int at = blockIdx.x;
+    if (a.begun != nullptr) {
+        at = a.begun[at];
+        if (at < 0 || at >= a.tiles) return;
+    }
     // (within the runs also where the lengths were changed under the first kernel)
-    const int run = max(a.plan[2 * blockIdx.x], 0);
-    const int parts = min(a.plan[2 * blockIdx.x + 1], a.runs - 1) - run + 1;
+    const int run = max(a.plan[2 * at], 0);
+    const int parts = min(a.plan[2 * at + 1], a.runs - 1) - run + 1;
     if (parts <= 1) return;
     int begin;
-    const int place = place_of_tile(a, blockIdx.x, lane, begin);
+    const int place = place_of_tile(a, at, lane, begin);
     const int first = start_of(a, place), rows = rows_of(a, place);
-    const int tile = blockIdx.x - begin;
+    const int tile = at - begin;
     if (tile < 0 || tile >= column_tiles(a, rows)) return;  // (below 0 where row starts do not ascend)
     const int col0 = tile << a.columns_log2, columns = rows * a.group;
     if (parts > kFewPartials) {
@@ -1107,7 +1218,6 @@ struct ChunkShape {
     size_t bytes;
 };
 
-constexpr int64_t kMostSplitSequences = 256;  // every workgroup reads all their lengths
 constexpr int64_t kFewTiles = 4;              // for each workgroup that the device holds
 
 ChunkShape shape_of(int64_t sequences, int64_t rows, int64_t heads, int64_t kv_heads, int64_t head_dim,
@@ -1117,7 +1227,7 @@ ChunkShape shape_of(int64_t sequences, int64_t rows, int64_t heads, int64_t kv_h
     const int64_t resident = plm::cu_count();
     s.columns = head_dim > 128 ? Layout<256, false>::kColumns : Layout<128, false>::kColumns;
     s.tiles = rows * group / s.columns + sequences + 2;
-    s.split = sequences <= kMostSplitSequences && rows * heads / s.columns < kFewTiles * resident &&
+    s.split = rows * heads / s.columns < kFewTiles * resident &&
               capacity > kTile * (static_cast<int64_t>(kStart + kJoin) + 1);
     s.runs = 0;
     s.work_shift = 0;
@@ -1127,6 +1237,7 @@ ChunkShape shape_of(int64_t sequences, int64_t rows, int64_t heads, int64_t kv_h
         while (s.tiles * (plm::ceil_div(capacity, kTile) + kTileWork) >> s.work_shift > kMostInt / 2) ++s.work_shift;
         s.bytes = static_cast<size_t>(2 * s.runs) * kv_heads * s.columns * (head_dim + 2) * sizeof(float) +
                   2 * sizeof(int) * s.tiles;
+        if (sequences > kFewSequences) s.bytes += (sizeof(Found) + sizeof(int)) * s.runs;
     }
     return s;
 }
@@ -1149,11 +1260,13 @@ int launch_kernel(const ChunkArgs& a, const ChunkShape& s, hipStream_t st) {
     }
     const int64_t g = 8 % a.kv_heads == 0 ? 8 / a.kv_heads : 1;
     const int64_t blocks = plm::ceil_div(a.pieces, g) * g * a.kv_heads;
+    if (a.found != nullptr)
+        hipLaunchKernelGGL(paged_chunk_find_kernel, dim3(static_cast<unsigned>(s.runs)), dim3(kFindThreads), 0, st, a);
     hipLaunchKernelGGL((paged_chunk_kernel<BF16, E8, DP>), dim3(static_cast<unsigned>(blocks)), dim3(64 * L::kWaves),
                        bytes, st, a);
     if (s.split)
         hipLaunchKernelGGL((paged_chunk_join_kernel<BF16>),
-                           dim3(static_cast<unsigned>(s.tiles), static_cast<unsigned>(a.kv_heads),
+                           dim3(static_cast<unsigned>(a.found != nullptr ? s.runs : s.tiles), static_cast<unsigned>(a.kv_heads),
                                 L::kColumns / kJoinColumns),
                            dim3(kJoinThreads), 0, st, a);
     return 0;
@@ -1209,6 +1322,10 @@ int run_chunk(ChunkArgs& a, const uint16_t* q, uint16_t* out, const int* row_sta
     a.part = static_cast<float*>(part);
     a.part_ml = a.part + 2 * s.runs * kv_heads * s.columns * head_dim;
     a.plan = s.split ? reinterpret_cast<int*>(a.part_ml + 2 * s.runs * kv_heads * s.columns * 2) : nullptr;
+    a.tiles = static_cast<int>(s.tiles);
+    const bool many = s.split && sequences > kFewSequences;
+    a.found = many ? reinterpret_cast<Found*>(a.plan + 2 * s.tiles) : nullptr;
+    a.begun = many ? reinterpret_cast<int*>(a.found + s.runs) : nullptr;
     a.by_page = divider_of(a.p.page_size);
     a.by_group = divider_of(static_cast<uint32_t>(a.group));
     // a scale of 0 would make NaN of hidden scores

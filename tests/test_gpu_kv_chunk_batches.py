@@ -220,3 +220,105 @@ def test_weight_on_a_few_of_many_e4m3_positions(nat, heads, kvh, dim, length, ro
     want, bound = pref.chunk(q, *caches, table, [length], [0, rows], 1.0, scales=scales, weight=2.0 ** -15)
     rest = 2.0 ** -8 * 2 * (length + rows) * math.exp(-21.0) * 448.0 * float(scales[1].max())
     pref.agree(got, want, bound + rest)
+
+
+def many(sequences, long, page, heads, kvh, dim, dtype, e4m3, seed):
+    """(q, caches, scales, table, lengths, starts): short sequences of 0 to 3 rows, idle ones among them, and a few long
+    ones, over random pages of a small pool."""
+    pool = 200
+    caches, scales, _ = pref.make_pages([pool * page], page, kvh, dim, E4M3 if e4m3 else dtype, seed, spare=0)
+    g = torch.Generator().manual_seed(seed + 1)
+    lengths = [(7 * b) % 150 if b % 11 else -1 for b in range(sequences)]
+    rows = [(3 * b) % 4 for b in range(sequences)]
+    for at, (length, n) in long.items():
+        lengths[at], rows[at] = length, n
+    cols = (max(x + r for x, r in zip(lengths, rows)) + page - 1) // page
+    table = torch.randint(0, pool, (sequences, cols), generator=g, dtype=torch.int32)
+    starts = [0]
+    for r in rows:
+        starts.append(starts[-1] + r)
+    return randn((starts[-1] + 3, heads, dim), dtype, seed + 2), caches, scales, table, lengths, starts
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("heads,kvh,dim", [(14, 2, 128), (4, 1, 64), (3, 1, 80)])
+@pytest.mark.parametrize("sequences", [62, 63, 256, 257, 300, 1100])
+def test_long_sequences_among_many(nat, e4m3, heads, kvh, dim, sequences):
+    long = {sequences // 3: (20000, 1), sequences - 1: (9000, 2), 0: (5000, 70)}
+    q, caches, scales, table, lengths, starts = many(sequences, long, 16, heads, kvh, dim, BF16, e4m3, sequences)
+    got = attend(nat, q, caches, scales, table, lengths, starts)
+    want, bound = pref.chunk(q, *caches, table, lengths, starts, dim ** -0.5, scales=scales,
+                             weight=E4M3_WEIGHT[BF16] if e4m3 else None)
+    pref.agree(got, want, bound)
+
+
+@pytest.mark.parametrize("sequences", [4000, 8191, 65535])
+def test_long_sequences_among_thousands(nat, sequences):
+    """Rows of a few sequences against those alone."""
+    long = {5: (30000, 1), sequences - 2: (12000, 3)}
+    q, caches, scales, table, lengths, starts = many(sequences, long, 16, 4, 1, 64, BF16, False, 3)
+    got = attend(nat, q, caches, scales, table, lengths, starts)
+    for b in (2, 5, 1001, sequences // 2, sequences - 2, sequences - 1):
+        mine = slice(starts[b], starts[b + 1])
+        want, bound = pref.chunk(q[mine], *caches, table[b:b + 1], lengths[b:b + 1], [0, starts[b + 1] - starts[b]], 64 ** -0.5)
+        pref.agree(got[mine], want, bound)
+    assert not bool(got[starts[-1]:].any())
+
+
+def test_scratch_of_many_sequences(nat):
+    """A caller's scratch is not left, whatever the call's sequences are split into."""
+    from pocketlm_amd import _lib
+
+    lib = _lib.load()
+    heads, kvh, dim, page = 14, 2, 128, 16
+    q, caches, scales, table, lengths, starts = many(700, {20: (30000, 1), 600: (4000, 90)}, page, heads, kvh, dim, BF16, False, 8)
+    table_d, rows = table.cuda(), q.shape[0]
+    need = lib.kv_paged_attention_chunk_scratch_bytes(700, rows, heads, kvh, dim, table.shape[1] * page)
+    held = torch.full((need + 65536,), 0xA5, dtype=torch.uint8, device="cuda")
+    for ls in (lengths, [x // 50 for x in lengths], [min(x * 30, 20000) for x in lengths], lengths):
+        want = attend(nat, q, caches, scales, table, ls, starts)
+        out = torch.full_like(q, 7.0)
+        lengths_d, starts_d = i32(ls), i32(starts)
+        lib.pocketlm_set_stream(torch.cuda.current_stream().cuda_stream)
+        assert 0 == lib.kv_paged_attention_chunk_u16(
+            q.data_ptr(), caches[0].data_ptr(), caches[1].data_ptr(), table_d.data_ptr(), lengths_d.data_ptr(),
+            starts_d.data_ptr(), out.data_ptr(), held.data_ptr(), need, rows, 700, heads, kvh, dim, heads * dim, dim,
+            table.shape[1], caches[0].shape[0], page, *caches[0].stride()[:3], dim ** -0.5, 1)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        assert bool((held[need:] == 0xA5).all())
+
+
+def test_time_of_one_long_sequence_among_many(nat):
+    """It is split over the device as among few: within twice the time (16 times where it is not split)."""
+    times = []
+    for sequences in (250, 300):
+        q, caches, scales, table, lengths, starts = many(sequences, {100: (60000, 1)}, 16, 28, 4, 128, BF16, False, 4)
+        where = (table.cuda(), i32(lengths), i32(starts))
+        times.append(milliseconds(lambda: nat.kv_paged_attention_chunk(q, *caches, *where)))
+    assert times[1] < 2 * times[0], times
+
+
+def test_many_sequences_in_a_graph(nat):
+    """Captured with short lengths, replayed with others that are split, in other orders; rows of no sequence are zero."""
+    q, caches, scales, table, lengths, starts = many(400, {7: (30000, 1), 300: (5000, 80)}, 16, 14, 2, 128, BF16, False, 6)
+    table_d, lengths_d, starts_d = table.cuda(), i32([50 if x >= 0 else -1 for x in lengths]), i32(starts)
+
+    def call():
+        return nat.kv_paged_attention_chunk(q, *caches, table_d, lengths_d, starts_d)
+
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for ls, ss in ((lengths, starts), (lengths[::-1], starts), ([x // 100 for x in lengths], starts), (lengths, [0] * 300 + starts[300:]),
+                   (lengths, starts)):
+        lengths_d.copy_(i32(ls))
+        starts_d.copy_(i32(ss))
+        want = call()
+        torch.cuda.synchronize()
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
