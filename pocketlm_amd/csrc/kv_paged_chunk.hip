@@ -49,7 +49,7 @@ struct ChunkArgs {
     const uint16_t* q;     // [rows][heads][head_dim]
     uint16_t* out;         // the same, contiguous
     const int* row_starts; // [sequences + 1]
-    float* part;           // [slot][kv head][column of a tile][head_dim], then the maxima and sums
+    float* part;           // [slot][kv head][column of a tile, of part_columns][head_dim], then the maxima and sums
     float* part_ml;
     int* plan;             // {the run that begins it, the one that ends it} of each tile; null: no tile is split
     struct Found* found;   // of each run, by a kernel of its own; null: each workgroup finds its run
@@ -63,6 +63,7 @@ struct ChunkArgs {
     int group;
     int head_dim;
     int columns_log2;      // of a tile
+    int part_columns;      // of a tile of the largest sequence that the rows may be
     int pieces;            // tiles of a head, and runs, at most
     int runs;              // at most
     uint32_t work_shift;   // so that a head's work stays in 32 bits
@@ -974,7 +975,7 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
     l = both_sum(l);
     // where column c's results go: a partial's, or the output's
     auto partial_of = [&](int c) {
-        return (static_cast<int64_t>(piece.slot) * a.kv_heads + kvh) * L::kColumns + (c - piece.tile * L::kColumns);
+        return (static_cast<int64_t>(piece.slot) * a.kv_heads + kvh) * a.part_columns + (c - piece.tile * L::kColumns);
     };
     auto output_of = [&](int c, int r) {
         return a.out + (static_cast<int64_t>(piece.first + r) * a.heads + kvh * a.group + c - r * a.group) * a.head_dim + 4 * half;
@@ -1118,8 +1119,8 @@ __device__ __forceinline__ void join_column(const ChunkArgs& a, int run, int par
     const int part_lane = lane & (LANES - 1), g = part_lane >> 4, j = lane & 15;
     // partial i: the first is its run's second
     auto slot = [](int i) { return max(2 * i, 1); };
-    const int64_t stride = static_cast<int64_t>(a.kv_heads) << a.columns_log2;
-    const int64_t from = ((static_cast<int64_t>(2 * run) * a.kv_heads + kvh) << a.columns_log2) + in;
+    const int64_t stride = static_cast<int64_t>(a.kv_heads) * a.part_columns;
+    const int64_t from = (static_cast<int64_t>(2 * run) * a.kv_heads + kvh) * a.part_columns + in;
     const f32x2* ml = reinterpret_cast<const f32x2*>(a.part_ml) + from;
     float m = -INFINITY;
     for (int i = part_lane; i < parts; i += LANES) m = fmaxf(m, ml[slot(i) * stride][0]);
@@ -1211,6 +1212,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_chunk_join_kernel(const Ch
 
 struct ChunkShape {
     int64_t columns;   // of a tile
+    int64_t part_columns;
     int64_t tiles;     // of a head, at most
     int64_t runs;      // of a head, at most
     bool split;
@@ -1226,6 +1228,7 @@ ChunkShape shape_of(int64_t sequences, int64_t rows, int64_t heads, int64_t kv_h
     const int64_t group = heads / kv_heads;
     const int64_t resident = plm::cu_count();
     s.columns = head_dim > 128 ? Layout<256, false>::kColumns : Layout<128, false>::kColumns;
+    s.part_columns = std::min(s.columns, rows * group);
     s.tiles = rows * group / s.columns + sequences + 2;
     s.split = rows * heads / s.columns < kFewTiles * resident &&
               capacity > kTile * (static_cast<int64_t>(kStart + kJoin) + 1);
@@ -1235,7 +1238,7 @@ ChunkShape shape_of(int64_t sequences, int64_t rows, int64_t heads, int64_t kv_h
     if (s.split) {
         s.runs = std::max<int64_t>(1, resident / kv_heads);
         while (s.tiles * (plm::ceil_div(capacity, kTile) + kTileWork) >> s.work_shift > kMostInt / 2) ++s.work_shift;
-        s.bytes = static_cast<size_t>(2 * s.runs) * kv_heads * s.columns * (head_dim + 2) * sizeof(float) +
+        s.bytes = static_cast<size_t>(2 * s.runs) * kv_heads * s.part_columns * (head_dim + 2) * sizeof(float) +
                   2 * sizeof(int) * s.tiles;
         if (sequences > kFewSequences) s.bytes += (sizeof(Found) + sizeof(int)) * s.runs;
     }
@@ -1320,8 +1323,9 @@ int run_chunk(ChunkArgs& a, const uint16_t* q, uint16_t* out, const int* row_sta
     a.runs = static_cast<int>(s.runs);
     a.work_shift = s.work_shift;
     a.part = static_cast<float*>(part);
-    a.part_ml = a.part + 2 * s.runs * kv_heads * s.columns * head_dim;
-    a.plan = s.split ? reinterpret_cast<int*>(a.part_ml + 2 * s.runs * kv_heads * s.columns * 2) : nullptr;
+    a.part_columns = static_cast<int>(s.part_columns);
+    a.part_ml = a.part + 2 * s.runs * kv_heads * s.part_columns * head_dim;
+    a.plan = s.split ? reinterpret_cast<int*>(a.part_ml + 2 * s.runs * kv_heads * s.part_columns * 2) : nullptr;
     a.tiles = static_cast<int>(s.tiles);
     const bool many = s.split && sequences > kFewSequences;
     a.found = many ? reinterpret_cast<Found*>(a.plan + 2 * s.tiles) : nullptr;

@@ -322,3 +322,31 @@ def test_many_sequences_in_a_graph(nat):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("heads,kvh,dim,rows", [(28, 4, 128, 1), (28, 4, 128, 36), (28, 4, 128, 37), (5, 5, 64, 3), (3, 1, 256, 50)])
+def test_scratch_of_few_rows(nat, heads, kvh, dim, rows):
+    """It holds partials of the columns that the rows have, and no more is written."""
+    from pocketlm_amd import _lib
+
+    lib = _lib.load()
+    page, length = 16, 30000
+    caches, _, table = pref.make_pages([200 * page], page, kvh, dim, BF16, 3, spare=0)
+    table = torch.randint(0, 200, (1, (length + rows + page - 1) // page), generator=torch.Generator().manual_seed(1),
+                          dtype=torch.int32)
+    q = randn((rows, heads, dim), BF16, 4)
+    need = lib.kv_paged_attention_chunk_scratch_bytes(1, rows, heads, kvh, dim, table.shape[1] * page)
+    # two partials of at most a tile's columns of each of at most 256 runs of all heads, and their plan
+    most = min(256 if dim <= 128 else 128, rows * heads // kvh)
+    assert 0 < need <= 2 * 256 * most * (dim + 2) * 4 + 65536
+    held = torch.full((need + 65536,), 0xA5, dtype=torch.uint8, device="cuda")
+    table_d, lengths, starts, out = table.cuda(), i32([length]), i32([0, rows]), torch.zeros_like(q)
+    want, bound = pref.chunk(q, *caches, table, [length], [0, rows], dim ** -0.5)
+    lib.pocketlm_set_stream(torch.cuda.current_stream().cuda_stream)
+    assert 0 == lib.kv_paged_attention_chunk_u16(
+        q.data_ptr(), caches[0].data_ptr(), caches[1].data_ptr(), table_d.data_ptr(), lengths.data_ptr(), starts.data_ptr(),
+        out.data_ptr(), held.data_ptr(), need, rows, 1, heads, kvh, dim, heads * dim, dim, table.shape[1], caches[0].shape[0], page,
+        *caches[0].stride()[:3], dim ** -0.5, 1)
+    torch.cuda.synchronize()
+    pref.agree(out, want, bound)
+    assert bool((held[need:] == 0xA5).all())
