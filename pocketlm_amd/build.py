@@ -6,15 +6,23 @@
 Each source under csrc/ is compiled to an object in csrc/_build/ (in
 parallel), then linked into pocketlm_amd/libpocketlm_hip.so.  Only the
 symbols declared in include/pocketlm_hip.h are exported.
+
+Where a kernel needs more vector registers than it has, hipcc can save one at
+the end of a divergent region before it enables the other lanes again, which
+then read back what was in memory before.  Such a kernel faults now and then, so
+the build reads each source's assembly and fails at such a store
+(masked_spills).
 """
 
 from __future__ import annotations
 
 import argparse
 import os
+import re
 import shutil
 import subprocess
 import sys
+import tempfile
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -51,12 +59,40 @@ def sources() -> list[Path]:
     return sorted(CSRC.glob("*.hip"))
 
 
+_LABEL = re.compile(r"^(?P<function>_\w+):|^(?:\.LBB|; %bb|\.Lfunc_end)")
+
+
+def masked_spills(assembly: str) -> list[str]:
+    """Stores of spilled vector registers in front of the instruction that ends
+    their block's divergent region, as "function: store"."""
+    found, function, stores = [], "", []
+    for line in assembly.splitlines():
+        label = _LABEL.match(line)
+        if label:
+            function, stores = label["function"] or function, []
+        elif "saveexec" in line:
+            stores = []
+        elif "Spill" in line and ("scratch_store" in line or "buffer_store" in line):
+            stores.append(f"{function}: {line.strip()}")
+        elif stores and "s_or_b64 exec, exec," in line:
+            found += stores
+            stores = []
+    return found
+
+
 def _compile(src: Path) -> Path:
     obj = BUILD_DIR / (src.stem + ".o")
-    cmd = [hipcc(), *COMMON_FLAGS, "-c", str(src), "-o", str(obj)]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{proc.stdout}\n{proc.stderr}")
+    with tempfile.TemporaryDirectory(dir=BUILD_DIR) as temps:
+        held = Path(temps) / obj.name
+        cmd = [hipcc(), *COMMON_FLAGS, "-save-temps=obj", "-c", str(src), "-o", str(held)]
+        proc = subprocess.run(cmd, capture_output=True, text=True)
+        if proc.returncode != 0:
+            raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{proc.stdout}\n{proc.stderr}")
+        listing = Path(temps) / f"{src.stem}-hip-amdgcn-amd-amdhsa-{ARCH}.s"
+        found = masked_spills(listing.read_text())
+        if found:
+            raise RuntimeError(f"{src.name}: registers spilled while lanes are off, use fewer:\n" + "\n".join(found))
+        os.replace(held, obj)
     return obj
 
 

@@ -524,7 +524,10 @@ __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, i
     typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
     typedef __attribute__((address_space(3))) const int lds_int;
     const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
-    const int lane = threadIdx.x & 63;
+    // (the lane's place anew for each piece: what follows from it is not kept in registers over the others, which
+    // took e4m3 kernels of heads of 65 to 128 past their 256)
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool second = wave >= 4;
     const int li = lane & 31, half = lane >> 5;
