@@ -350,3 +350,33 @@ def test_scratch_of_few_rows(nat, heads, kvh, dim, rows):
     torch.cuda.synchronize()
     pref.agree(out, want, bound)
     assert bool((held[need:] == 0xA5).all())
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("heads,kvh,dim", [(28, 4, 128), (6, 6, 64), (4, 2, 256), (3, 1, 80)])
+@pytest.mark.parametrize("rows,longest", [(3, 2500), (45, 700)])
+def test_values_that_are_not_finite_in_some_sequences(nat, e4m3, heads, kvh, dim, rows, longest):
+    """Workgroups that go from sequences with such values, seen by all, by some and by few of the rows, to others without
+    them, and pages that are not there."""
+    page, count = 16, 40
+    lengths = [(longest * (7 * b % count)) // count for b in range(count)]
+    g = torch.Generator().manual_seed(13)
+    starts = list(range(0, rows * count + 1, rows))
+    q = torch.randn((rows * count, heads, dim), generator=g).to(BF16).cuda()
+    caches, scales, table = pref.make_pages([x + rows for x in lengths], page, kvh, dim, E4M3 if e4m3 else BF16, 14,
+                                            dirt=float("nan"))
+    v = caches[1].view(torch.uint8) if e4m3 else caches[1]
+    bad = 0x7F if e4m3 else float("nan")
+    for b in range(0, count, 3):
+        for pos, at in ((lengths[b] + rows - 1, 5), (lengths[b] + rows // 2, 7), (lengths[b] // 2, 9)):
+            v[int(table[b, pos // page]), pos % page, b % kvh, at] = bad
+        if not e4m3:
+            v[int(table[b, lengths[b] // page]), lengths[b] % page, :, 11] = float("inf")
+    for b in range(0, count, 7):
+        if lengths[b] > 200:
+            table[b, 3] = -7
+    got = attend(nat, q, caches, scales, table, lengths, starts)
+    want, bound = pref.chunk(q, *caches, table, lengths, starts, dim ** -0.5, scales=scales,
+                             weight=E4M3_WEIGHT[BF16] if e4m3 else None)
+    assert bool(want.isnan().any()) and bool(want.isfinite().all(2).any())
+    pref.agree(got, want, bound)
