@@ -948,10 +948,11 @@ constexpr double kLittleBytes = 64.0 * (1 << 20);
 
 // e4m3 caches: three workgroups to a compute unit, where registers allow them and
 // the sequences hold more than this of 16-bit values, half of it in bytes: a wave has
-// half as many bytes in flight (48 sequences of up to 16381 positions, 4 heads of
-// 128, 133 us against 141 with two, 64 of 8000, 8 heads of 64 144 and 148; but 32
-// of 3000 with 2 rows, 4 heads of 128 37 and 31; head sizes below 128 that are not 64
-// or less take more registers: 48 of 16000, 5 heads of 96 193 and 177).
+// half as many bytes in flight (a batch called again and again: 48 sequences of up to
+// 16381 positions, 4 heads of 128, 131 us against 139 with two, 126 among other calls; 64
+// of 8000, 8 heads of 64 144 and 151; but 32 of 3000 with 2 rows, 4 heads of 128 37 and
+// 31; head sizes below 128 that are not 64 or less take more registers: 48 of 16000, 5
+// heads of 96 188 and 169).
 constexpr double kManyBytes = 512.0 * (1 << 20);
 
 struct AttnShape {

@@ -168,7 +168,7 @@ __device__ __forceinline__ int place_of_tile(const ChunkArgs& a, int at, int lan
 // of the work and a fifth of the longest; runs take their share, kStart for each tile
 // that they hold a part of, kJoin, and kJoinRuns where every workgroup leaves
 // partials of full tiles (67 MB at a head of 128).  28 and 4 heads of 128, whole / in runs: a prompt
-// of 500 rows 28 / 41 us, of 1500 56 / 67, of 2500 81 / 108, 16 of up to 200 rows 33 / 56; 37 rows
+// of 500 rows 29 / 41 us, of 1500 56 / 67, of 2500 81 / 108, 16 of up to 200 rows 33 / 56; 37 rows
 // behind 700 positions 34 / 27, 64 times 2 rows behind up to 4000 128 / 110.
 constexpr uint32_t kTileWork = 2;
 constexpr uint32_t kLeastWork = 4;  // of a run
@@ -413,7 +413,7 @@ __device__ __forceinline__ int swizzle(int position) {
 
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-// 16 bytes a lane to LDS, the wave's KB in lane order at `to` (see fp8_matmul.hip).  The wait is loads_barrier's.
+// 16 bytes a lane to LDS, the wave's KB in lane order at `to` (see fp8_matmul.hip).  The wait is `landed`'s.
 __device__ __forceinline__ void load_to_lds(const void* from, uint32_t to) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(to) : "m0", "memory");
 }
@@ -504,11 +504,13 @@ __device__ __forceinline__ void reset_cleared(lds_char* lds) {
 // long as without it.  Positions behind the last one seen are never read.
 //
 // Bound by the matrix cores' power and by the exponentials between them: two
-// prompts of up to 8191 rows of 28 and 4 heads of 128, 752 GFLOP, in 726 us, 1.03 PFLOP/s
-// (a library product of 8192^3 1.05 to 1.2); in step, with tiles three deep, the waves
-// took 818.  Over e4m3 pages 2048 rows behind 30000 positions, 911 GFLOP, in 952
-// us (1065 with each lane's page and scale found anew for each load).  Small calls wait for
-// memory and for the code: 37 rows behind 700 positions 20 us of kernel.
+// prompts of up to 8191 rows of 28 and 4 heads of 128, 752 GFLOP, in 717 to 776 us (as
+// the card is rested or in a row of calls), 0.97 to 1.05 PFLOP/s (a library product of
+// 8192^3 1.05 to 1.2); in step, with tiles three deep, the waves took 818.  Over e4m3
+// pages 2048 rows behind 30000 positions, 911 GFLOP, in 966 to 1050 us (1065 with each
+// lane's page and scale found anew for each load, against 952).  Small calls wait for
+// memory and for the code: 37 rows behind 700 positions 21 us of kernel; the look at
+// the tiles of the diagonal is 1 us of a prompt of 500 rows' 29.
 template <bool BF16, bool E8, int DP>
 __device__ __forceinline__ void attend(const ChunkArgs& a, const Piece& piece, int kvh, lds_char* lds) {
     using L = Layout<DP, E8>;
