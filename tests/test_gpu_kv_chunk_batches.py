@@ -21,7 +21,7 @@ E4M3_WEIGHT = {BF16: ref.HALF[BF16], F16: 2.0 ** -7 * ref.HALF[BF16]}
 def nat():
     from pocketlm_amd import native
 
-    assert native.native_paged_kv_available(), "libpocketlm_hip.so must load on the GPU box"
+    assert native.native_paged_kv_available(), "libpocketlm_hip.so must load"
     return native
 
 

@@ -19,7 +19,7 @@ POOL = 300
 def nat():
     from pocketlm_amd import native
 
-    assert native.native_paged_kv_available(), "libpocketlm_hip.so must load on the GPU box"
+    assert native.native_paged_kv_available(), "libpocketlm_hip.so must load"
     return native
 
 
